@@ -56,6 +56,91 @@ pub struct IrisModelDesc {
     pub layer_is_sliding: *const u8,
 }
 
+/// Key and value pages of one layer (include/iris_hip.h `IrisPagedKv`).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct IrisPagedKv {
+    pub k: *mut i32,
+    pub v: *mut i32,
+    pub pages: u32,
+    pub page_size: u32,
+    pub kv_heads: u32,
+    pub head_dim: u32,
+}
+
+/// The block tables and slot map of a pass (`IrisPagedPlan`).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct IrisPagedPlan {
+    pub lengths: *const i32,
+    pub added: *const i32,
+    pub parents: *const i32,
+    pub held: *const i32,
+    pub held_out: *mut i32,
+    pub table: *mut i32,
+    pub ring: *mut i32,
+    pub ring_state: *const i32,
+    pub ring_state_out: *mut i32,
+    pub row_start: *mut i32,
+    pub slots: *mut i32,
+    pub positions: *mut i32,
+    pub status: *mut i32,
+    pub requests: u32,
+    pub table_stride: u32,
+    pub pages: u32,
+    pub page_size: u32,
+    pub max_rows: u32,
+}
+
+/// Causal attention over packed prompts (`IrisPackedAttention`).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct IrisPackedAttention {
+    pub q: *const i32,
+    pub k: *const i32,
+    pub v: *const i32,
+    pub out: *mut i32,
+    pub row_start: *const i32,
+    pub status: *mut i32,
+    pub q_stride: u32,
+    pub k_stride: u32,
+    pub v_stride: u32,
+    pub out_stride: u32,
+    pub sequences: u32,
+    pub rows: u32,
+    pub max_length: u32,
+    pub heads: u32,
+    pub kv_heads: u32,
+    pub head_dim: u32,
+    pub window: u32,
+    pub scaled: i32,
+    pub scale_q32: u32,
+}
+
+/// Attention of drafted trees over the paged cache (`IrisTreeAttention`).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct IrisTreeAttention {
+    pub q: *const i32,
+    pub out: *mut i32,
+    pub row_start: *const i32,
+    pub lengths: *const i32,
+    pub parents: *const i32,
+    pub table: *const i32,
+    pub status: *mut i32,
+    pub q_stride: u32,
+    pub out_stride: u32,
+    pub requests: u32,
+    pub rows: u32,
+    pub table_stride: u32,
+    pub max_nodes: u32,
+    pub max_positions: u32,
+    pub heads: u32,
+    pub window: u32,
+    pub scaled: i32,
+    pub scale_q32: u32,
+}
+
 extern "C" {
     pub fn q8gpu_error(code: c_int) -> *const c_char;
     pub fn q8gpu_init() -> c_int;
@@ -257,5 +342,31 @@ extern "C" {
     ) -> c_int;
     pub fn iris_silu_device(x: *const i32, n: u32, out: *mut i32) -> c_int;
     pub fn iris_silu_table_device(x: *const i32, n: u32, out: *mut i32) -> c_int;
+    pub fn iris_paged_plan(plan: *const IrisPagedPlan, stream: *mut c_void) -> c_int;
+    pub fn iris_paged_store(
+        cache: *const IrisPagedKv,
+        k: *const i32,
+        k_stride: u32,
+        v: *const i32,
+        v_stride: u32,
+        slots: *const i32,
+        rows: u32,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn iris_attention_packed_workspace_bytes(a: *const IrisPackedAttention) -> u64;
+    pub fn iris_attention_packed(
+        a: *const IrisPackedAttention,
+        d_workspace: *mut c_void,
+        workspace_bytes: u64,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn iris_attention_tree_workspace_bytes(cache: *const IrisPagedKv, a: *const IrisTreeAttention) -> u64;
+    pub fn iris_attention_tree(
+        cache: *const IrisPagedKv,
+        a: *const IrisTreeAttention,
+        d_workspace: *mut c_void,
+        workspace_bytes: u64,
+        stream: *mut c_void,
+    ) -> c_int;
     pub fn iris_sha256_bytes(data: *const u8, len: u64, out: *mut u8) -> c_int;
 }

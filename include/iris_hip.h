@@ -390,6 +390,148 @@ int iris_silu_device(const int32_t* x, uint32_t n, int32_t* out);
  * reference. */
 int iris_silu_table_device(const int32_t* x, uint32_t n, int32_t* out);
 
+/* ------------------------------------------------------------------------
+ * Several requests over one paged cache: the operators of a pass (no
+ * counterpart in the reference, whose executor runs one sequence,
+ * crates/inference/direct/src/executor.rs:143-185). The arithmetic of a row
+ * is the reference's (crates/inference/kernels/src/mistral/layer.rs:274-318,
+ * crates/inference/kernels/src/prefill_range.rs:755-845), so a row's result
+ * has the same bits whichever rows share its launch.
+ *
+ * Every pointer inside these structs is device memory of the current device;
+ * the structs themselves are host memory, read before the call returns. Calls
+ * enqueue on `stream` (a hipStream_t; NULL = the null stream), allocate
+ * nothing, do not synchronise and can be captured into a graph. Work space
+ * holds nothing between calls; calls that may run at once need their own.
+ * What the device finds wrong (counts and indexes in device memory) it
+ * reports in *status; nothing is read or written out of bounds.
+ * ---------------------------------------------------------------------- */
+
+/* Key and value pages of one layer: [pages][kv_heads][page_size][head_dim]
+ * Q16.16 values each, 16-byte aligned. page_size is a power of two from 4 to
+ * 1024, head_dim a multiple of 4 up to 512, pages * page_size below 2^31. A
+ * slot is page * page_size + the place within the page. */
+typedef struct IrisPagedKv {
+    int32_t* k;
+    int32_t* v;
+    uint32_t pages, page_size, kv_heads, head_dim;
+} IrisPagedKv;
+
+/* A pass's block tables and slot map from the requests' lengths. Request b
+ * holds lengths[b] positions in held[b] pages, table[b][0 .. held[b]), and
+ * adds added[b] rows: it needs ceil((lengths[b] + added[b]) / page_size)
+ * pages. Pages it lacks come from the ring of free pages, those past its need
+ * go back to the ring (lengths = added = 0 returns them all), each in request
+ * order. The ring holds ring_state[1] pages from ring[ring_state[0]], modulo
+ * `pages`.
+ *   held_out[b]     the pages held now (may be held itself)
+ *   table           entries [held, need) written, the others left
+ *   ring            the entries behind the free pages: the returned ones
+ *   ring_state_out  first and count now (may be ring_state itself)
+ *   row_start       [requests + 1] first row of each request's added rows
+ *   slots           [max_rows] each added row's slot, -1 from the last row on
+ *   positions       (nullable) [max_rows] each added row's position,
+ *                   lengths[b] + its depth, -1 from the last row on
+ *   parents         (nullable) [max_rows] each row's parent in its request's
+ *                   tree of drafted rows, as IrisTreeAttention's (a row's
+ *                   depth is the number of its ancestors); null: row i of a
+ *                   request has depth i. A request then adds at most 64 rows.
+ *   status          0; or IRIS_E_RANGE where the rows, a request's pages or
+ *                   the free pages do not suffice, IRIS_E_INVALID for counts
+ *                   that cannot be: the state is then as it was, row_start is
+ *                   0 and slots and positions are -1. */
+typedef struct IrisPagedPlan {
+    const int32_t* lengths;
+    const int32_t* added;
+    const int32_t* parents;
+    const int32_t* held;
+    int32_t* held_out;
+    int32_t* table;
+    int32_t* ring;
+    const int32_t* ring_state;
+    int32_t* ring_state_out;
+    int32_t* row_start;
+    int32_t* slots;
+    int32_t* positions;
+    int32_t* status;
+    uint32_t requests, table_stride, pages, page_size, max_rows;
+} IrisPagedPlan;
+
+/* Builds them; at most 4096 requests. One call at a time changes a ring. */
+int iris_paged_plan(const IrisPagedPlan* plan, void* stream);
+
+/* Writes rows of keys and values (kv_heads * head_dim values each, strides in
+ * values, multiples of 4, 16-byte aligned) to their slots; a row whose slot is
+ * outside the cache (-1) is skipped. Two rows of one slot: either one. */
+int iris_paged_store(const IrisPagedKv* cache, const int32_t* k, uint32_t k_stride, const int32_t* v,
+                     uint32_t v_stride, const int32_t* slots, uint32_t rows, void* stream);
+
+/* Causal attention over whole prompts, packed row after row: row t of the
+ * sequence that starts at s = row_start[i] <= t < row_start[i + 1] sees rows
+ * [max(s, t + 1 - window), t] (window 0: from s). Query head h reads key head
+ * h / (heads / kv_heads). Strides are in values, multiples of 4; the arrays
+ * 16-byte aligned; out overlaps none of the others.
+ *   scaled      1: scores are the scaled dot product (scale_q32, mistral);
+ *               0: the requantized dot product (gemma)
+ *   rows        rows of q, k, v and out; rows from row_start[sequences] on
+ *               are left as they were
+ *   max_length  at least the longest sequence, at most 65535; a row that lies
+ *               deeper in its sequence is left as it was
+ *   status      (nullable) set to IRIS_E_RANGE where such a row was found;
+ *               never cleared here */
+typedef struct IrisPackedAttention {
+    const int32_t* q;
+    const int32_t* k;
+    const int32_t* v;
+    int32_t* out;
+    const int32_t* row_start;
+    int32_t* status;
+    uint32_t q_stride, k_stride, v_stride, out_stride;
+    uint32_t sequences, rows, max_length;
+    uint32_t heads, kv_heads, head_dim, window;
+    int32_t scaled;
+    uint32_t scale_q32;
+} IrisPackedAttention;
+
+/* Bytes of work space a call needs (0 for one that is refused). */
+uint64_t iris_attention_packed_workspace_bytes(const IrisPackedAttention* a);
+int iris_attention_packed(const IrisPackedAttention* a, void* d_workspace, uint64_t workspace_bytes, void* stream);
+
+/* Attention of each request's newest rows over its cached positions and, of
+ * the rows themselves, over their ancestors: request b's rows
+ * row_start[b] .. row_start[b + 1] (a tree of at most max_nodes <= 64 drafted
+ * tokens, or the one token of a decode step) lie in the cache behind its
+ * lengths[b] positions, in row order, at table[b]. Row i sees every position
+ * below lengths[b], itself, and the rows reached from it through parents
+ * (each a row of the request before its child; any other value: none). A row's
+ * position is lengths[b] + the number of its ancestors; with a window a row
+ * sees the last `window` positions up to its own.
+ *   parents        (nullable) null: each row's parent is the row before it
+ *   max_positions  at least the largest lengths[b] + rows of b, at most 2^20
+ *   status         (nullable) set to IRIS_E_RANGE where a request's rows or
+ *                  positions pass these bounds or its table (its rows are left
+ *                  as they were), to IRIS_E_INVALID where the table names a
+ *                  page outside the cache (read as zeros); never cleared here
+ * The rest as in IrisPackedAttention. */
+typedef struct IrisTreeAttention {
+    const int32_t* q;
+    int32_t* out;
+    const int32_t* row_start;
+    const int32_t* lengths;
+    const int32_t* parents;
+    const int32_t* table;
+    int32_t* status;
+    uint32_t q_stride, out_stride;
+    uint32_t requests, rows, table_stride, max_nodes, max_positions;
+    uint32_t heads, window;
+    int32_t scaled;
+    uint32_t scale_q32;
+} IrisTreeAttention;
+
+uint64_t iris_attention_tree_workspace_bytes(const IrisPagedKv* cache, const IrisTreeAttention* a);
+int iris_attention_tree(const IrisPagedKv* cache, const IrisTreeAttention* a, void* d_workspace,
+                        uint64_t workspace_bytes, void* stream);
+
 /* SHA-256 (FIPS 180-4) of `len` bytes into out[32]; the hash
  * iris_session_layer_pass uses. Host code only. */
 int iris_sha256_bytes(const uint8_t* data, uint64_t len, uint8_t* out);

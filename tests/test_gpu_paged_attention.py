@@ -1,0 +1,436 @@
+"""GPU: attention over packed prompts and of drafted trees over a paged cache,
+bit for bit against a plain 64-bit implementation with the oracle's softmax."""
+import random
+
+import numpy as np
+import pytest
+import torch
+
+from iris_amd import native, paged, scalars
+from tests import paged_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+LEFT = 123456789  # what rows that a call leaves hold
+
+
+@pytest.fixture(scope="module", autouse=True)
+def device():
+    native.check(native.lib().q8gpu_init(), "q8gpu_init")
+
+
+def values(rng, shape, kind):
+    """Q16.16 values: "normal" (three digits), "wide" (every int32), "mixed"
+    (normal with some of four and five digits), "sharp" (large, so that scores
+    differ by thousands), "ends" (the ends of the range), "same" (all equal)."""
+    if kind == "wide":
+        return rng.integers(-2 ** 31, 2 ** 31, shape, dtype=np.int64).astype(np.int32)
+    if kind == "ends":
+        return rng.choice(np.array([-2 ** 31, -2 ** 31 + 1, 2 ** 31 - 1, 0, 1, -1, -2 ** 23, 2 ** 23 - 1, 8355711, 8355712,
+                                    -8421504, -8421505], np.int64), shape).astype(np.int32)
+    if kind == "same":
+        return np.full(shape, 40000, np.int32)
+    x = rng.normal(0, 65536 * (16 if kind == "sharp" else 1), shape).round().astype(np.int64)
+    if kind == "mixed":
+        at = rng.random(shape) < 0.002
+        x = np.where(at, rng.integers(-2 ** 31, 2 ** 31, shape), x)
+    return x.astype(np.int32)
+
+
+def dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).cuda()
+
+
+def padded(a, extra):
+    """The rows of `a` at a stride of `extra` more values."""
+    out = torch.full((a.shape[0], a.shape[1] + extra), 77, dtype=torch.int32, device="cuda")
+    out[:, :a.shape[1]] = dev(a)
+    return out
+
+
+def scale_of(hd, scaled):
+    return scalars.attention_scale_q32(hd) if scaled else 0
+
+
+class Packed:
+    def __init__(self, rng, lens, heads, kv_heads, hd, window=0, scaled=True, kinds=("normal", "normal", "normal"),
+                 extra=(0, 0, 0, 0), behind=0, max_length=None):
+        self.starts = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+        rows = int(self.starts[-1]) + behind
+        self.heads, self.kv_heads, self.hd, self.window, self.scale = heads, kv_heads, hd, window, scale_of(hd, scaled)
+        self.q, self.k, self.v = (values(rng, (rows, n * hd), kind)
+                                  for n, kind in zip((heads, kv_heads, kv_heads), kinds))
+        self.t = [padded(x, e) for x, e in zip((self.q, self.k, self.v), extra)]
+        self.out = torch.full((rows, heads * hd + extra[3]), LEFT, dtype=torch.int32, device="cuda")
+        self.row_start, self.status = dev(self.starts), dev([0])
+        q, k, v = self.t
+        self.d = paged.PackedAttention(
+            q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=self.out.data_ptr(), row_start=self.row_start.data_ptr(),
+            status=self.status.data_ptr(), q_stride=q.stride(0), k_stride=k.stride(0), v_stride=v.stride(0),
+            out_stride=self.out.stride(0), sequences=len(lens), rows=rows, max_length=max_length or max(max(lens), 1),
+            heads=heads, kv_heads=kv_heads, head_dim=hd, window=window, scaled=int(scaled), scale_q32=self.scale)
+        self.size = paged.packed_workspace_bytes(self.d)
+        self.space = torch.full((max(self.size, 16),), 0xA5, dtype=torch.uint8, device="cuda")
+
+    def run(self, stream=None):
+        paged.attend_packed(self.d, self.space.data_ptr(), self.size, stream)
+
+    def want(self):
+        out = np.full(self.out.shape, LEFT, np.int32)
+        ref.packed(self.q, self.k, self.v, self.starts.tolist(), self.heads, self.kv_heads, self.hd, self.window,
+                   self.scale, out)
+        return out
+
+    def check(self):
+        torch.cuda.synchronize()
+        assert np.array_equal(self.out.cpu().numpy(), self.want())
+        assert self.status.item() == 0
+
+
+@pytest.mark.parametrize("heads, kv_heads, hd", [(1, 1, 4), (2, 1, 20), (4, 2, 64), (6, 2, 80), (8, 2, 128), (5, 5, 64),
+                                                 (8, 1, 256), (7, 1, 128), (2, 1, 512), (4, 4, 132)])
+@pytest.mark.parametrize("scaled", [True, False])
+def test_packed_heads(heads, kv_heads, hd, scaled):
+    rng = np.random.default_rng(hd + heads)
+    p = Packed(rng, [1, 17, 0, 64, 3, 66], heads, kv_heads, hd, scaled=scaled, extra=(4, 8, 12, 16), behind=3)
+    p.run()
+    p.check()
+
+
+@pytest.mark.parametrize("lens", [[1], [2], [15], [16], [17], [63], [64], [65], [129], [1] * 40, [0, 0, 5, 0], [100, 1, 1, 200],
+                                  [31, 33, 48, 16, 5, 250]])
+@pytest.mark.parametrize("window", [0, 1, 7, 64, 100])
+def test_packed_lengths_and_windows(lens, window):
+    rng = np.random.default_rng(sum(lens) + window)
+    p = Packed(rng, lens, 4, 2, 64, window=window)
+    p.run()
+    p.check()
+
+
+@pytest.mark.parametrize("kinds", [("wide", "wide", "wide"), ("normal", "wide", "normal"), ("wide", "normal", "normal"),
+                                   ("normal", "normal", "wide"), ("mixed", "mixed", "mixed"), ("ends", "ends", "ends"),
+                                   ("sharp", "sharp", "sharp"), ("same", "same", "ends"), ("normal", "normal", "ends"),
+                                   ("sharp", "normal", "mixed")])
+@pytest.mark.parametrize("heads, kv_heads, hd, scaled", [(4, 2, 64, True), (2, 2, 128, False), (4, 1, 256, False),
+                                                         (3, 1, 80, True), (2, 1, 512, True)])
+def test_packed_values(kinds, heads, kv_heads, hd, scaled):
+    rng = np.random.default_rng(hd)
+    p = Packed(rng, [37, 90, 16], heads, kv_heads, hd, scaled=scaled, kinds=kinds)
+    p.run()
+    p.check()
+
+
+@pytest.mark.parametrize("lens, window, hd", [([2700], 0, 64), ([700, 2400, 90], 0, 64), ([5000], 900, 128), ([1300, 1200], 0, 256),
+                                              ([1900], 0, 512)])
+def test_packed_long(lens, window, hd):
+    # Few heads; the rows that are compared: each sequence's ends and some between.
+    rng = np.random.default_rng(sum(lens))
+    p = Packed(rng, lens, 2, 1, hd, window=window, kinds=("sharp", "normal", "normal"))
+    p.run()
+    torch.cuda.synchronize()
+    got = p.out.cpu().numpy()
+    for a, b in zip(p.starts[:-1], p.starts[1:]):
+        n = b - a
+        rows = sorted({0, 1, n // 2, n - 17, n - 2, n - 1} | set(rng.integers(0, n, 10).tolist()))
+        at = np.arange(n)
+        seen = np.stack([(at <= r) & ((r - at < window) if window else True) for r in rows])
+        for h in range(2):
+            cols = slice(h * hd, h * hd + hd)
+            want = ref.attend(p.q[a:b][rows][:, cols], p.k[a:b], p.v[a:b], seen, p.scale)
+            assert np.array_equal(got[a:b][rows][:, cols], want)
+
+
+def test_packed_rows_deeper_than_max_length_are_left():
+    rng = np.random.default_rng(5)
+    p = Packed(rng, [40, 90, 20], 4, 2, 64, max_length=50)
+    p.run()
+    torch.cuda.synchronize()
+    got, want = p.out.cpu().numpy(), p.want()
+    want[40 + 50:130] = LEFT
+    assert np.array_equal(got, want) and p.status.item() == -5
+
+
+def test_packed_starts_that_cannot_be_stay_in_bounds():
+    # Every row's first row is clamped to what lies before it.
+    rng = np.random.default_rng(6)
+    p = Packed(rng, [30, 30, 30], 2, 1, 64)
+    for starts in ([0, -5, 30, 90], [50, 40, 30, 90], [0, 30, 200, 300], [0, 0, 0, -4], [-9, 2 ** 31 - 1, -2 ** 31, 90]):
+        p.row_start.copy_(dev(starts))
+        p.run()
+        torch.cuda.synchronize()
+
+
+def test_packed_result_is_the_same_beside_other_sequences():
+    rng = np.random.default_rng(8)
+    p = Packed(rng, [70, 200, 33], 4, 2, 128)
+    p.run()
+    torch.cuda.synchronize()
+    a, b = 70, 270
+    alone = Packed(rng, [200], 4, 2, 128)
+    for t, x in zip(alone.t, p.t):
+        t.copy_(x[a:b])
+    alone.run()
+    torch.cuda.synchronize()
+    assert torch.equal(alone.out, p.out[a:b])
+
+
+def replays(p, change):
+    """Two captured graphs of one call, replayed in turns with eager runs and
+    other inputs between."""
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            p.run(torch.cuda.current_stream().cuda_stream)
+        graphs.append(g)
+    for i in range(4):
+        change(i)
+        p.out.fill_(LEFT)
+        graphs[i % 2].replay()
+        torch.cuda.synchronize()
+        got = p.out.clone()
+        p.out.fill_(LEFT)
+        p.run(torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        assert torch.equal(got, p.out)
+        if i in (0, 3):
+            p.check()
+
+
+def test_packed_captured_and_replayed():
+    rng = np.random.default_rng(12)
+    p = Packed(rng, [50, 1, 80], 4, 2, 64)
+
+    def change(i):
+        p.q = values(rng, p.q.shape, "wide" if i == 2 else "normal")
+        p.t[0].copy_(dev(p.q))
+
+    replays(p, change)
+
+
+def test_packed_calls_at_once_on_two_streams():
+    rng = np.random.default_rng(13)
+    calls = [Packed(rng, lens, 8, 2, 128) for lens in ([300, 20], [17, 400])]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for c, s in zip(calls, streams):
+            c.run(s.cuda_stream)
+    for c in calls:
+        c.check()
+
+
+# ------------------------------------------------------------------ trees
+
+
+class Tree:
+    def __init__(self, rng, lengths, nodes, heads, kv_heads, hd, window=0, scaled=True, page=16, parents="random",
+                 kinds=("normal", "normal", "normal"), extra=(0, 0), behind=0, max_nodes=None, max_positions=None,
+                 spare_pages=2):
+        r = random.Random(int(rng.integers(1 << 30)))
+        n = len(lengths)
+        self.lengths, self.starts = list(lengths), [0] + list(np.cumsum(nodes))
+        rows = self.starts[-1] + behind
+        self.heads, self.window, self.scale = heads, window, scale_of(hd, scaled)
+        held = [-(-(x + m) // page) for x, m in zip(lengths, nodes)]
+        pages = sum(held) + spare_pages
+        order = list(range(pages))
+        r.shuffle(order)
+        self.table, at = np.full((n, max(max(held), 1) + 1), -1, np.int32), 0
+        for i, h in enumerate(held):
+            self.table[i, :h] = order[at:at + h]
+            at += h
+        if parents == "random":
+            parents = [r.choice([i - 1, r.randrange(i) if i else -1, max(i - 3, -1), -1, i + 1, -9]) for m in nodes
+                       for i in range(m)]
+        self.parents = parents
+        self.q = values(rng, (rows, heads * hd), kinds[0])
+        self.kp, self.vp = (values(rng, (pages, kv_heads, page, hd), kind) for kind in kinds[1:])
+        self.tq, self.tk, self.tv = padded(self.q, extra[0]), dev(self.kp), dev(self.vp)
+        self.out = torch.full((rows, heads * hd + extra[1]), LEFT, dtype=torch.int32, device="cuda")
+        self.t = dict(row_start=dev(self.starts), lengths=dev(lengths), table=dev(self.table), status=dev([0]))
+        if parents is not None:
+            self.t["parents"] = dev(list(parents) or [0])
+        self.c = paged.PagedKv(k=self.tk.data_ptr(), v=self.tv.data_ptr(), pages=pages, page_size=page, kv_heads=kv_heads,
+                               head_dim=hd)
+        self.d = paged.TreeAttention(
+            q=self.tq.data_ptr(), out=self.out.data_ptr(), **{k: v.data_ptr() for k, v in self.t.items()},
+            q_stride=self.tq.stride(0), out_stride=self.out.stride(0), requests=n, rows=rows,
+            table_stride=self.table.shape[1], max_nodes=max_nodes or max(max(nodes), 1),
+            max_positions=max_positions or max(max(x + m for x, m in zip(lengths, nodes)), 1), heads=heads, window=window,
+            scaled=int(scaled), scale_q32=self.scale)
+        self.size = paged.tree_workspace_bytes(self.c, self.d)
+        self.space = torch.full((max(self.size, 16),), 0xA5, dtype=torch.uint8, device="cuda")
+
+    def run(self, stream=None):
+        paged.attend_tree(self.c, self.d, self.space.data_ptr(), self.size, stream)
+
+    def want(self):
+        out = np.full(self.out.shape, LEFT, np.int32)
+        return ref.tree(self.q, self.kp, self.vp, self.table, self.starts, self.lengths, self.parents, self.heads,
+                        self.window, self.scale, out)
+
+    def check(self, status=0):
+        torch.cuda.synchronize()
+        assert np.array_equal(self.out.cpu().numpy(), self.want())
+        assert self.t["status"].item() == status
+
+
+HEADS = [(1, 1, 4), (2, 1, 20), (4, 2, 64), (6, 2, 80), (8, 2, 128), (5, 5, 64), (8, 1, 256), (7, 1, 128), (2, 1, 512),
+         (4, 4, 132), (32, 2, 64)]
+
+
+@pytest.mark.parametrize("heads, kv_heads, hd", HEADS)
+@pytest.mark.parametrize("scaled", [True, False])
+def test_tree_heads(heads, kv_heads, hd, scaled):
+    rng = np.random.default_rng(hd + heads)
+    t = Tree(rng, [0, 40, 7, 130], [3, 1, 0, 9], heads, kv_heads, hd, scaled=scaled, extra=(4, 8), behind=2)
+    t.run()
+    t.check()
+
+
+@pytest.mark.parametrize("lengths, nodes", [([0], [1]), ([1], [1]), ([15], [1]), ([16], [1]), ([63], [1]), ([64], [1]),
+                                            ([200], [64]), ([0], [64]), ([5, 0, 900], [0, 0, 2]), ([300] * 5, [1] * 5),
+                                            ([1, 2, 3, 70, 129, 400], [17, 33, 5, 16, 64, 2])])
+@pytest.mark.parametrize("window", [0, 1, 3, 65, 300])
+@pytest.mark.parametrize("page", [4, 16, 128])
+def test_tree_lengths_windows_and_pages(lengths, nodes, window, page):
+    rng = np.random.default_rng(sum(lengths) + window + page)
+    t = Tree(rng, lengths, nodes, 4, 2, 64, window=window, page=page)
+    t.run()
+    t.check()
+
+
+@pytest.mark.parametrize("kinds", [("wide", "wide", "wide"), ("normal", "wide", "normal"), ("wide", "normal", "normal"),
+                                   ("normal", "normal", "wide"), ("mixed", "mixed", "mixed"), ("ends", "ends", "ends"),
+                                   ("sharp", "sharp", "sharp"), ("same", "same", "ends")])
+@pytest.mark.parametrize("heads, kv_heads, hd, scaled", [(4, 2, 64, True), (2, 2, 128, False), (4, 1, 256, False),
+                                                         (3, 1, 80, True), (2, 1, 512, True)])
+def test_tree_values(kinds, heads, kv_heads, hd, scaled):
+    rng = np.random.default_rng(hd)
+    t = Tree(rng, [150, 20], [9, 21], heads, kv_heads, hd, scaled=scaled, kinds=kinds, page=32)
+    t.run()
+    t.check()
+
+
+@pytest.mark.parametrize("length, nodes, heads, kv_heads, hd, page, window", [
+    (9000, 2, 2, 1, 64, 64, 0), (3000, 1, 4, 1, 128, 16, 0), (20000, 1, 1, 1, 64, 256, 0), (6000, 5, 2, 2, 256, 32, 2500),
+    (4100, 7, 2, 1, 512, 16, 0)])
+def test_tree_long_contexts(length, nodes, heads, kv_heads, hd, page, window):
+    rng = np.random.default_rng(length)
+    t = Tree(rng, [length, 33], [nodes, 1], heads, kv_heads, hd, page=page, window=window,
+             kinds=("sharp", "normal", "normal"))
+    t.run()
+    t.check()
+
+
+def test_tree_of_null_parents_is_a_chain():
+    rng = np.random.default_rng(3)
+    t = Tree(rng, [77, 3], [12, 40], 4, 2, 64, parents=None)
+    t.run()
+    t.check()
+
+
+def test_tree_rows_equal_single_tokens():
+    # Row i of a chain, and one token over the cache that holds the rows before it.
+    rng = np.random.default_rng(4)
+    t = Tree(rng, [100], [6], 8, 2, 128, parents=None)
+    t.run()
+    torch.cuda.synchronize()
+    for i in range(6):
+        one = Tree(rng, [100 + i], [1], 8, 2, 128, parents=None)
+        one.c, one.t["table"] = t.c, t.t["table"]
+        one.d.table, one.d.table_stride = t.t["table"].data_ptr(), t.table.shape[1]
+        one.tq.copy_(t.tq[i:i + 1])
+        one.run()
+        torch.cuda.synchronize()
+        assert torch.equal(one.out[0], t.out[i])
+
+
+@pytest.mark.parametrize("length", [60, 3000])
+def test_tree_bad_pages_read_as_zeros(length):
+    rng = np.random.default_rng(9)
+    t = Tree(rng, [length, 30], [5, 2], 4, 2, 64)
+    for col, page in ((0, -1), (2, t.c.pages), (length // 16, 2 ** 31 - 1)):
+        t.table[0, col] = page
+    t.t["table"].copy_(dev(t.table))
+    t.run()
+    t.check(status=-1)
+
+
+@pytest.mark.parametrize("name, value, rows_left", [
+    ("lengths", -1, 1), ("lengths", 2 ** 31 - 1, 1), ("lengths", 57, 1), ("max_nodes", 3, 1), ("rows", 7, 2),
+    ("max_positions", 40, 1), ("table_stride", 3, 1)])
+def test_tree_requests_that_do_not_fit_are_left(name, value, rows_left):
+    # Request 1 of three passes a bound; the others are computed.
+    rng = np.random.default_rng(10)
+    t = Tree(rng, [20, 45, 9], [2, 5, 1], 4, 2, 64, max_positions=60)
+    want = t.want()
+    want[2:7] = LEFT
+    if name == "lengths":
+        t.t["lengths"][1] = value
+    elif name == "rows":
+        # the last request's rows pass the end of q and out
+        t.d.rows = value
+        want = t.want()
+        want[7:] = LEFT
+    elif name == "table_stride":
+        t.t["table"] = dev(t.table[:, :3])
+        t.d.table, t.d.table_stride = t.t["table"].data_ptr(), 3
+    else:
+        setattr(t.d, name, value)
+    t.run()
+    torch.cuda.synchronize()
+    assert np.array_equal(t.out.cpu().numpy(), want)
+    assert t.t["status"].item() == -5
+
+
+def test_tree_row_starts_that_cannot_be():
+    rng = np.random.default_rng(11)
+    t = Tree(rng, [20, 45, 9], [2, 5, 1], 4, 2, 64)
+    for starts in ([0, -3, 2, 4], [5, 2, 1, 0], [-1, 2, 7, 900], [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, 8]):
+        t.t["row_start"].copy_(dev(starts))
+        t.run()
+        torch.cuda.synchronize()
+
+
+def test_tree_captured_and_replayed():
+    rng = np.random.default_rng(14)
+    t = Tree(rng, [500, 40], [9, 3], 4, 2, 64, max_positions=520)
+
+    def change(i):
+        t.q = values(rng, t.q.shape, "wide" if i == 1 else "normal")
+        t.tq.copy_(dev(t.q))
+        t.lengths[1] = 40 + i  # the last rows' keys are others now, and still in the request's pages
+        t.t["lengths"].copy_(dev(t.lengths))
+
+    replays(t, change)
+
+
+def test_tree_calls_at_once_on_two_streams():
+    rng = np.random.default_rng(15)
+    calls = [Tree(rng, [700, 30], [4, 9], 8, 2, 128), Tree(rng, [90, 2100], [1, 2], 8, 2, 128)]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for c, s in zip(calls, streams):
+            c.run(s.cuda_stream)
+    for c in calls:
+        c.check()
+
+
+def test_tree_cache_past_four_gigabytes():
+    # Pages at the far end of 4.3 GB of keys.
+    kv_heads, hd, page, pages = 8, 128, 1024, 1050
+    rng = np.random.default_rng(16)
+    t = Tree(rng, [1500], [3], 8, 8, hd, page=page)
+    kp = torch.zeros(pages, kv_heads, page, hd, dtype=torch.int32, device="cuda")
+    vp = torch.zeros_like(kp)
+    for col in range(2):
+        kp[pages - 1 - col] = t.tk[int(t.table[0, col])]
+        vp[pages - 1 - col] = t.tv[int(t.table[0, col])]
+    t.t["table"][0, :2] = dev([pages - 1, pages - 2])
+    t.c = paged.PagedKv(k=kp.data_ptr(), v=vp.data_ptr(), pages=pages, page_size=page, kv_heads=kv_heads, head_dim=hd)
+    t.run()
+    t.check()
