@@ -1,0 +1,166 @@
+// Pieces of exact attention on the int8 matrix cores over rows of several
+// sequences.
+//
+// An int32 value is five signed byte digits, v = sum_l 256^l d_l; one below
+// 2^23 - 2^15 in magnitude three. A dot product modulo 2^64 is the sum over
+// pairs of digit planes of exact int32 products, each pair shifted by
+// 8 (l + m); pairs of one shift share an accumulator (at most five times
+// 512 * 2^14 < 2^26 each). The usual values need nine products per 64
+// dimensions, the widest 25.
+//
+// Tiles: scores are keys x queries (16 x 16): lane l holds query l % 16 and
+// keys 4 (l / 16) + i of the tile. Within a 64-dimension step the operand
+// byte 4 j + c of lane l is dimension 16 j + 4 (l / 16) + c, for queries and
+// keys alike: 16-byte loads of a row's four consecutive values. Weights are
+// the other product's left operand without leaving their lanes: byte 4 t + i
+// of a 64-key step is key 16 t + 4 (l / 16) + i. Value tiles hold, as column
+// l % 16 of tile t, dimension 4 (l % 16) + t of a 64-dimension block.
+#pragma once
+
+#include "detnum_dev.h"
+#include "paged.h"
+
+namespace {
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+
+constexpr uint32_t TILE_BYTES = 1024;  // a 16 x 64 operand: 16 bytes per lane
+constexpr int DIGITS = 5;              // of any int32
+constexpr int NARROW = 3;              // of the usual values
+constexpr int32_t BIG_WEIGHT = 32640;  // the first weight that needs a third digit
+
+// The four digit planes' dwords (byte c: value c's digit) of four values;
+// `seen` collects what tells whether a fourth digit was needed.
+__device__ __forceinline__ void split4(int4 v, uint32_t (&plane)[4], uint32_t& seen) {
+    const uint32_t bias = 0x80808080u;
+    const uint32_t x = ((uint32_t)v.x + bias) ^ bias, y = ((uint32_t)v.y + bias) ^ bias;
+    const uint32_t z = ((uint32_t)v.z + bias) ^ bias, w = ((uint32_t)v.w + bias) ^ bias;
+    seen |= x | y | z | w;
+    const uint32_t xy = __builtin_amdgcn_perm(y, x, 0x05010400u), zw = __builtin_amdgcn_perm(w, z, 0x05010400u);
+    const uint32_t xy2 = __builtin_amdgcn_perm(y, x, 0x07030602u), zw2 = __builtin_amdgcn_perm(w, z, 0x07030602u);
+    plane[0] = __builtin_amdgcn_perm(zw, xy, 0x05040100u);
+    plane[1] = __builtin_amdgcn_perm(zw, xy, 0x07060302u);
+    plane[2] = __builtin_amdgcn_perm(zw2, xy2, 0x05040100u);
+    plane[3] = __builtin_amdgcn_perm(zw2, xy2, 0x07060302u);
+}
+
+// The fifth digit's dword: one where the lower four cannot reach the value.
+__device__ __forceinline__ uint32_t fifth4(int4 v) {
+    const int32_t top = 0x7f7f7f7f;
+    return (uint32_t)(v.x > top) | (uint32_t)(v.y > top) << 8 | (uint32_t)(v.z > top) << 16 | (uint32_t)(v.w > top) << 24;
+}
+
+// Whether a fourth digit was needed anywhere in the wave.
+__device__ __forceinline__ bool is_wide(uint32_t seen) { return __any(seen >> 24) != 0; }
+
+// The scores of a lane's four keys from the accumulators of LD digits each.
+template <uint32_t HD, int LD>
+__device__ __forceinline__ void scores_of(const v4i (&acc)[2 * LD - 1], int scaled, uint32_t scale_q32, int32_t (&sc)[4]) {
+    constexpr int NS = 2 * LD - 1;
+    if constexpr (LD == NARROW) {
+        // The sum in double: exact below 2^53, else off by less than 2^-52 of
+        // itself; a score near a rounding tie (one in 2^14) is redone exactly.
+        const double scale = (double)scale_q32 * 0x1p-48;
+        bool slow = false;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            double s;
+            if constexpr (HD <= 128) {
+                // Neighbouring accumulators fit an int32 (2 HD 2^14 2^8 <= 2^30).
+                const int32_t low = acc[0][i] + (acc[1][i] << 8), mid = acc[2][i] + (acc[3][i] << 8);
+                s = fma(fma((double)acc[4][i], 65536.0, (double)mid), 65536.0, (double)low);
+            } else {
+                s = (double)acc[NS - 1][i];
+#pragma unroll
+                for (int j = NS - 2; j >= 0; j--) s = fma(s, 256.0, (double)acc[j][i]);
+            }
+            if (scaled) {
+                slow |= !dn::scaled_score_fast(s, scale, sc[i]);
+            } else {
+                sc[i] = dn::requantize((int64_t)s);
+                slow |= !(fabs(s) < 0x1p53);
+            }
+        }
+        if (!__any(slow)) return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint64_t s = 0;  // the wrapping i64 dot product
+#pragma unroll
+        for (int j = 0; j < NS && j < 8; j++) s += (uint64_t)(int64_t)acc[j][i] << (8 * j);
+        sc[i] = scaled ? dn::scaled_score_from_sum((int64_t)s, scale_q32) : dn::requantize((int64_t)s);
+    }
+}
+
+// One 64-dimension step's products into the accumulators.
+template <int LD>
+__device__ __forceinline__ void dot_step(const v4i (&kf)[LD], const v4i (&qf)[LD], v4i (&acc)[2 * LD - 1]) {
+#pragma unroll
+    for (int l = 0; l < LD; l++)
+#pragma unroll
+        for (int m = 0; m < LD; m++)
+            acc[l + m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[l], qf[m], acc[l + m], 0, 0, 0);
+}
+
+// A score's exp term below the row's maximum as it is kept between the
+// passes: 2^32 (the maximum's own) as 0xffffffff, which no other term is.
+__device__ __forceinline__ uint32_t kept_term(double e) { return e > 4294967295.0 ? 0xffffffffu : (uint32_t)e; }
+__device__ __forceinline__ double term_of(uint32_t kept) { return kept == 0xffffffffu ? 4294967296.0 : (double)kept; }
+
+// The weights of four kept terms and the reciprocal scales of the row's sum.
+// `slow` flags those near a rounding tie or of three digits; they are redone
+// exactly, the third digit left to on_big(i) and taken off the weight.
+template <class OnBig>
+__device__ __forceinline__ void weights_of(const uint32_t (&e)[4], uint64_t sum, double w_scale, double q_scale,
+                                           int32_t (&w)[4], int32_t& wsum, OnBig&& on_big) {
+    uint32_t slow = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const double t = term_of(e[i]) * w_scale + 0.5, fl = floor(t);
+        w[i] = (int32_t)fl;
+        slow |= (uint32_t)((fabs(t - fl - 0.5) > 0.5 - 0x1p-15) | (w[i] >= BIG_WEIGHT)) << i;
+    }
+    if (slow) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (!((slow >> i) & 1)) continue;
+            const uint64_t term = e[i] == 0xffffffffu ? (uint64_t)dn::ONE_ACC : e[i];
+            w[i] = dn::softmax_weight(term, sum, q_scale);
+            if (w[i] >= BIG_WEIGHT) {
+                on_big(i);
+                w[i] -= 65536;
+                wsum += 65536;
+            }
+        }
+    }
+    wsum += w[0] + w[1] + w[2] + w[3];
+}
+
+// The two digit planes' dwords of four weights in [-32896, 32640).
+__device__ __forceinline__ void weight_digits(const int32_t (&w)[4], uint32_t& low, uint32_t& high) {
+    uint32_t d[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) d[i] = (uint32_t)(w[i] + 0x8080) ^ 0x8080u;
+    const uint32_t a = __builtin_amdgcn_perm(d[1], d[0], 0x05010400u), b = __builtin_amdgcn_perm(d[3], d[2], 0x05010400u);
+    low = __builtin_amdgcn_perm(b, a, 0x05040100u);
+    high = __builtin_amdgcn_perm(b, a, 0x07060302u);
+}
+
+// Value products of one 64-key step: weights of two digits, values of LV.
+template <int LV>
+__device__ __forceinline__ void value_step(v4i w0, v4i w1, const v4i (&vf)[LV], v4i (&acc)[LV + 1]) {
+#pragma unroll
+    for (int b = 0; b < LV; b++) {
+        acc[b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w0, vf[b], acc[b], 0, 0, 0);
+        acc[b + 1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w1, vf[b], acc[b + 1], 0, 0, 0);
+    }
+}
+
+// The larger score, of equal ones the earlier key.
+__device__ __forceinline__ void take_best(int32_t& best, uint32_t& key, int32_t other, uint32_t other_key) {
+    const bool take = other > best || (other == best && other_key < key);
+    best = take ? other : best;
+    key = take ? other_key : key;
+}
+
+}  // namespace

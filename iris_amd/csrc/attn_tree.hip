@@ -1,31 +1,10 @@
-// Attention of rows of several sequences: packed prompts and drafted trees
-// over a paged cache.
+// Attention of drafted trees over a paged cache.
 #include <algorithm>
 
 #include "attn_common.h"
 #include "paged.h"
 
 namespace {
-
-// The request or sequence of row t: the last s[i] <= t.
-__device__ __forceinline__ uint32_t sequence_of(const int32_t* s, uint32_t n, uint32_t t) {
-    uint32_t lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (s[mid] <= (int32_t)t) lo = mid;
-        else hi = mid;
-    }
-    return lo;
-}
-
-struct PackedView {
-    const int32_t *k, *v;
-    size_t k_stride, v_stride;
-    uint32_t start;  // row of key 0
-    __device__ bool sees(uint32_t) const { return true; }
-    __device__ const int32_t* key(uint32_t j) const { return k + (start + j) * k_stride; }
-    __device__ const int32_t* value(uint32_t j) const { return v + (start + j) * v_stride; }
-};
 
 // One (row, head) by a workgroup of 256: keys [lo, hi) that the view sees.
 template <class View>
@@ -93,23 +72,6 @@ __device__ void attend_one(const View& view, const int32_t* q, int32_t* out, uin
             out[tid + 256 * c] = dn::requantize((int64_t)(acc[c] + (uint64_t)(resid * v[tid + 256 * c])));
 }
 
-__global__ __launch_bounds__(256) void packed_kernel(const IrisPackedAttention a, int32_t* space) {
-    const uint32_t t = blockIdx.x, h = blockIdx.y, g = h / (a.heads / a.kv_heads);
-    const uint32_t end = (uint32_t)min(max(a.row_start[a.sequences], 0), (int32_t)a.rows);
-    if (t >= end) return;
-    const int32_t s = a.row_start[sequence_of(a.row_start, a.sequences, t)];
-    const uint32_t start = (uint32_t)min(max(s, 0), (int32_t)t);
-    if (t - start >= a.max_length) {
-        if (a.status && threadIdx.x == 0) *a.status = IRIS_E_RANGE;
-        return;
-    }
-    const uint32_t n = t - start + 1, lo = a.window && n > a.window ? n - a.window : 0;
-    PackedView v{a.k + (size_t)g * a.head_dim, a.v + (size_t)g * a.head_dim, a.k_stride, a.v_stride, start};
-    attend_one(v, a.q + (size_t)t * a.q_stride + (size_t)h * a.head_dim,
-               a.out + (size_t)t * a.out_stride + (size_t)h * a.head_dim, lo, n, a.head_dim, a.scaled, a.scale_q32,
-               space + ((size_t)t * a.heads + h) * a.max_length);
-}
-
 // A place of zeros for keys whose page is outside the cache.
 __device__ const int32_t g_zeros[ATTN_MAX_HEAD_DIM] = {};
 
@@ -166,20 +128,6 @@ __global__ __launch_bounds__(256) void tree_kernel(const IrisPagedKv c, const Ir
 
 bool misaligned(const void* p) { return ((uintptr_t)p & 15) != 0; }
 
-int packed_check(const IrisPackedAttention* a) {
-    if (!a || !a->q || !a->k || !a->v || !a->out || !a->row_start) return IRIS_E_INVALID;
-    if (misaligned(a->q) || misaligned(a->k) || misaligned(a->v) || misaligned(a->out)) return IRIS_E_INVALID;
-    if (!a->heads || !a->kv_heads || a->heads % a->kv_heads || !a->head_dim || a->head_dim % 4 ||
-        a->head_dim > ATTN_MAX_HEAD_DIM || a->heads > 65535)
-        return IRIS_E_INVALID;
-    const uint64_t q = (uint64_t)a->heads * a->head_dim, kv = (uint64_t)a->kv_heads * a->head_dim;
-    if ((a->q_stride | a->k_stride | a->v_stride | a->out_stride) % 4) return IRIS_E_INVALID;
-    if (a->q_stride < q || a->out_stride < q || a->k_stride < kv || a->v_stride < kv) return IRIS_E_INVALID;
-    if (a->rows > INT32_MAX || a->sequences > INT32_MAX || a->max_length > ATTN_MAX_KEYS) return IRIS_E_RANGE;
-    if (!a->max_length && a->rows && a->sequences) return IRIS_E_INVALID;
-    return 0;
-}
-
 int tree_check(const IrisPagedKv* c, const IrisTreeAttention* a) {
     const int rc = iris_paged_check(c);
     if (rc) return rc;
@@ -198,21 +146,6 @@ int tree_check(const IrisPagedKv* c, const IrisTreeAttention* a) {
 }  // namespace
 
 extern "C" {
-
-uint64_t iris_attention_packed_workspace_bytes(const IrisPackedAttention* a) {
-    if (packed_check(a)) return 0;
-    return (uint64_t)a->rows * a->heads * a->max_length * 4;
-}
-
-int iris_attention_packed(const IrisPackedAttention* a, void* space, uint64_t bytes, void* stream) {
-    const int rc = packed_check(a);
-    if (rc) return rc;
-    if (!a->rows || !a->sequences) return 0;
-    if (!space || misaligned(space)) return IRIS_E_INVALID;
-    if (bytes < iris_attention_packed_workspace_bytes(a)) return IRIS_E_RANGE;
-    hipLaunchKernelGGL(packed_kernel, dim3(a->rows, a->heads), dim3(256), 0, (hipStream_t)stream, *a, (int32_t*)space);
-    return (int)hipGetLastError();
-}
 
 uint64_t iris_attention_tree_workspace_bytes(const IrisPagedKv* c, const IrisTreeAttention* a) {
     if (tree_check(c, a)) return 0;
