@@ -29,6 +29,14 @@ constexpr int DIGITS = 5;              // of any int32
 constexpr int NARROW = 3;              // of the usual values
 constexpr int32_t BIG_WEIGHT = 32640;  // the first weight that needs a third digit
 
+// Loads from device memory by a pointer the compiler cannot place (flat loads
+// would count as LDS accesses too, and every LDS wait as one for them).
+__device__ __forceinline__ int4 load4(const int32_t* p) {
+    const v4i v = *(const __attribute__((address_space(1))) v4i*)p;
+    return make_int4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ int32_t load1(const int32_t* p) { return *(const __attribute__((address_space(1))) int32_t*)p; }
+
 // The four digit planes' dwords (byte c: value c's digit) of four values;
 // `seen` collects what tells whether a fourth digit was needed.
 __device__ __forceinline__ void split4(int4 v, uint32_t (&plane)[4], uint32_t& seen) {
@@ -62,23 +70,28 @@ __device__ __forceinline__ void scores_of(const v4i (&acc)[2 * LD - 1], int scal
         // itself; a score near a rounding tie (one in 2^14) is redone exactly.
         const double scale = (double)scale_q32 * 0x1p-48;
         bool slow = false;
+        double s[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            double s;
             if constexpr (HD <= 128) {
                 // Neighbouring accumulators fit an int32 (2 HD 2^14 2^8 <= 2^30).
                 const int32_t low = acc[0][i] + (acc[1][i] << 8), mid = acc[2][i] + (acc[3][i] << 8);
-                s = fma(fma((double)acc[4][i], 65536.0, (double)mid), 65536.0, (double)low);
+                s[i] = fma(fma((double)acc[4][i], 65536.0, (double)mid), 65536.0, (double)low);
             } else {
-                s = (double)acc[NS - 1][i];
+                s[i] = (double)acc[NS - 1][i];
 #pragma unroll
-                for (int j = NS - 2; j >= 0; j--) s = fma(s, 256.0, (double)acc[j][i]);
+                for (int j = NS - 2; j >= 0; j--) s[i] = fma(s[i], 256.0, (double)acc[j][i]);
             }
-            if (scaled) {
-                slow |= !dn::scaled_score_fast(s, scale, sc[i]);
-            } else {
-                sc[i] = dn::requantize((int64_t)s);
-                slow |= !(fabs(s) < 0x1p53);
+        }
+        if (scaled) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) slow |= !dn::scaled_score_fast(s[i], scale, sc[i]);
+        } else {
+            // Ties to even of an exact sum: 2^-16 s is exact too.
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                sc[i] = (int32_t)fmin(fmax(rint(s[i] * 0x1p-16), -2147483648.0), 2147483647.0);
+                slow |= !(fabs(s[i]) < 0x1p53);
             }
         }
         if (!__any(slow)) return;

@@ -26,11 +26,12 @@ constexpr uint32_t STEP = 64;  // positions of a value product
 // The work space of a launch. Row tiles count a request's (drafted row, head)
 // pairs by sixteens, `row_tiles` per (request, key head).
 struct TreeSpace {
-    uint4* scores;     // [request, key head][row tile][key tile][64] scores, then exp terms
-    uint64_t* maxima;  // [..][row tile][chunk][16]: score and position, packed; 0: none seen
-    double* sums;      // [..][row tile][chunk][16]
-    int32_t* weights;  // [..][row tile][chunk][16] the weights' sum
-    uint64_t* partial; // [..][row tile][chunk][16][HD] weighted values
+    uint4* scores;      // [request, key head][row tile][chunk][key tile][64] scores, then exp terms
+    int32_t* maxima;    // [..][row tile][chunk][16]
+    uint32_t* firsts;   // [..][row tile][chunk][16] the first position of the row's maximum, ~0: not here
+    double* sums;       // [..][row tile][chunk][16] of the exp terms
+    int32_t* weights;   // [..][row tile][chunk][16] the weights' sum
+    uint64_t* partial;  // [..][row tile][chunk][16][HD] weighted values
     uint32_t row_tiles, chunks, chunk;  // positions per chunk, whole steps
 };
 
@@ -90,41 +91,52 @@ __device__ __forceinline__ RowView row_view(const IrisTreeAttention& a, const Re
     return v;
 }
 
-// The cache of one key head: where a position's values lie.
+// The cache of one key head, for positions [key0, key1) whose pages are in
+// LDS. Positions past the last one read the last one (no row sees them).
 struct Places {
-    const int32_t *k, *v, *table;
-    uint32_t pages, page_log, place_mask, last;
+    const int32_t *k, *v;
+    const uint32_t* page;  // of key0's page on
+    uint32_t pages, page_log, place_mask, first, last;
     size_t page_stride;
     uint32_t hd;
-    int32_t* status;
-    // Positions past the last one read the last one (no row sees them).
-    __device__ __forceinline__ const int32_t* at(const int32_t* base, uint32_t page, uint32_t key) const {
-        return page < pages ? base + page * page_stride + (size_t)(key & place_mask) * hd : g_zeros;
+    __device__ __forceinline__ const int32_t* at(const int32_t* base, uint32_t key) const {
+        key = min(key, last);
+        const uint32_t p = page[(key >> page_log) - first];
+        return p < pages ? base + p * page_stride + (size_t)(key & place_mask) * hd : g_zeros;
     }
-    __device__ __forceinline__ uint32_t page_of(uint32_t key) const { return (uint32_t)table[key >> page_log]; }
-    __device__ __forceinline__ uint32_t clamped(uint32_t key) const { return min(key, last); }
 };
 
-__device__ __forceinline__ Places places(const IrisPagedKv& c, const IrisTreeAttention& a, const Request& r, uint32_t g) {
-    const size_t head = (size_t)c.page_size * c.head_dim;
-    return Places{c.k + g * head, c.v + g * head, r.table, c.pages, 31u - __clz((int)c.page_size), c.page_size - 1,
-                  r.total - 1, c.kv_heads * head, c.head_dim, a.status};
-}
+constexpr uint32_t MAX_CHUNK = 1024;
+constexpr uint32_t CHUNK_PAGES = MAX_CHUNK / 4 + 1;
 
-__device__ __forceinline__ uint64_t pack_best(int32_t score, uint32_t key) {
-    return (uint64_t)((uint32_t)score ^ 0x80000000u) << 32 | (0xffffffffu - key);
+// The workgroup's places; s_page has CHUNK_PAGES entries. A barrier follows.
+__device__ __forceinline__ Places places(const IrisPagedKv& c, const IrisTreeAttention& a, const Request& r, uint32_t g,
+                                         uint32_t key0, uint32_t key1, uint32_t* s_page) {
+    const size_t head = (size_t)c.page_size * c.head_dim;
+    const uint32_t log = 31u - __clz((int)c.page_size), first = key0 >> log, n = ((key1 - 1) >> log) - first + 1;
+    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
+        const uint32_t p = (uint32_t)r.table[first + i];
+        s_page[i] = p;
+        if (p >= c.pages && a.status) *a.status = IRIS_E_INVALID;
+    }
+    return Places{c.k + g * head, c.v + g * head, s_page, c.pages, log, c.page_size - 1, first, key1 - 1, c.kv_heads * head,
+                  c.head_dim};
 }
-__device__ __forceinline__ int32_t packed_score(uint64_t p) { return (int32_t)((uint32_t)(p >> 32) ^ 0x80000000u); }
-__device__ __forceinline__ uint32_t packed_key(uint64_t p) { return 0xffffffffu - (uint32_t)p; }
 
 // A lane's four values of each 16-dimension piece of a 64-dimension step.
+// FULL: the head fills its operand tiles (no dimension past it).
+template <bool FULL>
 __device__ __forceinline__ void load_step(const int32_t* row, uint32_t ds, uint32_t hd, int4 (&v)[4]) {
-    const uint32_t d0 = ds * 64 + (threadIdx.x >> 4 & 3) * 4;
+    const uint32_t d0 = (threadIdx.x >> 4 & 3) * 4;
 #pragma unroll
     for (uint32_t j = 0; j < 4; j++) {
-        const uint32_t d = d0 + j * 16;
-        v[j] = *(const int4*)(row + (d < hd ? d : 0));
-        if (d >= hd) v[j] = make_int4(0, 0, 0, 0);
+        const uint32_t at = ds * 64 + j * 16;
+        if constexpr (FULL) {
+            v[j] = load4(row + d0 + at);
+        } else {
+            v[j] = load4(row + (d0 + at < hd ? d0 + at : 0));
+            if (d0 + at >= hd) v[j] = make_int4(0, 0, 0, 0);
+        }
     }
 }
 
@@ -138,99 +150,106 @@ __device__ __forceinline__ void step_digits(const int4 (&v)[4], v4i (&f)[LD], ui
     if constexpr (LD == DIGITS) f[4] = v4i{(int)fifth4(v[0]), (int)fifth4(v[1]), (int)fifth4(v[2]), (int)fifth4(v[3])};
 }
 
-// The row tiles a workgroup of the scores and values launches takes: LDS and
-// registers hold that many of a head size.
-constexpr uint32_t row_block(uint32_t hd) { return hd <= 128 ? 4 : hd <= 256 ? 2 : 1; }
+// The row tiles of a scores workgroup: LDS holds their operands (48 KB).
+constexpr uint32_t row_block(uint32_t hd) { return hd <= 128 ? 8 : 1024 / hd; }
 
-// ---- (1) scores
+// The chunks that hold positions of a request.
+__device__ __forceinline__ uint32_t chunks_of(const TreeSpace& s, const Request& r) {
+    return (r.total - r.base + s.chunk - 1) / s.chunk;
+}
 
-template <uint32_t HD, uint32_t RB>
+// ---- (1) scores and each chunk's maxima
+
+// A wave takes 16 positions at a time, splits their keys once and meets every
+// row tile's queries (digit planes in LDS) with them.
+template <uint32_t HD, bool FULL>
 __global__ __launch_bounds__(256, HD >= 512 ? 1 : HD >= 256 ? 2 : 3) void tree_scores_kernel(const IrisPagedKv c, const IrisTreeAttention a,
                                                                              const TreeSpace s) {
-    constexpr uint32_t DS = HD / 64;
-    extern __shared__ v4i s_q[];  // [RB][DS][DIGITS][64]: the rows' operand tiles
-    __shared__ uint64_t s_best[4][RB][16];
+    constexpr uint32_t DS = HD / 64, RB = row_block(HD);
+    extern __shared__ v4i s_q[];  // [tiles][DS][NARROW][64]
+    __shared__ int32_t s_max[RB][64];
+    __shared__ uint64_t s_mask[RB * 16];
+    __shared__ uint32_t s_lo[RB * 16], s_page[CHUNK_PAGES];
     __shared__ int32_t s_wide;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, grp = lane >> 4;
-    const uint32_t chunk = blockIdx.x, rt0 = blockIdx.y * RB, bg = blockIdx.z, b = bg / c.kv_heads, g = bg % c.kv_heads;
+    const uint32_t chunk = blockIdx.x, rt0 = blockIdx.y * RB, bg = blockIdx.z, g = bg % c.kv_heads;
     const uint32_t group = a.heads / c.kv_heads;
     Request r;
-    if (!read_request(c, a, b, r)) return;
+    if (!read_request(c, a, bg / c.kv_heads, r)) return;
     const uint32_t key0 = r.base + chunk * s.chunk, pairs = r.rows * group;
     if (key0 >= r.total || rt0 * 16 >= pairs) return;
-    const uint32_t key1 = min(key0 + s.chunk, r.total), tiles = (pairs - rt0 * 16 + 15) / 16;
-    const Places at = places(c, a, r, g);
+    const uint32_t key1 = min(key0 + s.chunk, r.total), tiles = min(RB, (pairs - rt0 * 16 + 15) / 16);
+    const Places at = places(c, a, r, g, key0, key1, s_page);
+    auto query = [&](uint32_t rt) {
+        const uint32_t pair = min((rt0 + rt) * 16 + (lane & 15), pairs - 1);
+        return a.q + (size_t)(r.row0 + pair / group) * a.q_stride + (size_t)(g * group + pair % group) * c.head_dim;
+    };
     if (tid == 0) s_wide = 0;
+    for (uint32_t i = tid; i < tiles * 64; i += 256) s_max[i / 64][i % 64] = INT32_MIN;
     __syncthreads();
     uint32_t seen = 0;
-    for (uint32_t i = wave; i < RB * DS; i += 4) {
-        const uint32_t rt = i / DS, ds = i % DS, pair = (rt0 + rt) * 16 + (lane & 15), node = pair / group;
-        if (rt >= tiles) continue;
+    for (uint32_t i = wave; i < tiles * DS; i += 4) {
         int4 v[4];
-        v4i f[DIGITS];
-        load_step(a.q + (size_t)(r.row0 + min(node, r.rows - 1)) * a.q_stride + (size_t)(g * group + pair % group) * c.head_dim, ds,
-                  c.head_dim, v);
-        step_digits<DIGITS>(v, f, seen);
+        v4i f[NARROW];
+        load_step<FULL>(query(i / DS), i % DS, c.head_dim, v);
+        step_digits<NARROW>(v, f, seen);
 #pragma unroll
-        for (int l = 0; l < DIGITS; l++) s_q[(i * DIGITS + l) * 64 + lane] = f[l];
+        for (int l = 0; l < NARROW; l++) s_q[(i * NARROW + l) * 64 + lane] = f[l];
     }
     if (is_wide(seen) && lane == 0) s_wide = 1;
-    RowView view[RB];
-#pragma unroll
-    for (uint32_t rt = 0; rt < RB; rt++) view[rt] = row_view(a, r, (rt0 + rt) * 16 + (lane & 15), group);
+    for (uint32_t rt = wave; rt < tiles; rt += 4) {
+        const RowView v = row_view(a, r, (rt0 + rt) * 16 + (lane & 15), group);
+        if (lane < 16) s_mask[rt * 16 + lane] = v.mask, s_lo[rt * 16 + lane] = v.lo;
+    }
     __syncthreads();
     const bool q_wide = s_wide;
-
-    int32_t best[RB];
-    uint32_t best_key[RB];
-#pragma unroll
-    for (uint32_t rt = 0; rt < RB; rt++) best[rt] = INT32_MIN, best_key[rt] = 0xffffffffu;
+    // Positions [all0, length) are seen by every row.
+    const uint32_t all0 = a.window && r.total > a.window ? r.total - a.window : 0;
     const uint32_t kt1 = (key1 - key0 + 15) / 16;
     uint4* out = s.scores + (((size_t)bg * s.row_tiles + rt0) * s.chunks + chunk) * (s.chunk / 16) * 64;
     const size_t rt_stride = (size_t)s.chunks * (s.chunk / 16) * 64;
     auto keep = [&](uint32_t kt, uint32_t rt, const int32_t (&sc)[4]) __attribute__((always_inline)) {
-        out[rt * rt_stride + kt * 64 + lane] = make_uint4((uint32_t)sc[0], (uint32_t)sc[1], (uint32_t)sc[2], (uint32_t)sc[3]);
+        if ((rt0 + rt) * 16 + (lane & 15) < pairs)
+            out[rt * rt_stride + kt * 64 + lane] = make_uint4((uint32_t)sc[0], (uint32_t)sc[1], (uint32_t)sc[2], (uint32_t)sc[3]);
+        const uint32_t first = key0 + kt * 16;
+        int32_t m;
+        if (first >= all0 && first + 16 <= r.length) {
+            m = max(max(sc[0], sc[1]), max(sc[2], sc[3]));
+        } else {
+            const RowView v{s_lo[rt * 16 + (lane & 15)], r.length, s_mask[rt * 16 + (lane & 15)]};
+            m = INT32_MIN;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t key = key0 + kt * 16 + 4 * grp + i;
-            const bool take = view[rt].sees(key) & ((sc[i] > best[rt]) | (best_key[rt] == 0xffffffffu));
-            best[rt] = take ? sc[i] : best[rt];
-            best_key[rt] = take ? key : best_key[rt];
+            for (int i = 0; i < 4; i++)
+                if (v.sees(first + 4 * grp + i)) m = max(m, sc[i]);
         }
+        atomicMax(&s_max[rt][lane], m);
     };
     // The next tile's keys are loaded during this one's products.
-    auto key_row = [&](uint32_t kt) {
-        const uint32_t key = at.clamped(key0 + kt * 16 + (lane & 15)), page = at.page_of(key);
-        if (page >= at.pages && at.status) *at.status = IRIS_E_INVALID;
-        return at.at(at.k, page, key);
-    };
     constexpr bool AHEAD = HD <= 256;
     int4 raw[AHEAD ? DS : 1][4];
-    const int32_t* row = wave < kt1 ? key_row(wave) : nullptr;
-    if constexpr (AHEAD)
-        if (row)
+    // (Past the last: it again, so that no load is behind a branch, where it
+    // would be waited for.)
+    auto load_ahead = [&](uint32_t kt) __attribute__((always_inline)) {
+        if constexpr (AHEAD) {
+            const int32_t* row = at.at(at.k, key0 + min(kt, kt1 - 1) * 16 + (lane & 15));
 #pragma unroll
-            for (uint32_t ds = 0; ds < DS; ds++) load_step(row, ds, c.head_dim, raw[ds]);
+            for (uint32_t ds = 0; ds < DS; ds++) load_step<FULL>(row, ds, c.head_dim, raw[ds]);
+        }
+    };
+    load_ahead(wave);
 #pragma unroll 1
     for (uint32_t kt = wave; kt < kt1; kt += 4) {
         v4i kf[DS][NARROW];
         uint32_t wide = 0;
-        const int32_t* here = row;
 #pragma unroll
         for (uint32_t ds = 0; ds < DS; ds++) {
-            if constexpr (!AHEAD) load_step(here, ds, c.head_dim, raw[0]);
+            if constexpr (!AHEAD) load_step<FULL>(at.at(at.k, key0 + kt * 16 + (lane & 15)), ds, c.head_dim, raw[0]);
             step_digits<NARROW>(raw[AHEAD ? ds : 0], kf[ds], wide);
         }
-        if (kt + 4 < kt1) {
-            row = key_row(kt + 4);
-            if constexpr (AHEAD)
-#pragma unroll
-                for (uint32_t ds = 0; ds < DS; ds++) load_step(row, ds, c.head_dim, raw[ds]);
-        }
         if (!q_wide && !is_wide(wide)) {
-#pragma unroll
-            for (uint32_t rt = 0; rt < RB; rt++) {
-                if (rt >= tiles) break;
+            load_ahead(kt + 4);
+#pragma unroll 1
+            for (uint32_t rt = 0; rt < tiles; rt++) {
                 v4i acc[2 * NARROW - 1];
 #pragma unroll
                 for (int j = 0; j < 2 * NARROW - 1; j++) acc[j] = v4i{0, 0, 0, 0};
@@ -238,7 +257,7 @@ __global__ __launch_bounds__(256, HD >= 512 ? 1 : HD >= 256 ? 2 : 3) void tree_s
                 for (uint32_t ds = 0; ds < DS; ds++) {
                     v4i qf[NARROW];
 #pragma unroll
-                    for (int l = 0; l < NARROW; l++) qf[l] = s_q[((rt * DS + ds) * DIGITS + l) * 64 + lane];
+                    for (int l = 0; l < NARROW; l++) qf[l] = s_q[((rt * DS + ds) * NARROW + l) * 64 + lane];
                     dot_step<NARROW>(kf[ds], qf, acc);
                 }
                 int32_t sc[4];
@@ -246,9 +265,8 @@ __global__ __launch_bounds__(256, HD >= 512 ? 1 : HD >= 256 ? 2 : 3) void tree_s
                 keep(kt, rt, sc);
             }
         } else {
-#pragma unroll
-            for (uint32_t rt = 0; rt < RB; rt++) {
-                if (rt >= tiles) break;
+#pragma unroll 1
+            for (uint32_t rt = 0; rt < tiles; rt++) {
                 v4i acc[2 * DIGITS - 1];
 #pragma unroll
                 for (int j = 0; j < 2 * DIGITS - 1; j++) acc[j] = v4i{0, 0, 0, 0};
@@ -256,263 +274,423 @@ __global__ __launch_bounds__(256, HD >= 512 ? 1 : HD >= 256 ? 2 : 3) void tree_s
                 for (uint32_t ds = 0; ds < DS; ds++) {
                     int4 v[4];
                     v4i f[DIGITS], qf[DIGITS];
-                    load_step(here, ds, c.head_dim, v);
+                    load_step<FULL>(at.at(at.k, key0 + kt * 16 + (lane & 15)), ds, c.head_dim, v);
                     step_digits<DIGITS>(v, f, wide);
-#pragma unroll
-                    for (int l = 0; l < DIGITS; l++) qf[l] = s_q[((rt * DS + ds) * DIGITS + l) * 64 + lane];
+                    load_step<FULL>(query(rt), ds, c.head_dim, v);
+                    step_digits<DIGITS>(v, qf, wide);
                     dot_step<DIGITS>(f, qf, acc);
                 }
                 int32_t sc[4];
                 scores_of<HD, DIGITS>(acc, a.scaled, a.scale_q32, sc);
                 keep(kt, rt, sc);
             }
+            load_ahead(kt + 4);
         }
     }
-#pragma unroll
-    for (uint32_t rt = 0; rt < RB; rt++) {
-        take_best(best[rt], best_key[rt], __shfl_xor(best[rt], 16), (uint32_t)__shfl_xor((int)best_key[rt], 16));
-        take_best(best[rt], best_key[rt], __shfl_xor(best[rt], 32), (uint32_t)__shfl_xor((int)best_key[rt], 32));
-        if (lane < 16) s_best[wave][rt][lane] = best_key[rt] == 0xffffffffu ? 0 : pack_best(best[rt], best_key[rt]);
-    }
     __syncthreads();
-    if (tid < RB * 16 && tid / 16 < tiles) {
+    if (tid < tiles * 16) {
         const uint32_t rt = tid / 16, i = tid % 16;
-        const uint64_t m = max(max(s_best[0][rt][i], s_best[1][rt][i]), max(s_best[2][rt][i], s_best[3][rt][i]));
-        s.maxima[(((size_t)bg * s.row_tiles + rt0 + rt) * s.chunks + chunk) * 16 + i] = m;
+        s.maxima[(((size_t)bg * s.row_tiles + rt0 + rt) * s.chunks + chunk) * 16 + i] =
+            max(max(s_max[rt][i], s_max[rt][16 + i]), max(s_max[rt][32 + i], s_max[rt][48 + i]));
     }
 }
 
-// The chunks that hold positions of a request.
-__device__ __forceinline__ uint32_t chunks_of(const TreeSpace& s, const Request& r) {
-    return (r.total - r.base + s.chunk - 1) / s.chunk;
-}
+// Few rows in a tile leave most lanes of a wave without one: a lane then takes
+// a row of `width` (a power of two, at least the rows) and one of 16 / width
+// key tiles at once.
+struct RowLanes {
+    uint32_t width, row, sub, slot;  // slot: the row's place in a key tile
+    __device__ __forceinline__ explicit RowLanes(uint32_t rows) {
+        const uint32_t lane = threadIdx.x & 63;
+        width = rows > 8 ? 16 : rows > 4 ? 8 : rows > 2 ? 4 : rows > 1 ? 2 : 1;
+        row = lane & (width - 1);
+        sub = (lane & 15) / width;
+        slot = (lane & 48) | row;
+    }
+};
 
-// A row's maximum over its chunks, for row lane % 16.
-__device__ __forceinline__ uint64_t row_maximum(const TreeSpace& s, size_t tile, uint32_t chunks) {
-    const uint32_t lane = threadIdx.x & 63;
-    uint64_t m = 0;
-    for (uint32_t i = lane >> 4; i < chunks; i += 4) m = max(m, s.maxima[(tile * s.chunks + i) * 16 + (lane & 15)]);
-    m = max(m, (uint64_t)__shfl_xor((unsigned long long)m, 16));
-    return max(m, (uint64_t)__shfl_xor((unsigned long long)m, 32));
-}
-
-// ---- (2) exp terms
+// ---- (2) exp terms in place of the scores, each chunk's sums and first maxima
 
 __global__ __launch_bounds__(256) void tree_terms_kernel(const IrisPagedKv c, const IrisTreeAttention a, const TreeSpace s) {
     __shared__ double s_sum[4][16];
+    __shared__ uint32_t s_first[4][16];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, grp = lane >> 4;
     const uint32_t chunk = blockIdx.x, rt = blockIdx.y, bg = blockIdx.z, group = a.heads / c.kv_heads;
     Request r;
     if (!read_request(c, a, bg / c.kv_heads, r)) return;
-    const uint32_t key0 = r.base + chunk * s.chunk;
-    if (key0 >= r.total || rt * 16 >= r.rows * group) return;
-    const uint32_t kt1 = (min(s.chunk, r.total - key0) + 15) / 16;
+    const uint32_t key0 = r.base + chunk * s.chunk, pairs = r.rows * group;
+    if (key0 >= r.total || rt * 16 >= pairs) return;
+    const uint32_t kt1 = (min(s.chunk, r.total - key0) + 15) / 16, rows = min(16u, pairs - rt * 16);
     const size_t tile = (size_t)bg * s.row_tiles + rt;
-    const uint32_t top = (uint32_t)packed_score(row_maximum(s, tile, chunks_of(s, r)));
-    const RowView view = row_view(a, r, rt * 16 + (lane & 15), group);
-    uint4* t = s.scores + (tile * s.chunks + chunk) * (s.chunk / 16) * 64 + lane;
+    const RowLanes l(rows);
+    const bool valid = l.row < rows;
+    // The row's maximum over its chunks.
+    int32_t top = INT32_MIN;
+    for (uint32_t i = lane / l.width; i < chunks_of(s, r); i += 64 / l.width)
+        top = max(top, valid ? s.maxima[(tile * s.chunks + i) * 16 + l.row] : INT32_MIN);
+    for (uint32_t off = l.width; off < 64; off <<= 1) top = max(top, __shfl_xor(top, (int)off));
+    const RowView view = row_view(a, r, valid ? rt * 16 + l.row : 0xffffffffu, group);
+    const uint32_t all0 = a.window && r.total > a.window ? r.total - a.window : 0, per = 16 / l.width;
+    uint4* t = s.scores + (tile * s.chunks + chunk) * (s.chunk / 16) * 64 + l.slot;
     double sum = 0;  // at most 2^20 terms of 2^32: exact
+    uint32_t found = 0xffffffffu;
 #pragma unroll 2
-    for (uint32_t kt = wave; kt < kt1; kt += 4) {
+    for (uint32_t k = wave * per; k < kt1; k += 4 * per) {
+        const uint32_t kt = k + l.sub, key = key0 + kt * 16 + 4 * grp;
+        if (!valid || kt >= kt1) continue;
         const uint4 sc = t[kt * 64];
         const uint32_t v[4] = {sc.x, sc.y, sc.z, sc.w};
         uint32_t e[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const double x = view.sees(key0 + kt * 16 + 4 * grp + i) ? dn::softmax_exp_f64(top - v[i]) : 0.0;
+            const bool sees = (key >= all0 && key + 4 <= r.length) || view.sees(key + i);
+            const double x = sees ? dn::softmax_exp_f64((uint32_t)top - v[i]) : 0.0;
+            if (sees && v[i] == (uint32_t)top) found = min(found, key + i);
             sum += x;
             e[i] = kept_term(x);
         }
         t[kt * 64] = make_uint4(e[0], e[1], e[2], e[3]);
     }
-    sum += __shfl_xor(sum, 16);
-    sum += __shfl_xor(sum, 32);
-    if (lane < 16) s_sum[wave][lane] = sum;
+    for (uint32_t off = l.width; off < 64; off <<= 1) {
+        sum += __shfl_xor(sum, (int)off);
+        found = min(found, (uint32_t)__shfl_xor((int)found, (int)off));
+    }
+    if (lane < l.width) s_sum[wave][lane] = sum, s_first[wave][lane] = found;
     __syncthreads();
-    if (tid < 16) s.sums[(tile * s.chunks + chunk) * 16 + tid] = s_sum[0][tid] + s_sum[1][tid] + s_sum[2][tid] + s_sum[3][tid];
+    if (tid < rows) {
+        const size_t to = (tile * s.chunks + chunk) * 16 + tid;
+        s.sums[to] = s_sum[0][tid] + s_sum[1][tid] + s_sum[2][tid] + s_sum[3][tid];
+        s.firsts[to] = min(min(s_first[0][tid], s_first[1][tid]), min(s_first[2][tid], s_first[3][tid]));
+    }
 }
 
-// ---- (3) weighted values
+// ---- (3) weights and weighted values
 
-// Waves: a 64-dimension block each, `RS` halves of the row tiles, and PARTS
-// of the steps.
-template <uint32_t HD, uint32_t RB>
-struct ValueShape {
-    static constexpr uint32_t DS = HD / 64, RS = RB == 4 ? 2 : 1, WAVES = std::max(4u, DS) * RS, PARTS = WAVES / RS / DS, RW = RB / RS;
+// What turns a row's exp terms into weights.
+struct RowScale {
+    double w, q;
+    uint64_t sum;
 };
 
-constexpr uint32_t BATCH = 4;  // steps whose weights are in LDS at a time
+// Lane row `row` of tile `tile`, the lanes of one row at strides of `width`.
+__device__ __forceinline__ RowScale row_scale(const TreeSpace& s, size_t tile, uint32_t chunks, uint32_t row, uint32_t width,
+                                              bool valid) {
+    const uint32_t lane = threadIdx.x & 63;
+    double sum = 0;
+    for (uint32_t i = lane / width; i < chunks; i += 64 / width) sum += valid ? s.sums[(tile * s.chunks + i) * 16 + row] : 0.0;
+    for (uint32_t off = width; off < 64; off <<= 1) sum += __shfl_xor(sum, (int)off);
+    return valid ? RowScale{65536.0 / sum, 4294967296.0 / sum, (uint64_t)sum} : RowScale{0.0, 0.0, 1};
+}
 
-template <uint32_t HD, uint32_t RB>
-__global__ __launch_bounds__((ValueShape<HD, RB>::WAVES * 64), 2) void tree_values_kernel(const IrisPagedKv c,
-                                                                                       const IrisTreeAttention a,
-                                                                                       const TreeSpace s) {
-    using S = ValueShape<HD, RB>;
-    constexpr uint32_t WAVES = S::WAVES, RW = S::RW;
-    extern __shared__ uint64_t s_sums[];  // [RB][16][HD], then the weights' digits [RB][BATCH][2][64] uint4
-    __shared__ int32_t s_wsum[RB][16], s_nbig[RB][16], s_big[RB][16][2];
-    uint4* s_w = (uint4*)(s_sums + RB * 16 * HD);
+// A step's values for one 64-dimension block: dimensions d .. d + 3 of the
+// lane's sixteen positions, four in a row at a time.
+template <bool FULL>
+__device__ __forceinline__ void load_values(const Places& at, uint32_t key, uint32_t d, int4 (&v)[4][4]) {
+#pragma unroll
+    for (uint32_t t = 0; t < 4; t++)
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) v[t][i] = load4(at.at(at.v, key + 16 * t + i) + (FULL || d < at.hd ? d : 0));
+}
+
+__device__ __forceinline__ int4 column(const int4 (&v)[4], int k) {
+    auto of = [&](int4 x) { return k == 0 ? x.x : k == 1 ? x.y : k == 2 ? x.z : x.w; };
+    return make_int4(of(v[0]), of(v[1]), of(v[2]), of(v[3]));
+}
+
+// What the fourth and fifth digits of the values add to a lane's four rows.
+__device__ __forceinline__ void upper_values(v4i w0, v4i w1, const int4 (&x)[4], uint64_t (&add)[4]) {
+    uint32_t seen = 0;
+    v4i f[DIGITS];
+    step_digits<DIGITS>(x, f, seen);
+    const v4i upper[2] = {f[3], f[4]};
+    v4i up[3] = {v4i{0, 0, 0, 0}, v4i{0, 0, 0, 0}, v4i{0, 0, 0, 0}};
+    value_step<2>(w0, w1, upper, up);
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+        add[q] = ((uint64_t)(int64_t)up[0][q] << 24) + ((uint64_t)(int64_t)up[1][q] << 32) + ((uint64_t)(int64_t)up[2][q] << 40);
+}
+
+// At most two weights of a row need a third digit: 65536 v more for each.
+struct BigWeights {
+    int32_t count[16];
+    uint32_t key[16][2];
+    __device__ __forceinline__ void add(uint32_t row, uint32_t k) {
+        const int n = atomicAdd(&count[row], 1);
+        if (n < 2) key[row][n] = k;
+    }
+};
+
+// One row tile: a wave takes a 64-dimension block and PARTS of the steps; the
+// chunk's weights, as operands, lie in LDS.
+template <uint32_t HD, bool FULL>
+__global__ __launch_bounds__((HD / 64 > 4 ? HD : 256), 2) void tree_values_kernel(const IrisPagedKv c, const IrisTreeAttention a,
+                                                                                const TreeSpace s) {
+    constexpr uint32_t DS = HD / 64, WAVES = DS > 4 ? DS : 4, PARTS = WAVES / DS;
+    extern __shared__ uint64_t s_sums[];  // [16][HD], then the weights' digits [steps][2][64] uint4
+    __shared__ BigWeights s_big;
+    __shared__ int32_t s_wsum[16];
+    __shared__ uint32_t s_page[CHUNK_PAGES];
+    uint4* s_w = (uint4*)(s_sums + 16 * HD);
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, grp = lane >> 4;
-    const uint32_t chunk = blockIdx.x, rt0 = blockIdx.y * RB, bg = blockIdx.z, g = bg % c.kv_heads, group = a.heads / c.kv_heads;
+    const uint32_t chunk = blockIdx.x, bg = blockIdx.z, g = bg % c.kv_heads, group = a.heads / c.kv_heads;
+    Request r;
+    if (!read_request(c, a, bg / c.kv_heads, r)) return;
+    const uint32_t key0 = r.base + chunk * s.chunk, rows = r.rows * group;
+    if (key0 >= r.total) return;
+    const uint32_t n = min(s.chunk, r.total - key0), steps = (n + STEP - 1) / STEP, kt1 = (n + 15) / 16;
+    const Places at = places(c, a, r, g, key0, key0 + n, s_page);
+    for (uint32_t i = tid; i < 16 * HD; i += WAVES * 64) s_sums[i] = 0;
+    for (uint32_t i = tid; i < steps * 128; i += WAVES * 64) s_w[i] = make_uint4(0, 0, 0, 0);
+    if (tid < 16) s_wsum[tid] = 0, s_big.count[tid] = 0;
+    __syncthreads();
+    const uint32_t block = wave % DS, part = wave / DS, d = block * 64 + 4 * (lane & 15);
+    {
+        const RowLanes l(rows);
+        const bool valid = l.row < rows;
+        const RowScale sc = row_scale(s, bg, chunks_of(s, r), l.row, l.width, valid);
+        const uint4* t = s.scores + ((size_t)bg * s.chunks + chunk) * (s.chunk / 16) * 64 + l.slot;
+        const uint32_t per = 16 / l.width;
+        int32_t wsum = 0;
+        for (uint32_t k = wave * per; k < kt1; k += WAVES * per) {
+            const uint32_t kt = k + l.sub;
+            if (!valid || kt >= kt1) continue;
+            const uint4 x = t[kt * 64];
+            const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+            int32_t w[4];
+            weights_of(e, sc.sum, sc.w, sc.q, w, wsum, [&](int j) { s_big.add(l.row, key0 + kt * 16 + 4 * grp + j); });
+            uint32_t low, high;
+            weight_digits(w, low, high);
+            uint32_t* to = (uint32_t*)(s_w + (size_t)(kt / 4) * 128 + l.slot) + kt % 4;
+            to[0] = low;
+            to[256] = high;
+        }
+        for (uint32_t off = l.width; off < 64; off <<= 1) wsum += __shfl_xor(wsum, (int)off);
+        if (lane < l.width && valid) atomicAdd(&s_wsum[lane], wsum);
+    }
+    __syncthreads();
+    v4i acc[4][NARROW + 1];
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int j = 0; j < NARROW + 1; j++) acc[t][j] = v4i{0, 0, 0, 0};
+#pragma unroll 1
+    for (uint32_t step = part; step < steps; step += PARTS) {
+        int4 v[4][4];
+        load_values<FULL>(at, key0 + step * STEP + 4 * grp, d, v);
+        const uint4 x0 = s_w[step * 128 + lane], x1 = s_w[step * 128 + 64 + lane];
+        const v4i w0 = v4i{(int)x0.x, (int)x0.y, (int)x0.z, (int)x0.w}, w1 = v4i{(int)x1.x, (int)x1.y, (int)x1.z, (int)x1.w};
+        uint32_t seen = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int4 x[4] = {column(v[0], k), column(v[1], k), column(v[2], k), column(v[3], k)};
+            v4i f[NARROW];
+            step_digits<NARROW>(x, f, seen);
+            value_step<NARROW>(w0, w1, f, acc[k]);
+        }
+        if (is_wide(seen)) {
+#pragma unroll 1
+            for (int k = 0; k < 4; k++) {
+                int4 x[4];
+#pragma unroll
+                for (uint32_t t = 0; t < 4; t++) {
+                    int32_t y[4];
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; i++)
+                        y[i] = load1(at.at(at.v, key0 + step * STEP + 4 * grp + 16 * t + i) + (d < at.hd ? d + k : 0));
+                    x[t] = make_int4(y[0], y[1], y[2], y[3]);
+                }
+                uint64_t add[4];
+                upper_values(w0, w1, x, add);
+#pragma unroll
+                for (uint32_t q = 0; q < 4; q++)
+                    if (4 * grp + q < rows) atomicAdd((unsigned long long*)&s_sums[(4 * grp + q) * HD + d + k], add[q]);
+            }
+        }
+    }
+#pragma unroll
+    for (uint32_t q = 0; q < 4; q++) {
+        if (4 * grp + q >= rows) break;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            uint64_t t = 0;
+#pragma unroll
+            for (int j = 0; j < NARROW + 1; j++) t += (uint64_t)(int64_t)acc[k][j][q] << (8 * j);
+            atomicAdd((unsigned long long*)&s_sums[(4 * grp + q) * HD + d + k], t);
+        }
+    }
+    __syncthreads();
+    uint64_t* out = s.partial + ((size_t)bg * s.chunks + chunk) * 16 * HD;
+    for (uint32_t i = tid; i < rows * HD; i += WAVES * 64) {
+        const uint32_t row = i / HD, dim = i % HD;
+        uint64_t t = s_sums[i];
+        if (dim < c.head_dim)
+            for (int j = 0; j < s_big.count[row]; j++) t += (uint64_t)((int64_t)65536 * load1(at.at(at.v, s_big.key[row][j]) + dim));
+        out[i] = t;
+    }
+    if (tid < rows) s.weights[((size_t)bg * s.chunks + chunk) * 16 + tid] = s_wsum[tid];
+}
+
+// Dimensions of a many-rows workgroup.
+constexpr uint32_t value_dims(uint32_t hd) { return hd < 128 ? hd : 128; }
+
+// NW row tiles, a wave each, which forms its own weights in registers; the
+// workgroup splits each step's values once, into LDS, a step ahead.
+template <uint32_t HD, uint32_t NW, bool FULL>
+__global__ __launch_bounds__(NW * 64, 2) void tree_values_many_kernel(const IrisPagedKv c, const IrisTreeAttention a,
+                                                                      const TreeSpace s) {
+    constexpr uint32_t VD = value_dims(HD), BLOCKS = VD / 64, UNITS = BLOCKS * 4, PER = (UNITS + NW - 1) / NW, TILES = VD / 16;
+    __shared__ v4i s_v[2][TILES][NARROW][64];
+    __shared__ int32_t s_wide[2];
+    __shared__ BigWeights s_big[NW];
+    __shared__ uint32_t s_page[CHUNK_PAGES];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, grp = lane >> 4;
+    const uint32_t chunk = blockIdx.x, bg = blockIdx.z, g = bg % c.kv_heads, group = a.heads / c.kv_heads;
+    const uint32_t dim0 = blockIdx.y % (HD / VD) * VD, rt0 = blockIdx.y / (HD / VD) * NW;
     Request r;
     if (!read_request(c, a, bg / c.kv_heads, r)) return;
     const uint32_t key0 = r.base + chunk * s.chunk, pairs = r.rows * group;
     if (key0 >= r.total || rt0 * 16 >= pairs) return;
-    const uint32_t steps = (min(s.chunk, r.total - key0) + STEP - 1) / STEP, tiles = (pairs - rt0 * 16 + 15) / 16;
-    const uint32_t kt1 = (min(s.chunk, r.total - key0) + 15) / 16;
-    const Places at = places(c, a, r, g);
-    for (uint32_t i = tid; i < RB * 16 * HD; i += WAVES * 64) s_sums[i] = 0;
-    if (tid < RB * 16) s_wsum[tid / 16][tid % 16] = 0, s_nbig[tid / 16][tid % 16] = 0;
+    const uint32_t n = min(s.chunk, r.total - key0), steps = (n + STEP - 1) / STEP, kt1 = (n + 15) / 16;
+    const Places at = places(c, a, r, g, key0, key0 + n, s_page);
+    const uint32_t rt = rt0 + wave, row = rt * 16 + (lane & 15);
+    const bool has_rt = rt * 16 < pairs, valid = row < pairs;
+    const size_t tile = (size_t)bg * s.row_tiles + min(rt, s.row_tiles - 1);
+    if (tid < 2) s_wide[tid] = 0;
+    if (lane < 16) s_big[wave].count[lane] = 0;
+    __syncthreads();
+    const RowScale sc = row_scale(s, tile, chunks_of(s, r), lane & 15, 16, valid);
 
-    // The weights of (row tile, step of the batch) items, dealt to the waves.
-    const size_t tile0 = (size_t)bg * s.row_tiles + rt0;
-    const uint32_t chunks = chunks_of(s, r);
-    auto row_sum = [&](uint32_t rt) {
-        double sum = 0;
-        for (uint32_t i = grp; i < chunks; i += 4) sum += s.sums[((tile0 + rt) * s.chunks + i) * 16 + (lane & 15)];
-        sum += __shfl_xor(sum, 16);
-        return sum + __shfl_xor(sum, 32);
-    };
-    // An item is always taken by a wave with the same row tile.
-    const uint32_t my_rt = wave % RB;
-    const bool has_rt = my_rt < tiles;
-    const double sum = has_rt ? row_sum(my_rt) : 1.0;
-    const bool valid = has_rt && (rt0 + my_rt) * 16 + (lane & 15) < pairs;
-    const double w_scale = valid ? 65536.0 / sum : 0.0, q_scale = valid ? 4294967296.0 / sum : 0.0;
-    const uint64_t total = valid ? (uint64_t)sum : 1;
-    int32_t wsum = 0;
-
-    const uint32_t block = wave % S::DS, part = wave / S::DS % S::PARTS, half = wave / S::DS / S::PARTS;
-    const uint32_t d = block * 64 + 4 * (lane & 15);
-    v4i acc[RW][4][NARROW + 1];
+    // A unit of a step's values: positions 16 t + 4 q + i (lane: t, and
+    // dimensions 4 n ..) of one block and q.
+    int4 raw[PER][4];
+    auto load_raw = [&](uint32_t step) __attribute__((always_inline)) {
 #pragma unroll
-    for (uint32_t rt = 0; rt < RW; rt++)
+        for (uint32_t u = 0; u < PER; u++) {
+            const uint32_t unit = wave + u * NW;
+            if (unit >= UNITS) break;
+            const uint32_t d = dim0 + unit / 4 * 64 + 4 * (lane & 15), key = key0 + step * STEP + 16 * grp + 4 * (unit % 4);
 #pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int j = 0; j < NARROW + 1; j++) acc[rt][t][j] = v4i{0, 0, 0, 0};
-    // Four positions in a row lie in one page.
-    auto load_values = [&](uint32_t step, int4 (&v)[4][4]) __attribute__((always_inline)) {
-#pragma unroll
-        for (uint32_t t = 0; t < 4; t++) {
-            const uint32_t key = key0 + step * STEP + 16 * t + 4 * grp;
-            const uint32_t page = at.page_of(at.clamped(key));
-#pragma unroll
-            for (uint32_t i = 0; i < 4; i++)
-                v[t][i] = *(const int4*)(at.at(at.v, page, at.clamped(key + i)) + (d < c.head_dim ? d : 0));
+            for (uint32_t i = 0; i < 4; i++) raw[u][i] = load4(at.at(at.v, key + i) + (FULL || d < at.hd ? d : 0));
         }
     };
-    __syncthreads();
-#pragma unroll 1
-    for (uint32_t batch = 0; batch < steps; batch += BATCH) {
-        if (has_rt)
-#pragma unroll 1
-            for (uint32_t i = wave / RB; i < BATCH; i += WAVES / RB) {
-                v4i w0 = v4i{0, 0, 0, 0}, w1 = v4i{0, 0, 0, 0};
-                const uint4* t = s.scores + (((tile0 + my_rt) * s.chunks + chunk) * (s.chunk / 16) + (batch + i) * 4) * 64 + lane;
+    auto split_raw = [&](uint32_t step) __attribute__((always_inline)) {
+        uint32_t seen = 0;
 #pragma unroll
-                for (uint32_t k = 0; k < 4; k++) {
-                    const uint32_t kt = (batch + i) * 4 + k;
-                    uint32_t low = 0, high = 0;
-                    if (kt < kt1) {
-                        const uint4 x = t[k * 64];
-                        const uint32_t e[4] = {x.x, x.y, x.z, x.w};
-                        int32_t w[4];
-                        weights_of(e, total, w_scale, q_scale, w, wsum, [&](int j) {
-                            const int n = atomicAdd(&s_nbig[my_rt][lane & 15], 1);
-                            if (n < 2) s_big[my_rt][lane & 15][n] = (int32_t)(key0 + kt * 16 + 4 * grp + j);
-                        });
-                        weight_digits(w, low, high);
-                    }
-                    w0[k] = (int)low, w1[k] = (int)high;
-                }
-                s_w[((my_rt * BATCH + i) * 2) * 64 + lane] = make_uint4(w0[0], w0[1], w0[2], w0[3]);
-                s_w[((my_rt * BATCH + i) * 2 + 1) * 64 + lane] = make_uint4(w1[0], w1[1], w1[2], w1[3]);
-            }
-        __syncthreads();
-#pragma unroll 1
-        for (uint32_t i = part; i < BATCH && batch + i < steps; i += S::PARTS) {
-            int4 v[4][4];
-            load_values(batch + i, v);
-            v4i w0[RW], w1[RW];
-#pragma unroll
-            for (uint32_t rt = 0; rt < RW; rt++) {
-                const uint4* p = s_w + (((half * RW + rt) * BATCH + i) * 2) * 64 + lane;
-                const uint4 x = p[0], y = p[64];
-                w0[rt] = v4i{(int)x.x, (int)x.y, (int)x.z, (int)x.w};
-                w1[rt] = v4i{(int)y.x, (int)y.y, (int)y.z, (int)y.w};
-            }
-            auto column = [&](int k, uint32_t t) {
-                auto of = [&](int4 x) { return k == 0 ? x.x : k == 1 ? x.y : k == 2 ? x.z : x.w; };
-                return make_int4(of(v[t][0]), of(v[t][1]), of(v[t][2]), of(v[t][3]));
-            };
-            uint32_t seen = 0;
+        for (uint32_t u = 0; u < PER; u++) {
+            const uint32_t unit = wave + u * NW;
+            if (unit >= UNITS) break;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const int4 x[4] = {column(k, 0), column(k, 1), column(k, 2), column(k, 3)};
-                v4i f[NARROW];
-                step_digits<NARROW>(x, f, seen);
+                uint32_t p[4];
+                split4(column(raw[u], k), p, seen);
 #pragma unroll
-                for (uint32_t rt = 0; rt < RW; rt++) value_step<NARROW>(w0[rt], w1[rt], f, acc[rt][k]);
+                for (int l = 0; l < NARROW; l++)
+                    ((uint32_t*)&s_v[step & 1][unit / 4 * 4 + k][l][unit % 4 * 16 + (lane & 15)])[grp] = p[l];
             }
-            // Values of more digits: the two upper planes' products, straight
-            // to the sums.
-            if (is_wide(seen)) {
+        }
+        if (is_wide(seen) && lane == 0) s_wide[step & 1] = (int32_t)step + 1;
+    };
+    const uint4* t = s.scores + (tile * s.chunks + chunk) * (s.chunk / 16) * 64 + lane;
+    uint4 terms[4];
+    auto load_terms = [&](uint32_t step) __attribute__((always_inline)) {
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int4 x[4] = {column(k, 0), column(k, 1), column(k, 2), column(k, 3)};
-                    v4i f[DIGITS];
-                    step_digits<DIGITS>(x, f, seen);
+        for (uint32_t k = 0; k < 4; k++) terms[k] = t[min(step * 4 + k, kt1 - 1) * 64];
+    };
+    v4i acc[TILES][NARROW + 1];
+#pragma unroll
+    for (uint32_t k = 0; k < TILES; k++)
+#pragma unroll
+        for (int j = 0; j < NARROW + 1; j++) acc[k][j] = v4i{0, 0, 0, 0};
+    int32_t wsum = 0;
+    uint64_t* out = s.partial + (tile * s.chunks + chunk) * 16 * HD + dim0;
+    bool added = false;  // the lane's own sums in `out` hold upper digits' products
+    load_raw(0);
+    load_terms(0);
 #pragma unroll 1
-                    for (uint32_t rt = 0; rt < RW; rt++) {
-                        if (half * RW + rt >= tiles) break;
-                        const uint4* p = s_w + (((half * RW + rt) * BATCH + i) * 2) * 64 + lane;
-                        const uint4 y0 = p[0], y1 = p[64];
-                        const v4i a0 = v4i{(int)y0.x, (int)y0.y, (int)y0.z, (int)y0.w}, a1 = v4i{(int)y1.x, (int)y1.y, (int)y1.z, (int)y1.w};
-                        const v4i upper[2] = {f[3], f[4]};
-                        v4i up[3] = {v4i{0, 0, 0, 0}, v4i{0, 0, 0, 0}, v4i{0, 0, 0, 0}};
-                        value_step<2>(a0, a1, upper, up);
+    for (uint32_t step = 0; step < steps; step++) {
+        split_raw(step);
+        if (step + 1 < steps) load_raw(step + 1);
+        v4i w0 = v4i{0, 0, 0, 0}, w1 = v4i{0, 0, 0, 0};
+        if (has_rt) {
 #pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            const uint64_t t = (uint64_t)(int64_t)up[0][q] << 24;
-                            const uint64_t sum3 = t + ((uint64_t)(int64_t)up[1][q] << 32) + ((uint64_t)(int64_t)up[2][q] << 40);
-                            atomicAdd((unsigned long long*)&s_sums[((half * RW + rt) * 16 + 4 * grp + q) * HD + d + k], sum3);
-                        }
-                    }
+            for (uint32_t k = 0; k < 4; k++) {
+                const uint32_t kt = step * 4 + k;
+                const bool live = valid && kt < kt1;
+                const uint4 x = terms[k];
+                const uint32_t e[4] = {live ? x.x : 0, live ? x.y : 0, live ? x.z : 0, live ? x.w : 0};
+                int32_t w[4];
+                weights_of(e, sc.sum, sc.w, sc.q, w, wsum,
+                           [&](int j) { s_big[wave].add(lane & 15, key0 + kt * 16 + 4 * grp + j); });
+                uint32_t low, high;
+                weight_digits(w, low, high);
+                w0[k] = (int)low, w1[k] = (int)high;
+            }
+            if (step + 1 < steps) load_terms(step + 1);
+        }
+        lds_barrier();
+        if (!has_rt) continue;
+#pragma unroll
+        for (uint32_t k = 0; k < TILES; k++) {
+            v4i f[NARROW];
+#pragma unroll
+            for (int l = 0; l < NARROW; l++) f[l] = s_v[step & 1][k][l][lane];
+            value_step<NARROW>(w0, w1, f, acc[k]);
+        }
+        if (s_wide[step & 1] == (int32_t)step + 1) {
+            // Every (row, dimension) is one lane's own: it adds to its sums.
+#pragma unroll 1
+            for (uint32_t k = 0; k < TILES; k++) {
+                const uint32_t d = dim0 + k / 4 * 64 + 4 * (lane & 15) + k % 4;
+                int4 x[4];
+#pragma unroll
+                for (uint32_t i = 0; i < 4; i++) {
+                    int32_t y[4];
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; j++)
+                        y[j] = load1(at.at(at.v, key0 + step * STEP + 4 * grp + 16 * i + j) + (d < at.hd ? d : 0));
+                    x[i] = make_int4(y[0], y[1], y[2], y[3]);
+                }
+                uint64_t more[4];
+                upper_values(w0, w1, x, more);
+#pragma unroll
+                for (uint32_t q = 0; q < 4; q++) {
+                    uint64_t* to = out + (size_t)(4 * grp + q) * HD + (d - dim0);
+                    *to = added ? *to + more[q] : more[q];
                 }
             }
+            added = true;
         }
-        __syncthreads();
     }
+    if (!has_rt) return;
     wsum += __shfl_xor(wsum, 16);
     wsum += __shfl_xor(wsum, 32);
-    if (has_rt && lane < 16) atomicAdd(&s_wsum[my_rt][lane], wsum);
+    if (lane < 16 && valid && dim0 == 0) s.weights[(tile * s.chunks + chunk) * 16 + lane] = wsum;
+    // The wave's own large weights: its LDS accesses are in order.
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-    for (uint32_t rt = 0; rt < RW; rt++) {
-        if (half * RW + rt >= tiles) break;
+    for (uint32_t b = 0; b < BLOCKS; b++) {
+        const uint32_t d = dim0 + b * 64 + 4 * (lane & 15);
 #pragma unroll
-        for (int k = 0; k < 4; k++)
+        for (uint32_t q = 0; q < 4; q++) {
+            const uint32_t i = 4 * grp + q;
+            if (rt * 16 + i >= pairs) continue;
+            uint64_t* to = out + (size_t)i * HD + (d - dim0);
+            uint64_t sum[4];
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                uint64_t t = 0;
+            for (int k = 0; k < 4; k++) {
+                sum[k] = added ? to[k] : 0;
 #pragma unroll
-                for (int j = 0; j < NARROW + 1; j++) t += (uint64_t)(int64_t)acc[rt][k][j][q] << (8 * j);
-                uint64_t* to = &s_sums[((half * RW + rt) * 16 + 4 * grp + q) * HD + d + k];
-                atomicAdd((unsigned long long*)to, t);
+                for (int j = 0; j < NARROW + 1; j++) sum[k] += (uint64_t)(int64_t)acc[b * 4 + k][j][q] << (8 * j);
             }
-    }
-    __syncthreads();
-    const uint32_t rows = min(RB, tiles) * 16;
-    for (uint32_t i = tid; i < rows * HD; i += WAVES * 64) {
-        const uint32_t row = i / HD, dim = i % HD, rt = row / 16;
-        uint64_t t = s_sums[i];
-        for (int j = 0; j < s_nbig[rt][row % 16]; j++) {  // at most two
-            const uint32_t key = (uint32_t)s_big[rt][row % 16][j];
-            if (dim < c.head_dim) t += (uint64_t)((int64_t)65536 * at.at(at.v, at.page_of(key), key)[dim]);
+            for (int j = 0; j < s_big[wave].count[i]; j++) {
+                const int4 x = load4(at.at(at.v, s_big[wave].key[i][j]) + (d < at.hd ? d : 0));
+                sum[0] += (uint64_t)((int64_t)65536 * x.x), sum[1] += (uint64_t)((int64_t)65536 * x.y);
+                sum[2] += (uint64_t)((int64_t)65536 * x.z), sum[3] += (uint64_t)((int64_t)65536 * x.w);
+            }
+            *(ulonglong2*)to = make_ulonglong2(sum[0], sum[1]);
+            *(ulonglong2*)(to + 2) = make_ulonglong2(sum[2], sum[3]);
         }
-        s.partial[(((tile0 + rt) * s.chunks + chunk) * 16 + row % 16) * HD + dim] = t;
     }
-    if (tid < rows) s.weights[((tile0 + tid / 16) * s.chunks + chunk) * 16 + tid % 16] = s_wsum[tid / 16][tid % 16];
 }
 
 // ---- (4) the chunks joined: a workgroup per (drafted row, head)
@@ -520,28 +698,34 @@ __global__ __launch_bounds__((ValueShape<HD, RB>::WAVES * 64), 2) void tree_valu
 __global__ __launch_bounds__(256) void tree_join_kernel(const IrisPagedKv c, const IrisTreeAttention a, const TreeSpace s,
                                                         uint32_t hd_padded) {
     __shared__ uint64_t s_part[256];
-    const uint32_t tid = threadIdx.x, bg = blockIdx.y, g = bg % c.kv_heads, group = a.heads / c.kv_heads, pair = blockIdx.x;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, bg = blockIdx.y, g = bg % c.kv_heads, group = a.heads / c.kv_heads;
+    const uint32_t pair = blockIdx.x;
     Request r;
     if (!read_request(c, a, bg / c.kv_heads, r)) return;
     if (pair >= r.rows * group) return;
     const size_t tile = (size_t)bg * s.row_tiles + pair / 16;
     const uint32_t i = pair % 16, chunks = chunks_of(s, r);
-    uint64_t best = 0;
+    uint32_t key = 0xffffffffu;
     int32_t wsum = 0;
-    for (uint32_t k = 0; k < chunks; k++) {
-        best = max(best, s.maxima[(tile * s.chunks + k) * 16 + i]);
+    for (uint32_t k = lane; k < chunks; k += 64) {
+        key = min(key, s.firsts[(tile * s.chunks + k) * 16 + i]);
         wsum += s.weights[(tile * s.chunks + k) * 16 + i];
     }
+    for (int off = 1; off < 64; off <<= 1) {
+        key = min(key, (uint32_t)__shfl_xor((int)key, off));
+        wsum += __shfl_xor(wsum, off);
+    }
     const int64_t resid = dn::sub_sat(dn::ONE_ACT, wsum);
-    const uint32_t key = packed_key(best);
-    const Places at = places(c, a, r, g);
-    const int32_t* v = at.at(at.v, at.page_of(key), key);
+    const uint32_t log = 31u - __clz((int)c.page_size), page = (uint32_t)r.table[key >> log];
+    const int32_t* v = page < c.pages ? c.v + (((size_t)page * c.kv_heads + g) * c.page_size + (key & (c.page_size - 1))) * c.head_dim
+                                      : g_zeros;
     int32_t* out = a.out + (size_t)(r.row0 + pair / group) * a.out_stride + (size_t)(g * group + pair % group) * c.head_dim;
     // Up to 256 dimensions at a time, the chunks dealt to what threads are left.
     const uint32_t width = min(hd_padded, 256u), parts = 256 / width, part = tid / width;
     for (uint32_t d0 = 0; d0 < c.head_dim; d0 += width) {
         const uint32_t d = d0 + tid % width;
         uint64_t t = 0;
+#pragma unroll 4
         for (uint32_t k = part; k < chunks; k += parts) t += s.partial[((tile * s.chunks + k) * 16 + i) * hd_padded + d];
         s_part[tid] = t;
         __syncthreads();
@@ -579,9 +763,8 @@ uint64_t tree_space(const IrisPagedKv& c, const IrisTreeAttention& a, uint8_t* b
     s->row_tiles = (a.max_nodes * group + 15) / 16;
     // Positions that a request's rows look at, from a multiple of STEP on.
     const uint64_t span = std::min<uint64_t>(a.max_positions, a.window ? (uint64_t)a.window + a.max_nodes + STEP : a.max_positions);
-    const uint64_t blocks = bg * ((s->row_tiles + row_block(hd) - 1) / row_block(hd));
-    const uint64_t want = std::max<uint64_t>(1, 1024 / blocks);
-    s->chunk = (uint32_t)std::max<uint64_t>(128, ((span + want - 1) / want + 127) & ~127ull);
+    const uint64_t want = std::max<uint64_t>(1, 1024 / bg);
+    s->chunk = (uint32_t)std::min<uint64_t>(MAX_CHUNK, std::max<uint64_t>(128, ((span + want - 1) / want + 127) & ~127ull));
     s->chunks = (uint32_t)((span + s->chunk - 1) / s->chunk);
     uint64_t at = 0;
     auto take = [&](auto*& p, uint64_t bytes) {
@@ -590,34 +773,35 @@ uint64_t tree_space(const IrisPagedKv& c, const IrisTreeAttention& a, uint8_t* b
     };
     const uint64_t parts = bg * s->row_tiles * s->chunks;
     take(s->scores, parts * (s->chunk / 16) * TILE_BYTES);
-    take(s->maxima, parts * 16 * 8);
+    take(s->maxima, parts * 16 * 4);
+    take(s->firsts, parts * 16 * 4);
     take(s->sums, parts * 16 * 8);
     take(s->weights, parts * 16 * 4);
     take(s->partial, parts * 16 * hd * 8);
     return at;
 }
 
-template <uint32_t HD, uint32_t RB>
-int tree_launch_block(const IrisPagedKv& c, const IrisTreeAttention& a, const TreeSpace& s, hipStream_t stream) {
-    const uint32_t bg = a.requests * c.kv_heads, blocks = (s.row_tiles + RB - 1) / RB;
-    const size_t q_lds = RB * (HD / 64) * DIGITS * TILE_BYTES, v_lds = RB * 16 * HD * 8 + RB * BATCH * 2 * TILE_BYTES;
-    hipError_t st = paged_lds_limit((const void*)tree_scores_kernel<HD, RB>, q_lds);
-    if (st == hipSuccess) st = paged_lds_limit((const void*)tree_values_kernel<HD, RB>, v_lds);
+template <uint32_t HD, bool FULL>
+int tree_launch(const IrisPagedKv& c, const IrisTreeAttention& a, const TreeSpace& s, hipStream_t stream) {
+    const uint32_t bg = a.requests * c.kv_heads, RB = row_block(HD), few = std::min(s.row_tiles, RB);
+    const size_t q_lds = (size_t)few * (HD / 64) * NARROW * TILE_BYTES, v_lds = 16 * HD * 8 + (size_t)s.chunk / STEP * 2 * TILE_BYTES;
+    hipError_t st = paged_lds_limit((const void*)tree_values_kernel<HD, FULL>, v_lds);
     if (st != hipSuccess) return (int)st;
-    hipLaunchKernelGGL((tree_scores_kernel<HD, RB>), dim3(s.chunks, blocks, bg), dim3(256), q_lds, stream, c, a, s);
+    hipLaunchKernelGGL((tree_scores_kernel<HD, FULL>), dim3(s.chunks, (s.row_tiles + RB - 1) / RB, bg), dim3(256), q_lds, stream, c,
+                       a, s);
     hipLaunchKernelGGL(tree_terms_kernel, dim3(s.chunks, s.row_tiles, bg), dim3(256), 0, stream, c, a, s);
-    hipLaunchKernelGGL((tree_values_kernel<HD, RB>), dim3(s.chunks, blocks, bg), dim3(ValueShape<HD, RB>::WAVES * 64), v_lds,
-                       stream, c, a, s);
+    if (s.row_tiles == 1)
+        hipLaunchKernelGGL((tree_values_kernel<HD, FULL>), dim3(s.chunks, 1, bg), dim3(HD > 256 ? HD : 256), v_lds, stream, c, a, s);
+    else
+        hipLaunchKernelGGL((tree_values_many_kernel<HD, 8, FULL>), dim3(s.chunks, (s.row_tiles + 7) / 8 * (HD / value_dims(HD)), bg),
+                           dim3(512), 0, stream, c, a, s);
     hipLaunchKernelGGL(tree_join_kernel, dim3(a.max_nodes * (a.heads / c.kv_heads), bg), dim3(256), 0, stream, c, a, s, HD);
     return (int)hipGetLastError();
 }
 
 template <uint32_t HD>
-int tree_launch(const IrisPagedKv& c, const IrisTreeAttention& a, const TreeSpace& s, hipStream_t stream) {
-    if (s.row_tiles == 1) return tree_launch_block<HD, 1>(c, a, s, stream);
-    if constexpr (row_block(HD) >= 2)
-        if (s.row_tiles == 2 || row_block(HD) == 2) return tree_launch_block<HD, 2>(c, a, s, stream);
-    return tree_launch_block<HD, row_block(HD)>(c, a, s, stream);
+int tree_launch_head(const IrisPagedKv& c, const IrisTreeAttention& a, const TreeSpace& s, hipStream_t stream) {
+    return c.head_dim == HD ? tree_launch<HD, true>(c, a, s, stream) : tree_launch<HD, false>(c, a, s, stream);
 }
 
 }  // namespace
@@ -638,10 +822,10 @@ int iris_attention_tree(const IrisPagedKv* c, const IrisTreeAttention* a, void* 
     TreeSpace s;
     if (bytes < tree_space(*c, *a, (uint8_t*)space, &s)) return IRIS_E_RANGE;
     switch (padded_head(c->head_dim)) {
-        case 64: return tree_launch<64>(*c, *a, s, (hipStream_t)stream);
-        case 128: return tree_launch<128>(*c, *a, s, (hipStream_t)stream);
-        case 256: return tree_launch<256>(*c, *a, s, (hipStream_t)stream);
-        default: return tree_launch<512>(*c, *a, s, (hipStream_t)stream);
+        case 64: return tree_launch_head<64>(*c, *a, s, (hipStream_t)stream);
+        case 128: return tree_launch_head<128>(*c, *a, s, (hipStream_t)stream);
+        case 256: return tree_launch_head<256>(*c, *a, s, (hipStream_t)stream);
+        default: return tree_launch_head<512>(*c, *a, s, (hipStream_t)stream);
     }
 }
 
