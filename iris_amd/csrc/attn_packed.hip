@@ -135,7 +135,7 @@ __device__ __forceinline__ void value_block_planes(const int32_t* x, size_t stri
 template <uint32_t HD>
 __global__ __launch_bounds__(256) void packed_planes_kernel(const IrisPackedAttention a, const PackedSpace s) {
     constexpr uint32_t DS = HD / 64;
-    uint32_t task = blockIdx.x * 4 + (threadIdx.x >> 6);
+    uint32_t task = blockIdx.x * 4 + wave_index();
     const uint32_t key_tiles = s.steps * 4, lane = threadIdx.x & 63;
     if (task < key_tiles * a.kv_heads) {
         const uint32_t g = task % a.kv_heads, kt = task / a.kv_heads;
@@ -179,7 +179,7 @@ template <int NW>
 struct PackedSmem {
     int32_t best[NW][16];
     uint32_t best_key[NW][16];
-    double sum[NW][16];
+    double sum[NW][16], total[16];
     int32_t wsum[16], nbig[16], big[16][2];
     int32_t wide_scores, wide_values;
 };
@@ -195,7 +195,7 @@ __device__ __forceinline__ void packed_rows(const IrisPackedAttention& a, const 
                                             uint4* tiles, uint4* spill, PackedSmem<NW>& sm) {
     constexpr uint32_t DS = HD / 64, DT = HD / 16, PARTS = key_parts<HD, NW>(), DTW = DT * PARTS / NW;
     constexpr bool HOLD = HD <= 128;  // the queries' operands stay in registers
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, grp = lane >> 4;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = wave_index(), grp = lane >> 4;
     const uint32_t g = h / (a.heads / a.kv_heads);
 
     // This lane's row and the keys [first, row] it sees.
@@ -330,16 +330,19 @@ __device__ __forceinline__ void packed_rows(const IrisPackedAttention& a, const 
     sum += __shfl_xor(sum, 32);
     if (lane < 16) sm.sum[wave][lane] = sum;
     __syncthreads();
-    sum = sm.sum[0][lane & 15];
+    if (tid < 16) {
+        sum = sm.sum[0][tid];
 #pragma unroll
-    for (int v = 1; v < NW; v++) sum += sm.sum[v][lane & 15];
+        for (int v = 1; v < NW; v++) sum += sm.sum[v][tid];
+        sm.total[tid] = sum;
+    }
+    __syncthreads();
 
     // (3) the weights' digits in place of the terms: the low digits of a
     // tile's four keys per lane as dword `lane`, the high ones as dword
     // 64 + lane. Tiles of the first and last step that no row sees: zeros.
     {
-        const double w_scale = valid ? 65536.0 / sum : 0.0, q_scale = valid ? 4294967296.0 / sum : 0.0;
-        const uint64_t total = valid ? (uint64_t)sum : 1;
+        const RowScale scale(&sm.total[lane & 15], valid);
         int32_t wsum = 0;
 #pragma unroll 1
         for (uint32_t kt = base + wave; kt < ks1 * 4; kt += NW) {
@@ -349,7 +352,7 @@ __device__ __forceinline__ void packed_rows(const IrisPackedAttention& a, const 
                 const uint4 k = t[lane];
                 const uint32_t e[4] = {k.x, k.y, k.z, k.w};
                 int32_t w[4];
-                weights_of(e, total, w_scale, q_scale, w, wsum, [&](int i) {
+                weights_of(e, scale, scale.w, w, wsum, [&](int i) {
                     const int at = atomicAdd(&sm.nbig[lane & 15], 1);
                     if (at < 2) sm.big[lane & 15][at] = (int32_t)(kt * 16 + 4 * grp + i);
                 });

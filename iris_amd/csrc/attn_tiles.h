@@ -29,6 +29,10 @@ constexpr int DIGITS = 5;              // of any int32
 constexpr int NARROW = 3;              // of the usual values
 constexpr int32_t BIG_WEIGHT = 32640;  // the first weight that needs a third digit
 
+// The wave's index in its workgroup, known to be the same in every lane (what
+// follows from it stays in scalar registers).
+__device__ __forceinline__ uint32_t wave_index() { return (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
+
 // Loads from device memory by a pointer the compiler cannot place (flat loads
 // would count as LDS accesses too, and every LDS wait as one for them).
 __device__ __forceinline__ int4 load4(const int32_t* p) {
@@ -118,38 +122,64 @@ __device__ __forceinline__ void dot_step(const v4i (&kf)[LD], const v4i (&qf)[LD
 // A score's exp term below the row's maximum as it is kept between the
 // passes: 2^32 (the maximum's own) as 0xffffffff, which no other term is.
 __device__ __forceinline__ uint32_t kept_term(double e) { return e > 4294967295.0 ? 0xffffffffu : (uint32_t)e; }
-__device__ __forceinline__ double term_of(uint32_t kept) { return kept == 0xffffffffu ? 4294967296.0 : (double)kept; }
 
-// The weights of four kept terms and the reciprocal scales of the row's sum.
-// `slow` flags those near a rounding tie or of three digits; they are redone
-// exactly, the third digit left to on_big(i) and taken off the weight.
+// What turns a row's exp terms into weights: 2^16 over their sum (zero for a
+// lane without a row: all its weights are zero), and whether a weight may need
+// three digits. The sum itself is read again where a weight is formed exactly.
+struct RowScale {
+    double w;
+    bool big;
+    const double* sum;
+    __device__ __forceinline__ RowScale(const double* total, bool valid) : sum(total) {
+        w = valid ? 65536.0 / *total : 0.0;
+        big = w * 4294967296.0 >= (double)BIG_WEIGHT - 1.0;
+    }
+};
+
+__device__ __forceinline__ int32_t exact_weight(uint32_t kept, double total) {
+    return dn::softmax_weight(kept == 0xffffffffu ? (uint64_t)dn::ONE_ACC : kept, (uint64_t)total, 4294967296.0 / total);
+}
+
+// The weights of four kept terms, two digits each. A quotient estimated in
+// double is off by under 2^-29 (and 2^-16 where the kept term stands for
+// 2^32), the quotient's own rounding in 32 fraction bits moves it by at most
+// 2^-17: within 2^-15 of a rounding tie, and where a third digit is needed,
+// the weight is formed again exactly (one in 2^14), the third digit left to
+// on_big(i) and taken off the weight.
 template <class OnBig>
-__device__ __forceinline__ void weights_of(const uint32_t (&e)[4], uint64_t sum, double w_scale, double q_scale,
-                                           int32_t (&w)[4], int32_t& wsum, OnBig&& on_big) {
-    uint32_t slow = 0;
+__device__ __forceinline__ void weights_of(const uint32_t (&e)[4], const RowScale& s, double w_scale, int32_t (&w)[4],
+                                           int32_t& wsum, OnBig&& on_big) {
+    bool slow = s.big;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const double t = term_of(e[i]) * w_scale + 0.5, fl = floor(t);
-        w[i] = (int32_t)fl;
-        slow |= (uint32_t)((fabs(t - fl - 0.5) > 0.5 - 0x1p-15) | (w[i] >= BIG_WEIGHT)) << i;
+        const double t = (double)e[i] * w_scale, n = rint(t);
+        w[i] = (int32_t)n;
+        slow |= fabs(t - n) > 0.5 - 0x1p-15;
     }
-    if (slow) {
-#pragma unroll
+    if (__any(slow)) {
+        // One piece of code for the four: four copies of it in every loop
+        // would not stay in the instruction cache.
+#pragma unroll 1
         for (int i = 0; i < 4; i++) {
-            if (!((slow >> i) & 1)) continue;
-            const uint64_t term = e[i] == 0xffffffffu ? (uint64_t)dn::ONE_ACC : e[i];
-            w[i] = dn::softmax_weight(term, sum, q_scale);
-            if (w[i] >= BIG_WEIGHT) {
+            const uint32_t kept = i == 0 ? e[0] : i == 1 ? e[1] : i == 2 ? e[2] : e[3];
+            int32_t x = i == 0 ? w[0] : i == 1 ? w[1] : i == 2 ? w[2] : w[3];
+            const double t = (double)kept * w_scale;
+            if (fabs(t - rint(t)) > 0.5 - 0x1p-15) x = exact_weight(kept, *s.sum);
+            if (x >= BIG_WEIGHT) {
                 on_big(i);
-                w[i] -= 65536;
+                x -= 65536;
                 wsum += 65536;
             }
+            w[0] = i == 0 ? x : w[0], w[1] = i == 1 ? x : w[1], w[2] = i == 2 ? x : w[2], w[3] = i == 3 ? x : w[3];
         }
     }
     wsum += w[0] + w[1] + w[2] + w[3];
 }
 
-// The two digit planes' dwords of four weights in [-32896, 32640).
+// What two digits hold of a weight: the weight, or 65536 less.
+__device__ __forceinline__ int32_t two_digits(int32_t w) { return ((w + 0x8080) & 0xffff) - 0x8080; }
+
+// The two digit planes' dwords of four weights, of each what two_digits() says.
 __device__ __forceinline__ void weight_digits(const int32_t (&w)[4], uint32_t& low, uint32_t& high) {
     uint32_t d[4];
 #pragma unroll

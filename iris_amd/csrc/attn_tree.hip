@@ -18,8 +18,8 @@
 
 namespace {
 
-// A place of zeros for positions whose page is outside the cache.
-__device__ const int32_t g_zeros[ATTN_MAX_HEAD_DIM] = {};
+// Four rows of zeros for positions whose page is outside the cache.
+__device__ const int32_t g_zeros[4 * ATTN_MAX_HEAD_DIM] = {};
 
 constexpr uint32_t STEP = 64;  // positions of a value product
 
@@ -91,36 +91,36 @@ __device__ __forceinline__ RowView row_view(const IrisTreeAttention& a, const Re
     return v;
 }
 
-// The cache of one key head, for positions [key0, key1) whose pages are in
-// LDS. Positions past the last one read the last one (no row sees them).
+// The cache of one key head, for positions [key0, key1) whose pages' offsets
+// are in LDS. Positions past the last one read the last one (no row sees them).
 struct Places {
     const int32_t *k, *v;
-    const uint32_t* page;  // of key0's page on
-    uint32_t pages, page_log, place_mask, first, last;
-    size_t page_stride;
-    uint32_t hd;
+    const uint64_t* page;  // offsets in values, of key0's page on; ~0: outside the cache
+    uint32_t page_log, place_mask, first, last, hd;
     __device__ __forceinline__ const int32_t* at(const int32_t* base, uint32_t key) const {
         key = min(key, last);
-        const uint32_t p = page[(key >> page_log) - first];
-        return p < pages ? base + p * page_stride + (size_t)(key & place_mask) * hd : g_zeros;
+        const uint64_t p = page[(key >> page_log) - first];
+        return p != ~0ull ? base + (p + (key & place_mask) * hd) : g_zeros;
     }
+    // The first of four positions in a row (key a multiple of four), which
+    // lie in one page; those past the last one are there, but not written.
+    __device__ __forceinline__ const int32_t* four(const int32_t* base, uint32_t key) const { return at(base, min(key, last & ~3u)); }
 };
 
-constexpr uint32_t MAX_CHUNK = 1024;
+constexpr uint32_t MAX_CHUNK = 512;
 constexpr uint32_t CHUNK_PAGES = MAX_CHUNK / 4 + 1;
 
 // The workgroup's places; s_page has CHUNK_PAGES entries. A barrier follows.
 __device__ __forceinline__ Places places(const IrisPagedKv& c, const IrisTreeAttention& a, const Request& r, uint32_t g,
-                                         uint32_t key0, uint32_t key1, uint32_t* s_page) {
+                                         uint32_t key0, uint32_t key1, uint64_t* s_page) {
     const size_t head = (size_t)c.page_size * c.head_dim;
     const uint32_t log = 31u - __clz((int)c.page_size), first = key0 >> log, n = ((key1 - 1) >> log) - first + 1;
     for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
         const uint32_t p = (uint32_t)r.table[first + i];
-        s_page[i] = p;
+        s_page[i] = p < c.pages ? p * (c.kv_heads * head) : ~0ull;
         if (p >= c.pages && a.status) *a.status = IRIS_E_INVALID;
     }
-    return Places{c.k + g * head, c.v + g * head, s_page, c.pages, log, c.page_size - 1, first, key1 - 1, c.kv_heads * head,
-                  c.head_dim};
+    return Places{c.k + g * head, c.v + g * head, s_page, log, c.page_size - 1, first, key1 - 1, c.head_dim};
 }
 
 // A lane's four values of each 16-dimension piece of a 64-dimension step.
@@ -169,10 +169,11 @@ __global__ __launch_bounds__(256, HD >= 512 ? 1 : HD >= 256 ? 2 : 3) void tree_s
     extern __shared__ v4i s_q[];  // [tiles][DS][NARROW][64]
     __shared__ int32_t s_max[RB][64];
     __shared__ uint64_t s_mask[RB * 16];
-    __shared__ uint32_t s_lo[RB * 16], s_page[CHUNK_PAGES];
+    __shared__ uint32_t s_lo[RB * 16];
+    __shared__ uint64_t s_page[CHUNK_PAGES];
     __shared__ int32_t s_wide;
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, grp = lane >> 4;
-    const uint32_t chunk = blockIdx.x, rt0 = blockIdx.y * RB, bg = blockIdx.z, g = bg % c.kv_heads;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = wave_index(), grp = lane >> 4;
+    const uint32_t chunk = blockIdx.y, rt0 = blockIdx.z * RB, bg = blockIdx.x, g = bg % c.kv_heads;
     const uint32_t group = a.heads / c.kv_heads;
     Request r;
     if (!read_request(c, a, bg / c.kv_heads, r)) return;
@@ -314,8 +315,8 @@ struct RowLanes {
 __global__ __launch_bounds__(256) void tree_terms_kernel(const IrisPagedKv c, const IrisTreeAttention a, const TreeSpace s) {
     __shared__ double s_sum[4][16];
     __shared__ uint32_t s_first[4][16];
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, grp = lane >> 4;
-    const uint32_t chunk = blockIdx.x, rt = blockIdx.y, bg = blockIdx.z, group = a.heads / c.kv_heads;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = wave_index(), grp = lane >> 4;
+    const uint32_t chunk = blockIdx.y, rt = blockIdx.z, bg = blockIdx.x, group = a.heads / c.kv_heads;
     Request r;
     if (!read_request(c, a, bg / c.kv_heads, r)) return;
     const uint32_t key0 = r.base + chunk * s.chunk, pairs = r.rows * group;
@@ -366,20 +367,15 @@ __global__ __launch_bounds__(256) void tree_terms_kernel(const IrisPagedKv c, co
 
 // ---- (3) weights and weighted values
 
-// What turns a row's exp terms into weights.
-struct RowScale {
-    double w, q;
-    uint64_t sum;
-};
-
-// Lane row `row` of tile `tile`, the lanes of one row at strides of `width`.
-__device__ __forceinline__ RowScale row_scale(const TreeSpace& s, size_t tile, uint32_t chunks, uint32_t row, uint32_t width,
-                                              bool valid) {
+// The sum of lane row `row` of tile `tile` over its chunks, the lanes of one
+// row at strides of `width`.
+__device__ __forceinline__ double row_sum(const TreeSpace& s, size_t tile, uint32_t chunks, uint32_t row, uint32_t width,
+                                          bool valid) {
     const uint32_t lane = threadIdx.x & 63;
     double sum = 0;
     for (uint32_t i = lane / width; i < chunks; i += 64 / width) sum += valid ? s.sums[(tile * s.chunks + i) * 16 + row] : 0.0;
     for (uint32_t off = width; off < 64; off <<= 1) sum += __shfl_xor(sum, (int)off);
-    return valid ? RowScale{65536.0 / sum, 4294967296.0 / sum, (uint64_t)sum} : RowScale{0.0, 0.0, 1};
+    return sum;
 }
 
 // A step's values for one 64-dimension block: dimensions d .. d + 3 of the
@@ -387,9 +383,11 @@ __device__ __forceinline__ RowScale row_scale(const TreeSpace& s, size_t tile, u
 template <bool FULL>
 __device__ __forceinline__ void load_values(const Places& at, uint32_t key, uint32_t d, int4 (&v)[4][4]) {
 #pragma unroll
-    for (uint32_t t = 0; t < 4; t++)
+    for (uint32_t t = 0; t < 4; t++) {
+        const int32_t* p = at.four(at.v, key + 16 * t) + (FULL || d < at.hd ? d : 0);
 #pragma unroll
-        for (uint32_t i = 0; i < 4; i++) v[t][i] = load4(at.at(at.v, key + 16 * t + i) + (FULL || d < at.hd ? d : 0));
+        for (uint32_t i = 0; i < 4; i++) v[t][i] = load4(p + i * at.hd);
+    }
 }
 
 __device__ __forceinline__ int4 column(const int4 (&v)[4], int k) {
@@ -429,10 +427,11 @@ __global__ __launch_bounds__((HD / 64 > 4 ? HD : 256), 2) void tree_values_kerne
     extern __shared__ uint64_t s_sums[];  // [16][HD], then the weights' digits [steps][2][64] uint4
     __shared__ BigWeights s_big;
     __shared__ int32_t s_wsum[16];
-    __shared__ uint32_t s_page[CHUNK_PAGES];
+    __shared__ double s_total[WAVES][16];
+    __shared__ uint64_t s_page[CHUNK_PAGES];
     uint4* s_w = (uint4*)(s_sums + 16 * HD);
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, grp = lane >> 4;
-    const uint32_t chunk = blockIdx.x, bg = blockIdx.z, g = bg % c.kv_heads, group = a.heads / c.kv_heads;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = wave_index(), grp = lane >> 4;
+    const uint32_t chunk = blockIdx.y, bg = blockIdx.x, g = bg % c.kv_heads, group = a.heads / c.kv_heads;
     Request r;
     if (!read_request(c, a, bg / c.kv_heads, r)) return;
     const uint32_t key0 = r.base + chunk * s.chunk, rows = r.rows * group;
@@ -447,7 +446,9 @@ __global__ __launch_bounds__((HD / 64 > 4 ? HD : 256), 2) void tree_values_kerne
     {
         const RowLanes l(rows);
         const bool valid = l.row < rows;
-        const RowScale sc = row_scale(s, bg, chunks_of(s, r), l.row, l.width, valid);
+        const double total = row_sum(s, bg, chunks_of(s, r), l.row, l.width, valid);
+        s_total[wave][lane & 15] = total;
+        const RowScale sc(&s_total[wave][lane & 15], valid);
         const uint4* t = s.scores + ((size_t)bg * s.chunks + chunk) * (s.chunk / 16) * 64 + l.slot;
         const uint32_t per = 16 / l.width;
         int32_t wsum = 0;
@@ -457,7 +458,7 @@ __global__ __launch_bounds__((HD / 64 > 4 ? HD : 256), 2) void tree_values_kerne
             const uint4 x = t[kt * 64];
             const uint32_t e[4] = {x.x, x.y, x.z, x.w};
             int32_t w[4];
-            weights_of(e, sc.sum, sc.w, sc.q, w, wsum, [&](int j) { s_big.add(l.row, key0 + kt * 16 + 4 * grp + j); });
+            weights_of(e, sc, sc.w, w, wsum, [&](int j) { s_big.add(l.row, key0 + kt * 16 + 4 * grp + j); });
             uint32_t low, high;
             weight_digits(w, low, high);
             uint32_t* to = (uint32_t*)(s_w + (size_t)(kt / 4) * 128 + l.slot) + kt % 4;
@@ -496,7 +497,7 @@ __global__ __launch_bounds__((HD / 64 > 4 ? HD : 256), 2) void tree_values_kerne
                     int32_t y[4];
 #pragma unroll
                     for (uint32_t i = 0; i < 4; i++)
-                        y[i] = load1(at.at(at.v, key0 + step * STEP + 4 * grp + 16 * t + i) + (d < at.hd ? d + k : 0));
+                        y[i] = load1(at.four(at.v, key0 + step * STEP + 4 * grp + 16 * t) + i * at.hd + (d < at.hd ? d + k : 0));
                     x[t] = make_int4(y[0], y[1], y[2], y[3]);
                 }
                 uint64_t add[4];
@@ -530,181 +531,279 @@ __global__ __launch_bounds__((HD / 64 > 4 ? HD : 256), 2) void tree_values_kerne
     if (tid < rows) s.weights[((size_t)bg * s.chunks + chunk) * 16 + tid] = s_wsum[tid];
 }
 
-// Dimensions of a many-rows workgroup.
-constexpr uint32_t value_dims(uint32_t hd) { return hd < 128 ? hd : 128; }
+// Weights that an estimate leaves open (near a rounding tie, or of three
+// digits): (row, position in the chunk) of each, settled after the loop over
+// the steps, so that the loop keeps its registers. Past the list's end every
+// position of the chunk is looked at again.
+struct OpenWeights {
+    static constexpr uint32_t ROOM = 64;
+    uint32_t count;
+    uint32_t at[ROOM];  // position << 4 | row
+    int32_t add[ROOM];  // what the loop's weight lacks
+    __device__ __forceinline__ void push(uint32_t row, uint32_t position) {
+        const uint32_t n = atomicAdd(&count, 1u);
+        if (n < ROOM) at[n] = position << 4 | row;
+    }
+};
 
-// NW row tiles, a wave each, which forms its own weights in registers; the
-// workgroup splits each step's values once, into LDS, a step ahead.
-template <uint32_t HD, uint32_t NW, bool FULL>
-__global__ __launch_bounds__(NW * 64, 2) void tree_values_many_kernel(const IrisPagedKv c, const IrisTreeAttention a,
-                                                                      const TreeSpace s) {
-    constexpr uint32_t VD = value_dims(HD), BLOCKS = VD / 64, UNITS = BLOCKS * 4, PER = (UNITS + NW - 1) / NW, TILES = VD / 16;
-    __shared__ v4i s_v[2][TILES][NARROW][64];
-    __shared__ int32_t s_wide[2];
-    __shared__ BigWeights s_big[NW];
-    __shared__ uint32_t s_page[CHUNK_PAGES];
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, grp = lane >> 4;
-    const uint32_t chunk = blockIdx.x, bg = blockIdx.z, g = bg % c.kv_heads, group = a.heads / c.kv_heads;
-    const uint32_t dim0 = blockIdx.y % (HD / VD) * VD, rt0 = blockIdx.y / (HD / VD) * NW;
+// The estimate of a weight, and whether it is left open.
+__device__ __forceinline__ int32_t estimate(uint32_t kept, double w_scale, bool& open) {
+    const double t = (double)kept * w_scale, n = rint(t);
+    open = fabs(t - n) > 0.5 - 0x1p-15 || n >= (double)BIG_WEIGHT;
+    return (int32_t)n;
+}
+
+// Several row tiles: a workgroup takes MANY of them and 128 dimensions (64 of
+// a head of 64), a wave per (row tile, 64-dimension block). Each step's values
+// are split once, and its weights formed once, into LDS, a step ahead of the
+// products that read them.
+constexpr uint32_t MANY = 4;
+constexpr uint32_t value_blocks(uint32_t hd) { return hd < 128 ? 1 : 2; }
+
+template <uint32_t HD, bool FULL>
+__global__ __launch_bounds__(MANY * value_blocks(HD) * 64, 4) void tree_values_many_kernel(const IrisPagedKv c,
+                                                                                       const IrisTreeAttention a,
+                                                                                       const TreeSpace s) {
+    constexpr uint32_t BLOCKS = value_blocks(HD), WAVES = MANY * BLOCKS, VD = 64 * BLOCKS, KT = 4 / BLOCKS;
+    __shared__ v4i s_v[2][BLOCKS * 4][NARROW][64];
+    __shared__ uint4 s_w[2][MANY][2][64];
+    __shared__ int32_t s_wsum[MANY][16];
+    __shared__ uint32_t s_wide;  // a bit per step whose values need more digits
+    __shared__ OpenWeights s_open[MANY];
+    __shared__ double s_total[WAVES][16];
+    __shared__ uint64_t s_page[CHUNK_PAGES];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = wave_index(), grp = lane >> 4;
+    const uint32_t chunk = blockIdx.y, bg = blockIdx.x, g = bg % c.kv_heads, group = a.heads / c.kv_heads;
+    const uint32_t dim0 = blockIdx.z % (HD / VD) * VD, rt0 = blockIdx.z / (HD / VD) * MANY;
     Request r;
     if (!read_request(c, a, bg / c.kv_heads, r)) return;
     const uint32_t key0 = r.base + chunk * s.chunk, pairs = r.rows * group;
     if (key0 >= r.total || rt0 * 16 >= pairs) return;
     const uint32_t n = min(s.chunk, r.total - key0), steps = (n + STEP - 1) / STEP, kt1 = (n + 15) / 16;
     const Places at = places(c, a, r, g, key0, key0 + n, s_page);
-    const uint32_t rt = rt0 + wave, row = rt * 16 + (lane & 15);
+    const uint32_t my = wave % MANY, block = wave / MANY, rt = rt0 + my, row = rt * 16 + (lane & 15);
     const bool has_rt = rt * 16 < pairs, valid = row < pairs;
-    const size_t tile = (size_t)bg * s.row_tiles + min(rt, s.row_tiles - 1);
-    if (tid < 2) s_wide[tid] = 0;
-    if (lane < 16) s_big[wave].count[lane] = 0;
+    const size_t tile = (size_t)bg * s.row_tiles + (has_rt ? rt : rt0);
+    if (tid == 0) s_wide = 0;
+    if (tid < MANY * 16) s_wsum[tid / 16][tid % 16] = 0;
+    if (tid < MANY) s_open[tid].count = 0;
     __syncthreads();
-    const RowScale sc = row_scale(s, tile, chunks_of(s, r), lane & 15, 16, valid);
 
-    // A unit of a step's values: positions 16 t + 4 q + i (lane: t, and
-    // dimensions 4 n ..) of one block and q.
-    int4 raw[PER][4];
+    // This wave's share of a step's values: dimensions 4 n .. of its block, at
+    // positions 16 t + 4 `my` + i (lane: t and n).
+    const uint32_t split_d = dim0 + block * 64 + 4 * (lane & 15);
+    int4 raw[4];
     auto load_raw = [&](uint32_t step) __attribute__((always_inline)) {
+        const int32_t* p = at.four(at.v, key0 + step * STEP + 16 * grp + 4 * my) + (FULL || split_d < at.hd ? split_d : 0);
 #pragma unroll
-        for (uint32_t u = 0; u < PER; u++) {
-            const uint32_t unit = wave + u * NW;
-            if (unit >= UNITS) break;
-            const uint32_t d = dim0 + unit / 4 * 64 + 4 * (lane & 15), key = key0 + step * STEP + 16 * grp + 4 * (unit % 4);
-#pragma unroll
-            for (uint32_t i = 0; i < 4; i++) raw[u][i] = load4(at.at(at.v, key + i) + (FULL || d < at.hd ? d : 0));
-        }
+        for (uint32_t i = 0; i < 4; i++) raw[i] = load4(p + i * at.hd);
     };
-    auto split_raw = [&](uint32_t step) __attribute__((always_inline)) {
-        uint32_t seen = 0;
-#pragma unroll
-        for (uint32_t u = 0; u < PER; u++) {
-            const uint32_t unit = wave + u * NW;
-            if (unit >= UNITS) break;
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                uint32_t p[4];
-                split4(column(raw[u], k), p, seen);
-#pragma unroll
-                for (int l = 0; l < NARROW; l++)
-                    ((uint32_t*)&s_v[step & 1][unit / 4 * 4 + k][l][unit % 4 * 16 + (lane & 15)])[grp] = p[l];
-            }
-        }
-        if (is_wide(seen) && lane == 0) s_wide[step & 1] = (int32_t)step + 1;
-    };
+    load_raw(0);
+    const double total = row_sum(s, tile, chunks_of(s, r), lane & 15, 16, valid), scale = valid ? 65536.0 / total : 0.0;
+    s_total[wave][lane & 15] = valid ? total : 0.0;
+    // And of its weights: key tiles block * KT ..
     const uint4* t = s.scores + (tile * s.chunks + chunk) * (s.chunk / 16) * 64 + lane;
-    uint4 terms[4];
+    uint4 terms[KT];
     auto load_terms = [&](uint32_t step) __attribute__((always_inline)) {
 #pragma unroll
-        for (uint32_t k = 0; k < 4; k++) terms[k] = t[min(step * 4 + k, kt1 - 1) * 64];
+        for (uint32_t k = 0; k < KT; k++) terms[k] = t[min(step * 4 + block * KT + k, kt1 - 1) * 64];
     };
-    v4i acc[TILES][NARROW + 1];
+    load_terms(0);
+    v4i acc[4][NARROW + 1];
 #pragma unroll
-    for (uint32_t k = 0; k < TILES; k++)
+    for (int k = 0; k < 4; k++)
 #pragma unroll
         for (int j = 0; j < NARROW + 1; j++) acc[k][j] = v4i{0, 0, 0, 0};
     int32_t wsum = 0;
-    uint64_t* out = s.partial + (tile * s.chunks + chunk) * 16 * HD + dim0;
-    bool added = false;  // the lane's own sums in `out` hold upper digits' products
-    load_raw(0);
-    load_terms(0);
+    uint64_t* out = s.partial + (tile * s.chunks + chunk) * 16 * HD + split_d;
 #pragma unroll 1
     for (uint32_t step = 0; step < steps; step++) {
-        split_raw(step);
-        if (step + 1 < steps) load_raw(step + 1);
-        v4i w0 = v4i{0, 0, 0, 0}, w1 = v4i{0, 0, 0, 0};
-        if (has_rt) {
+        const uint32_t buf = step & 1;
+        uint32_t seen = 0;
 #pragma unroll
-            for (uint32_t k = 0; k < 4; k++) {
-                const uint32_t kt = step * 4 + k;
-                const bool live = valid && kt < kt1;
-                const uint4 x = terms[k];
-                const uint32_t e[4] = {live ? x.x : 0, live ? x.y : 0, live ? x.z : 0, live ? x.w : 0};
-                int32_t w[4];
-                weights_of(e, sc.sum, sc.w, sc.q, w, wsum,
-                           [&](int j) { s_big[wave].add(lane & 15, key0 + kt * 16 + 4 * grp + j); });
-                uint32_t low, high;
-                weight_digits(w, low, high);
-                w0[k] = (int)low, w1[k] = (int)high;
-            }
-            if (step + 1 < steps) load_terms(step + 1);
+        for (int k = 0; k < 4; k++) {
+            uint32_t p[4];
+            split4(column(raw, k), p, seen);
+#pragma unroll
+            for (int l = 0; l < NARROW; l++) ((uint32_t*)&s_v[buf][block * 4 + k][l][my * 16 + (lane & 15)])[grp] = p[l];
         }
+        if (is_wide(seen) && lane == 0) atomicOr(&s_wide, 1u << step);
+        load_raw(min(step + 1, steps - 1));
+#pragma unroll
+        for (uint32_t k = 0; k < KT; k++) {
+            const uint32_t kt = step * 4 + block * KT + k;
+            const uint4 x = terms[k];
+            const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+            const double w_scale = kt < kt1 ? scale : 0.0;
+            int32_t w[4];
+            bool open[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) w[i] = estimate(e[i], w_scale, open[i]);
+            if (__any(open[0] | open[1] | open[2] | open[3])) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (open[i]) s_open[my].push(lane & 15, kt * 16 + 4 * grp + i);
+            }
+            wsum += w[0] + w[1] + w[2] + w[3];
+            uint32_t low, high;
+            weight_digits(w, low, high);
+            ((uint32_t*)&s_w[buf][my][0][lane])[block * KT + k] = low;
+            ((uint32_t*)&s_w[buf][my][1][lane])[block * KT + k] = high;
+        }
+        load_terms(min(step + 1, steps - 1));
         lds_barrier();
         if (!has_rt) continue;
+        const uint4 x0 = s_w[buf][my][0][lane], x1 = s_w[buf][my][1][lane];
+        const v4i w0 = v4i{(int)x0.x, (int)x0.y, (int)x0.z, (int)x0.w}, w1 = v4i{(int)x1.x, (int)x1.y, (int)x1.z, (int)x1.w};
 #pragma unroll
-        for (uint32_t k = 0; k < TILES; k++) {
+        for (int k = 0; k < 4; k++) {
             v4i f[NARROW];
 #pragma unroll
-            for (int l = 0; l < NARROW; l++) f[l] = s_v[step & 1][k][l][lane];
+            for (int l = 0; l < NARROW; l++) f[l] = s_v[buf][block * 4 + k][l][lane];
             value_step<NARROW>(w0, w1, f, acc[k]);
         }
-        if (s_wide[step & 1] == (int32_t)step + 1) {
-            // Every (row, dimension) is one lane's own: it adds to its sums.
-#pragma unroll 1
-            for (uint32_t k = 0; k < TILES; k++) {
-                const uint32_t d = dim0 + k / 4 * 64 + 4 * (lane & 15) + k % 4;
-                int4 x[4];
-#pragma unroll
-                for (uint32_t i = 0; i < 4; i++) {
-                    int32_t y[4];
-#pragma unroll
-                    for (uint32_t j = 0; j < 4; j++)
-                        y[j] = load1(at.at(at.v, key0 + step * STEP + 4 * grp + 16 * i + j) + (d < at.hd ? d : 0));
-                    x[i] = make_int4(y[0], y[1], y[2], y[3]);
-                }
-                uint64_t more[4];
-                upper_values(w0, w1, x, more);
-#pragma unroll
-                for (uint32_t q = 0; q < 4; q++) {
-                    uint64_t* to = out + (size_t)(4 * grp + q) * HD + (d - dim0);
-                    *to = added ? *to + more[q] : more[q];
-                }
-            }
-            added = true;
-        }
     }
-    if (!has_rt) return;
-    wsum += __shfl_xor(wsum, 16);
-    wsum += __shfl_xor(wsum, 32);
-    if (lane < 16 && valid && dim0 == 0) s.weights[(tile * s.chunks + chunk) * 16 + lane] = wsum;
-    // The wave's own large weights: its LDS accesses are in order.
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-    for (uint32_t b = 0; b < BLOCKS; b++) {
-        const uint32_t d = dim0 + b * 64 + 4 * (lane & 15);
+    // The sums so far; every (row, dimension) is one lane's own, which adds
+    // what follows to its own entries.
+    if (has_rt)
 #pragma unroll
         for (uint32_t q = 0; q < 4; q++) {
-            const uint32_t i = 4 * grp + q;
-            if (rt * 16 + i >= pairs) continue;
-            uint64_t* to = out + (size_t)i * HD + (d - dim0);
             uint64_t sum[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                sum[k] = added ? to[k] : 0;
+                sum[k] = 0;
 #pragma unroll
-                for (int j = 0; j < NARROW + 1; j++) sum[k] += (uint64_t)(int64_t)acc[b * 4 + k][j][q] << (8 * j);
+                for (int j = 0; j < NARROW + 1; j++) sum[k] += (uint64_t)(int64_t)acc[k][j][q] << (8 * j);
             }
-            for (int j = 0; j < s_big[wave].count[i]; j++) {
-                const int4 x = load4(at.at(at.v, s_big[wave].key[i][j]) + (d < at.hd ? d : 0));
-                sum[0] += (uint64_t)((int64_t)65536 * x.x), sum[1] += (uint64_t)((int64_t)65536 * x.y);
-                sum[2] += (uint64_t)((int64_t)65536 * x.z), sum[3] += (uint64_t)((int64_t)65536 * x.w);
-            }
+            if (rt * 16 + 4 * grp + q >= pairs) continue;
+            uint64_t* to = out + (size_t)(4 * grp + q) * HD;
             *(ulonglong2*)to = make_ulonglong2(sum[0], sum[1]);
             *(ulonglong2*)(to + 2) = make_ulonglong2(sum[2], sum[3]);
+        }
+    wsum += __shfl_xor(wsum, 16);
+    wsum += __shfl_xor(wsum, 32);
+    if (lane < 16) atomicAdd(&s_wsum[my][lane], wsum);
+    __syncthreads();
+
+    // The open weights: what the loop's lack, a lane each (of the tile's first
+    // wave), or of every position.
+    const int32_t* terms0 = (const int32_t*)(s.scores + (tile * s.chunks + chunk) * (s.chunk / 16) * 64);
+    auto lacking = [&](uint32_t i, uint32_t position, int32_t& off) __attribute__((always_inline)) {
+        const uint32_t kept = (uint32_t)load1(terms0 + ((position / 16 * 64 + position % 16 / 4 * 16 + i) * 4 + position % 4));
+        const double sum = s_total[wave][i];
+        bool open;
+        const int32_t n = estimate(kept, 65536.0 / sum, open), w = open ? exact_weight(kept, sum) : n;
+        off = w - n;
+        return w - two_digits(n);
+    };
+    const uint32_t open_count = s_open[my].count;
+    const bool listed = open_count <= OpenWeights::ROOM;
+    if (has_rt && block == 0) {
+        if (listed) {
+            if (lane < open_count) {
+                const uint32_t x = s_open[my].at[lane];
+                int32_t off;
+                s_open[my].add[lane] = lacking(x & 15, x >> 4, off);
+                if (off) atomicAdd(&s_wsum[my][x & 15], off);
+            }
+        } else if (valid) {
+            int32_t all = 0;
+#pragma unroll 1
+            for (uint32_t k = grp; k < n; k += 4) {
+                int32_t off;
+                lacking(lane & 15, k, off);
+                all += off;
+            }
+            atomicAdd(&s_wsum[my][lane & 15], all);
+        }
+    }
+    __syncthreads();
+    if (!has_rt) return;
+    if (block == 0 && lane < 16 && valid && dim0 == 0) s.weights[(tile * s.chunks + chunk) * 16 + lane] = s_wsum[my][lane];
+#pragma unroll 1
+    for (uint32_t q = 0; q < 4; q++) {
+        const uint32_t i = 4 * grp + q;
+        if (rt * 16 + i >= pairs) continue;
+        uint64_t* to = out + (size_t)i * HD;
+#pragma unroll 1
+        for (uint32_t j = 0; j < (listed ? open_count : n); j++) {
+            uint32_t position = j;
+            int32_t more, off;
+            if (listed) {
+                if ((s_open[my].at[j] & 15) != i) continue;
+                position = s_open[my].at[j] >> 4, more = s_open[my].add[j];
+            } else {
+                more = lacking(i, j, off);
+            }
+            if (!more) continue;
+            const int4 x = load4(at.at(at.v, key0 + position) + (split_d < at.hd ? split_d : 0));
+            to[0] += (uint64_t)((int64_t)more * x.x), to[1] += (uint64_t)((int64_t)more * x.y);
+            to[2] += (uint64_t)((int64_t)more * x.z), to[3] += (uint64_t)((int64_t)more * x.w);
+        }
+    }
+    // Values of more digits: their steps' weights formed again, the upper
+    // planes' products added.
+    const uint32_t wide = s_wide;
+#pragma unroll 1
+    for (uint32_t step = 0; step < steps; step++) {
+        if (!((wide >> step) & 1)) continue;
+        v4i w0, w1;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) {
+            const uint4 x = t[min(step * 4 + k, kt1 - 1) * 64];
+            const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+            int32_t w[4];
+            bool open;
+#pragma unroll
+            for (int i = 0; i < 4; i++) w[i] = estimate(e[i], step * 4 + k < kt1 ? scale : 0.0, open);
+            uint32_t low, high;
+            weight_digits(w, low, high);
+            w0[k] = (int)low, w1[k] = (int)high;
+        }
+#pragma unroll 1
+        for (int k = 0; k < 4; k++) {
+            int4 x[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+                const int32_t* p = at.four(at.v, key0 + step * STEP + 4 * grp + 16 * i) + (split_d < at.hd ? split_d + k : 0);
+                x[i] = make_int4(load1(p), load1(p + at.hd), load1(p + 2 * at.hd), load1(p + 3 * at.hd));
+            }
+            uint64_t more[4];
+            upper_values(w0, w1, x, more);
+#pragma unroll
+            for (uint32_t q = 0; q < 4; q++)
+                if (rt * 16 + 4 * grp + q < pairs) out[(size_t)(4 * grp + q) * HD + k] += more[q];
         }
     }
 }
 
-// ---- (4) the chunks joined: a workgroup per (drafted row, head)
+// ---- (4) the chunks joined: a wave per (drafted row, head), or four that
+// share the chunks where there are many (SPLIT)
 
-__global__ __launch_bounds__(256) void tree_join_kernel(const IrisPagedKv c, const IrisTreeAttention a, const TreeSpace s,
-                                                        uint32_t hd_padded) {
-    __shared__ uint64_t s_part[256];
-    const uint32_t tid = threadIdx.x, lane = tid & 63, bg = blockIdx.y, g = bg % c.kv_heads, group = a.heads / c.kv_heads;
-    const uint32_t pair = blockIdx.x;
+template <uint32_t HD, bool SPLIT>
+__global__ __launch_bounds__(256) void tree_join_kernel(const IrisPagedKv c, const IrisTreeAttention a, const TreeSpace s) {
+    constexpr uint32_t PIECES = HD > 128 ? HD / 128 : 1, PARTS = SPLIT ? 4 : 1;
+    __shared__ uint64_t s_part[SPLIT ? 4 : 1][SPLIT ? HD : 1];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = wave_index();
+    const uint32_t bg = blockIdx.x, g = bg % c.kv_heads, group = a.heads / c.kv_heads;
+    const uint32_t pair = SPLIT ? blockIdx.y : blockIdx.y * 4 + wave, part = SPLIT ? wave : 0;
     Request r;
     if (!read_request(c, a, bg / c.kv_heads, r)) return;
     if (pair >= r.rows * group) return;
     const size_t tile = (size_t)bg * s.row_tiles + pair / 16;
     const uint32_t i = pair % 16, chunks = chunks_of(s, r);
+    // Two dimensions per lane (HD 64: a half of the lanes has them).
+    uint64_t t[PIECES][2];
+#pragma unroll
+    for (uint32_t p = 0; p < PIECES; p++) t[p][0] = t[p][1] = 0;
+    const uint64_t* from = s.partial + (tile * s.chunks * 16 + i) * HD + (2 * lane) % HD;
+#pragma unroll 4
+    for (uint32_t k = part; k < chunks; k += PARTS)
+#pragma unroll
+        for (uint32_t p = 0; p < PIECES; p++) {
+            const ulonglong2 x = *(const ulonglong2*)(from + (size_t)k * 16 * HD + p * 128);
+            t[p][0] += x.x, t[p][1] += x.y;
+        }
     uint32_t key = 0xffffffffu;
     int32_t wsum = 0;
     for (uint32_t k = lane; k < chunks; k += 64) {
@@ -715,25 +814,29 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const IrisPagedKv c, con
         key = min(key, (uint32_t)__shfl_xor((int)key, off));
         wsum += __shfl_xor(wsum, off);
     }
+    if constexpr (SPLIT) {
+#pragma unroll
+        for (uint32_t p = 0; p < PIECES; p++)
+            if (2 * lane < HD) s_part[wave][p * 128 + 2 * lane] = t[p][0], s_part[wave][p * 128 + 2 * lane + 1] = t[p][1];
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (uint32_t p = 0; p < PIECES; p++)
+#pragma unroll
+            for (uint32_t w = 1; w < 4; w++)
+                t[p][0] += s_part[w][p * 128 + (2 * lane) % HD], t[p][1] += s_part[w][p * 128 + (2 * lane) % HD + 1];
+    }
     const int64_t resid = dn::sub_sat(dn::ONE_ACT, wsum);
     const uint32_t log = 31u - __clz((int)c.page_size), page = (uint32_t)r.table[key >> log];
     const int32_t* v = page < c.pages ? c.v + (((size_t)page * c.kv_heads + g) * c.page_size + (key & (c.page_size - 1))) * c.head_dim
                                       : g_zeros;
     int32_t* out = a.out + (size_t)(r.row0 + pair / group) * a.out_stride + (size_t)(g * group + pair % group) * c.head_dim;
-    // Up to 256 dimensions at a time, the chunks dealt to what threads are left.
-    const uint32_t width = min(hd_padded, 256u), parts = 256 / width, part = tid / width;
-    for (uint32_t d0 = 0; d0 < c.head_dim; d0 += width) {
-        const uint32_t d = d0 + tid % width;
-        uint64_t t = 0;
-#pragma unroll 4
-        for (uint32_t k = part; k < chunks; k += parts) t += s.partial[((tile * s.chunks + k) * 16 + i) * hd_padded + d];
-        s_part[tid] = t;
-        __syncthreads();
-        if (tid < width && d < c.head_dim) {
-            for (uint32_t p = 1; p < parts; p++) t += s_part[p * width + tid];
-            out[d] = dn::requantize((int64_t)(t + (uint64_t)(resid * v[d])));
-        }
-        __syncthreads();
+#pragma unroll
+    for (uint32_t p = 0; p < PIECES; p++) {
+        const uint32_t d = p * 128 + 2 * lane;
+        if (2 * lane < HD && d < c.head_dim)
+            *(int2*)(out + d) = make_int2(dn::requantize((int64_t)(t[p][0] + (uint64_t)(resid * load1(v + d)))),
+                                          dn::requantize((int64_t)(t[p][1] + (uint64_t)(resid * load1(v + d + 1)))));
     }
 }
 
@@ -781,21 +884,28 @@ uint64_t tree_space(const IrisPagedKv& c, const IrisTreeAttention& a, uint8_t* b
     return at;
 }
 
+// Workgroups of one chunk follow each other request by request: consecutive
+// ones go to the chiplets in turn, and how many chunks a request has is its own
+// (with the chunks in front, one chiplet had every request's first chunk: the
+// values of 32 trees at up to 8000 took twice the time).
 template <uint32_t HD, bool FULL>
 int tree_launch(const IrisPagedKv& c, const IrisTreeAttention& a, const TreeSpace& s, hipStream_t stream) {
     const uint32_t bg = a.requests * c.kv_heads, RB = row_block(HD), few = std::min(s.row_tiles, RB);
     const size_t q_lds = (size_t)few * (HD / 64) * NARROW * TILE_BYTES, v_lds = 16 * HD * 8 + (size_t)s.chunk / STEP * 2 * TILE_BYTES;
     hipError_t st = paged_lds_limit((const void*)tree_values_kernel<HD, FULL>, v_lds);
     if (st != hipSuccess) return (int)st;
-    hipLaunchKernelGGL((tree_scores_kernel<HD, FULL>), dim3(s.chunks, (s.row_tiles + RB - 1) / RB, bg), dim3(256), q_lds, stream, c,
+    hipLaunchKernelGGL((tree_scores_kernel<HD, FULL>), dim3(bg, s.chunks, (s.row_tiles + RB - 1) / RB), dim3(256), q_lds, stream, c,
                        a, s);
-    hipLaunchKernelGGL(tree_terms_kernel, dim3(s.chunks, s.row_tiles, bg), dim3(256), 0, stream, c, a, s);
+    hipLaunchKernelGGL(tree_terms_kernel, dim3(bg, s.chunks, s.row_tiles), dim3(256), 0, stream, c, a, s);
     if (s.row_tiles == 1)
-        hipLaunchKernelGGL((tree_values_kernel<HD, FULL>), dim3(s.chunks, 1, bg), dim3(HD > 256 ? HD : 256), v_lds, stream, c, a, s);
+        hipLaunchKernelGGL((tree_values_kernel<HD, FULL>), dim3(bg, s.chunks), dim3(HD > 256 ? HD : 256), v_lds, stream, c, a, s);
     else
-        hipLaunchKernelGGL((tree_values_many_kernel<HD, 8, FULL>), dim3(s.chunks, (s.row_tiles + 7) / 8 * (HD / value_dims(HD)), bg),
-                           dim3(512), 0, stream, c, a, s);
-    hipLaunchKernelGGL(tree_join_kernel, dim3(a.max_nodes * (a.heads / c.kv_heads), bg), dim3(256), 0, stream, c, a, s, HD);
+        hipLaunchKernelGGL((tree_values_many_kernel<HD, FULL>),
+                           dim3(bg, s.chunks, (s.row_tiles + MANY - 1) / MANY * (HD / (64 * value_blocks(HD)))),
+                           dim3(MANY * value_blocks(HD) * 64), 0, stream, c, a, s);
+    const uint32_t pairs = a.max_nodes * (a.heads / c.kv_heads);
+    if (s.chunks > 8) hipLaunchKernelGGL((tree_join_kernel<HD, true>), dim3(bg, pairs), dim3(256), 0, stream, c, a, s);
+    else hipLaunchKernelGGL((tree_join_kernel<HD, false>), dim3(bg, (pairs + 3) / 4), dim3(256), 0, stream, c, a, s);
     return (int)hipGetLastError();
 }
 
