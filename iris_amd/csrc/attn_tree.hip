@@ -173,7 +173,7 @@ __global__ __launch_bounds__(256, HD >= 512 ? 1 : HD >= 256 ? 2 : 3) void tree_s
     __shared__ uint64_t s_page[CHUNK_PAGES];
     __shared__ int32_t s_wide;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = wave_index(), grp = lane >> 4;
-    const uint32_t chunk = blockIdx.y, rt0 = blockIdx.z * RB, bg = blockIdx.x, g = bg % c.kv_heads;
+    const uint32_t chunk = blockIdx.x, rt0 = blockIdx.z * RB, bg = blockIdx.y, g = bg % c.kv_heads;
     const uint32_t group = a.heads / c.kv_heads;
     Request r;
     if (!read_request(c, a, bg / c.kv_heads, r)) return;
@@ -316,7 +316,7 @@ __global__ __launch_bounds__(256) void tree_terms_kernel(const IrisPagedKv c, co
     __shared__ double s_sum[4][16];
     __shared__ uint32_t s_first[4][16];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = wave_index(), grp = lane >> 4;
-    const uint32_t chunk = blockIdx.y, rt = blockIdx.z, bg = blockIdx.x, group = a.heads / c.kv_heads;
+    const uint32_t chunk = blockIdx.x, rt = blockIdx.z, bg = blockIdx.y, group = a.heads / c.kv_heads;
     Request r;
     if (!read_request(c, a, bg / c.kv_heads, r)) return;
     const uint32_t key0 = r.base + chunk * s.chunk, pairs = r.rows * group;
@@ -431,7 +431,7 @@ __global__ __launch_bounds__((HD / 64 > 4 ? HD : 256), 2) void tree_values_kerne
     __shared__ uint64_t s_page[CHUNK_PAGES];
     uint4* s_w = (uint4*)(s_sums + 16 * HD);
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = wave_index(), grp = lane >> 4;
-    const uint32_t chunk = blockIdx.y, bg = blockIdx.x, g = bg % c.kv_heads, group = a.heads / c.kv_heads;
+    const uint32_t chunk = blockIdx.x, bg = blockIdx.y, g = bg % c.kv_heads, group = a.heads / c.kv_heads;
     Request r;
     if (!read_request(c, a, bg / c.kv_heads, r)) return;
     const uint32_t key0 = r.base + chunk * s.chunk, rows = r.rows * group;
@@ -573,7 +573,7 @@ __global__ __launch_bounds__(MANY * value_blocks(HD) * 64, 4) void tree_values_m
     __shared__ double s_total[WAVES][16];
     __shared__ uint64_t s_page[CHUNK_PAGES];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = wave_index(), grp = lane >> 4;
-    const uint32_t chunk = blockIdx.y, bg = blockIdx.x, g = bg % c.kv_heads, group = a.heads / c.kv_heads;
+    const uint32_t chunk = blockIdx.x, bg = blockIdx.y, g = bg % c.kv_heads, group = a.heads / c.kv_heads;
     const uint32_t dim0 = blockIdx.z % (HD / VD) * VD, rt0 = blockIdx.z / (HD / VD) * MANY;
     Request r;
     if (!read_request(c, a, bg / c.kv_heads, r)) return;
@@ -894,14 +894,14 @@ int tree_launch(const IrisPagedKv& c, const IrisTreeAttention& a, const TreeSpac
     const size_t q_lds = (size_t)few * (HD / 64) * NARROW * TILE_BYTES, v_lds = 16 * HD * 8 + (size_t)s.chunk / STEP * 2 * TILE_BYTES;
     hipError_t st = paged_lds_limit((const void*)tree_values_kernel<HD, FULL>, v_lds);
     if (st != hipSuccess) return (int)st;
-    hipLaunchKernelGGL((tree_scores_kernel<HD, FULL>), dim3(bg, s.chunks, (s.row_tiles + RB - 1) / RB), dim3(256), q_lds, stream, c,
+    hipLaunchKernelGGL((tree_scores_kernel<HD, FULL>), dim3(s.chunks | 1, bg, (s.row_tiles + RB - 1) / RB), dim3(256), q_lds, stream, c,
                        a, s);
-    hipLaunchKernelGGL(tree_terms_kernel, dim3(bg, s.chunks, s.row_tiles), dim3(256), 0, stream, c, a, s);
+    hipLaunchKernelGGL(tree_terms_kernel, dim3(s.chunks | 1, bg, s.row_tiles), dim3(256), 0, stream, c, a, s);
     if (s.row_tiles == 1)
-        hipLaunchKernelGGL((tree_values_kernel<HD, FULL>), dim3(bg, s.chunks), dim3(HD > 256 ? HD : 256), v_lds, stream, c, a, s);
+        hipLaunchKernelGGL((tree_values_kernel<HD, FULL>), dim3(s.chunks | 1, bg), dim3(HD > 256 ? HD : 256), v_lds, stream, c, a, s);
     else
         hipLaunchKernelGGL((tree_values_many_kernel<HD, FULL>),
-                           dim3(bg, s.chunks, (s.row_tiles + MANY - 1) / MANY * (HD / (64 * value_blocks(HD)))),
+                           dim3(s.chunks | 1, bg, (s.row_tiles + MANY - 1) / MANY * (HD / (64 * value_blocks(HD)))),
                            dim3(MANY * value_blocks(HD) * 64), 0, stream, c, a, s);
     const uint32_t pairs = a.max_nodes * (a.heads / c.kv_heads);
     if (s.chunks > 8) hipLaunchKernelGGL((tree_join_kernel<HD, true>), dim3(bg, pairs), dim3(256), 0, stream, c, a, s);
