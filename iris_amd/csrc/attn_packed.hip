@@ -178,10 +178,9 @@ __global__ __launch_bounds__(256) void packed_planes_kernel(const IrisPackedAtte
 template <int NW>
 struct PackedSmem {
     int32_t best[NW][16];
-    uint32_t best_key[NW][16];
     double sum[NW][16], total[16];
+    uint32_t first[16];
     int32_t wsum[16], nbig[16], big[16][2];
-    int32_t wide_scores, wide_values;
 };
 
 // The parts of the keys that the waves of one dimension tile share.
@@ -194,7 +193,7 @@ template <uint32_t HD, int NW, bool SPILL>
 __device__ __forceinline__ void packed_rows(const IrisPackedAttention& a, const PackedSpace& s, uint32_t qt, uint32_t h,
                                             uint4* tiles, uint4* spill, PackedSmem<NW>& sm) {
     constexpr uint32_t DS = HD / 64, DT = HD / 16, PARTS = key_parts<HD, NW>(), DTW = DT * PARTS / NW;
-    constexpr bool HOLD = HD <= 128;  // the queries' operands stay in registers
+    constexpr bool HOLD = HD <= 256;  // the queries' operands stay in registers
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = wave_index(), grp = lane >> 4;
     const uint32_t g = h / (a.heads / a.kv_heads);
 
@@ -202,130 +201,178 @@ __device__ __forceinline__ void packed_rows(const IrisPackedAttention& a, const 
     const uint32_t row = qt * 16 + (lane & 15);
     const int32_t first = row < a.rows ? s.first[row] : -1;
     const bool valid = first >= 0;
-    uint32_t lo = valid ? (uint32_t)first : 0xffffffffu;
+    uint32_t lo = valid ? (uint32_t)first : 0xffffffffu, all0 = valid ? (uint32_t)first : 0;
     int32_t hi = valid ? (int32_t)row : -1;
+    uint32_t all1 = valid ? row : 0xffffffffu;
 #pragma unroll
     for (int off = 1; off < 16; off <<= 1) {
         lo = min(lo, (uint32_t)__shfl_xor((int)lo, off));
         hi = max(hi, __shfl_xor(hi, off));
+        all0 = max(all0, (uint32_t)__shfl_xor((int)all0, off));
+        all1 = min(all1, (uint32_t)__shfl_xor((int)all1, off));
     }
-    if (hi < 0) return;  // uniform: no row is computed
+    // The same in every lane: scalars from here on. Every row sees the keys
+    // [all0, all1].
+    lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)lo);
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    all0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)all0);
+    all1 = (uint32_t)__builtin_amdgcn_readfirstlane((int)all1);
+    if (hi < 0) return;  // no row is computed
     const uint32_t span = valid ? row - (uint32_t)first : 0;
     auto sees = [&](uint32_t key) { return valid & (key - (uint32_t)first <= span); };
     // Tiles [ta, tb) hold keys that are seen; steps are whole.
     const uint32_t ks0 = lo / 64, ks1 = (uint32_t)hi / 64 + 1, base = ks0 * 4, ta = lo / 16, tb = (uint32_t)hi / 16 + 1;
-    auto tile = [&](uint32_t kt) -> uint4* {
-        const uint32_t i = kt - base;
-        if (SPILL && i >= s.lds_tiles) return spill + (size_t)(i - s.lds_tiles) * 64;
-        return tiles + i * 64;
+    // A tile's place: in LDS, or past it in the work space. (Two kinds of
+    // access: a pointer to either would make all of them flat ones.)
+    auto spilled = [&](uint32_t kt) { return SPILL && kt - base >= s.lds_tiles; };
+    auto in_lds = [&](uint32_t kt) { return tiles + (kt - base) * 64; };
+    typedef __attribute__((address_space(1))) v4i global_v4i;
+    typedef __attribute__((address_space(1))) uint32_t global_u32;
+    auto in_space = [&](uint32_t kt) { return spill + (size_t)(kt - base - s.lds_tiles) * 64; };
+    auto put = [&](uint32_t kt, uint32_t x, uint32_t y, uint32_t z, uint32_t w) __attribute__((always_inline)) {
+        if (spilled(kt)) *(global_v4i*)(in_space(kt) + lane) = v4i{(int)x, (int)y, (int)z, (int)w};
+        else in_lds(kt)[lane] = make_uint4(x, y, z, w);
     };
-
-    if (tid == 0) sm.wide_scores = s.q_wide[(size_t)h * s.q_tiles + qt], sm.wide_values = 0;
-    if (tid < 16) sm.wsum[tid] = 0, sm.nbig[tid] = 0;
-    __syncthreads();
-    {
-        const uint8_t* kw = s.k_wide + (size_t)g * s.steps * 4;
-        for (uint32_t i = ta + tid; i < tb; i += NW * 64)
-            if (kw[i]) sm.wide_scores = 1;
-        const uint8_t* vw = s.v_wide + (size_t)g * s.steps * DS;
-        for (uint32_t i = ks0 * DS + tid; i < ks1 * DS; i += NW * 64)
-            if (vw[i]) sm.wide_values = 1;
-    }
-    __syncthreads();
-    const bool wide_scores = sm.wide_scores, wide_values = sm.wide_values;
-
-    // (1) scores and the first maximum; a lane's keys run in increasing order.
-    const int8_t* qb = s.q + ((size_t)h * s.q_tiles + qt) * DS * TILE_BYTES + lane * 16;
-    const int8_t* kb = s.k + (size_t)g * s.steps * 4 * DS * TILE_BYTES + lane * 16;
-    int32_t best = INT32_MIN;
-    uint32_t best_key = 0xffffffffu;
-    auto keep = [&](uint32_t kt, const int32_t (&sc)[4]) {
-        tile(kt)[lane] = make_uint4((uint32_t)sc[0], (uint32_t)sc[1], (uint32_t)sc[2], (uint32_t)sc[3]);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t key = kt * 16 + 4 * grp + i;
-            const bool take = sees(key) & ((sc[i] > best) | (best_key == 0xffffffffu));
-            best = take ? sc[i] : best;
-            best_key = take ? key : best_key;
+    auto get = [&](uint32_t kt, uint32_t (&v)[4]) __attribute__((always_inline)) {
+        if (spilled(kt)) {
+            const v4i x = *(const global_v4i*)(in_space(kt) + lane);
+            v[0] = (uint32_t)x[0], v[1] = (uint32_t)x[1], v[2] = (uint32_t)x[2], v[3] = (uint32_t)x[3];
+        } else {
+            const uint4 x = in_lds(kt)[lane];
+            v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
         }
     };
-    if (!wide_scores) {
-        v4i qf[HOLD ? DS : 1][NARROW];
-        if constexpr (HOLD)
+
+    if (tid < 16) sm.wsum[tid] = 0, sm.nbig[tid] = 0, sm.first[tid] = 0xffffffffu;
+
+    // (1) scores and the maxima.
+    const int8_t* qb = s.q + ((size_t)h * s.q_tiles + qt) * DS * TILE_BYTES + lane * 16;
+    const int8_t* kb = s.k + (size_t)g * s.steps * 4 * DS * TILE_BYTES + lane * 16;
+    v4i qf[HOLD ? DS : 1][NARROW];
+    if constexpr (HOLD)
 #pragma unroll
-            for (uint32_t ds = 0; ds < DS; ds++)
+        for (uint32_t ds = 0; ds < DS; ds++)
 #pragma unroll
-                for (int l = 0; l < NARROW; l++) qf[ds][l] = *(const v4i*)(qb + l * s.q_plane + ds * TILE_BYTES);
+            for (int l = 0; l < NARROW; l++) qf[ds][l] = *(const v4i*)(qb + l * s.q_plane + ds * TILE_BYTES);
+    auto whole = [&](uint32_t kt) { return kt * 16 >= all0 && kt * 16 + 15 <= all1; };
+    int32_t best = INT32_MIN;
+    auto keep = [&](uint32_t kt, const int32_t (&sc)[4]) __attribute__((always_inline)) {
+        put(kt, (uint32_t)sc[0], (uint32_t)sc[1], (uint32_t)sc[2], (uint32_t)sc[3]);
+        if (whole(kt)) {
+            best = max(max(best, sc[0]), max(sc[1], max(sc[2], sc[3])));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) best = sees(kt * 16 + 4 * grp + i) ? max(best, sc[i]) : best;
+        }
+    };
+    {
+        // The next tile's keys are loaded during this one's products, where
+        // the registers allow. (Past the last: it again.)
+        constexpr bool AHEAD = HD <= 128;
+        const uint8_t* kw = s.k_wide + (size_t)g * s.steps * 4;
+        const uint32_t q_wide = s.q_wide[(size_t)h * s.q_tiles + qt];
+        uint32_t any_wide = 0;
+        v4i kf[AHEAD ? DS : 1][NARROW];
+        uint32_t k_wide = 0;
+        auto load_keys = [&](uint32_t kt) __attribute__((always_inline)) {
+            k_wide = kw[kt];
+            if constexpr (AHEAD)
+#pragma unroll
+                for (uint32_t ds = 0; ds < DS; ds++)
+#pragma unroll
+                    for (int l = 0; l < NARROW; l++) kf[ds][l] = *(const v4i*)(kb + l * s.kv_plane + ((size_t)kt * DS + ds) * TILE_BYTES);
+        };
+        load_keys(min(ta + wave, tb - 1));
 #pragma unroll 1
         for (uint32_t kt = ta + wave; kt < tb; kt += NW) {
+            const uint32_t wide = (uint32_t)__builtin_amdgcn_readfirstlane((int)(k_wide | q_wide));
+            if (wide) {  // tiles of more digits: below
+                any_wide = 1;
+                load_keys(min(kt + NW, tb - 1));
+                continue;
+            }
             v4i acc[2 * NARROW - 1];
 #pragma unroll
             for (int j = 0; j < 2 * NARROW - 1; j++) acc[j] = v4i{0, 0, 0, 0};
 #pragma unroll
             for (uint32_t ds = 0; ds < DS; ds++) {
-                v4i kf[NARROW];
+                if constexpr (AHEAD) {
+                    dot_step<NARROW>(kf[ds], qf[ds], acc);
+                } else {
+                    v4i k[NARROW], q[NARROW];
 #pragma unroll
-                for (int l = 0; l < NARROW; l++) {
-                    kf[l] = *(const v4i*)(kb + l * s.kv_plane + ((size_t)kt * DS + ds) * TILE_BYTES);
-                    if constexpr (!HOLD) qf[0][l] = *(const v4i*)(qb + l * s.q_plane + ds * TILE_BYTES);
+                    for (int l = 0; l < NARROW; l++) {
+                        k[l] = *(const v4i*)(kb + l * s.kv_plane + ((size_t)kt * DS + ds) * TILE_BYTES);
+                        q[l] = HOLD ? qf[HOLD ? ds : 0][l] : *(const v4i*)(qb + l * s.q_plane + ds * TILE_BYTES);
+                    }
+                    dot_step<NARROW>(k, q, acc);
                 }
-                dot_step<NARROW>(kf, qf[HOLD ? ds : 0], acc);
             }
+            load_keys(min(kt + NW, tb - 1));
             int32_t sc[4];
             scores_of<HD, NARROW>(acc, a.scaled, a.scale_q32, sc);
             keep(kt, sc);
         }
-    } else {
+        if (any_wide)
 #pragma unroll 1
-        for (uint32_t kt = ta + wave; kt < tb; kt += NW) {
-            // A narrow tile's upper planes were not written: its digits there
-            // are zero.
-            const bool kw = s.k_wide[(size_t)g * s.steps * 4 + kt], qw = s.q_wide[(size_t)h * s.q_tiles + qt];
-            v4i acc[2 * DIGITS - 1];
+            for (uint32_t kt = ta + wave; kt < tb; kt += NW) {
+                // A narrow tile's upper planes were not written: its digits
+                // there are zero.
+                const uint32_t kwide = kw[kt];
+                if (!(kwide | q_wide)) continue;
+                v4i acc[2 * DIGITS - 1];
 #pragma unroll
-            for (int j = 0; j < 2 * DIGITS - 1; j++) acc[j] = v4i{0, 0, 0, 0};
+                for (int j = 0; j < 2 * DIGITS - 1; j++) acc[j] = v4i{0, 0, 0, 0};
 #pragma unroll 1
-            for (uint32_t ds = 0; ds < DS; ds++) {
-                v4i kf[DIGITS], qf[DIGITS];
+                for (uint32_t ds = 0; ds < DS; ds++) {
+                    v4i k[DIGITS], q[DIGITS];
 #pragma unroll
-                for (int l = 0; l < DIGITS; l++) {
-                    kf[l] = qf[l] = v4i{0, 0, 0, 0};
-                    if (l < NARROW || kw) kf[l] = *(const v4i*)(kb + l * s.kv_plane + ((size_t)kt * DS + ds) * TILE_BYTES);
-                    if (l < NARROW || qw) qf[l] = *(const v4i*)(qb + l * s.q_plane + ds * TILE_BYTES);
+                    for (int l = 0; l < DIGITS; l++) {
+                        k[l] = q[l] = v4i{0, 0, 0, 0};
+                        if (l < NARROW || kwide) k[l] = *(const v4i*)(kb + l * s.kv_plane + ((size_t)kt * DS + ds) * TILE_BYTES);
+                        if (l < NARROW || q_wide) q[l] = *(const v4i*)(qb + l * s.q_plane + ds * TILE_BYTES);
+                    }
+                    dot_step<DIGITS>(k, q, acc);
                 }
-                dot_step<DIGITS>(kf, qf, acc);
+                int32_t sc[4];
+                scores_of<HD, DIGITS>(acc, a.scaled, a.scale_q32, sc);
+                keep(kt, sc);
             }
-            int32_t sc[4];
-            scores_of<HD, DIGITS>(acc, a.scaled, a.scale_q32, sc);
-            keep(kt, sc);
-        }
     }
-    take_best(best, best_key, __shfl_xor(best, 16), (uint32_t)__shfl_xor((int)best_key, 16));
-    take_best(best, best_key, __shfl_xor(best, 32), (uint32_t)__shfl_xor((int)best_key, 32));
-    if (lane < 16) sm.best[wave][lane] = best, sm.best_key[wave][lane] = best_key;
+    best = max(best, __shfl_xor(best, 16));
+    best = max(best, __shfl_xor(best, 32));
+    if (lane < 16) sm.best[wave][lane] = best;
     __syncthreads();
-    best = sm.best[0][lane & 15];
-    best_key = sm.best_key[0][lane & 15];
 #pragma unroll
-    for (int v = 1; v < NW; v++) take_best(best, best_key, sm.best[v][lane & 15], sm.best_key[v][lane & 15]);
+    for (int v = 0; v < NW; v++) best = max(best, sm.best[v][lane & 15]);
 
-    // (2) the exp terms in place of the scores, and their sum (at most 2^16
-    // terms of 2^32: exact in double, in any order).
+    // (2) the exp terms in place of the scores, their sum (at most 2^16 terms
+    // of 2^32: exact in double, in any order), and where the maximum is first.
     double sum = 0;
-#pragma unroll 1
+    uint32_t found = 0xffffffffu;
+#pragma unroll 2
     for (uint32_t kt = ta + wave; kt < tb; kt += NW) {
-        uint4* t = tile(kt) + lane;
-        const uint4 sc = *t;
-        const uint32_t v[4] = {sc.x, sc.y, sc.z, sc.w};
-        uint32_t e[4];
+        uint32_t v[4], e[4];
+        double x[4];
+        get(kt, v);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const double x = sees(kt * 16 + 4 * grp + i) ? dn::softmax_exp_f64((uint32_t)best - v[i]) : 0.0;
-            sum += x;
-            e[i] = kept_term(x);
+        for (int i = 0; i < 4; i++) x[i] = softmax_term((uint32_t)best - v[i], &e[i]);
+        if (!whole(kt)) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (!sees(kt * 16 + 4 * grp + i)) x[i] = 0, e[i] = 0;
         }
-        *t = make_uint4(e[0], e[1], e[2], e[3]);
+        if (max(max(e[0], e[1]), max(e[2], e[3])) == 0xffffffffu) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (e[i] == 0xffffffffu) found = min(found, kt * 16 + 4 * grp + i);
+        }
+        sum += (x[0] + x[1]) + (x[2] + x[3]);
+        put(kt, e[0], e[1], e[2], e[3]);
     }
+    found = min(found, (uint32_t)__shfl_xor((int)found, 16));
+    found = min(found, (uint32_t)__shfl_xor((int)found, 32));
+    if (lane < 16) atomicMin(&sm.first[lane], found);
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
     if (lane < 16) sm.sum[wave][lane] = sum;
@@ -346,11 +393,10 @@ __device__ __forceinline__ void packed_rows(const IrisPackedAttention& a, const 
         int32_t wsum = 0;
 #pragma unroll 1
         for (uint32_t kt = base + wave; kt < ks1 * 4; kt += NW) {
-            uint4* t = tile(kt);
             uint32_t low = 0, high = 0;
             if (kt >= ta && kt < tb) {
-                const uint4 k = t[lane];
-                const uint32_t e[4] = {k.x, k.y, k.z, k.w};
+                uint32_t e[4];
+                get(kt, e);
                 int32_t w[4];
                 weights_of(e, scale, scale.w, w, wsum, [&](int i) {
                     const int at = atomicAdd(&sm.nbig[lane & 15], 1);
@@ -358,61 +404,92 @@ __device__ __forceinline__ void packed_rows(const IrisPackedAttention& a, const 
                 });
                 weight_digits(w, low, high);
             }
-            ((uint32_t*)t)[lane] = low;
-            ((uint32_t*)t)[64 + lane] = high;
+            if (spilled(kt)) {
+                global_u32* t = (global_u32*)in_space(kt);
+                t[lane] = low;
+                t[64 + lane] = high;
+            } else {
+                uint32_t* t = (uint32_t*)in_lds(kt);
+                t[lane] = low;
+                t[64 + lane] = high;
+            }
         }
         wsum += __shfl_xor(wsum, 16);
         wsum += __shfl_xor(wsum, 32);
         if (lane < 16) atomicAdd(&sm.wsum[lane], wsum);
     }
-    if (wave == 0 && lane < 16) sm.best_key[0][lane] = best_key;
     if constexpr (SPILL) __threadfence_block();
     __syncthreads();
 
     // (4) weighted values: a wave's dimension tiles over its part of the steps.
     const uint32_t dt0 = wave % (NW / PARTS) * DTW, part = wave / (NW / PARTS);
     const int8_t* vb = s.v + (size_t)g * s.steps * DT * TILE_BYTES + lane * 16;
-    uint64_t tot[DTW][4];
-    auto values = [&](auto digits) __attribute__((always_inline)) {
-        constexpr int LV = decltype(digits)::value;
-        v4i acc[DTW][LV + 1];
+    const uint8_t* vw = s.v_wide + (size_t)g * s.steps * DS + dt0 / 4;
+    auto load_weights = [&](uint32_t ks, v4i& w0, v4i& w1) __attribute__((always_inline)) {
 #pragma unroll
-        for (uint32_t d = 0; d < DTW; d++)
-#pragma unroll
-            for (int j = 0; j < LV + 1; j++) acc[d][j] = v4i{0, 0, 0, 0};
-#pragma unroll 1
-        for (uint32_t ks = ks0 + part; ks < ks1; ks += PARTS) {
-            v4i w0, w1;
-#pragma unroll
-            for (uint32_t t = 0; t < 4; t++) {
-                const uint32_t* p = (const uint32_t*)tile(ks * 4 + t);
+        for (uint32_t t = 0; t < 4; t++) {
+            if (spilled(ks * 4 + t)) {
+                const global_u32* p = (const global_u32*)in_space(ks * 4 + t);
+                w0[t] = (int)p[lane];
+                w1[t] = (int)p[64 + lane];
+            } else {
+                const uint32_t* p = (const uint32_t*)in_lds(ks * 4 + t);
                 w0[t] = (int)p[lane];
                 w1[t] = (int)p[64 + lane];
             }
+        }
+    };
+    v4i acc[DTW][NARROW + 1];
+#pragma unroll
+    for (uint32_t d = 0; d < DTW; d++)
+#pragma unroll
+        for (int j = 0; j < NARROW + 1; j++) acc[d][j] = v4i{0, 0, 0, 0};
+    uint32_t any_wide = 0;
+#pragma unroll 1
+    for (uint32_t ks = ks0 + part; ks < ks1; ks += PARTS) {
+        v4i vf[DTW][NARROW];
+        uint32_t wide = 0;
+#pragma unroll
+        for (uint32_t d = 0; d < DTW; d++) {
+#pragma unroll
+            for (int b = 0; b < NARROW; b++)
+                vf[d][b] = *(const v4i*)(vb + b * s.kv_plane + ((size_t)ks * DT + dt0 + d) * TILE_BYTES);
+            if (d % 4 == 0) wide |= (uint32_t)vw[ks * DS + d / 4] << d / 4;
+        }
+        v4i w0, w1;
+        load_weights(ks, w0, w1);
+#pragma unroll
+        for (uint32_t d = 0; d < DTW; d++) value_step<NARROW>(w0, w1, vf[d], acc[d]);
+        any_wide |= wide;
+    }
+    uint64_t tot[DTW][4];
+#pragma unroll
+    for (uint32_t d = 0; d < DTW; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            tot[d][i] = 0;
+#pragma unroll
+            for (int j = 0; j < NARROW + 1; j++) tot[d][i] += (uint64_t)(int64_t)acc[d][j][i] << (8 * j);
+        }
+    if (__any(any_wide))  // values of more digits: the two upper planes' products
+#pragma unroll 1
+        for (uint32_t ks = ks0 + part; ks < ks1; ks += PARTS) {
+            v4i w0, w1;
+            load_weights(ks, w0, w1);
 #pragma unroll
             for (uint32_t d = 0; d < DTW; d++) {
-                v4i vf[LV];
-                const bool vw = LV == NARROW || s.v_wide[((size_t)g * s.steps + ks) * DS + (dt0 + d) / 4];
+                if (!vw[ks * DS + d / 4]) continue;
+                v4i up[3] = {v4i{0, 0, 0, 0}, v4i{0, 0, 0, 0}, v4i{0, 0, 0, 0}}, upper[2];
 #pragma unroll
-                for (int b = 0; b < LV; b++) {
-                    vf[b] = v4i{0, 0, 0, 0};
-                    if (b < NARROW || vw)
-                        vf[b] = *(const v4i*)(vb + b * s.kv_plane + ((size_t)ks * DT + dt0 + d) * TILE_BYTES);
-                }
-                value_step<LV>(w0, w1, vf, acc[d]);
+                for (int b = 0; b < 2; b++)
+                    upper[b] = *(const v4i*)(vb + (NARROW + b) * s.kv_plane + ((size_t)ks * DT + dt0 + d) * TILE_BYTES);
+                value_step<2>(w0, w1, upper, up);
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int j = 0; j < 3; j++) tot[d][i] += (uint64_t)(int64_t)up[j][i] << (24 + 8 * j);
             }
         }
-#pragma unroll
-        for (uint32_t d = 0; d < DTW; d++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                tot[d][i] = 0;
-#pragma unroll
-                for (int j = 0; j < LV + 1; j++) tot[d][i] += (uint64_t)(int64_t)acc[d][j][i] << (8 * j);
-            }
-    };
-    if (!wide_values) values(std::integral_constant<int, NARROW>{});
-    else values(std::integral_constant<int, DIGITS>{});
     __syncthreads();  // the weights are read: their place takes the sums
     uint64_t* sums = (uint64_t*)tiles;  // [part][16][HD]
 #pragma unroll
@@ -432,7 +509,7 @@ __device__ __forceinline__ void packed_rows(const IrisPackedAttention& a, const 
         const uint32_t r = c / hd4, d = c % hd4 * 4, out_row = qt * 16 + r;
         if (out_row >= a.rows || s.first[out_row] < 0) continue;
         const int64_t resid = dn::sub_sat(dn::ONE_ACT, sm.wsum[r]);
-        const int4 vm = *(const int4*)(v + (size_t)sm.best_key[0][r] * a.v_stride + d);
+        const int4 vm = *(const int4*)(v + (size_t)sm.first[r] * a.v_stride + d);
         const int32_t vv[4] = {vm.x, vm.y, vm.z, vm.w};
         uint64_t t[4];
 #pragma unroll
@@ -464,8 +541,7 @@ __device__ __forceinline__ void packed_place(const IrisPackedAttention& a, const
 }
 
 template <uint32_t HD, int NW>
-__global__ __launch_bounds__(NW * 64, HD >= 512 ? 2 : 4) void packed_lds_kernel(const IrisPackedAttention a,
-                                                                              const PackedSpace s) {
+__global__ __launch_bounds__(NW * 64, HD >= 512 ? 2 : 4) void packed_lds_kernel(const IrisPackedAttention a, const PackedSpace s) {
     extern __shared__ uint4 s_tiles[];
     __shared__ PackedSmem<NW> sm;
     uint32_t qt, h;
@@ -508,8 +584,15 @@ int packed_check(const IrisPackedAttention* a) {
 uint32_t padded_head(uint32_t hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : 512; }
 
 constexpr uint32_t LDS_BYTES = 160 * 1024;
-constexpr int PACKED_WAVES = 8;
-constexpr uint32_t PACKED_GROUPS = 512;  // of a launch whose tiles pass LDS
+constexpr uint32_t PACKED_GROUPS = 256;  // of a launch whose tiles pass LDS
+
+// The waves of a workgroup: sixteen to a CU (one head size's registers allow
+// no more), in as many workgroups as their score tiles leave LDS for, so that
+// one's waits are another's work.
+inline int packed_waves(uint32_t hd, uint32_t lds_tiles) {
+    if (hd > 256) return 8;
+    return lds_tiles <= 38 ? 4 : lds_tiles <= 78 ? 8 : 16;
+}
 
 // Carves the work space (base may be null) and returns its bytes.
 uint64_t packed_space(const IrisPackedAttention& a, uint8_t* base, PackedSpace* s) {
@@ -521,7 +604,7 @@ uint64_t packed_space(const IrisPackedAttention& a, uint8_t* base, PackedSpace* 
     // A tile of rows sees at most this many keys, in whole steps.
     const uint32_t span = std::min(std::min(a.max_length, a.window ? a.window : a.max_length) + 15, a.rows);
     const uint32_t tiles = std::min(((span + 126) / 64) * 4, s->steps * 4);
-    const uint32_t room = (LDS_BYTES - (uint32_t)sizeof(PackedSmem<PACKED_WAVES>) - 64) / TILE_BYTES;
+    const uint32_t room = (LDS_BYTES - (uint32_t)sizeof(PackedSmem<16>) - 64) / TILE_BYTES;
     s->lds_tiles = std::min(tiles, room);
     s->spill_tiles = tiles - s->lds_tiles;
     uint64_t at = 0;
@@ -540,11 +623,8 @@ uint64_t packed_space(const IrisPackedAttention& a, uint8_t* base, PackedSpace* 
     return at;
 }
 
-template <uint32_t HD>
-int packed_launch(const IrisPackedAttention& a, const PackedSpace& s, hipStream_t stream) {
-    constexpr int NW = PACKED_WAVES;
-    const uint32_t tasks = s.steps * 4 * a.kv_heads + s.steps * (HD / 64) * a.kv_heads + s.q_tiles * a.heads + (a.rows + 63) / 64;
-    hipLaunchKernelGGL(packed_planes_kernel<HD>, dim3((tasks + 3) / 4), dim3(256), 0, stream, a, s);
+template <uint32_t HD, int NW>
+int packed_launch_waves(const IrisPackedAttention& a, const PackedSpace& s, hipStream_t stream) {
     const uint32_t items = s.q_tiles * a.heads;
     const size_t lds = std::max<size_t>((size_t)s.lds_tiles * TILE_BYTES, (size_t)key_parts<HD, NW>() * 16 * HD * 8);
     const void* kernel = s.spill_tiles ? (const void*)packed_spill_kernel<HD, NW> : (const void*)packed_lds_kernel<HD, NW>;
@@ -555,6 +635,18 @@ int packed_launch(const IrisPackedAttention& a, const PackedSpace& s, hipStream_
     else
         hipLaunchKernelGGL((packed_lds_kernel<HD, NW>), dim3(items), dim3(NW * 64), lds, stream, a, s);
     return (int)hipGetLastError();
+}
+
+template <uint32_t HD>
+int packed_launch(const IrisPackedAttention& a, const PackedSpace& s, hipStream_t stream) {
+    const uint32_t tasks = s.steps * 4 * a.kv_heads + s.steps * (HD / 64) * a.kv_heads + s.q_tiles * a.heads + (a.rows + 63) / 64;
+    hipLaunchKernelGGL(packed_planes_kernel<HD>, dim3((tasks + 3) / 4), dim3(256), 0, stream, a, s);
+    const int waves = packed_waves(HD, s.lds_tiles);
+    if constexpr (HD <= 256) {
+        if (waves == 4) return packed_launch_waves<HD, 4>(a, s, stream);
+        if (waves == 16) return packed_launch_waves<HD, 16>(a, s, stream);
+    }
+    return packed_launch_waves<HD, 8>(a, s, stream);
 }
 
 }  // namespace

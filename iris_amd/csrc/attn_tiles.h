@@ -19,6 +19,7 @@
 
 #include "detnum_dev.h"
 #include "paged.h"
+#include "softmax_double.h"
 
 namespace {
 
@@ -87,16 +88,17 @@ __device__ __forceinline__ void scores_of(const v4i (&acc)[2 * LD - 1], int scal
                 for (int j = NS - 2; j >= 0; j--) s[i] = fma(s[i], 256.0, (double)acc[j][i]);
             }
         }
-        if (scaled) {
+        // The integer nearest t = sum * scale / 2^48 by a rounding addend; the
+        // reference's floor at 2^-32 moves t by under 2^-16. Unscaled, t =
+        // sum / 2^16 of an exact sum rounds to even as the reference does.
+        const double unit = scaled ? scale : 0x1p-16;
 #pragma unroll
-            for (int i = 0; i < 4; i++) slow |= !dn::scaled_score_fast(s[i], scale, sc[i]);
-        } else {
-            // Ties to even of an exact sum: 2^-16 s is exact too.
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                sc[i] = (int32_t)fmin(fmax(rint(s[i] * 0x1p-16), -2147483648.0), 2147483647.0);
-                slow |= !(fabs(s[i]) < 0x1p53);
-            }
+        for (int i = 0; i < 4; i++) {
+            const double t = fma(s[i], unit, SOFTMAX_ROUND), n = t - SOFTMAX_ROUND;
+            sc[i] = (int32_t)(uint32_t)softmax_bits(t);
+            slow |= !(fabs(n) < 2147483647.0);
+            if (scaled) slow |= !(fabs(fma(s[i], unit, -n)) <= 0.5 - 0x1p-15);
+            else slow |= !(fabs(s[i]) < 0x1p53);
         }
         if (!__any(slow)) return;
     }
@@ -119,10 +121,6 @@ __device__ __forceinline__ void dot_step(const v4i (&kf)[LD], const v4i (&qf)[LD
             acc[l + m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[l], qf[m], acc[l + m], 0, 0, 0);
 }
 
-// A score's exp term below the row's maximum as it is kept between the
-// passes: 2^32 (the maximum's own) as 0xffffffff, which no other term is.
-__device__ __forceinline__ uint32_t kept_term(double e) { return e > 4294967295.0 ? 0xffffffffu : (uint32_t)e; }
-
 // What turns a row's exp terms into weights: 2^16 over their sum (zero for a
 // lane without a row: all its weights are zero), and whether a weight may need
 // three digits. The sum itself is read again where a weight is formed exactly.
@@ -140,21 +138,27 @@ __device__ __forceinline__ int32_t exact_weight(uint32_t kept, double total) {
     return dn::softmax_weight(kept == 0xffffffffu ? (uint64_t)dn::ONE_ACC : kept, (uint64_t)total, 4294967296.0 / total);
 }
 
-// The weights of four kept terms, two digits each. A quotient estimated in
-// double is off by under 2^-29 (and 2^-16 where the kept term stands for
-// 2^32), the quotient's own rounding in 32 fraction bits moves it by at most
-// 2^-17: within 2^-15 of a rounding tie, and where a third digit is needed,
-// the weight is formed again exactly (one in 2^14), the third digit left to
-// on_big(i) and taken off the weight.
+// The integer nearest a weight's quotient as double has it: off by under
+// 2^-29 (and 2^-16 where the kept term stands for 2^32), while the quotient's
+// own rounding in 32 fraction bits moves it by at most 2^-17. So unless it is
+// near a rounding tie, within 2^-15 (one in 2^14), this is the weight.
+__device__ __forceinline__ int32_t nearest_weight(uint32_t kept, double w_scale, bool& near) {
+    const double k = (double)kept, t = fma(k, w_scale, SOFTMAX_ROUND);
+    near = fabs(fma(k, w_scale, SOFTMAX_ROUND - t)) > 0.5 - 0x1p-15;
+    return (int32_t)(uint32_t)softmax_bits(t);
+}
+
+// The weights of four kept terms, two digits each; those near a tie are formed
+// again exactly, a third digit is left to on_big(i) and taken off the weight.
 template <class OnBig>
 __device__ __forceinline__ void weights_of(const uint32_t (&e)[4], const RowScale& s, double w_scale, int32_t (&w)[4],
                                            int32_t& wsum, OnBig&& on_big) {
     bool slow = s.big;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const double t = (double)e[i] * w_scale, n = rint(t);
-        w[i] = (int32_t)n;
-        slow |= fabs(t - n) > 0.5 - 0x1p-15;
+        bool near;
+        w[i] = nearest_weight(e[i], w_scale, near);
+        slow |= near;
     }
     if (__any(slow)) {
         // One piece of code for the four: four copies of it in every loop
@@ -163,8 +167,9 @@ __device__ __forceinline__ void weights_of(const uint32_t (&e)[4], const RowScal
         for (int i = 0; i < 4; i++) {
             const uint32_t kept = i == 0 ? e[0] : i == 1 ? e[1] : i == 2 ? e[2] : e[3];
             int32_t x = i == 0 ? w[0] : i == 1 ? w[1] : i == 2 ? w[2] : w[3];
-            const double t = (double)kept * w_scale;
-            if (fabs(t - rint(t)) > 0.5 - 0x1p-15) x = exact_weight(kept, *s.sum);
+            bool near;
+            nearest_weight(kept, w_scale, near);
+            if (near) x = exact_weight(kept, *s.sum);
             if (x >= BIG_WEIGHT) {
                 on_big(i);
                 x -= 65536;

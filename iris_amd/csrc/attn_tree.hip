@@ -338,18 +338,26 @@ __global__ __launch_bounds__(256) void tree_terms_kernel(const IrisPagedKv c, co
 #pragma unroll 2
     for (uint32_t k = wave * per; k < kt1; k += 4 * per) {
         const uint32_t kt = k + l.sub, key = key0 + kt * 16 + 4 * grp;
-        if (!valid || kt >= kt1) continue;
-        const uint4 sc = t[kt * 64];
+        const bool live = valid && kt < kt1;
+        const uint4 sc = live ? t[kt * 64] : make_uint4(0, 0, 0, 0);
         const uint32_t v[4] = {sc.x, sc.y, sc.z, sc.w};
+        const bool whole = key0 + k * 16 >= all0 && key0 + (k + per) * 16 <= r.length;
         uint32_t e[4];
+        double x[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const bool sees = (key >= all0 && key + 4 <= r.length) || view.sees(key + i);
-            const double x = sees ? dn::softmax_exp_f64((uint32_t)top - v[i]) : 0.0;
-            if (sees && v[i] == (uint32_t)top) found = min(found, key + i);
-            sum += x;
-            e[i] = kept_term(x);
+        for (int i = 0; i < 4; i++) x[i] = softmax_term((uint32_t)top - v[i], &e[i]);
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (!view.sees(key + i)) x[i] = 0, e[i] = 0;
         }
+        if (!live) continue;
+        if (max(max(e[0], e[1]), max(e[2], e[3])) == 0xffffffffu) {  // the maximum itself
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (e[i] == 0xffffffffu) found = min(found, key + i);
+        }
+        sum += (x[0] + x[1]) + (x[2] + x[3]);
         t[kt * 64] = make_uint4(e[0], e[1], e[2], e[3]);
     }
     for (uint32_t off = l.width; off < 64; off <<= 1) {
@@ -548,9 +556,9 @@ struct OpenWeights {
 
 // The estimate of a weight, and whether it is left open.
 __device__ __forceinline__ int32_t estimate(uint32_t kept, double w_scale, bool& open) {
-    const double t = (double)kept * w_scale, n = rint(t);
-    open = fabs(t - n) > 0.5 - 0x1p-15 || n >= (double)BIG_WEIGHT;
-    return (int32_t)n;
+    const int32_t n = nearest_weight(kept, w_scale, open);
+    open |= n >= BIG_WEIGHT;
+    return n;
 }
 
 // Several row tiles: a workgroup takes MANY of them and 128 dimensions (64 of
