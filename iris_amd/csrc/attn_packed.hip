@@ -26,7 +26,7 @@ struct PackedSpace {
     int32_t* first;             // [rows] the first key a row sees, -1: the row is left
     uint4* spill;               // [workgroups][spill_tiles][64] score tiles past those in LDS
     uint32_t q_tiles, steps;    // 16-row tiles; 64-key steps
-    uint32_t lds_tiles, spill_tiles;
+    uint32_t lds_tiles, spill_tiles, waves, groups;
 };
 
 // The sequence of row t: the last s[i] <= t.
@@ -584,14 +584,32 @@ int packed_check(const IrisPackedAttention* a) {
 uint32_t padded_head(uint32_t hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : 512; }
 
 constexpr uint32_t LDS_BYTES = 160 * 1024;
-constexpr uint32_t PACKED_GROUPS = 256;  // of a launch whose tiles pass LDS
+constexpr uint32_t CUS = 256;  // an MI355X
 
-// The waves of a workgroup: sixteen to a CU (one head size's registers allow
-// no more), in as many workgroups as their score tiles leave LDS for, so that
-// one's waits are another's work.
-inline int packed_waves(uint32_t hd, uint32_t lds_tiles) {
-    if (hd > 256) return 8;
-    return lds_tiles <= 38 ? 4 : lds_tiles <= 78 ? 8 : 16;
+// How a launch's (rows, head) items are taken: by workgroups of `waves`, with
+// `tiles` score tiles in LDS (the rest in the work space) and, where some are
+// there, `groups` workgroups.
+struct PackedShape {
+    uint32_t waves, tiles, groups;
+};
+
+// A CU's registers hold sixteen waves of a head size up to 256, eight of 512.
+// Tiles of up to a half (a quarter) of LDS: workgroups of eight (four) waves,
+// so that one's waits are another's work. More than that: where the items are
+// many, still two workgroups of eight waves to a CU with the tiles past 76 in
+// the work space, else one of sixteen waves with 157 tiles. us, two of eight /
+// one of sixteen: 4096 rows x 32 heads of 128 1349 / 1419, 2048 x 32 of 128 357
+// / 371, 1300 x 32 of 128 159 / 172, 2000 x 8 of 512 256 / 307; 2300 x 8 of 256
+// 175 / 161, 2000 x 4 of 64 52 / 44. Few items: sixteen waves for each, eight
+// for twice as many, while there are tiles for them.
+inline PackedShape packed_shape(uint32_t hd, uint32_t items, uint32_t tiles) {
+    const uint32_t one = (LDS_BYTES - 4096) / TILE_BYTES, two = (LDS_BYTES / 2 - 4096) / TILE_BYTES,
+                   four = (LDS_BYTES / 4 - 4096) / TILE_BYTES;
+    if (tiles > two && (hd > 256 || items >= 8 * CUS)) return {8, two, 2 * CUS};
+    if (hd > 256) return {8, tiles, 0};
+    if (tiles > two) return {16, std::min(tiles, one), CUS};
+    const uint32_t filled = items < CUS ? 16 : items < 2 * CUS ? 8 : 4;
+    return {std::max(tiles > four ? 8u : 4u, std::min(filled, tiles >= 16 ? 16u : tiles >= 8 ? 8u : 4u)), tiles, 0};
 }
 
 // Carves the work space (base may be null) and returns its bytes.
@@ -604,8 +622,10 @@ uint64_t packed_space(const IrisPackedAttention& a, uint8_t* base, PackedSpace* 
     // A tile of rows sees at most this many keys, in whole steps.
     const uint32_t span = std::min(std::min(a.max_length, a.window ? a.window : a.max_length) + 15, a.rows);
     const uint32_t tiles = std::min(((span + 126) / 64) * 4, s->steps * 4);
-    const uint32_t room = (LDS_BYTES - (uint32_t)sizeof(PackedSmem<16>) - 64) / TILE_BYTES;
-    s->lds_tiles = std::min(tiles, room);
+    const PackedShape shape = packed_shape((uint32_t)hd, s->q_tiles * a.heads, tiles);
+    s->waves = shape.waves;
+    s->groups = shape.groups;
+    s->lds_tiles = shape.tiles;
     s->spill_tiles = tiles - s->lds_tiles;
     uint64_t at = 0;
     auto take = [&](auto*& p, uint64_t bytes) {
@@ -619,7 +639,7 @@ uint64_t packed_space(const IrisPackedAttention& a, uint8_t* base, PackedSpace* 
     take(s->k_wide, (uint64_t)a.kv_heads * s->steps * 4);
     take(s->v_wide, (uint64_t)a.kv_heads * s->steps * (hd / 64));
     take(s->first, (uint64_t)a.rows * 4);
-    take(s->spill, s->spill_tiles ? (uint64_t)PACKED_GROUPS * s->spill_tiles * TILE_BYTES : 0);
+    take(s->spill, (uint64_t)s->groups * s->spill_tiles * TILE_BYTES);
     return at;
 }
 
@@ -627,13 +647,17 @@ template <uint32_t HD, int NW>
 int packed_launch_waves(const IrisPackedAttention& a, const PackedSpace& s, hipStream_t stream) {
     const uint32_t items = s.q_tiles * a.heads;
     const size_t lds = std::max<size_t>((size_t)s.lds_tiles * TILE_BYTES, (size_t)key_parts<HD, NW>() * 16 * HD * 8);
-    const void* kernel = s.spill_tiles ? (const void*)packed_spill_kernel<HD, NW> : (const void*)packed_lds_kernel<HD, NW>;
-    const hipError_t st = paged_lds_limit(kernel, lds);
+    if constexpr (NW > 4) {
+        if (s.spill_tiles) {
+            const hipError_t st = paged_lds_limit((const void*)packed_spill_kernel<HD, NW>, lds);
+            if (st != hipSuccess) return (int)st;
+            hipLaunchKernelGGL((packed_spill_kernel<HD, NW>), dim3(std::min(items, s.groups)), dim3(NW * 64), lds, stream, a, s);
+            return (int)hipGetLastError();
+        }
+    }
+    const hipError_t st = paged_lds_limit((const void*)packed_lds_kernel<HD, NW>, lds);
     if (st != hipSuccess) return (int)st;
-    if (s.spill_tiles)
-        hipLaunchKernelGGL((packed_spill_kernel<HD, NW>), dim3(std::min(items, PACKED_GROUPS)), dim3(NW * 64), lds, stream, a, s);
-    else
-        hipLaunchKernelGGL((packed_lds_kernel<HD, NW>), dim3(items), dim3(NW * 64), lds, stream, a, s);
+    hipLaunchKernelGGL((packed_lds_kernel<HD, NW>), dim3(items), dim3(NW * 64), lds, stream, a, s);
     return (int)hipGetLastError();
 }
 
@@ -641,10 +665,9 @@ template <uint32_t HD>
 int packed_launch(const IrisPackedAttention& a, const PackedSpace& s, hipStream_t stream) {
     const uint32_t tasks = s.steps * 4 * a.kv_heads + s.steps * (HD / 64) * a.kv_heads + s.q_tiles * a.heads + (a.rows + 63) / 64;
     hipLaunchKernelGGL(packed_planes_kernel<HD>, dim3((tasks + 3) / 4), dim3(256), 0, stream, a, s);
-    const int waves = packed_waves(HD, s.lds_tiles);
     if constexpr (HD <= 256) {
-        if (waves == 4) return packed_launch_waves<HD, 4>(a, s, stream);
-        if (waves == 16) return packed_launch_waves<HD, 16>(a, s, stream);
+        if (s.waves == 4) return packed_launch_waves<HD, 4>(a, s, stream);
+        if (s.waves == 16) return packed_launch_waves<HD, 16>(a, s, stream);
     }
     return packed_launch_waves<HD, 8>(a, s, stream);
 }
