@@ -40,6 +40,11 @@ __device__ __forceinline__ int4 load4(const int32_t* p) {
     const v4i v = *(const __attribute__((address_space(1))) v4i*)p;
     return make_int4(v[0], v[1], v[2], v[3]);
 }
+__device__ __forceinline__ int2 load2(const int32_t* p) {
+    typedef int v2i __attribute__((ext_vector_type(2)));
+    const v2i v = *(const __attribute__((address_space(1))) v2i*)p;
+    return make_int2(v[0], v[1]);
+}
 __device__ __forceinline__ int32_t load1(const int32_t* p) { return *(const __attribute__((address_space(1))) int32_t*)p; }
 
 // The four digit planes' dwords (byte c: value c's digit) of four values;

@@ -33,6 +33,7 @@ struct TreeSpace {
     int32_t* weights;   // [..][row tile][chunk][16] the weights' sum
     uint64_t* partial;  // [..][row tile][chunk][16][HD] weighted values
     uint32_t row_tiles, chunks, chunk;  // positions per chunk, whole steps
+    uint32_t short_tiles;  // key tiles of a request where the short form is taken, else 0
 };
 
 // A request as a workgroup finds it.
@@ -188,6 +189,21 @@ __global__ __launch_bounds__(256, HD >= 512 ? 1 : HD >= 256 ? 2 : 3) void tree_s
     if (tid == 0) s_wide = 0;
     for (uint32_t i = tid; i < tiles * 64; i += 256) s_max[i / 64][i % 64] = INT32_MIN;
     __syncthreads();
+    const uint32_t kt1 = (key1 - key0 + 15) / 16;
+    // The next tile's keys are loaded during this one's products, the first
+    // while the queries are prepared.
+    constexpr bool AHEAD = HD <= 256;
+    int4 raw[AHEAD ? DS : 1][4];
+    // (Past the last: it again, so that no load is behind a branch, where it
+    // would be waited for.)
+    auto load_ahead = [&](uint32_t kt) __attribute__((always_inline)) {
+        if constexpr (AHEAD) {
+            const int32_t* row = at.at(at.k, key0 + min(kt, kt1 - 1) * 16 + (lane & 15));
+#pragma unroll
+            for (uint32_t ds = 0; ds < DS; ds++) load_step<FULL>(row, ds, c.head_dim, raw[ds]);
+        }
+    };
+    load_ahead(wave);
     uint32_t seen = 0;
     for (uint32_t i = wave; i < tiles * DS; i += 4) {
         int4 v[4];
@@ -206,7 +222,6 @@ __global__ __launch_bounds__(256, HD >= 512 ? 1 : HD >= 256 ? 2 : 3) void tree_s
     const bool q_wide = s_wide;
     // Positions [all0, length) are seen by every row.
     const uint32_t all0 = a.window && r.total > a.window ? r.total - a.window : 0;
-    const uint32_t kt1 = (key1 - key0 + 15) / 16;
     uint4* out = s.scores + (((size_t)bg * s.row_tiles + rt0) * s.chunks + chunk) * (s.chunk / 16) * 64;
     const size_t rt_stride = (size_t)s.chunks * (s.chunk / 16) * 64;
     auto keep = [&](uint32_t kt, uint32_t rt, const int32_t (&sc)[4]) __attribute__((always_inline)) {
@@ -225,19 +240,7 @@ __global__ __launch_bounds__(256, HD >= 512 ? 1 : HD >= 256 ? 2 : 3) void tree_s
         }
         atomicMax(&s_max[rt][lane], m);
     };
-    // The next tile's keys are loaded during this one's products.
-    constexpr bool AHEAD = HD <= 256;
-    int4 raw[AHEAD ? DS : 1][4];
-    // (Past the last: it again, so that no load is behind a branch, where it
-    // would be waited for.)
-    auto load_ahead = [&](uint32_t kt) __attribute__((always_inline)) {
-        if constexpr (AHEAD) {
-            const int32_t* row = at.at(at.k, key0 + min(kt, kt1 - 1) * 16 + (lane & 15));
-#pragma unroll
-            for (uint32_t ds = 0; ds < DS; ds++) load_step<FULL>(row, ds, c.head_dim, raw[ds]);
-        }
-    };
-    load_ahead(wave);
+    uint32_t any_wide = 0;
 #pragma unroll 1
     for (uint32_t kt = wave; kt < kt1; kt += 4) {
         v4i kf[DS][NARROW];
@@ -247,25 +250,41 @@ __global__ __launch_bounds__(256, HD >= 512 ? 1 : HD >= 256 ? 2 : 3) void tree_s
             if constexpr (!AHEAD) load_step<FULL>(at.at(at.k, key0 + kt * 16 + (lane & 15)), ds, c.head_dim, raw[0]);
             step_digits<NARROW>(raw[AHEAD ? ds : 0], kf[ds], wide);
         }
-        if (!q_wide && !is_wide(wide)) {
-            load_ahead(kt + 4);
+        load_ahead(kt + 4);
+        if (q_wide || is_wide(wide)) {  // more digits: below
+            any_wide = 1;
+            continue;
+        }
 #pragma unroll 1
-            for (uint32_t rt = 0; rt < tiles; rt++) {
-                v4i acc[2 * NARROW - 1];
+        for (uint32_t rt = 0; rt < tiles; rt++) {
+            v4i acc[2 * NARROW - 1];
 #pragma unroll
-                for (int j = 0; j < 2 * NARROW - 1; j++) acc[j] = v4i{0, 0, 0, 0};
+            for (int j = 0; j < 2 * NARROW - 1; j++) acc[j] = v4i{0, 0, 0, 0};
 #pragma unroll
-                for (uint32_t ds = 0; ds < DS; ds++) {
-                    v4i qf[NARROW];
+            for (uint32_t ds = 0; ds < DS; ds++) {
+                v4i qf[NARROW];
 #pragma unroll
-                    for (int l = 0; l < NARROW; l++) qf[l] = s_q[((rt * DS + ds) * NARROW + l) * 64 + lane];
-                    dot_step<NARROW>(kf[ds], qf, acc);
-                }
-                int32_t sc[4];
-                scores_of<HD, NARROW>(acc, a.scaled, a.scale_q32, sc);
-                keep(kt, rt, sc);
+                for (int l = 0; l < NARROW; l++) qf[l] = s_q[((rt * DS + ds) * NARROW + l) * 64 + lane];
+                dot_step<NARROW>(kf[ds], qf, acc);
             }
-        } else {
+            int32_t sc[4];
+            scores_of<HD, NARROW>(acc, a.scaled, a.scale_q32, sc);
+            keep(kt, rt, sc);
+        }
+    }
+    if (any_wide)
+#pragma unroll 1
+        for (uint32_t kt = wave; kt < kt1; kt += 4) {
+            const int32_t* row = at.at(at.k, key0 + kt * 16 + (lane & 15));
+            uint32_t wide = 0;
+#pragma unroll 1
+            for (uint32_t ds = 0; ds < DS; ds++) {
+                int4 v[4];
+                v4i f[NARROW];
+                load_step<FULL>(row, ds, c.head_dim, v);
+                step_digits<NARROW>(v, f, wide);
+            }
+            if (!q_wide && !is_wide(wide)) continue;  // above
 #pragma unroll 1
             for (uint32_t rt = 0; rt < tiles; rt++) {
                 v4i acc[2 * DIGITS - 1];
@@ -275,7 +294,7 @@ __global__ __launch_bounds__(256, HD >= 512 ? 1 : HD >= 256 ? 2 : 3) void tree_s
                 for (uint32_t ds = 0; ds < DS; ds++) {
                     int4 v[4];
                     v4i f[DIGITS], qf[DIGITS];
-                    load_step<FULL>(at.at(at.k, key0 + kt * 16 + (lane & 15)), ds, c.head_dim, v);
+                    load_step<FULL>(row, ds, c.head_dim, v);
                     step_digits<DIGITS>(v, f, wide);
                     load_step<FULL>(query(rt), ds, c.head_dim, v);
                     step_digits<DIGITS>(v, qf, wide);
@@ -285,9 +304,7 @@ __global__ __launch_bounds__(256, HD >= 512 ? 1 : HD >= 256 ? 2 : 3) void tree_s
                 scores_of<HD, DIGITS>(acc, a.scaled, a.scale_q32, sc);
                 keep(kt, rt, sc);
             }
-            load_ahead(kt + 4);
         }
-    }
     __syncthreads();
     if (tid < tiles * 16) {
         const uint32_t rt = tid / 16, i = tid % 16;
@@ -848,6 +865,209 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const IrisPagedKv c, con
     }
 }
 
+// ---- (2) to (4) in one launch, for positions whose score tiles LDS holds: a
+// workgroup per (request, key head), row tile and 32 dimensions
+
+constexpr uint32_t SHORT_WAVES = 16;
+constexpr uint32_t SHORT_DIMS = 32;
+constexpr uint32_t SHORT_TILES = (160 * 1024 - 16 * SHORT_DIMS * 8 - 8192) / (TILE_BYTES + 32);
+
+template <bool FULL>
+__global__ __launch_bounds__(SHORT_WAVES * 64, 4) void tree_short_kernel(const IrisPagedKv c, const IrisTreeAttention a,
+                                                                       const TreeSpace s) {
+    constexpr uint32_t NW = SHORT_WAVES, DIMS = SHORT_DIMS;
+    extern __shared__ uint4 s_tile[];  // score tiles, sums [16][DIMS], page offsets
+    uint64_t* s_sums = (uint64_t*)(s_tile + s.short_tiles * 64);
+    uint64_t* s_page = s_sums + 16 * DIMS;
+    __shared__ int32_t s_wsum[16];
+    __shared__ double s_sum[NW][16], s_total[16];
+    __shared__ uint32_t s_first[16];
+    __shared__ BigWeights s_big;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = wave_index(), grp = lane >> 4;
+    const uint32_t bg = blockIdx.x, rt = blockIdx.y, g = bg % c.kv_heads, group = a.heads / c.kv_heads;
+    Request r;
+    if (!read_request(c, a, bg / c.kv_heads, r)) return;
+    const uint32_t pairs = r.rows * group;
+    if (rt * 16 >= pairs) return;
+    const uint32_t rows = min(16u, pairs - rt * 16), key0 = r.base, n = r.total - key0;
+    const uint32_t kt1 = (n + 15) / 16, steps = (n + STEP - 1) / STEP, chunks = chunks_of(s, r);
+    const Places at = places(c, a, r, g, key0, r.total, s_page);
+    if (tid < 16) s_wsum[tid] = 0, s_first[tid] = 0xffffffffu, s_big.count[tid] = 0;
+    for (uint32_t i = tid; i < 16 * DIMS; i += NW * 64) s_sums[i] = 0;
+    const RowLanes l(rows);
+    const bool valid = l.row < rows;
+    const uint32_t per = 16 / l.width;
+    const size_t tile = (size_t)bg * s.row_tiles + rt;
+    int32_t top = INT32_MIN;
+    for (uint32_t i = lane / l.width; i < chunks; i += 64 / l.width)
+        top = max(top, valid ? s.maxima[(tile * s.chunks + i) * 16 + l.row] : INT32_MIN);
+    for (uint32_t off = l.width; off < 64; off <<= 1) top = max(top, __shfl_xor(top, (int)off));
+    const RowView view = row_view(a, r, valid ? rt * 16 + l.row : 0xffffffffu, group);
+    const uint32_t all0 = a.window && r.total > a.window ? r.total - a.window : 0;
+    // The first scores before the values: loads return in order.
+    const uint4* from = s.scores + tile * s.chunks * (s.chunk / 16) * 64 + l.slot;  // chunk by chunk: tile by tile
+    uint4 sc = from[min(wave * per + l.sub, kt1 - 1) * 64];
+    __syncthreads();
+
+    // A wave's first values are on their way during the softmax.
+    // (Value tile k, column n: dimension 2 n + k.)
+    const uint32_t d2 = 2 * (lane & 15), d = blockIdx.z * DIMS + d2;
+    int2 v[4][4];
+    auto load_pairs = [&](uint32_t step) __attribute__((always_inline)) {
+#pragma unroll
+        for (uint32_t t = 0; t < 4; t++) {
+            const int32_t* p = at.four(at.v, key0 + min(step, steps - 1) * STEP + 4 * grp + 16 * t) + (FULL || d < at.hd ? d : 0);
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) v[t][i] = load2(p + i * at.hd);
+        }
+    };
+    load_pairs(wave);
+
+    // (2) exp terms, their sum, the first maximum.
+    double sum = 0;
+    uint32_t found = 0xffffffffu;
+#pragma unroll 1
+    for (uint32_t k = wave * per; k < kt1; k += NW * per) {
+        const uint32_t kt = k + l.sub, key = key0 + kt * 16 + 4 * grp;
+        const bool live = valid && kt < kt1;
+        const uint32_t x[4] = {sc.x, sc.y, sc.z, sc.w};
+        if (k + NW * per < kt1) sc = from[min(kt + NW * per, kt1 - 1) * 64];
+        uint32_t e[4];
+        double t[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) t[i] = softmax_term((uint32_t)top - x[i], &e[i]);
+        if (!(key0 + k * 16 >= all0 && key0 + (k + per) * 16 <= r.length)) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (!view.sees(key + i)) t[i] = 0, e[i] = 0;
+        }
+        if (!live) continue;
+        if (max(max(e[0], e[1]), max(e[2], e[3])) == 0xffffffffu) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (e[i] == 0xffffffffu) found = min(found, key + i);
+        }
+        sum += (t[0] + t[1]) + (t[2] + t[3]);
+        s_tile[kt * 64 + l.slot] = make_uint4(e[0], e[1], e[2], e[3]);
+    }
+    for (uint32_t off = l.width; off < 64; off <<= 1) {
+        sum += __shfl_xor(sum, (int)off);
+        found = min(found, (uint32_t)__shfl_xor((int)found, (int)off));
+    }
+    if (lane < l.width) s_sum[wave][lane] = sum;
+    if (lane < l.width && valid) atomicMin(&s_first[lane], found);
+    lds_barrier();
+    if (tid < 16) {
+        double t = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < NW; w++) t += s_sum[w][min(tid, l.width - 1)];
+        s_total[tid] = t;
+    }
+    lds_barrier();
+
+    // (3) the weights' digits in place of the terms: the low digits as dword
+    // `slot` of a tile, the high ones as dword 64 + slot. A wave has read all
+    // of its tiles' terms before it writes there. (Rows past the last: what
+    // was there; their sums are not looked at.)
+    {
+        const RowScale scale(&s_total[l.row], valid);
+        int32_t wsum = 0;
+#pragma unroll 1
+        for (uint32_t k = wave * per; k < steps * 4; k += NW * per) {
+            const uint32_t kt = k + l.sub;
+            const uint4 x = s_tile[min(kt, kt1 - 1) * 64 + l.slot];
+            const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+            int32_t w[4];
+            weights_of(e, scale, kt < kt1 ? scale.w : 0.0, w, wsum,
+                       [&](int j) { s_big.add(l.row, key0 + kt * 16 + 4 * grp + j); });
+            uint32_t low, high;
+            weight_digits(w, low, high);
+            if (kt < steps * 4) {
+                uint32_t* to = (uint32_t*)(s_tile + kt * 64);
+                to[l.slot] = low;
+                to[64 + l.slot] = high;
+            }
+        }
+        for (uint32_t off = l.width; off < 64; off <<= 1) wsum += __shfl_xor(wsum, (int)off);
+        if (lane < l.width && valid) atomicAdd(&s_wsum[lane], wsum);
+    }
+    lds_barrier();
+
+    // (4) weighted values: a wave takes its part of the steps. A thread
+    // finishes one (row, dimension); the first maximum's value is on its way.
+    static_assert(16 * DIMS <= NW * 64, "an output per thread");
+    const uint32_t my_row = tid / DIMS, my_dim = blockIdx.z * DIMS + tid % DIMS;
+    const bool mine = my_row < rows && my_dim < c.head_dim;
+    const int32_t first_value = mine ? load1(at.at(at.v, s_first[my_row]) + my_dim) : 0;
+    auto load_weights = [&](uint32_t step, v4i& w0, v4i& w1) __attribute__((always_inline)) {
+#pragma unroll
+        for (uint32_t t = 0; t < 4; t++) {
+            const uint32_t* p = (const uint32_t*)(s_tile + (step * 4 + t) * 64);
+            w0[t] = (int)p[lane];
+            w1[t] = (int)p[64 + lane];
+        }
+    };
+    v4i acc[2][NARROW + 1];
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int j = 0; j < NARROW + 1; j++) acc[t][j] = v4i{0, 0, 0, 0};
+    uint32_t any_wide = 0;
+#pragma unroll 1
+    for (uint32_t step = wave; step < steps; step += NW) {
+        v4i w0, w1;
+        load_weights(step, w0, w1);
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            int4 x[4];
+#pragma unroll
+            for (uint32_t t = 0; t < 4; t++)
+                x[t] = k ? make_int4(v[t][0].y, v[t][1].y, v[t][2].y, v[t][3].y) : make_int4(v[t][0].x, v[t][1].x, v[t][2].x, v[t][3].x);
+            v4i f[NARROW];
+            step_digits<NARROW>(x, f, any_wide);
+            value_step<NARROW>(w0, w1, f, acc[k]);
+        }
+        load_pairs(step + NW);
+    }
+#pragma unroll
+    for (uint32_t q = 0; q < 4; q++) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            uint64_t t = 0;
+#pragma unroll
+            for (int j = 0; j < NARROW + 1; j++) t += (uint64_t)(int64_t)acc[k][j][q] << (8 * j);
+            if (4 * grp + q < rows && wave < steps) atomicAdd((unsigned long long*)&s_sums[(4 * grp + q) * DIMS + d2 + k], t);
+        }
+    }
+    if (is_wide(any_wide))
+#pragma unroll 1
+        for (uint32_t step = wave; step < steps; step += NW) {
+            v4i w0, w1;
+            load_weights(step, w0, w1);
+#pragma unroll 1
+            for (int k = 0; k < 2; k++) {
+                int4 x[4];
+#pragma unroll
+                for (uint32_t t = 0; t < 4; t++) {
+                    const int32_t* p = at.four(at.v, key0 + step * STEP + 4 * grp + 16 * t) + (d < at.hd ? d + k : 0);
+                    x[t] = make_int4(load1(p), load1(p + at.hd), load1(p + 2 * at.hd), load1(p + 3 * at.hd));
+                }
+                uint64_t more[4];
+                upper_values(w0, w1, x, more);
+#pragma unroll
+                for (uint32_t q = 0; q < 4; q++)
+                    if (4 * grp + q < rows) atomicAdd((unsigned long long*)&s_sums[(4 * grp + q) * DIMS + d2 + k], more[q]);
+            }
+        }
+    __syncthreads();
+    if (!mine) return;
+    uint64_t t = s_sums[tid] + (uint64_t)((int64_t)dn::sub_sat(dn::ONE_ACT, s_wsum[my_row]) * first_value);
+    for (int j = 0; j < s_big.count[my_row]; j++) t += (uint64_t)((int64_t)65536 * load1(at.at(at.v, s_big.key[my_row][j]) + my_dim));
+    const uint32_t pair = rt * 16 + my_row;
+    a.out[(size_t)(r.row0 + pair / group) * a.out_stride + (size_t)(g * group + pair % group) * c.head_dim + my_dim] =
+        dn::requantize((int64_t)t);
+}
+
 bool misaligned(const void* p) { return ((uintptr_t)p & 15) != 0; }
 
 int tree_check(const IrisPagedKv* c, const IrisTreeAttention* a) {
@@ -874,8 +1094,16 @@ uint64_t tree_space(const IrisPagedKv& c, const IrisTreeAttention& a, uint8_t* b
     s->row_tiles = (a.max_nodes * group + 15) / 16;
     // Positions that a request's rows look at, from a multiple of STEP on.
     const uint64_t span = std::min<uint64_t>(a.max_positions, a.window ? (uint64_t)a.window + a.max_nodes + STEP : a.max_positions);
+    const uint64_t tiles = (span + STEP - 1) / STEP * 4;
+    // Where its workgroups (sixteen waves: one to a CU) are there all at once.
+    // us, short / long: 1 token at 700 (32 heads of 128, 32 workgroups) 18.4 /
+    // 24.1, 8 at 700 (256) 20.2 / 28.2, 8 at up to 2100 (256) 31.6 / 36.1, a tree
+    // of 32 at 700 (256) 33.8 / 44, 12 of 9 in a window of 1024 (heads of 256, 480)
+    // 50 / 40, 32 at 700 (1024) 60 / 45.
+    const uint64_t groups = bg * s->row_tiles * ((c.head_dim + SHORT_DIMS - 1) / SHORT_DIMS);
+    s->short_tiles = tiles <= SHORT_TILES && groups <= 256 ? (uint32_t)tiles : 0;
     const uint64_t want = std::max<uint64_t>(1, 1024 / bg);
-    s->chunk = (uint32_t)std::min<uint64_t>(MAX_CHUNK, std::max<uint64_t>(128, ((span + want - 1) / want + 127) & ~127ull));
+    s->chunk = (uint32_t)std::min<uint64_t>(MAX_CHUNK, std::max<uint64_t>(STEP, ((span + want - 1) / want + STEP - 1) & ~uint64_t(STEP - 1)));
     s->chunks = (uint32_t)((span + s->chunk - 1) / s->chunk);
     uint64_t at = 0;
     auto take = [&](auto*& p, uint64_t bytes) {
@@ -888,7 +1116,7 @@ uint64_t tree_space(const IrisPagedKv& c, const IrisTreeAttention& a, uint8_t* b
     take(s->firsts, parts * 16 * 4);
     take(s->sums, parts * 16 * 8);
     take(s->weights, parts * 16 * 4);
-    take(s->partial, parts * 16 * hd * 8);
+    if (!s->short_tiles) take(s->partial, parts * 16 * hd * 8);
     return at;
 }
 
@@ -904,6 +1132,13 @@ int tree_launch(const IrisPagedKv& c, const IrisTreeAttention& a, const TreeSpac
     if (st != hipSuccess) return (int)st;
     hipLaunchKernelGGL((tree_scores_kernel<HD, FULL>), dim3(s.chunks | 1, bg, (s.row_tiles + RB - 1) / RB), dim3(256), q_lds, stream, c,
                        a, s);
+    if (s.short_tiles) {
+        const size_t lds = (size_t)s.short_tiles * TILE_BYTES + 16 * SHORT_DIMS * 8 + ((size_t)s.short_tiles * 4 + 2) * 8;
+        st = paged_lds_limit((const void*)tree_short_kernel<FULL>, lds);
+        if (st != hipSuccess) return (int)st;
+        hipLaunchKernelGGL(tree_short_kernel<FULL>, dim3(bg, s.row_tiles, (c.head_dim + SHORT_DIMS - 1) / SHORT_DIMS), dim3(SHORT_WAVES * 64), lds, stream, c, a, s);
+        return (int)hipGetLastError();
+    }
     hipLaunchKernelGGL(tree_terms_kernel, dim3(s.chunks | 1, bg, s.row_tiles), dim3(256), 0, stream, c, a, s);
     if (s.row_tiles == 1)
         hipLaunchKernelGGL((tree_values_kernel<HD, FULL>), dim3(s.chunks | 1, bg), dim3(HD > 256 ? HD : 256), v_lds, stream, c, a, s);
@@ -936,9 +1171,10 @@ int iris_attention_tree(const IrisPagedKv* c, const IrisTreeAttention* a, void* 
     const int rc = tree_check(c, a);
     if (rc) return rc;
     if (!a->rows || !a->requests) return 0;
-    if (!space || misaligned(space)) return IRIS_E_INVALID;
     TreeSpace s;
-    if (bytes < tree_space(*c, *a, (uint8_t*)space, &s)) return IRIS_E_RANGE;
+    const uint64_t need = tree_space(*c, *a, (uint8_t*)space, &s);
+    if (need && (!space || misaligned(space))) return IRIS_E_INVALID;
+    if (bytes < need) return IRIS_E_RANGE;
     switch (padded_head(c->head_dim)) {
         case 64: return tree_launch_head<64>(*c, *a, s, (hipStream_t)stream);
         case 128: return tree_launch_head<128>(*c, *a, s, (hipStream_t)stream);
