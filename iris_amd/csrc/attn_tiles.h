@@ -209,11 +209,4 @@ __device__ __forceinline__ void value_step(v4i w0, v4i w1, const v4i (&vf)[LV], 
     }
 }
 
-// The larger score, of equal ones the earlier key.
-__device__ __forceinline__ void take_best(int32_t& best, uint32_t& key, int32_t other, uint32_t other_key) {
-    const bool take = other > best || (other == best && other_key < key);
-    best = take ? other : best;
-    key = take ? other_key : key;
-}
-
 }  // namespace

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from iris_amd import native, paged, scalars
+from oracle import cpu
 from tests import paged_reference as ref
 
 pytestmark = pytest.mark.gpu
@@ -138,6 +139,63 @@ def test_packed_long(lens, window, hd):
             cols = slice(h * hd, h * hd + hd)
             want = ref.attend(p.q[a:b][rows][:, cols], p.k[a:b], p.v[a:b], seen, p.scale)
             assert np.array_equal(got[a:b][rows][:, cols], want)
+
+
+def check_some_rows(p, rng):
+    """Each sequence's ends and some rows between, three heads."""
+    torch.cuda.synchronize()
+    got = p.out.cpu().numpy()
+    group = p.heads // p.kv_heads
+    for a, b in zip(p.starts[:-1], p.starts[1:]):
+        n = int(b - a)
+        rows = sorted({0, n - 1} | set(rng.integers(0, n, 5).tolist()))
+        at = np.arange(n)
+        seen = np.stack([(at <= r) & ((r - at < p.window) if p.window else True) for r in rows])
+        for h in sorted({0, p.heads // 2, p.heads - 1}):
+            cols, kv = slice(h * p.hd, h * p.hd + p.hd), slice(h // group * p.hd, h // group * p.hd + p.hd)
+            want = ref.attend(p.q[a:b][rows][:, cols], p.k[a:b, kv], p.v[a:b, kv], seen, p.scale)
+            assert np.array_equal(got[a:b][rows][:, cols], want)
+    assert p.status.item() == 0
+
+
+@pytest.mark.parametrize("hd, kv_heads", [(64, 4), (128, 2), (256, 1), (80, 4)])
+@pytest.mark.parametrize("lens, heads", [([300, 77, 250], 16), ([90, 200], 16), ([700, 130, 90], 8), ([1000], 4), ([1400], 32),
+                                         ([2700], 4)])
+def test_packed_launch_shapes(lens, heads, hd, kv_heads):
+    # Four, eight and sixteen waves a tile, scores in LDS and behind it.
+    rng = np.random.default_rng(hd + heads + lens[0])
+    p = Packed(rng, lens, heads, min(kv_heads, heads), hd, kinds=("sharp", "mixed", "mixed"))
+    p.run()
+    check_some_rows(p, rng)
+
+
+def tied_difference(n):
+    """A score difference d for which n - 1 keys that far below the largest
+    have weights within 2^-17 of a rounding tie, and the weight before rounding."""
+    term = cpu.lib().dn_softmax_exp_term
+    for d in range(1, 700000):
+        e = term(-d * 65536)
+        total = (1 << 32) + (n - 1) * e
+        if abs((e * 65536) % total - total // 2) < total >> 17 and e * 65536 // total:
+            return d
+    raise AssertionError("no such difference")
+
+
+@pytest.mark.parametrize("n", [100, 333])
+def test_packed_weights_near_ties(n):
+    # The last row of every sequence: all its weights but one are near a tie.
+    rng = np.random.default_rng(n)
+    p = Packed(rng, [n] * 9, 2, 1, 64, scaled=False)
+    d = tied_difference(n)
+    for t, x in zip(p.t, (p.q, p.k)):
+        x[:] = 0
+        x[:, ::64] = 65536
+    p.k[:] = 0
+    p.k[p.starts[1:] - 1, 0] = d
+    for t, x in zip(p.t, (p.q, p.k)):
+        t.copy_(dev(x))
+    p.run()
+    p.check()
 
 
 def test_packed_rows_deeper_than_max_length_are_left():
@@ -321,6 +379,73 @@ def test_tree_long_contexts(length, nodes, heads, kv_heads, hd, page, window):
     rng = np.random.default_rng(length)
     t = Tree(rng, [length, 33], [nodes, 1], heads, kv_heads, hd, page=page, window=window,
              kinds=("sharp", "normal", "normal"))
+    t.run()
+    t.check()
+
+
+# Bounds on the positions that are far from what is held: the same rows by the
+# kernels for long spans, in chunks of several sizes.
+LONG = [2600, 30000, 300000]
+
+
+@pytest.mark.parametrize("heads, kv_heads, hd", HEADS)
+@pytest.mark.parametrize("max_positions", LONG)
+def test_tree_heads_in_long_spans(heads, kv_heads, hd, max_positions):
+    rng = np.random.default_rng(hd + heads)
+    t = Tree(rng, [0, 40, 7, 130], [3, 1, 0, 9], heads, kv_heads, hd, extra=(4, 8), behind=2, max_positions=max_positions)
+    t.run()
+    t.check()
+
+
+@pytest.mark.parametrize("kinds", [("wide", "wide", "wide"), ("normal", "wide", "normal"), ("normal", "normal", "wide"),
+                                   ("mixed", "mixed", "mixed"), ("ends", "ends", "ends"), ("sharp", "sharp", "sharp"),
+                                   ("same", "same", "ends")])
+@pytest.mark.parametrize("heads, kv_heads, hd, scaled", [(4, 2, 64, True), (2, 2, 128, False), (12, 1, 256, False),
+                                                         (9, 1, 80, True), (6, 1, 512, True), (32, 2, 128, True)])
+@pytest.mark.parametrize("max_positions", [2600, 300000])
+def test_tree_values_in_long_spans(kinds, heads, kv_heads, hd, scaled, max_positions):
+    rng = np.random.default_rng(hd)
+    t = Tree(rng, [150, 20], [9, 5], heads, kv_heads, hd, scaled=scaled, kinds=kinds, page=32, max_positions=max_positions)
+    t.run()
+    t.check()
+
+
+@pytest.mark.parametrize("lengths, nodes", [([0], [1]), ([63], [1]), ([64], [1]), ([200], [64]), ([5, 0, 900], [0, 0, 2]),
+                                            ([1, 2, 3, 70, 129, 400], [17, 33, 5, 16, 64, 2])])
+@pytest.mark.parametrize("window", [0, 3, 65])
+@pytest.mark.parametrize("heads", [2, 16])
+def test_tree_lengths_in_long_spans(lengths, nodes, window, heads):
+    rng = np.random.default_rng(sum(lengths) + window)
+    t = Tree(rng, lengths, nodes, heads, 2, 64, window=window, page=4 if heads == 2 else 64, max_positions=5000,
+             kinds=("sharp", "normal", "mixed"))
+    t.run()
+    t.check()
+
+
+@pytest.mark.parametrize("requests, heads, kv_heads, hd", [(70, 8, 4, 64), (40, 8, 2, 256), (300, 2, 1, 128)])
+def test_tree_of_many_requests(requests, heads, kv_heads, hd):
+    # Short spans, but more workgroups than the card holds at once.
+    rng = np.random.default_rng(requests)
+    t = Tree(rng, rng.integers(0, 150, requests).tolist(), rng.integers(0, 3, requests).tolist(), heads, kv_heads, hd)
+    t.run()
+    t.check()
+
+
+@pytest.mark.parametrize("n", [101, 700])
+@pytest.mark.parametrize("heads", [1, 40])
+@pytest.mark.parametrize("max_positions", [None, 2600, 300000])
+def test_tree_weights_near_ties(n, heads, max_positions):
+    # Every row's own key is its largest, all others' weights are near a tie.
+    rng = np.random.default_rng(n)
+    t = Tree(rng, [n - 1], [3], heads, 1, 64, scaled=False, parents=[-1] * 3, max_positions=max_positions)
+    t.q[:], t.kp[:] = 0, 0
+    t.q[:, ::64] = 65536
+    d = tied_difference(n)
+    for i in range(3):
+        at = n - 1 + i
+        t.kp[t.table[0, at // 16], 0, at % 16, 0] = d
+    t.tq.copy_(dev(t.q))
+    t.tk.copy_(dev(t.kp))
     t.run()
     t.check()
 
