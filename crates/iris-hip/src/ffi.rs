@@ -20,6 +20,12 @@ pub struct IrisSession {
     _private: [u8; 0],
 }
 
+
+#[repr(C)]
+pub struct IrisBatch {
+    _private: [u8; 0],
+}
+
 pub const IRIS_FAMILY_MISTRAL_DENSE: i32 = 0;
 pub const IRIS_FAMILY_GEMMA_DENSE: i32 = 1;
 pub const IRIS_NOALLOC_SCRATCH_BYTES: u64 = 32 << 20;
@@ -368,5 +374,31 @@ extern "C" {
         workspace_bytes: u64,
         stream: *mut c_void,
     ) -> c_int;
+    pub fn iris_batch_create(
+        model: *mut IrisModel,
+        requests: u32,
+        pages: u32,
+        page_size: u32,
+        max_positions: u32,
+        max_rows: u32,
+        out: *mut *mut IrisBatch,
+    ) -> c_int;
+    pub fn iris_batch_free(batch: *mut IrisBatch);
+    pub fn iris_batch_prefill(
+        batch: *mut IrisBatch,
+        ids: *const i32,
+        counts: *const u32,
+        out_tokens: *mut i32,
+    ) -> c_int;
+    pub fn iris_batch_step(
+        batch: *mut IrisBatch,
+        ids: *const i32,
+        parents: *const i32,
+        counts: *const u32,
+        out_tokens: *mut i32,
+        out_kept: *mut u32,
+    ) -> c_int;
+    pub fn iris_batch_release(batch: *mut IrisBatch, request: u32) -> c_int;
+    pub fn iris_batch_length(batch: *const IrisBatch, request: u32, out: *mut u32) -> c_int;
     pub fn iris_sha256_bytes(data: *const u8, len: u64, out: *mut u8) -> c_int;
 }

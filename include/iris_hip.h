@@ -532,6 +532,47 @@ uint64_t iris_attention_tree_workspace_bytes(const IrisPagedKv* cache, const Iri
 int iris_attention_tree(const IrisPagedKv* cache, const IrisTreeAttention* a, void* d_workspace,
                         uint64_t workspace_bytes, void* stream);
 
+/* Greedy generation of several requests at a time over one paged cache of
+ * `pages` pages of page_size positions (of every layer that has keys of its
+ * own), each up to max_positions (at most 2^20), in passes of up to max_rows
+ * rows; at most 4096 requests, requests * kv_heads at most 65535. Both
+ * families. Every call is synchronous, on a stream of the batch's own; calls
+ * of one batch must not overlap. A refused call (IRIS_E_INVALID, _SCALE,
+ * _RANGE, _STATE of a request's length) changes nothing; after any other
+ * error the batch's state is unknown and every call but iris_batch_free
+ * returns IRIS_E_STATE. */
+typedef struct IrisBatch IrisBatch;
+int iris_batch_create(IrisModel* model, uint32_t requests, uint32_t pages, uint32_t page_size, uint32_t max_positions,
+                      uint32_t max_rows, IrisBatch** out);
+void iris_batch_free(IrisBatch* batch);
+
+/* The prompts of requests of length 0, packed: request i's counts[i] ids (0:
+ * none for it; at most 65535) follow those before it in `ids`. out_tokens[i]
+ * is the first maximum of the logits behind request i's last row, the token
+ * that iris_session_generate selects first (-1 where counts[i] is 0).
+ * IRIS_E_STATE for a prompt to a request that holds positions, IRIS_E_RANGE
+ * where rows, positions or pages do not suffice. */
+int iris_batch_prefill(IrisBatch* batch, const int32_t* ids, const uint32_t* counts, int32_t* out_tokens);
+
+/* One pass of requests that hold positions: request i's counts[i] rows (0 to
+ * 64) are its last selected token and, behind it, drafted ones. parents (null:
+ * each row's is the row before it) names each row's parent among the request's
+ * rows, as IrisTreeAttention's. From row 0 on, a row's selection is the first
+ * maximum of its logits, and the path goes on to the first later row whose
+ * parent that row is and whose token is that selection. The path's rows are
+ * kept: out_kept[i] of them (at least 1 where counts[i] is not 0), and
+ * out_tokens has their selections where the request's rows are in `ids` (-1
+ * behind them). They are what iris_session_generate selects one by one: the
+ * last of them is the next call's row 0. IRIS_E_STATE for rows of a request of
+ * length 0. A request's rows need room for all of them, kept or not. */
+int iris_batch_step(IrisBatch* batch, const int32_t* ids, const int32_t* parents, const uint32_t* counts,
+                    int32_t* out_tokens, uint32_t* out_kept);
+
+/* Empties a request: its length is 0 and its pages are free for the next call. */
+int iris_batch_release(IrisBatch* batch, uint32_t request);
+/* Positions a request holds. */
+int iris_batch_length(const IrisBatch* batch, uint32_t request, uint32_t* out);
+
 /* SHA-256 (FIPS 180-4) of `len` bytes into out[32]; the hash
  * iris_session_layer_pass uses. Host code only. */
 int iris_sha256_bytes(const uint8_t* data, uint64_t len, uint8_t* out);

@@ -55,7 +55,7 @@ __global__ __launch_bounds__(NT) void gemma_qkv_finish_kernel(const GemmaQkvArgs
     for (uint32_t i = tid; i < hd; i += NT)
         s_v[i] = (is_q || is_k) ? dn::mul_sat(dn::mul_sat(s_v[i], scale), nw[i]) : dn::mul_sat(s_v[i], scale);
     __syncthreads();
-    const uint32_t pos = (uint32_t)(*a.d_pos) + t;
+    const uint32_t pos = a.positions ? (uint32_t)a.positions[t] : (uint32_t)(*a.d_pos) + t;
     if ((is_q || is_k) && pos != 0 && a.rotary_dim != 0) {
         const uint32_t half = a.rotary_dim / 2;
         for (uint32_t i = tid; i < half; i += NT) {
@@ -74,10 +74,16 @@ __global__ __launch_bounds__(NT) void gemma_qkv_finish_kernel(const GemmaQkvArgs
         for (uint32_t i = tid; i < hd; i += NT) dst[i] = s_v[i];
     } else if (is_k) {
         const size_t kbase = (size_t)(h - a.heads) * hd;
+        if (a.positions) {
+            int32_t* dst = a.k_rows + (size_t)t * ((size_t)a.kv_heads * hd) + kbase;
+            for (uint32_t i = tid; i < hd; i += NT) dst[i] = s_v[i];
+            return;
+        }
         for (uint32_t i = tid; i < hd; i += NT) a.k_cache[(kbase + i) * a.k_pos_stride + pos] = s_v[i];
     } else {
         const size_t vbase = (size_t)(h - a.heads - a.kv_heads) * hd;
-        int32_t* dst = a.v_cache + (size_t)pos * ((size_t)a.kv_heads * hd) + vbase;
+        int32_t* dst = (a.positions ? a.v_rows + (size_t)t * ((size_t)a.kv_heads * hd)
+                                    : a.v_cache + (size_t)pos * ((size_t)a.kv_heads * hd)) + vbase;
         for (uint32_t i = tid; i < hd; i += NT) dst[i] = s_v[i];
     }
 }
@@ -251,7 +257,8 @@ int iris_gemma_qkv_finish_launch(const GemmaQkvArgs& a, uint32_t rows, hipStream
     if (a.head_dim == 0 || a.head_dim > GEMMA_MAX_HEAD_DIM || a.rotary_dim > a.head_dim || a.rotary_dim % 2)
         return IRIS_E_INVALID;
     if (rows == 0) return 0;
-    hipLaunchKernelGGL(gemma_qkv_finish_kernel, dim3(a.heads + 2 * a.kv_heads, rows), dim3(NT), 0, stream, a);
+    const uint32_t kv = a.positions && !a.k_rows ? 0 : 2 * a.kv_heads;
+    hipLaunchKernelGGL(gemma_qkv_finish_kernel, dim3(a.heads + kv, rows), dim3(NT), 0, stream, a);
     return (int)hipGetLastError();
 }
 

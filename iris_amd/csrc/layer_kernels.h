@@ -113,6 +113,11 @@ struct GemmaQkvArgs {
     int32_t* k_cache;        // transposed: [kv_heads*head_dim][k_pos_stride]
     uint32_t k_pos_stride;
     int32_t* v_cache;        // [position][kv_heads*head_dim]
+    // Rows of several requests (null: one session's): each row's position, in
+    // place of *d_pos + row; the keys and values go to rows [rows][kv_heads *
+    // head_dim] of their own, null where only the queries are wanted.
+    const int32_t* positions;
+    int32_t *k_rows, *v_rows;
 };
 
 struct I32GemvArgs {
@@ -169,9 +174,10 @@ int iris_i32_gemv_launch(const I32GemvArgs& a, uint32_t tokens, hipStream_t stre
 int iris_silu_table(const int32_t** out);
 int iris_ple_prepare_launch(const PleArgs& a, uint32_t segments, uint32_t rows, hipStream_t stream);
 // (sin, cos) in Q30 (mistral.rs:84-109) of position * inv_freq[j] for the
-// `rows` positions from *d_pos and j < half: out[row][j][2].
+// `rows` positions from *d_pos and j < half: out[row][j][2]. With `each`, row's
+// position is d_pos[row].
 int iris_rope_table_launch(const int64_t* inv_freq, uint32_t half, const int32_t* d_pos, uint32_t rows, int64_t* out,
-                           hipStream_t stream);
+                           hipStream_t stream, bool each = false);
 // K cache positions pos0..pos0 + count as rows of kvw values (out), or rows
 // into the cache: kv_rows.hip.
 int iris_kv_rows_launch(bool out, int32_t* cache, uint32_t stride, uint32_t pos0, uint32_t count, uint32_t kvw,

@@ -417,12 +417,13 @@ __global__ void embed_rows_kernel(const int32_t* ids, const uint8_t* embed_raw, 
 }
 
 __global__ __launch_bounds__(256) void rope_table_kernel(const int64_t* inv_freq, uint32_t half, const int32_t* d_pos,
-                                                         uint32_t rows, int64_t* out) {
+                                                         uint32_t rows, int64_t* out, bool each) {
     const uint32_t i = blockIdx.x * 256 + threadIdx.x;
     if (i >= rows * half) return;
     const uint32_t row = i / half, j = i % half;
     int64_t s, c;
-    dn::sin_cos_q30((int64_t)((uint32_t)(*d_pos) + row) * inv_freq[j], s, c);
+    const uint32_t pos = each ? (uint32_t)d_pos[row] : (uint32_t)(*d_pos) + row;
+    dn::sin_cos_q30((int64_t)pos * inv_freq[j], s, c);
     out[2 * (size_t)i] = s;
     out[2 * (size_t)i + 1] = c;
 }
@@ -509,10 +510,10 @@ extern "C" int iris_silu_table_device(const int32_t* d_x, uint32_t n, int32_t* d
 }
 
 int iris_rope_table_launch(const int64_t* inv_freq, uint32_t half, const int32_t* d_pos, uint32_t rows, int64_t* out,
-                           hipStream_t stream) {
+                           hipStream_t stream, bool each) {
     if (rows == 0 || half == 0) return 0;
     hipLaunchKernelGGL(rope_table_kernel, dim3((rows * half + 255) / 256), dim3(256), 0, stream, inv_freq, half, d_pos,
-                       rows, out);
+                       rows, out, each);
     return (int)hipGetLastError();
 }
 

@@ -430,13 +430,6 @@ void iris_model_free(IrisModel* m) {
 
 // ---------------------------------------------------------------- session
 
-// Where a checkpointing pass leaves each layer's rows: a device copy per
-// layer, and an event recorded on the pass's stream once it is made.
-struct CkptSink {
-    int32_t* dev;        // [layers][rows][hidden]
-    hipEvent_t* events;  // [layers]
-};
-
 static int checkpoint_layer(IrisSession* s, const CkptSink* sink, uint32_t l, uint32_t rows) {
     if (!sink) return 0;
     const size_t n = (size_t)rows * s->model->d.hidden;
@@ -477,18 +470,24 @@ static int mistral_layer(IrisSession* s, uint32_t l, uint32_t rows, bool slots, 
         g.prologue = PRO_RMSNORM;
         g.norm_w = L.norm_attn;
         g.norm_eps = d.norm_eps;
-        g.epilogue = EPI_ROPE_KV;
-        g.out = s->q;
-        g.out_stride = qw;
-        g.d_pos = s->d_pos;
-        g.inv_freq = m->inv_freq;
-        g.rope_sc = s->rope_sc;
-        g.head_dim = d.head_dim;
-        g.q_rows = qw;
-        g.kv_rows = kvw;
-        g.k_cache = s->k_cache[l];
-        g.k_pos_stride = s->k_pos_stride;
-        g.v_cache = s->v_cache[l];
+        if (s->batch) {  // rows of several requests: plain rows here
+            g.epilogue = EPI_STORE;
+            g.out = s->qkv;
+            g.out_stride = qw + 2 * kvw;
+        } else {
+            g.epilogue = EPI_ROPE_KV;
+            g.out = s->q;
+            g.out_stride = qw;
+            g.d_pos = s->d_pos;
+            g.inv_freq = m->inv_freq;
+            g.rope_sc = s->rope_sc;
+            g.head_dim = d.head_dim;
+            g.q_rows = qw;
+            g.kv_rows = kvw;
+            g.k_cache = s->k_cache[l];
+            g.k_pos_stride = s->k_pos_stride;
+            g.v_cache = s->v_cache[l];
+        }
         if (slots && ssq_x_in) {
             g.ssq_in = s->ssq_x;
             g.ssq_n = h_tiles;
@@ -496,32 +495,37 @@ static int mistral_layer(IrisSession* s, uint32_t l, uint32_t rows, bool slots, 
         with_gemm_space(g, s, rows);
         RT_CHECK(iris_gemv_launch(g, st));
         // 2. attention.
-        AttnArgs a{};
-        a.q = s->q;
-        a.q_stride = qw;
-        a.k_cache = s->k_cache[l];
-        a.k_pos_stride = s->k_pos_stride;
-        a.v_cache = s->v_cache[l];
-        a.kv_stride = kvw;
-        a.ctx = s->ctx;
-        a.ctx_stride = qw;
-        a.d_pos = s->d_pos;
-        a.heads = d.heads;
-        a.kv_heads = d.kv_heads;
-        a.head_dim = d.head_dim;
-        a.scaled = 1;
-        a.scale_q32 = d.attention_scale_q32;
-        a.window = 0;
-        a.planes = s->attn_planes;
-        a.scores = s->scores;
-        // One row: the values launch leaves the context row's digit planes
-        // for the O product.
-        const bool ctx_planes = iris_attention_decode_applies(a, rows, s->max_positions);
-        if (ctx_planes) {
-            a.ctx_planes = s->ctx_planes;
-            a.ctx_counts = s->ctx_counts;
+        bool ctx_planes = false;
+        if (s->batch) {
+            RT_CHECK(iris_batch_attention(s, l, rows));
+        } else {
+            AttnArgs a{};
+            a.q = s->q;
+            a.q_stride = qw;
+            a.k_cache = s->k_cache[l];
+            a.k_pos_stride = s->k_pos_stride;
+            a.v_cache = s->v_cache[l];
+            a.kv_stride = kvw;
+            a.ctx = s->ctx;
+            a.ctx_stride = qw;
+            a.d_pos = s->d_pos;
+            a.heads = d.heads;
+            a.kv_heads = d.kv_heads;
+            a.head_dim = d.head_dim;
+            a.scaled = 1;
+            a.scale_q32 = d.attention_scale_q32;
+            a.window = 0;
+            a.planes = s->attn_planes;
+            a.scores = s->scores;
+            // One row: the values launch leaves the context row's digit planes
+            // for the O product.
+            ctx_planes = iris_attention_decode_applies(a, rows, s->max_positions);
+            if (ctx_planes) {
+                a.ctx_planes = s->ctx_planes;
+                a.ctx_counts = s->ctx_counts;
+            }
+            RT_CHECK(iris_attention_launch(a, rows, s->max_positions, st));
         }
-        RT_CHECK(iris_attention_launch(a, rows, s->max_positions, st));
         // 3. attended = W_o ctx + x.
         g = GemvArgs{};
         g.w = q8_view(L.wo);
@@ -597,7 +601,8 @@ static int mistral_pass(IrisSession* s, uint32_t rows, const CkptSink* sink) {
     // The rows' RoPE (sin, cos) pairs, shared by every layer (for a one-row
     // pass after a selection, the selection kernel has formed them).
     if (!(rows == 1 && s->rope_ready) && d.layers)
-        RT_CHECK(iris_rope_table_launch(m->inv_freq, d.head_dim / 2, s->d_pos, rows, s->rope_sc, s->stream));
+        RT_CHECK(iris_rope_table_launch(m->inv_freq, d.head_dim / 2, s->d_pos, rows, s->rope_sc, s->stream,
+                                        s->batch != nullptr));
     s->rope_ready = false;
     // One row: sums of squares pass from each residual product to the norm
     // after it (hidden rows in 16-row tiles, within the slot count).
@@ -719,50 +724,55 @@ static int gemma_layer(IrisSession* s, uint32_t l, uint32_t rows, bool carry) {
         g.out_stride = qkvw;
         with_gemm_space(g, s, rows);
         RT_CHECK(iris_gemv_launch(g, st));
-        // 2. per-head norms and RoPE, K/V into the layer's own cache (:607-647)
-        GemmaQkvArgs qa{};
-        qa.qkv = s->qkv;
-        qa.qkv_stride = qkvw;
-        qa.heads = d.heads;
-        qa.kv_heads = d.kv_heads;
-        qa.head_dim = hd;
-        qa.rotary_dim = L.rotary_dim;
-        qa.q_norm = L.q_norm;
-        qa.k_norm = L.k_norm;
-        qa.eps = d.norm_eps;
-        qa.inv_freq = L.inv_freq;
-        qa.d_pos = s->d_pos;
-        qa.q_out = s->q;
-        qa.q_stride = qw;
-        qa.k_cache = s->k_cache[l];
-        qa.k_pos_stride = s->k_pos_stride;
-        qa.v_cache = s->v_cache[l];
-        RT_CHECK(iris_gemma_qkv_finish_launch(qa, rows, st));
-        // 3. attention over the window of the source layer's cache (:692-845)
-        AttnArgs a{};
-        a.q = s->q;
-        a.q_stride = qw;
-        a.k_cache = s->k_cache[L.kv_source];
-        a.k_pos_stride = s->k_pos_stride;
-        a.v_cache = s->v_cache[L.kv_source];
-        a.kv_stride = kvw;
-        a.ctx = s->ctx;
-        a.ctx_stride = qw;
-        a.d_pos = s->d_pos;
-        a.heads = d.heads;
-        a.kv_heads = d.kv_heads;
-        a.head_dim = hd;
-        a.scaled = 0;
-        a.window = L.window;
-        a.planes = s->attn_planes;
-        a.scores = s->scores;
-        // One row: the context row's digit planes too, for the O product.
-        const bool ctx_planes = iris_attention_decode_applies(a, rows, s->max_positions);
-        if (ctx_planes) {
-            a.ctx_planes = s->ctx_planes;
-            a.ctx_counts = s->ctx_counts;
+        bool ctx_planes = false;
+        if (s->batch) {
+            RT_CHECK(iris_batch_attention(s, l, rows));
+        } else {
+            // 2. per-head norms and RoPE, K/V into the layer's own cache (:607-647)
+            GemmaQkvArgs qa{};
+            qa.qkv = s->qkv;
+            qa.qkv_stride = qkvw;
+            qa.heads = d.heads;
+            qa.kv_heads = d.kv_heads;
+            qa.head_dim = hd;
+            qa.rotary_dim = L.rotary_dim;
+            qa.q_norm = L.q_norm;
+            qa.k_norm = L.k_norm;
+            qa.eps = d.norm_eps;
+            qa.inv_freq = L.inv_freq;
+            qa.d_pos = s->d_pos;
+            qa.q_out = s->q;
+            qa.q_stride = qw;
+            qa.k_cache = s->k_cache[l];
+            qa.k_pos_stride = s->k_pos_stride;
+            qa.v_cache = s->v_cache[l];
+            RT_CHECK(iris_gemma_qkv_finish_launch(qa, rows, st));
+            // 3. attention over the window of the source layer's cache (:692-845)
+            AttnArgs a{};
+            a.q = s->q;
+            a.q_stride = qw;
+            a.k_cache = s->k_cache[L.kv_source];
+            a.k_pos_stride = s->k_pos_stride;
+            a.v_cache = s->v_cache[L.kv_source];
+            a.kv_stride = kvw;
+            a.ctx = s->ctx;
+            a.ctx_stride = qw;
+            a.d_pos = s->d_pos;
+            a.heads = d.heads;
+            a.kv_heads = d.kv_heads;
+            a.head_dim = hd;
+            a.scaled = 0;
+            a.window = L.window;
+            a.planes = s->attn_planes;
+            a.scores = s->scores;
+            // One row: the context row's digit planes too, for the O product.
+            ctx_planes = iris_attention_decode_applies(a, rows, s->max_positions);
+            if (ctx_planes) {
+                a.ctx_planes = s->ctx_planes;
+                a.ctx_counts = s->ctx_counts;
+            }
+            RT_CHECK(iris_attention_launch(a, rows, s->max_positions, st));
         }
-        RT_CHECK(iris_attention_launch(a, rows, s->max_positions, st));
         // 4. attended = rms_norm(W_o ctx, post_attention) + x  (:879-892)
         g = GemvArgs{};
         g.w = q8_view(L.wo);
@@ -886,7 +896,7 @@ static int gemma_layer(IrisSession* s, uint32_t l, uint32_t rows, bool carry) {
 // row fits the slot counts and the staged-row limits).
 static bool gemma_carries(const IrisSession* s, uint32_t rows, const CkptSink* sink) {
     const uint32_t H = s->model->d.hidden;
-    return rows == 1 && !sink && H % 4 == 0 && (H + Q8_TILE_ROWS - 1) / Q8_TILE_ROWS <= GEMV_SSQ_SLOTS &&
+    return rows == 1 && !sink && !s->batch && H % 4 == 0 && (H + Q8_TILE_ROWS - 1) / Q8_TILE_ROWS <= GEMV_SSQ_SLOTS &&
            H <= 4096 && H <= I32_GEMV_MAX_STAGED;
 }
 
@@ -904,7 +914,7 @@ static int gemma_pass(IrisSession* s, uint32_t rows, const CkptSink* sink) {
     return 0;
 }
 
-static int session_pass(IrisSession* s, uint32_t rows, const CkptSink* sink) {
+int iris_session_pass(IrisSession* s, uint32_t rows, const CkptSink* sink) {
     s->ssq_x_valid = false;
     s->carry.pending = false;
     if (s->model->d.family == IRIS_FAMILY_GEMMA_DENSE) return gemma_pass(s, rows, sink);
@@ -969,7 +979,7 @@ static int session_head_select(IrisSession* s, uint32_t rows) {
 // gemma-dense model with layers its PLE row, has a non-finite block scale
 // (dequantize_row, q8.rs:76-92, when model.rs:316-330 or the PLE prepare
 // reads the row).
-static bool embedding_refused(const IrisModel* m, int32_t id) {
+bool iris_embedding_refused(const IrisModel* m, int32_t id) {
     return (!m->embed_bad.empty() && m->embed_bad[id]) || (!m->ple_bad.empty() && m->ple_bad[id]);
 }
 
@@ -980,7 +990,7 @@ static int session_reset_and_embed(IrisSession* s, const int32_t* ids, uint32_t 
     s->rope_ready = false;
     for (uint32_t i = 0; i < count; i++) {
         if (ids[i] < 0 || (uint32_t)ids[i] >= m->d.vocab) return IRIS_E_INVALID;
-        if (embedding_refused(m, ids[i])) return IRIS_E_SCALE;
+        if (iris_embedding_refused(m, ids[i])) return IRIS_E_SCALE;
     }
     RT_CHECK(iris_set_counters_launch(s->d_pos, (int32_t)start, s->d_step, 0, s->stream));
     RT_CHECK(hipMemcpyAsync(s->ids, ids, (size_t)count * 4, hipMemcpyHostToDevice, s->stream));
@@ -1088,7 +1098,7 @@ static int ensure_graph(IrisSession* s, bool fresh) {
     }
     hipGraph_t graph = nullptr;
     RT_CHECK(hipStreamBeginCapture(s->stream, hipStreamCaptureModeThreadLocal));
-    int rc = session_pass(s, 1, nullptr);
+    int rc = iris_session_pass(s, 1, nullptr);
     if (rc == 0) rc = session_head_select(s, 1);
     hipError_t st = hipStreamEndCapture(s->stream, &graph);
     if (rc == 0) rc = (int)st;
@@ -1100,7 +1110,7 @@ static int ensure_graph(IrisSession* s, bool fresh) {
 
 static int session_decode_pass(IrisSession* s, int use_graph) {
     if (!use_graph) {
-        RT_CHECK(session_pass(s, 1, nullptr));
+        RT_CHECK(iris_session_pass(s, 1, nullptr));
         return session_head_select(s, 1);
     }
     RT_CHECK(ensure_graph(s, false));
@@ -1112,8 +1122,14 @@ extern "C" {
 int iris_session_create(IrisModel* m, uint32_t max_positions, uint32_t max_rows, IrisSession** out) {
     if (!m || !out || !m->finalized || max_positions == 0 || max_rows == 0) return IRIS_E_INVALID;
     *out = nullptr;
-    const IrisModelDesc& d = m->d;
     if (max_rows > max_positions || max_positions > ATTN_MAX_KEYS) return IRIS_E_RANGE;
+    return iris_session_make(m, max_positions, max_rows, nullptr, out);
+}
+
+}  // extern "C"
+
+int iris_session_make(IrisModel* m, uint32_t max_positions, uint32_t max_rows, IrisBatch* batch, IrisSession** out) {
+    const IrisModelDesc& d = m->d;
     iris_gemv_prepare();
     IrisSession* s = new (std::nothrow) IrisSession();
     if (!s) return IRIS_E_NOMEM;
@@ -1121,13 +1137,14 @@ int iris_session_create(IrisModel* m, uint32_t max_positions, uint32_t max_rows,
     s->max_positions = max_positions;
     s->k_pos_stride = (max_positions + 63) & ~63u;
     s->max_rows = max_rows;
+    s->batch = batch;
     const size_t qw = (size_t)d.heads * m->max_head_dim;
     hipError_t st = hipStreamCreate(&s->stream);
     s->k_cache.assign(d.layers, nullptr);
     s->v_cache.assign(d.layers, nullptr);
     s->kv_lo.assign(d.layers, 0);
     s->kv_hi.assign(d.layers, 0);
-    for (uint32_t l = 0; l < d.layers && st == hipSuccess; l++) {
+    for (uint32_t l = 0; l < d.layers && st == hipSuccess && !batch; l++) {
         const size_t kvw = m->layers[l].kv_rows;
         st = hipMalloc((void**)&s->k_cache[l], (size_t)s->k_pos_stride * kvw * 4);
         if (st == hipSuccess) st = hipMalloc((void**)&s->v_cache[l], (size_t)max_positions * kvw * 4);
@@ -1142,7 +1159,7 @@ int iris_session_create(IrisModel* m, uint32_t max_positions, uint32_t max_rows,
     if (st == hipSuccess) st = hipMalloc((void**)&s->ssq_x, GEMV_SSQ_SLOTS * sizeof(int64_t));
     if (st == hipSuccess) st = hipMalloc((void**)&s->ssq_att, GEMV_SSQ_SLOTS * sizeof(int64_t));
     alloc(&s->q, (size_t)max_rows * qw);
-    alloc(&s->scores, attn_scores_ints(d.heads, s->k_pos_stride));
+    if (!batch) alloc(&s->scores, attn_scores_ints(d.heads, s->k_pos_stride));
     alloc(&s->ctx, (size_t)max_rows * qw);
     alloc(&s->gated, (size_t)max_rows * m->max_ffn);
     {
@@ -1179,6 +1196,8 @@ int iris_session_create(IrisModel* m, uint32_t max_positions, uint32_t max_rows,
         alloc(&s->token_limbs, (size_t)gemm_limb_ints((uint32_t)widest, max_rows));
         if (st == hipSuccess) st = hipMalloc((void**)&s->gated_gemm_planes, gemm_planes_bytes(m->max_ffn, max_rows));
         alloc(&s->gated_gemm_limbs, (size_t)gemm_limb_ints(m->max_ffn, max_rows));
+    }
+    if (max_rows > 1 && !batch) {
         AttnPlanes& ap = s->attn_planes;
         ap.qt_cap = (max_rows + 15) / 16;
         ap.ks_cap = (max_positions + 63) / 64;
@@ -1192,20 +1211,22 @@ int iris_session_create(IrisModel* m, uint32_t max_positions, uint32_t max_rows,
         alloc8((void**)&ap.kv_limbs, 2ull * d.kv_heads * ap.ks_cap);
         alloc8((void**)&ap.e_store, attn_e_store_bytes(d.heads, ap.qt_cap, ap.ks_cap));
     }
+    if (d.family == IRIS_FAMILY_GEMMA_DENSE || batch) alloc(&s->qkv, (size_t)max_rows * m->max_qkv);
     if (d.family == IRIS_FAMILY_GEMMA_DENSE) {
         const size_t lp = (size_t)d.layers * d.ple_width;
-        alloc(&s->qkv, (size_t)max_rows * m->max_qkv);
         alloc(&s->tmp, (size_t)max_rows * d.hidden);
         alloc(&s->ple_proj, (size_t)max_rows * lp);
         alloc(&s->ple_rows, (size_t)max_rows * lp);
         alloc(&s->ple_gated, (size_t)max_rows * d.ple_width);
     }
-    alloc(&s->logits, d.vocab);
     alloc(&s->ids, max_rows);
-    alloc(&s->tokens, max_positions + 1);
-    alloc(&s->d_pos, 1);
-    alloc(&s->d_step, 1);
-    if (st == hipSuccess) st = hipMalloc((void**)&s->sel_partial, (size_t)m->head->tiles * sizeof(uint64_t));
+    alloc(&s->d_pos, batch ? max_rows : 1);
+    if (!batch) {
+        alloc(&s->logits, d.vocab);
+        alloc(&s->tokens, max_positions + 1);
+        alloc(&s->d_step, 1);
+    }
+    if (st == hipSuccess && !batch) st = hipMalloc((void**)&s->sel_partial, (size_t)m->head->tiles * sizeof(uint64_t));
     if (st != hipSuccess) {
         iris_session_free(s);
         return (int)st;
@@ -1213,6 +1234,8 @@ int iris_session_create(IrisModel* m, uint32_t max_positions, uint32_t max_rows,
     *out = s;
     return 0;
 }
+
+extern "C" {
 
 void iris_session_free(IrisSession* s) {
     if (!s) return;
@@ -1326,7 +1349,7 @@ static int session_generate(IrisSession* s, const int32_t* prompt, uint32_t prom
         return 0;
     };
     RT_CHECK(session_reset_and_embed(s, prompt, prompt_len));
-    RT_CHECK(session_pass(s, prompt_len, nullptr));
+    RT_CHECK(iris_session_pass(s, prompt_len, nullptr));
     RT_CHECK(session_head_select(s, prompt_len));
     if (use_graph && tokens > 1) RT_CHECK(ensure_graph(s, true));
     RT_CHECK(step_done(0));
@@ -1351,7 +1374,7 @@ static int session_generate(IrisSession* s, const int32_t* prompt, uint32_t prom
     // Each selection but the last is embedded for the next pass
     // (executor.rs:157-183): a refused row fails the run there.
     for (uint32_t t = 0; t + 1 < count; t++)
-        if (embedding_refused(m, out_tokens[t])) return IRIS_E_SCALE;
+        if (iris_embedding_refused(m, out_tokens[t])) return IRIS_E_SCALE;
     *out_count = count;
     cover_all(s, 0, (uint32_t)end, true);
     return 0;
@@ -1408,7 +1431,7 @@ static int layer_range_run(IrisSession* s, const int32_t* ids, uint32_t count, u
     const IrisModelDesc& d = m->d;
     if (!out_rows && !out_hashes) {
         RT_CHECK(session_reset_and_embed(s, ids, count, start_position));
-        RT_CHECK(session_pass(s, count, nullptr));
+        RT_CHECK(iris_session_pass(s, count, nullptr));
         return (int)hipStreamSynchronize(s->stream);
     }
     RT_CHECK(ensure_checkpoint_space(s));
@@ -1418,7 +1441,7 @@ static int layer_range_run(IrisSession* s, const int32_t* ids, uint32_t count, u
     hipEvent_t* on_host = on_device + layers;
     const CkptSink sink{s->ckpt_dev, on_device};
     RT_CHECK(session_reset_and_embed(s, ids, count, start_position));
-    RT_CHECK(session_pass(s, count, &sink));
+    RT_CHECK(iris_session_pass(s, count, &sink));
     // A layer's hash is one serial chain over its rows (about 2 GB/s), the
     // longest part of a pass of few layers, so it starts with the first
     // quarter to arrive, and the copy into the caller's rows, with its page
@@ -1603,7 +1626,7 @@ int iris_session_time_pass(IrisSession* s, const int32_t* ids, uint32_t count, d
     uncover_all(s, 0, count, true);
     int rc = session_reset_and_embed(s, ids, count);
     if (rc == 0) rc = (int)hipEventRecord(e0, s->stream);
-    if (rc == 0) rc = session_pass(s, count, nullptr);
+    if (rc == 0) rc = iris_session_pass(s, count, nullptr);
     if (rc == 0) rc = (int)hipEventRecord(e1, s->stream);
     float t = 0.f;
     if (rc == 0) rc = (int)hipEventSynchronize(e1);
@@ -1638,7 +1661,7 @@ int iris_session_time_decode_launches(IrisSession* s, const int32_t* prompt, uin
     uncover_all(s, 0, (uint32_t)end, true);
     int rc = session_reset_and_embed(s, prompt, prompt_len);
     if (rc == 0) rc = (int)hipEventRecord(e0, s->stream);
-    if (rc == 0) rc = session_pass(s, prompt_len, nullptr);
+    if (rc == 0) rc = iris_session_pass(s, prompt_len, nullptr);
     if (rc == 0) rc = session_head_select(s, prompt_len);
     // Capture (outside the timed region) before timing the replays.
     if (rc == 0) rc = (int)hipEventRecord(e1, s->stream);
@@ -1659,7 +1682,7 @@ int iris_session_time_decode_launches(IrisSession* s, const int32_t* prompt, uin
         std::vector<int32_t> ids(steps + 1);
         rc = (int)hipMemcpy(ids.data(), s->tokens, (size_t)(steps + 1) * 4, hipMemcpyDeviceToHost);
         for (uint32_t t = 0; rc == 0 && t < steps; t++)
-            if (embedding_refused(s->model, ids[t])) rc = IRIS_E_SCALE;
+            if (iris_embedding_refused(s->model, ids[t])) rc = IRIS_E_SCALE;
     }
     hipEventDestroy(e0);
     hipEventDestroy(e1);

@@ -70,8 +70,13 @@ struct IrisModel {
 
 constexpr uint32_t CKPT_PIECES = 4, LOGITS_SLOTS = 4;
 
+struct IrisBatch;  // runtime_batch.hip
+
 struct IrisSession {
     IrisModel* model = nullptr;
+    // A batch's rows, buffers and stream: no caches of its own, d_pos holds
+    // each row's position, and the attention is iris_batch_attention.
+    IrisBatch* batch = nullptr;
     uint32_t max_positions = 0, max_rows = 0;
     uint32_t k_pos_stride = 0;  // positions per row of the transposed K cache: max_positions rounded up to 64
     hipStream_t stream = nullptr;
@@ -150,6 +155,23 @@ struct IrisSession {
     hipGraphExec_t graph_exec = nullptr;
     bool graph_keep_logits = false;
 };
+
+// Where a checkpointing pass leaves each layer's rows: a device copy per
+// layer, and an event recorded on the pass's stream once it is made.
+struct CkptSink {
+    int32_t* dev;        // [layers][rows][hidden]
+    hipEvent_t* events;  // [layers]
+};
+
+// A session's buffers; with `batch`, those of its passes (no K/V caches).
+int iris_session_make(IrisModel* m, uint32_t max_positions, uint32_t max_rows, IrisBatch* batch, IrisSession** out);
+// Every layer over the `rows` rows in s->x, their output back in s->x.
+int iris_session_pass(IrisSession* s, uint32_t rows, const CkptSink* sink);
+// A batch's step between a layer's q|k|v product (s->qkv) and its O product:
+// rotation, cache store and attention, into s->ctx.
+int iris_batch_attention(IrisSession* s, uint32_t layer, uint32_t rows);
+// True when embedding token `id` is refused.
+bool iris_embedding_refused(const IrisModel* m, int32_t id);
 
 // SHA-256 (FIPS 180-4): whole 64-byte blocks as they come, then the rest
 // (under 64 bytes).

@@ -58,6 +58,12 @@ def _declare():
                                                         C.POINTER(C.c_double), vp]),
         "iris_session_time_pass": (C.c_int, [vp, vp, u32, C.POINTER(C.c_double)]),
         "iris_session_read_kv": (C.c_int, [vp, u32, u32, u32, vp, vp]),
+        "iris_batch_create": (C.c_int, [vp, u32, u32, u32, u32, u32, pp]),
+        "iris_batch_free": (None, [vp]),
+        "iris_batch_prefill": (C.c_int, [vp, vp, vp, vp]),
+        "iris_batch_step": (C.c_int, [vp, vp, vp, vp, vp, vp]),
+        "iris_batch_release": (C.c_int, [vp, u32]),
+        "iris_batch_length": (C.c_int, [vp, u32, C.POINTER(u32)]),
         "iris_sha256_bytes": (C.c_int, [vp, u64, vp]),
     }
     for name, (res, args) in sig.items():
@@ -292,6 +298,159 @@ class Session:
     def free(self):
         if getattr(self, "_h", None):
             native.lib().iris_session_free(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+class Batch:
+    """Up to ``requests`` requests at a time over one paged K/V cache of
+    ``pages`` pages of ``page_size`` positions, each request up to
+    ``max_positions``, in passes of up to ``max_rows`` rows (iris_batch_*). A
+    request's tokens are those ``Session.generate`` selects for its prompt,
+    whatever runs beside it."""
+
+    MAX_STEP_ROWS = 64  # rows of one request in one step
+
+    def __init__(self, dm: DeviceModel, requests: int, pages: int, page_size: int, max_positions: int, max_rows: int):
+        L = _declare()
+        self.dm, self.requests, self.pages, self.page_size = dm, requests, pages, page_size
+        self.max_positions, self.max_rows = max_positions, max_rows
+        h = C.c_void_p()
+        native.check(L.iris_batch_create(dm.handle, requests, pages, page_size, max_positions, max_rows, C.byref(h)),
+                     "batch create")
+        self._h = h
+
+    def _gather(self, rows: dict):
+        """The requests' rows one after the other: (ids, counts)."""
+        for i in rows:
+            if not 0 <= i < self.requests:
+                raise ValueError(f"request {i} of {self.requests}")
+        parts = [np.ascontiguousarray(rows.get(i, ()), dtype=np.int32) for i in range(self.requests)]
+        return np.concatenate(parts), np.array([p.size for p in parts], dtype=np.uint32)
+
+    def prefill(self, prompts: dict) -> dict:
+        """{request: ids} into empty requests -> {request: next token}."""
+        ids, counts = self._gather(prompts)
+        out = np.empty(self.requests, dtype=np.int32)
+        native.check(native.lib().iris_batch_prefill(self._h, ids.ctypes.data, counts.ctypes.data, out.ctypes.data),
+                     "batch prefill")
+        return {i: int(out[i]) for i in range(self.requests) if counts[i]}
+
+    def step(self, rows: dict, parents: dict | None = None) -> dict:
+        """{request: [last token, drafted ids...]} (and, of requests whose
+        drafts are a tree, {request: each row's parent row}; the others' are
+        chains) -> {request: the tokens selected along the kept path}."""
+        ids, counts = self._gather(rows)
+        par = None
+        if parents:
+            chains = {i: range(-1, int(counts[i]) - 1) for i in range(self.requests)}
+            par, n = self._gather({**chains, **parents})
+            if not np.array_equal(n, counts):
+                raise ValueError("parents must name one row per row")
+        tokens = np.empty(max(ids.size, 1), dtype=np.int32)
+        kept = np.empty(self.requests, dtype=np.uint32)
+        native.check(native.lib().iris_batch_step(self._h, ids.ctypes.data, None if par is None else par.ctypes.data,
+                                                  counts.ctypes.data, tokens.ctypes.data, kept.ctypes.data), "batch step")
+        at = [0] + np.cumsum(counts, dtype=np.int64).tolist()
+        return {i: tokens[at[i]:at[i] + kept[i]].tolist() for i in range(self.requests) if counts[i]}
+
+    def release(self, request: int):
+        """Empties a request; its pages are free for the next call."""
+        native.check(native.lib().iris_batch_release(self._h, request), "batch release")
+
+    def length(self, request: int) -> int:
+        n = C.c_uint32()
+        native.check(native.lib().iris_batch_length(self._h, request, C.byref(n)), "batch length")
+        return n.value
+
+    def generate(self, prompts, tokens: int, draft=None) -> list:
+        """Greedy generation for each prompt: a list of GenerateResult, as
+        ``Session.generate`` gives them (without logits), over requests that
+        are all empty. Prompts wait until a request and enough pages for all
+        their positions are free.
+        ``draft(index, ids)`` (optional), called with a prompt's index and the
+        ids so far, proposes what may follow: (ids, parents), parents[j] the
+        place in ``ids`` of row j's parent, -1 for the last of the ids so far;
+        or (ids, None) for a chain. The tokens do not depend on it."""
+        prompts = [np.ascontiguousarray(p, dtype=np.int32) for p in prompts]
+        eos = self.dm.model.eos_token_ids
+        results = [GenerateResult([], None) for _ in prompts]
+        if tokens == 0:
+            return results
+        room = [p.size + tokens - 1 for p in prompts]  # positions a prompt's passes fill
+        pages = [-(-n // self.page_size) for n in room]
+        for p, n, held in zip(prompts, room, pages):
+            if p.size == 0:
+                raise native.IrisError(-1, "batch generate")
+            if n > min(self.max_positions, self.dm.desc.max_positions) or held > self.pages or p.size > self.max_rows:
+                raise native.IrisError(-5, "batch generate")
+        if any(self.length(i) for i in range(self.requests)):
+            raise native.IrisError(-4, "batch generate")
+        waiting, running = list(range(len(prompts))), {}  # request -> prompt
+
+        def took(request, new):
+            """The request's next tokens; True when it has ended."""
+            r = results[running[request]]
+            for t in new:
+                r.token_ids.append(t)
+                if t in eos or len(r.token_ids) == tokens:
+                    r.stop_reason = "eos" if t in eos else "max_new_tokens"
+                    self.release(request)
+                    del running[request]
+                    return True
+            return False
+
+        try:
+            while waiting or running:
+                start, rows = {}, 0
+                free = self.pages - sum(pages[p] for p in running.values())
+                for request in range(self.requests):
+                    if request in running or not waiting:
+                        continue
+                    p = waiting[0]
+                    if pages[p] > free or rows + prompts[p].size > self.max_rows:
+                        break
+                    start[request] = running[request] = waiting.pop(0)
+                    free -= pages[p]
+                    rows += prompts[p].size
+                if start:
+                    for request, token in self.prefill({r: prompts[p] for r, p in start.items()}).items():
+                        took(request, [token])
+                step, trees, rows = {}, {}, 0
+                for n, (request, p) in enumerate(running.items()):
+                    left = self.max_rows - rows - (len(running) - n)  # rows beside one of each request behind
+                    if rows == self.max_rows:
+                        break  # the others' turn comes with the next pass
+                    ids, last = results[p].token_ids, [results[p].token_ids[-1]]
+                    more = min(room[p] - prompts[p].size - len(ids) + 1, self.MAX_STEP_ROWS) - 1
+                    more = max(min(more, left), 0)
+                    if draft is not None and more:
+                        drafted, above = draft(p, prompts[p].tolist() + ids)
+                        last += [int(t) for t in drafted[:more]]
+                        if above is not None:
+                            trees[request] = [-1] + [int(a) + 1 for a in above[:more]]
+                    step[request] = last
+                    rows += len(last)
+                if step:
+                    done = self.step(step, trees)
+                    # A request that has had its turn goes to the back.
+                    for request, new in done.items():
+                        if not took(request, new):
+                            running[request] = running.pop(request)
+        except Exception:
+            for i in list(running):
+                self.release(i)
+            raise
+        return results
+
+    def free(self):
+        if getattr(self, "_h", None):
+            native.lib().iris_batch_free(self._h)
             self._h = None
 
     def __del__(self):

@@ -1,0 +1,227 @@
+"""GPU: several requests at a time over one paged cache, against the session
+that runs one (its tokens are the oracle's, tests/test_gpu_direct.py): prompts
+packed, single tokens, chains and trees of drafts, pages that come and go."""
+import random
+
+import numpy as np
+import pytest
+
+from iris_amd import native, synth
+from iris_amd.direct import Batch, DeviceModel, Session
+from oracle import cpu
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def device():
+    native.check(native.lib().q8gpu_init(), "q8gpu_init")
+
+
+def parity_gemma(eos=()):
+    return synth.gemma_model(synth.parity_gemma_shape(), 256, seed=5, eos_token_ids=eos)
+
+
+MODELS = {
+    "mistral": lambda: synth.mistral_model(128, 2, 4, 2, 32, 256, 512, seed=21, per_row_scale=False),
+    "mistral wide heads": lambda: synth.mistral_model(256, 3, 6, 2, 128, 512, 512, seed=22),
+    "mistral odd heads": lambda: synth.mistral_model(96, 2, 3, 3, 32, 160, 320, seed=23, per_row_scale=False, tied_head=True),
+    "gemma": lambda: synth.tiny_gemma(),
+    "gemma windows": parity_gemma,
+    "gemma two head sizes": lambda: synth.gemma4_e2b_scaled(),
+    "no layers": lambda: synth.mistral_model(128, 0, 4, 2, 32, 256, 512, seed=24),
+}
+_made = {}
+
+
+def made(name):
+    """The model on the device and its single-request session's tokens."""
+    if name not in _made:
+        dm = DeviceModel(MODELS[name]())
+        _made[name] = dm, Session(dm, 256, 160), {}
+    return _made[name]
+
+
+def alone(name, prompt, tokens):
+    dm, s, known = made(name)
+    key = (tuple(int(i) for i in prompt), tokens)
+    if key not in known:
+        known[key] = s.generate(prompt, tokens)
+    return known[key]
+
+
+def prompts(name, lens, seed=1):
+    vocab = made(name)[0].model.vocab
+    return [synth.token_ids(seed + i, n, vocab).astype(np.int32) for i, n in enumerate(lens)]
+
+
+def drafter(name, ps, tokens, seed, tree):
+    """Proposals that hold the true continuation or parts of it, and others."""
+    r, vocab = random.Random(seed), made(name)[0].model.vocab
+
+    def draft(p, ids):
+        true = alone(name, ps[p], tokens).token_ids[len(ids) - len(ps[p]):]
+        good = true[:r.randrange(0, 9)]
+        if not tree:
+            ids = good + [r.randrange(vocab) for _ in range(r.randrange(3))]
+            return (ids, None) if r.random() < 0.8 else (ids, list(range(-1, len(ids) - 1)))
+        out, above, spine = [], [], -1
+        for t in good:
+            for _ in range(r.randrange(3)):  # others beside the true one, and below each other
+                out.append(r.randrange(vocab))
+                above.append(r.choice([spine, spine, len(out) - 2, -1]))
+            out.append(t)
+            above.append(spine)
+            spine = len(out) - 1
+        for _ in range(r.randrange(3)):
+            out.append(r.randrange(vocab))
+            above.append(spine)
+        return out[:63], above[:63]
+
+    return draft
+
+
+@pytest.mark.parametrize("name", list(MODELS))
+@pytest.mark.parametrize("how", ["plain", "chain", "tree"])
+def test_batch_generates_what_a_session_does(name, how):
+    tokens, lens = 24, [5, 1, 37, 64, 12, 3, 90, 17]
+    ps = prompts(name, lens)
+    want = [alone(name, p, tokens) for p in ps]
+    b = Batch(made(name)[0], 5, 60, 16, 256, 160)
+    draft = None if how == "plain" else drafter(name, ps, tokens, 7, how == "tree")
+    for _ in range(2):  # and over pages that others have left
+        got = b.generate(ps, tokens, draft)
+        assert [g.token_ids for g in got] == [w.token_ids for w in want]
+        assert [g.stop_reason for g in got] == [w.stop_reason for w in want]
+
+
+def test_batch_tokens_are_the_oracles():
+    m = MODELS["mistral"]()
+    ps = [synth.token_ids(40 + i, n, 512).astype(np.int32) for i, n in enumerate((9, 2, 21))]
+    got = Batch(DeviceModel(m), 3, 30, 4, 64, 64).generate(ps, 8)
+    for p, g in zip(ps, got):
+        assert g.token_ids == cpu.OracleRun(m, 64).generate(list(p), 8, keep_logits=True)[0]
+
+
+def test_selected_tokens_vary():
+    # So that a wrong row, position or page would show in the tokens.
+    seen = {t for n in ("mistral", "gemma windows", "gemma two head sizes") for p in prompts(n, [5, 37, 64, 12, 90, 17])
+            for t in alone(n, p, 24).token_ids}
+    assert len(seen) > 20
+
+
+@pytest.mark.parametrize("name", ["mistral wide heads", "gemma windows"])
+def test_batch_stops_at_end_ids(name):
+    ps = prompts(name, [5, 37, 64, 12])
+    free = [alone(name, p, 24).token_ids for p in ps]
+    m = MODELS[name]()
+    m.eos_token_ids = (free[0][3], free[2][7])
+    dm = DeviceModel(m)
+    s = Session(dm, 256, 160)
+    want = [s.generate(p, 24) for p in ps]
+    assert {w.stop_reason for w in want} >= {"eos"}
+    for tree in (False, True):
+        got = Batch(dm, 3, 40, 16, 256, 160).generate(ps, 24, drafter(name, ps, 24, 3, tree))
+        assert [g.token_ids for g in got] == [w.token_ids for w in want]
+        assert [g.stop_reason for g in got] == [w.stop_reason for w in want]
+
+
+@pytest.mark.parametrize("requests, pages, page, rows", [(1, 8, 16, 96), (8, 9, 16, 90), (4, 30, 4, 90), (6, 2, 128, 128),
+                                                         (3, 200, 4, 91)])
+def test_batch_of_few_pages_and_rows(requests, pages, page, rows):
+    name, tokens = "mistral", 20
+    ps = prompts(name, [90, 3, 40, 40, 2, 61, 8], seed=60)
+    b = Batch(made(name)[0], requests, pages, page, 256, rows)
+    got = b.generate(ps, tokens, drafter(name, ps, tokens, 9, True))
+    assert [g.token_ids for g in got] == [alone(name, p, tokens).token_ids for p in ps]
+    assert all(b.length(i) == 0 for i in range(requests))
+
+
+@pytest.mark.parametrize("name", ["mistral", "gemma two head sizes"])
+def test_step_keeps_the_path_of_the_selections(name):
+    ps = prompts(name, [30, 7], seed=80)
+    true = [alone(name, p, 12).token_ids for p in ps]
+    b = Batch(made(name)[0], 4, 20, 16, 128, 64)
+    assert b.prefill({1: ps[0], 3: ps[1]}) == {1: true[0][0], 3: true[1][0]}
+    assert [b.length(i) for i in range(4)] == [0, 30, 0, 7]
+    # Request 1: the true tokens at rows 2, 5 and 6 among others; a second copy
+    # of a true token stands behind the first. Request 3 is a single token.
+    wrong = (true[0][1] + 1) % made(name)[0].model.vocab
+    rows = [true[0][0], wrong, true[0][1], true[0][1], wrong, true[0][2], true[0][3], wrong]
+    parents = [-1, 0, 0, 0, 1, 2, 5, 6]
+    got = b.step({1: rows, 3: [true[1][0]]}, {1: parents})
+    assert got == {1: true[0][1:5], 3: [true[1][1]]}
+    assert [b.length(i) for i in range(4)] == [0, 34, 0, 8]
+    for j in range(5, 8):
+        got = b.step({1: [true[0][j - 1]], 3: [true[1][j - 4], true[1][j - 4]]})
+        assert got[1] == [true[0][j]] and got[3][0] == true[1][j - 3]
+        b_len = b.length(3)
+        if len(got[3]) == 2:  # the repeated token was the model's choice too
+            break
+    b.release(1)
+    assert b.length(1) == 0 and b.length(3) == b_len
+    again = b.prefill({1: ps[0], 0: ps[0]})
+    assert again == {0: true[0][0], 1: true[0][0]}
+
+
+def refused(code, call):
+    with pytest.raises(native.IrisError) as e:
+        call()
+    assert e.value.code == code
+
+
+def test_batch_refusals_change_nothing():
+    name = "mistral"
+    dm = made(name)[0]
+    b = Batch(dm, 2, 4, 16, 48, 40)
+    p = prompts(name, [20, 30], seed=90)
+    true = alone(name, p[0], 8).token_ids
+    refused(-1, lambda: b.prefill({0: [512]}))
+    refused(-1, lambda: b.prefill({0: [-1]}))
+    refused(-5, lambda: b.prefill({0: [1] * 41}))                # rows
+    refused(-5, lambda: Batch(dm, 2, 2, 16, 48, 64).prefill({0: [1] * 20, 1: [1] * 20}))  # pages
+    refused(-5, lambda: Batch(dm, 2, 9, 16, 48, 64).prefill({0: [1] * 49}))  # positions
+    refused(-4, lambda: b.step({0: [1]}))                        # nothing held
+    assert b.prefill({0: p[0]}) == {0: true[0]}
+    refused(-4, lambda: b.prefill({0: p[1]}))                    # holds positions
+    refused(-4, lambda: b.generate([p[1]], 2))
+    refused(-5, lambda: b.step({0: [true[0]] * 29}))             # positions
+    refused(-5, lambda: b.prefill({1: [1] * 40}))                # pages
+    refused(-1, lambda: b.step({0: [true[0], 512]}))
+    assert b.length(0) == 20
+    for j in range(1, 8):
+        assert b.step({0: [true[j - 1]]}) == {0: [true[j]]}
+    with pytest.raises(ValueError):
+        b.step({2: [1]})
+    with pytest.raises(ValueError):
+        b.step({0: [1, 2]}, {0: [-1]})
+
+
+def test_batch_of_too_many_rows_of_a_request():
+    b = Batch(made("mistral")[0], 1, 99, 16, 400, 200)
+    first = b.prefill({0: [1, 2, 3]})[0]
+    refused(-5, lambda: b.step({0: [first] * 65}))
+    assert len(b.step({0: [first] * 64})[0]) >= 1
+
+
+@pytest.mark.parametrize("kw, code", [
+    (dict(requests=0), -1), (dict(pages=0), -1), (dict(page_size=0), -1), (dict(page_size=24), -1), (dict(page_size=2048), -1),
+    (dict(max_positions=0), -1), (dict(max_rows=0), -1), (dict(requests=4097), -5), (dict(max_positions=(1 << 20) + 1), -5),
+    (dict(pages=1 << 27), -5)])
+def test_batch_create_refusals(kw, code):
+    args = dict(requests=2, pages=4, page_size=16, max_positions=64, max_rows=32)
+    refused(code, lambda: Batch(made("mistral")[0], **{**args, **kw}))
+
+
+def test_two_batches_and_a_session_in_turns():
+    name = "gemma windows"
+    ps = prompts(name, [25, 6], seed=95)
+    true = [alone(name, p, 10).token_ids for p in ps]
+    dm, s, _ = made(name)
+    bs = [Batch(dm, 2, 20, 16, 64, 64) for _ in ps]
+    for b, p, t in zip(bs, ps, true):
+        assert b.prefill({1: p}) == {1: t[0]}
+    for j in range(1, 10):
+        for b, t in zip(bs, true):
+            assert b.step({1: [t[j - 1]]}) == {1: [t[j]]}
+        assert s.generate(ps[j % 2], 10).token_ids == true[j % 2]
