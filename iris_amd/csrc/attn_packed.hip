@@ -185,7 +185,7 @@ struct PackedSmem {
 
 // The parts of the keys that the waves of one dimension tile share.
 template <uint32_t HD, int NW>
-constexpr uint32_t key_parts() { return NW * 16 > HD ? NW * 16 / HD : 1; }
+constexpr uint32_t key_parts() { return NW * 32 > HD ? NW * 32 / HD : 1; }
 
 // One (16 rows, head). NW waves; SPILL: tiles past s.lds_tiles in the work
 // space (`spill`).
@@ -445,22 +445,44 @@ __device__ __forceinline__ void packed_rows(const IrisPackedAttention& a, const 
 #pragma unroll
         for (int j = 0; j < NARROW + 1; j++) acc[d][j] = v4i{0, 0, 0, 0};
     uint32_t any_wide = 0;
-#pragma unroll 1
-    for (uint32_t ks = ks0 + part; ks < ks1; ks += PARTS) {
-        v4i vf[DTW][NARROW];
-        uint32_t wide = 0;
+    auto load_values = [&](uint32_t ks, v4i (&vf)[DTW][NARROW]) __attribute__((always_inline)) {
 #pragma unroll
         for (uint32_t d = 0; d < DTW; d++) {
 #pragma unroll
             for (int b = 0; b < NARROW; b++)
                 vf[d][b] = *(const v4i*)(vb + b * s.kv_plane + ((size_t)ks * DT + dt0 + d) * TILE_BYTES);
-            if (d % 4 == 0) wide |= (uint32_t)vw[ks * DS + d / 4] << d / 4;
+            if (d % 4 == 0) any_wide |= vw[ks * DS + d / 4];
         }
+    };
+    auto add_values = [&](uint32_t ks, const v4i (&vf)[DTW][NARROW]) __attribute__((always_inline)) {
         v4i w0, w1;
         load_weights(ks, w0, w1);
 #pragma unroll
         for (uint32_t d = 0; d < DTW; d++) value_step<NARROW>(w0, w1, vf[d], acc[d]);
-        any_wide |= wide;
+    };
+    // A step's values are loaded during the step before, where the registers
+    // allow. (Past the last: it again.)
+    if constexpr (DTW <= 2) {
+        v4i even[DTW][NARROW], odd[DTW][NARROW];
+        uint32_t ks = ks0 + part;
+        if (ks < ks1) load_values(ks, even);
+#pragma unroll 1
+        for (; ks + PARTS < ks1; ks += 2 * PARTS) {
+            load_values(ks + PARTS, odd);
+            __builtin_amdgcn_sched_barrier(0);  // (the loads stay ahead of the products)
+            add_values(ks, even);
+            load_values(min(ks + 2 * PARTS, ks1 - 1), even);
+            __builtin_amdgcn_sched_barrier(0);
+            add_values(ks + PARTS, odd);
+        }
+        if (ks < ks1) add_values(ks, even);
+    } else {
+#pragma unroll 1
+        for (uint32_t ks = ks0 + part; ks < ks1; ks += PARTS) {
+            v4i vf[DTW][NARROW];
+            load_values(ks, vf);
+            add_values(ks, vf);
+        }
     }
     uint64_t tot[DTW][4];
 #pragma unroll
