@@ -108,7 +108,7 @@ struct Places {
     __device__ __forceinline__ const int32_t* four(const int32_t* base, uint32_t key) const { return at(base, min(key, last & ~3u)); }
 };
 
-constexpr uint32_t MAX_CHUNK = 512;
+constexpr uint32_t MAX_CHUNK = 1024;
 constexpr uint32_t CHUNK_PAGES = MAX_CHUNK / 4 + 1;
 
 // The workgroup's places; s_page has CHUNK_PAGES entries. A barrier follows.
@@ -1102,6 +1102,11 @@ uint64_t tree_space(const IrisPagedKv& c, const IrisTreeAttention& a, uint8_t* b
     // 50 / 40, 32 at 700 (1024) 60 / 45.
     const uint64_t groups = bg * s->row_tiles * ((c.head_dim + SHORT_DIMS - 1) / SHORT_DIMS);
     s->short_tiles = tiles <= SHORT_TILES && groups <= 256 ? (uint32_t)tiles : 0;
+    // About 1024 workgroups, of at most 1024 positions: each begins with some
+    // microseconds of dependent loads, and its sums are written and read again.
+    // us, at most 512 / 1024 / 2048 positions: 4 tokens at up to 32700 145 / 127 /
+    // 127, 32 trees of 25 at up to 8000 563 / 520 / 582, 16 tokens at up to 20000
+    // 280 / 290 / 357, 64 at up to 2000 122 / 128 / 129.
     const uint64_t want = std::max<uint64_t>(1, 1024 / bg);
     s->chunk = (uint32_t)std::min<uint64_t>(MAX_CHUNK, std::max<uint64_t>(STEP, ((span + want - 1) / want + STEP - 1) & ~uint64_t(STEP - 1)));
     s->chunks = (uint32_t)((span + s->chunk - 1) / s->chunk);
