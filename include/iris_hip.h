@@ -462,7 +462,8 @@ int iris_paged_plan(const IrisPagedPlan* plan, void* stream);
 
 /* Writes rows of keys and values (kv_heads * head_dim values each, strides in
  * values, multiples of 4, 16-byte aligned) to their slots; a row whose slot is
- * outside the cache (-1) is skipped. Two rows of one slot: either one. */
+ * outside the cache (-1) is skipped. Two rows of one slot: either one. At most
+ * 2^24 - 1 rows. */
 int iris_paged_store(const IrisPagedKv* cache, const int32_t* k, uint32_t k_stride, const int32_t* v,
                      uint32_t v_stride, const int32_t* slots, uint32_t rows, void* stream);
 
@@ -473,8 +474,9 @@ int iris_paged_store(const IrisPagedKv* cache, const int32_t* k, uint32_t k_stri
  * 16-byte aligned; out overlaps none of the others.
  *   scaled      1: scores are the scaled dot product (scale_q32, mistral);
  *               0: the requantized dot product (gemma)
- *   rows        rows of q, k, v and out; rows from row_start[sequences] on
- *               are left as they were
+ *   rows        rows of q, k, v and out, rows * heads under 2^26 (and rows *
+ *               (heads + 24 kv_heads) under 2^30); rows from
+ *               row_start[sequences] on are left as they were
  *   max_length  at least the longest sequence, at most 65535; a row that lies
  *               deeper in its sequence is left as it was
  *   status      (nullable) set to IRIS_E_RANGE where such a row was found;
@@ -512,7 +514,8 @@ int iris_attention_packed(const IrisPackedAttention* a, void* d_workspace, uint6
  *                  positions pass these bounds or its table (its rows are left
  *                  as they were), to IRIS_E_INVALID where the table names a
  *                  page outside the cache (read as zeros); never cleared here
- * The rest as in IrisPackedAttention. */
+ * requests * kv_heads and max_nodes * heads / kv_heads are at most 65535. The
+ * rest as in IrisPackedAttention. */
 typedef struct IrisTreeAttention {
     const int32_t* q;
     int32_t* out;
@@ -535,8 +538,8 @@ int iris_attention_tree(const IrisPagedKv* cache, const IrisTreeAttention* a, vo
 /* Greedy generation of several requests at a time over one paged cache of
  * `pages` pages of page_size positions (of every layer that has keys of its
  * own), each up to max_positions (at most 2^20), in passes of up to max_rows
- * rows; at most 4096 requests, requests * kv_heads at most 65535. Both
- * families. Every call is synchronous, on a stream of the batch's own; calls
+ * rows (at most 65535); at most 4096 requests, requests * kv_heads at most
+ * 65535. Both families. Every call is synchronous, on a stream of the batch's own; calls
  * of one batch must not overlap. A refused call (IRIS_E_INVALID, _SCALE,
  * _RANGE, _STATE of a request's length) changes nothing; after any other
  * error the batch's state is unknown and every call but iris_batch_free

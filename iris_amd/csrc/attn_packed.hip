@@ -598,8 +598,10 @@ int packed_check(const IrisPackedAttention* a) {
     if (a->q_stride < q || a->out_stride < q || a->k_stride < kv || a->v_stride < kv) return IRIS_E_INVALID;
     if (a->rows > INT32_MAX - 64u || a->sequences > INT32_MAX || a->max_length > ATTN_MAX_KEYS) return IRIS_E_RANGE;
     if (!a->max_length && a->rows && a->sequences) return IRIS_E_INVALID;
-    // Workgroups and waves are counted in 32 bits.
-    if (((uint64_t)a->rows / 16 + 8) * (a->heads + 24ull * a->kv_heads) > INT32_MAX) return IRIS_E_RANGE;
+    // A launch has under 2^32 threads: up to 1024 for 16 rows of a head, 64 for
+    // a tile of digit planes.
+    if (((uint64_t)a->rows + 15) / 16 * a->heads >= 1u << 22) return IRIS_E_RANGE;
+    if (((uint64_t)a->rows / 16 + 8) * (a->heads + 24ull * a->kv_heads) >= 1u << 26) return IRIS_E_RANGE;
     return 0;
 }
 

@@ -1081,7 +1081,9 @@ int tree_check(const IrisPagedKv* c, const IrisTreeAttention* a) {
         return IRIS_E_INVALID;
     if (a->max_nodes > TREE_MAX_NODES || a->max_positions > TREE_MAX_POSITIONS || a->rows > INT32_MAX)
         return IRIS_E_RANGE;
-    if ((uint64_t)a->requests * c->kv_heads > 65535) return IRIS_E_RANGE;  // a launch's third dimension
+    // A launch's second and third dimensions.
+    if ((uint64_t)a->requests * c->kv_heads > 65535 || (uint64_t)a->max_nodes * (a->heads / c->kv_heads) > 65535)
+        return IRIS_E_RANGE;
     return 0;
 }
 

@@ -220,8 +220,9 @@ int iris_paged_store(const IrisPagedKv* c, const int32_t* k, uint32_t k_stride, 
     if (rc) return rc;
     const uint64_t width = (uint64_t)c->kv_heads * c->head_dim;
     if (!k || !v || !slots || misaligned(k) || misaligned(v) || k_stride % 4 || v_stride % 4 || k_stride < width ||
-        v_stride < width || rows > INT32_MAX)
+        v_stride < width)
         return IRIS_E_INVALID;
+    if (rows >= 1u << 24) return IRIS_E_RANGE;  // a launch has under 2^32 threads
     if (!rows) return 0;
     hipLaunchKernelGGL(store_kernel, dim3(rows), dim3(256), 0, (hipStream_t)stream, *c, k, k_stride, v, v_stride, slots,
                        rows);

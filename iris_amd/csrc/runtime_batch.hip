@@ -387,7 +387,8 @@ int iris_batch_create(IrisModel* m, uint32_t requests, uint32_t pages, uint32_t 
     if (!m || !out || !m->finalized || !requests || !pages || !max_positions || !max_rows) return IRIS_E_INVALID;
     *out = nullptr;
     const IrisModelDesc& d = m->d;
-    if (requests > 4096 || (d.layers && (uint64_t)requests * d.kv_heads > 65535) || max_positions > TREE_MAX_POSITIONS)
+    // Rows are a launch's second dimension in the layers' kernels.
+    if (requests > 4096 || max_rows > 65535 || max_positions > TREE_MAX_POSITIONS)
         return IRIS_E_RANGE;
     // What the paged operators take, layer by layer (the addresses stand for
     // the pass's; nothing is read).

@@ -207,7 +207,7 @@ def test_batch_of_too_many_rows_of_a_request():
 @pytest.mark.parametrize("kw, code", [
     (dict(requests=0), -1), (dict(pages=0), -1), (dict(page_size=0), -1), (dict(page_size=24), -1), (dict(page_size=2048), -1),
     (dict(max_positions=0), -1), (dict(max_rows=0), -1), (dict(requests=4097), -5), (dict(max_positions=(1 << 20) + 1), -5),
-    (dict(pages=1 << 27), -5)])
+    (dict(max_rows=65536), -5), (dict(pages=1 << 27), -5)])
 def test_batch_create_refusals(kw, code):
     args = dict(requests=2, pages=4, page_size=16, max_positions=64, max_rows=32)
     refused(code, lambda: Batch(made("mistral")[0], **{**args, **kw}))

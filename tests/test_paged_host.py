@@ -67,6 +67,11 @@ def test_store_refusals(args):
     refused(lambda: paged.store(cache(), *args, 3), -1)
 
 
+def test_store_of_too_many_rows():
+    refused(lambda: paged.store(cache(), A, 128, A, 128, A, 1 << 24), -5)
+    paged.store(cache(), A, 128, A, 128, A, 0)
+
+
 @pytest.mark.parametrize("kw, code", [
     (dict(q=None), -1), (dict(k=None), -1), (dict(v=None), -1), (dict(out=None), -1), (dict(row_start=None), -1),
     (dict(q=A + 4), -1), (dict(k=A + 4), -1), (dict(v=A + 4), -1), (dict(out=A + 4), -1), (dict(q_stride=258), -1),
@@ -74,7 +79,8 @@ def test_store_refusals(args):
     (dict(k_stride=124), -1), (dict(v_stride=124), -1), (dict(out_stride=252), -1), (dict(heads=0), -1),
     (dict(kv_heads=0), -1), (dict(heads=3), -1), (dict(head_dim=0), -1), (dict(head_dim=66), -1),
     (dict(head_dim=516, q_stride=4096, k_stride=4096, v_stride=4096, out_stride=4096), -1), (dict(max_length=0), -1),
-    (dict(max_length=65536), -5), (dict(rows=1 << 31), -5)])
+    (dict(max_length=65536), -5), (dict(rows=1 << 31), -5), (dict(rows=(1 << 24) + 1), -5),
+    (dict(rows=1 << 20, heads=64, kv_heads=64, q_stride=4096, k_stride=4096, v_stride=4096, out_stride=4096), -5)])
 def test_packed_refusals(kw, code):
     refused(lambda: paged.attend_packed(packed(**kw), A, 1 << 40), code)
     assert paged.packed_workspace_bytes(packed(**kw)) == 0
@@ -97,7 +103,7 @@ def test_packed_workspace():
     (dict(out_stride=258), -1), (dict(q_stride=252), -1), (dict(out_stride=252), -1), (dict(heads=0), -1),
     (dict(heads=3), -1), (dict(table_stride=0), -1), (dict(max_nodes=0), -1), (dict(max_positions=0), -1),
     (dict(max_nodes=65), -5), (dict(max_positions=(1 << 20) + 1), -5), (dict(rows=1 << 31), -5),
-    (dict(requests=65536), -5)])
+    (dict(requests=65536), -5), (dict(heads=2050, max_nodes=64, q_stride=1 << 18, out_stride=1 << 18), -5)])
 def test_tree_refusals(kw, code):
     refused(lambda: paged.attend_tree(cache(), tree(**kw), A, 1 << 40), code)
     assert paged.tree_workspace_bytes(cache(), tree(**kw)) == 0
