@@ -174,7 +174,7 @@ __device__ __forceinline__ uint32_t chunks_of(const TreeSpace& s, const Request&
 // 65 us, 206 MB of keys at 3.2 TB/s; a workgroup's first loads depend on each
 // other (request, pages, keys), and twelve waves a CU hide only a part of it
 // (sixteen spill registers: 85 us). 32 trees of 25 at up to 8000: 160 us, the
-// matrix cores and the vector units in half of the cycles each.
+// vector units issue in 42% of the cycles, the matrix cores are busy in 18%.
 template <uint32_t HD, bool FULL>
 __global__ __launch_bounds__(256, HD >= 512 ? 1 : HD >= 256 ? 2 : 3) void tree_scores_kernel(const IrisPagedKv c, const IrisTreeAttention a,
                                                                              const TreeSpace s) {
@@ -1174,6 +1174,8 @@ int tree_launch(const IrisPagedKv& c, const IrisTreeAttention& a, const TreeSpac
                            dim3(s.chunks | 1, bg, (s.row_tiles + MANY - 1) / MANY * (HD / (64 * value_blocks(HD)))),
                            dim3(MANY * value_blocks(HD) * 64), 0, stream, c, a, s);
     const uint32_t pairs = a.max_nodes * (a.heads / c.kv_heads);
+    // us, shared by four waves / one: 4 tokens at up to 32700 (32 chunks) 5.0 / 7.0,
+    // 12 trees of 9 in a window (18) 6.0 / 6.5, 32 of 25 at up to 8000 (8) 33 / 17.
     if (s.chunks > 8) hipLaunchKernelGGL((tree_join_kernel<HD, true>), dim3(bg, pairs), dim3(256), 0, stream, c, a, s);
     else hipLaunchKernelGGL((tree_join_kernel<HD, false>), dim3(bg, (pairs + 3) / 4), dim3(256), 0, stream, c, a, s);
     return (int)hipGetLastError();
