@@ -225,3 +225,34 @@ def test_two_batches_and_a_session_in_turns():
         for b, t in zip(bs, true):
             assert b.step({1: [t[j - 1]]}) == {1: [t[j]]}
         assert s.generate(ps[j % 2], 10).token_ids == true[j % 2]
+
+
+def test_step_of_more_rows_than_logits_are_held_for():
+    # 3 requests of 41 rows: the last token and the 40 that follow it.
+    name = "mistral wide heads"
+    ps = prompts(name, [9, 30, 2], seed=110)
+    true = [alone(name, p, 43).token_ids for p in ps]
+    b = Batch(made(name)[0], 3, 40, 16, 128, 130)
+    b.prefill(dict(enumerate(ps)))
+    got = b.step({i: t[:41] for i, t in enumerate(true)})
+    assert got == {i: t[1:42] for i, t in enumerate(true)}
+    assert b.step({i: [t[41]] for i, t in enumerate(true)}) == {i: [t[42]] for i, t in enumerate(true)}
+
+
+@pytest.mark.parametrize("name", ["mistral", "gemma windows"])
+def test_batch_of_one_row(name):
+    b = Batch(made(name)[0], 2, 9, 4, 32, 1)
+    ps = [np.array([5], np.int32), np.array([300], np.int32)]
+    assert [g.token_ids for g in b.generate(ps, 9)] == [alone(name, p, 9).token_ids for p in ps]
+
+
+def test_batch_refuses_a_row_without_finite_scales():
+    m = synth.mistral_model(128, 1, 4, 2, 32, 256, 512, seed=25, per_row_scale=False)
+    raw = m.tensors["model.language_model.embed_tokens.weight"].copy()
+    raw[7, 35] = 0x7C  # the second block's scale
+    m.tensors["model.language_model.embed_tokens.weight"] = raw
+    b = Batch(DeviceModel(m), 2, 8, 16, 64, 32)
+    refused(-2, lambda: b.prefill({0: [1, 7]}))
+    token = b.prefill({0: [1, 6]})[0]
+    refused(-2, lambda: b.step({0: [token, 7]}))
+    assert len(b.step({0: [token]})[0]) == 1
