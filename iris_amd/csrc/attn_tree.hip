@@ -119,13 +119,23 @@ struct Places {
 constexpr uint32_t MAX_CHUNK = 1024;
 constexpr uint32_t CHUNK_PAGES = MAX_CHUNK / 4 + 1;
 
+// This thread's table entry of the `count` positions from key0 on, where no
+// window moves them: on its way while the request is read.
+__device__ __forceinline__ uint32_t early_page(const IrisPagedKv& c, const IrisTreeAttention& a, uint32_t request, uint32_t key0,
+                                               uint32_t count) {
+    const uint32_t log = 31u - __clz((int)c.page_size);
+    if (a.window || threadIdx.x > count >> log) return 0;
+    const int32_t* table = a.table + (size_t)request * a.table_stride;
+    return (uint32_t)load1(table + min((key0 >> log) + threadIdx.x, a.table_stride - 1));
+}
+
 // The workgroup's places; s_page has CHUNK_PAGES entries. A barrier follows.
 __device__ __forceinline__ Places places(const IrisPagedKv& c, const IrisTreeAttention& a, const Request& r, uint32_t g,
-                                         uint32_t key0, uint32_t key1, uint64_t* s_page) {
+                                         uint32_t key0, uint32_t key1, uint64_t* s_page, uint32_t early) {
     const size_t head = (size_t)c.page_size * c.head_dim;
     const uint32_t log = 31u - __clz((int)c.page_size), first = key0 >> log, n = ((key1 - 1) >> log) - first + 1;
     for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
-        const uint32_t p = (uint32_t)r.table[first + i];
+        const uint32_t p = i == threadIdx.x && !a.window ? early : (uint32_t)r.table[first + i];
         s_page[i] = p < c.pages ? p * (c.kv_heads * head) : ~0ull;
         if (p >= c.pages && a.status) *a.status = IRIS_E_INVALID;
     }
@@ -188,12 +198,13 @@ __global__ __launch_bounds__(256, HD >= 512 ? 1 : HD >= 256 ? 2 : 3) void tree_s
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = wave_index(), grp = lane >> 4;
     const uint32_t chunk = blockIdx.x, rt0 = blockIdx.z * RB, bg = blockIdx.y, g = bg % c.kv_heads;
     const uint32_t group = a.heads / c.kv_heads;
+    const uint32_t early = early_page(c, a, bg / c.kv_heads, chunk * s.chunk, s.chunk);
     Request r;
     if (!read_request(c, a, bg / c.kv_heads, r)) return;
     const uint32_t key0 = r.base + chunk * s.chunk, pairs = r.rows * group;
     if (key0 >= r.total || rt0 * 16 >= pairs) return;
     const uint32_t key1 = min(key0 + s.chunk, r.total), tiles = min(RB, (pairs - rt0 * 16 + 15) / 16);
-    const Places at = places(c, a, r, g, key0, key1, s_page);
+    const Places at = places(c, a, r, g, key0, key1, s_page, early);
     auto query = [&](uint32_t rt) {
         const uint32_t pair = min((rt0 + rt) * 16 + (lane & 15), pairs - 1);
         return a.q + (size_t)(r.row0 + pair / group) * a.q_stride + (size_t)(g * group + pair % group) * c.head_dim;
@@ -472,12 +483,13 @@ __global__ __launch_bounds__((HD / 64 > 4 ? HD : 256), 2) void tree_values_kerne
     uint4* s_w = (uint4*)(s_sums + 16 * HD);
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = wave_index(), grp = lane >> 4;
     const uint32_t chunk = blockIdx.x, bg = blockIdx.y, g = bg % c.kv_heads, group = a.heads / c.kv_heads;
+    const uint32_t early = early_page(c, a, bg / c.kv_heads, chunk * s.chunk, s.chunk);
     Request r;
     if (!read_request(c, a, bg / c.kv_heads, r)) return;
     const uint32_t key0 = r.base + chunk * s.chunk, rows = r.rows * group;
     if (key0 >= r.total) return;
     const uint32_t n = min(s.chunk, r.total - key0), steps = (n + STEP - 1) / STEP, kt1 = (n + 15) / 16;
-    const Places at = places(c, a, r, g, key0, key0 + n, s_page);
+    const Places at = places(c, a, r, g, key0, key0 + n, s_page, early);
     for (uint32_t i = tid; i < 16 * HD; i += WAVES * 64) s_sums[i] = 0;
     for (uint32_t i = tid; i < steps * 128; i += WAVES * 64) s_w[i] = make_uint4(0, 0, 0, 0);
     if (tid < 16) s_wsum[tid] = 0, s_big.count[tid] = 0;
@@ -617,12 +629,13 @@ __global__ __launch_bounds__(MANY * value_blocks(HD) * 64, 4) void tree_values_m
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = wave_index(), grp = lane >> 4;
     const uint32_t chunk = blockIdx.x, bg = blockIdx.y, g = bg % c.kv_heads, group = a.heads / c.kv_heads;
     const uint32_t dim0 = blockIdx.z % (HD / VD) * VD, rt0 = blockIdx.z / (HD / VD) * MANY;
+    const uint32_t early = early_page(c, a, bg / c.kv_heads, chunk * s.chunk, s.chunk);
     Request r;
     if (!read_request(c, a, bg / c.kv_heads, r)) return;
     const uint32_t key0 = r.base + chunk * s.chunk, pairs = r.rows * group;
     if (key0 >= r.total || rt0 * 16 >= pairs) return;
     const uint32_t n = min(s.chunk, r.total - key0), steps = (n + STEP - 1) / STEP, kt1 = (n + 15) / 16;
-    const Places at = places(c, a, r, g, key0, key0 + n, s_page);
+    const Places at = places(c, a, r, g, key0, key0 + n, s_page, early);
     const uint32_t my = wave % MANY, block = wave / MANY, rt = rt0 + my, row = rt * 16 + (lane & 15);
     const bool has_rt = rt * 16 < pairs, valid = row < pairs;
     const size_t tile = (size_t)bg * s.row_tiles + (has_rt ? rt : rt0);
@@ -905,13 +918,14 @@ __global__ __launch_bounds__(SHORT_WAVES * 64, 4) void tree_short_kernel(const I
     __shared__ BigWeights s_big;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = wave_index(), grp = lane >> 4;
     const uint32_t bg = blockIdx.x, rt = blockIdx.y, g = bg % c.kv_heads, group = a.heads / c.kv_heads;
+    const uint32_t early = early_page(c, a, bg / c.kv_heads, 0, s.short_tiles * 16);
     Request r;
     if (!read_request(c, a, bg / c.kv_heads, r)) return;
     const uint32_t pairs = r.rows * group;
     if (rt * 16 >= pairs) return;
     const uint32_t rows = min(16u, pairs - rt * 16), key0 = r.base, n = r.total - key0;
     const uint32_t kt1 = (n + 15) / 16, steps = (n + STEP - 1) / STEP, chunks = chunks_of(s, r);
-    const Places at = places(c, a, r, g, key0, r.total, s_page);
+    const Places at = places(c, a, r, g, key0, r.total, s_page, early);
     if (tid < 16) s_wsum[tid] = 0, s_first[tid] = 0xffffffffu, s_big.count[tid] = 0;
     for (uint32_t i = tid; i < 16 * DIMS; i += NW * 64) s_sums[i] = 0;
     const RowLanes l(rows);
