@@ -1061,6 +1061,7 @@ __global__ __launch_bounds__(SHORT_WAVES * 64, 4) void tree_short_kernel(const I
             step_digits<NARROW>(x, f, any_wide);
             value_step<NARROW>(w0, w1, f, acc[k]);
         }
+        if (step + NW >= steps) break;
         load_pairs(step + NW);
     }
 #pragma unroll
@@ -1093,7 +1094,7 @@ __global__ __launch_bounds__(SHORT_WAVES * 64, 4) void tree_short_kernel(const I
                     if (4 * grp + q < rows) atomicAdd((unsigned long long*)&s_sums[(4 * grp + q) * DIMS + d2 + k], more[q]);
             }
         }
-    __syncthreads();
+    lds_barrier();
     if (!mine) return;
     uint64_t t = s_sums[tid] + (uint64_t)((int64_t)dn::sub_sat(dn::ONE_ACT, s_wsum[my_row]) * first_value);
     for (int j = 0; j < s_big.count[my_row]; j++) t += (uint64_t)((int64_t)65536 * load1(at.at(at.v, s_big.key[my_row][j]) + my_dim));
