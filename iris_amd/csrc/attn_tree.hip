@@ -328,7 +328,7 @@ __global__ __launch_bounds__(256, HD >= 512 ? 1 : HD >= 256 ? 2 : 3) void tree_s
                 keep(kt, rt, sc);
             }
         }
-    __syncthreads();
+    lds_barrier();  // (keys past the last may be under way)
     if (tid < tiles * 16) {
         const uint32_t rt = tid / 16, i = tid % 16;
         s.maxima[(((size_t)bg * s.row_tiles + rt0 + rt) * s.chunks + chunk) * 16 + i] =
@@ -738,7 +738,7 @@ __global__ __launch_bounds__(MANY * value_blocks(HD) * 64, 4) void tree_values_m
     wsum += __shfl_xor(wsum, 16);
     wsum += __shfl_xor(wsum, 32);
     if (lane < 16) atomicAdd(&s_wsum[my][lane], wsum);
-    __syncthreads();
+    lds_barrier();
 
     // The open weights: what the loop's lack, a lane each (of the tile's first
     // wave), or of every position.
