@@ -18,7 +18,7 @@
 // Trees of many rows are bound by the exact softmax and by what goes through the
 // work space (four bytes per score and head, written twice and read twice): 32
 // trees of 25 at up to 8000, 502 us. Short spans are bound by latency: 1 token
-// at 700 positions 17.2 us.
+// at 700 positions 16.2 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -899,7 +899,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const IrisPagedKv c, con
 // ---- (2) to (4) in one launch, for positions whose score tiles LDS holds: a
 // workgroup per (request, key head), row tile and 32 dimensions. Each forms all
 // terms and weights of its rows: more arithmetic, fewer launches. Bound by
-// latency: 1 token at 700 positions 12.0 us, behind 6.8 of the scores.
+// latency: 1 token at 700 positions 11.3 us, behind 6.5 of the scores.
 
 constexpr uint32_t SHORT_WAVES = 16;
 constexpr uint32_t SHORT_DIMS = 32;
@@ -1133,10 +1133,10 @@ uint64_t tree_space(const IrisPagedKv& c, const IrisTreeAttention& a, uint8_t* b
     const uint64_t span = std::min<uint64_t>(a.max_positions, a.window ? (uint64_t)a.window + a.max_nodes + STEP : a.max_positions);
     const uint64_t tiles = (span + STEP - 1) / STEP * 4;
     // Where its workgroups (sixteen waves: one to a CU) are there all at once.
-    // us, short / long: 1 token at 700 (32 heads of 128, 32 workgroups) 18.4 /
-    // 24.1, 8 at 700 (256) 20.2 / 28.2, 8 at up to 2100 (256) 31.6 / 36.1, a tree
-    // of 32 at 700 (256) 33.8 / 44, 12 of 9 in a window of 1024 (heads of 256, 480)
-    // 50 / 40, 32 at 700 (1024) 60 / 45.
+    // us, short / long: 1 token at 700 (32 heads of 128, 32 workgroups) 17.2 /
+    // 24.1, 8 at 700 (256) 19.4 / 28.2, 8 at up to 2100 (256) 29.7 / 36.1, a tree
+    // of 32 at 700 (256) 32.0 / 44, 12 of 9 in a window of 1024 (heads of 256, 480)
+    // 50 / 39, 32 at 700 (1024) 60 / 43.
     const uint64_t groups = bg * s->row_tiles * ((c.head_dim + SHORT_DIMS - 1) / SHORT_DIMS);
     s->short_tiles = tiles <= SHORT_TILES && groups <= 256 ? (uint32_t)tiles : 0;
     // About 1024 workgroups, of at most 1024 positions: each begins with some
