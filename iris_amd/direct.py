@@ -443,8 +443,8 @@ class Batch:
                         if not took(request, new):
                             running[request] = running.pop(request)
         except Exception:
-            for i in list(running):
-                self.release(i)
+            for i in running:
+                native.lib().iris_batch_release(self._h, i)  # (refused after a failed pass)
             raise
         return results
 

@@ -256,3 +256,15 @@ def test_batch_refuses_a_row_without_finite_scales():
     token = b.prefill({0: [1, 6]})[0]
     refused(-2, lambda: b.step({0: [token, 7]}))
     assert len(b.step({0: [token]})[0]) == 1
+
+
+def test_generate_after_a_draft_that_fails():
+    name = "mistral"
+    ps = prompts(name, [12, 30], seed=120)
+    b = Batch(made(name)[0], 2, 8, 16, 64, 64)
+    for bad, error in ((lambda p, ids: 1 / 0, ZeroDivisionError), (lambda p, ids: ([3, 4], [-1]), ValueError),
+                       (lambda p, ids: ([512], None), native.IrisError)):
+        with pytest.raises(error):
+            b.generate(ps, 9, bad)
+        assert [b.length(0), b.length(1)] == [0, 0]
+    assert [g.token_ids for g in b.generate(ps, 9)] == [alone(name, p, 9).token_ids for p in ps]

@@ -146,3 +146,15 @@ def test_rust_structs_match_the_header(name):
         want += [(n.strip(), rust[m.group(1)]) for n in m.group(2).split(",")]
     body = re.search(r"pub struct %s \{(.*?)\n\}" % name, open(ffi).read(), flags=re.S).group(1)
     assert re.findall(r"pub (\w+): ([^,]+),", body) == want
+
+
+def test_batch_refuses_null_handles():
+    import ctypes as C
+    from iris_amd import direct
+    L, h, n = direct._declare(), C.c_void_p(), C.c_uint32()
+    assert L.iris_batch_create(None, 1, 1, 16, 16, 16, C.byref(h)) == -1
+    assert L.iris_batch_prefill(None, A, A, A) == -1
+    assert L.iris_batch_step(None, A, None, A, A, A) == -1
+    assert L.iris_batch_release(None, 0) == -1
+    assert L.iris_batch_length(None, 0, C.byref(n)) == -1
+    L.iris_batch_free(None)
