@@ -422,7 +422,7 @@ typedef struct IrisPagedKv {
  * adds added[b] rows: it needs ceil((lengths[b] + added[b]) / page_size)
  * pages. Pages it lacks come from the ring of free pages, those past its need
  * go back to the ring (lengths = added = 0 returns them all), each in request
- * order. The ring holds ring_state[1] pages from ring[ring_state[0]], modulo
+ * order; pages are taken before others go back. The ring holds ring_state[1] pages from ring[ring_state[0]], modulo
  * `pages`.
  *   held_out[b]     the pages held now (may be held itself)
  *   table           entries [held, need) written, the others left

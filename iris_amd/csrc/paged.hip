@@ -95,7 +95,8 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(const IrisPagedPlan 
     }
     int status = s_status == 2 ? IRIS_E_INVALID : s_status == 1 ? IRIS_E_RANGE : 0;
     if (!status && (total.rows > p.max_rows || total.pops > free)) status = IRIS_E_RANGE;
-    if (!status && free - total.pops + total.pushes > p.pages) status = IRIS_E_INVALID;
+    // (More than the ring has places for: pages would go back to where others are taken.)
+    if (!status && free + total.pushes > p.pages) status = IRIS_E_INVALID;
     const bool ok = status == 0;
     const bool first = blockIdx.x == 0;
     for (uint32_t b = b0; b < b1; b++) {

@@ -112,7 +112,7 @@ def plan(lengths, added, parents, held, table, ring, ring_state, pages, page, ma
     back = sum(max(0, h - d) for d, h in zip(need, held))
     if max(need) > stride or sum(added) > max_rows or grow > free or (parents is not None and max(added) > 64):
         return *fail, -5
-    if free - grow + back > pages:
+    if free + back > pages:
         return *fail, -1
     slots, positions, starts, taken, given = [], [], [0], 0, []
     for i in range(n):

@@ -138,7 +138,8 @@ def test_plan_all_pages_return_and_are_taken_again():
     (dict(max_rows=5), -5), (dict(ring_state=[0, 0]), -5), (dict(lengths=[-1, 3]), -1), (dict(added=[-2, 30]), -1),
     (dict(held=[-1, 1]), -1), (dict(held=[99, 1]), -1), (dict(held=[0, 1]), -1), (dict(added=[500, 3]), -5),
     (dict(ring_state=[-1, 4]), -1), (dict(ring_state=[0, 99]), -1), (dict(ring_state=[8, 4]), -1),
-    (dict(added=[2 ** 31 - 1, 2 ** 31 - 1], max_rows=2 ** 31 - 1), None), (dict(lengths=[2 ** 31 - 1, 0]), -1)])
+    (dict(added=[2 ** 31 - 1, 2 ** 31 - 1], max_rows=2 ** 31 - 1), None), (dict(lengths=[2 ** 31 - 1, 0]), -1),
+    (dict(added=[0, 30], held=[4, 1], ring_state=[0, 8]), -1)])
 @pytest.mark.parametrize("in_place", [False, True])
 def test_plan_that_cannot_be(change, code, in_place):
     s = dict(lengths=[17, 3], added=[20, 14], held=[2, 1], ring_state=[0, 4], max_rows=40)
