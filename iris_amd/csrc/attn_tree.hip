@@ -23,13 +23,12 @@
 #include <type_traits>
 
 #include "attn_tiles.h"
+#include "tree_chunks.h"
 
 namespace {
 
 // Four rows of zeros for positions whose page is outside the cache.
 __device__ const int32_t g_zeros[4 * ATTN_MAX_HEAD_DIM] = {};
-
-constexpr uint32_t STEP = 64;  // positions of a value product
 
 // The work space of a launch. Row tiles count a request's (drafted row, head)
 // pairs by sixteens, `row_tiles` per (request, key head).
@@ -116,15 +115,13 @@ struct Places {
     __device__ __forceinline__ const int32_t* four(const int32_t* base, uint32_t key) const { return at(base, min(key, last & ~3u)); }
 };
 
-constexpr uint32_t MAX_CHUNK = 1024;
-constexpr uint32_t CHUNK_PAGES = MAX_CHUNK / 4 + 1;
-
 // This thread's table entry of the `count` positions from key0 on, where no
-// window moves them: on its way while the request is read.
+// window moves them: on its way while the request is read. (0 where places()
+// asks for none: from most_pages on.)
 __device__ __forceinline__ uint32_t early_page(const IrisPagedKv& c, const IrisTreeAttention& a, uint32_t request, uint32_t key0,
                                                uint32_t count) {
     const uint32_t log = 31u - __clz((int)c.page_size);
-    if (a.window || threadIdx.x > count >> log) return 0;
+    if (a.window || threadIdx.x >= most_pages(count, log)) return 0;
     const int32_t* table = a.table + (size_t)request * a.table_stride;
     return (uint32_t)load1(table + min((key0 >> log) + threadIdx.x, a.table_stride - 1));
 }
@@ -1139,13 +1136,7 @@ uint64_t tree_space(const IrisPagedKv& c, const IrisTreeAttention& a, uint8_t* b
     // 50 / 39, 32 at 700 (1024) 60 / 43.
     const uint64_t groups = bg * s->row_tiles * ((c.head_dim + SHORT_DIMS - 1) / SHORT_DIMS);
     s->short_tiles = tiles <= SHORT_TILES && groups <= 256 ? (uint32_t)tiles : 0;
-    // About 1024 workgroups, of at most 1024 positions: each begins with some
-    // microseconds of dependent loads, and its sums are written and read again.
-    // us, at most 512 / 1024 / 2048 positions: 4 tokens at up to 32700 145 / 127 /
-    // 127, 32 trees of 25 at up to 8000 563 / 520 / 582, 16 tokens at up to 20000
-    // 280 / 290 / 357, 64 at up to 2000 122 / 128 / 129.
-    const uint64_t want = std::max<uint64_t>(1, 1024 / bg);
-    s->chunk = (uint32_t)std::min<uint64_t>(MAX_CHUNK, std::max<uint64_t>(STEP, ((span + want - 1) / want + STEP - 1) & ~uint64_t(STEP - 1)));
+    s->chunk = chunk_positions(span, bg);
     s->chunks = (uint32_t)((span + s->chunk - 1) / s->chunk);
     uint64_t at = 0;
     auto take = [&](auto*& p, uint64_t bytes) {

@@ -268,3 +268,23 @@ def test_generate_after_a_draft_that_fails():
             b.generate(ps, 9, bad)
         assert [b.length(0), b.length(1)] == [0, 0]
     assert [g.token_ids for g in b.generate(ps, 9)] == [alone(name, p, 9).token_ids for p in ps]
+
+
+def test_batch_of_long_requests():
+    # Positions past the short form's, pages of more positions than a chunk's
+    # length divides, a work space that grows from call to call.
+    name = "mistral wide heads"
+    dm = made(name)[0]
+    lens, tokens = [1400, 1351, 700, 90], 40
+    ps = [synth.token_ids(130 + i, n, dm.model.vocab).astype(np.int32) for i, n in enumerate(lens)]
+    s = Session(dm, 2048, 1400)
+    want = [s.generate(p, tokens).token_ids for p in ps]
+
+    def draft(p, ids):  # the true next two of every third place, else a wrong one
+        at = len(ids) - lens[p]
+        return (want[p][at:at + 2] if at % 3 == 0 else [(want[p][at] + 1) % dm.model.vocab]), None
+
+    for page, requests in ((256, 64), (1024, 64), (16, 4)):
+        b = Batch(dm, requests, 8192 // page, page, 2048, 3600)
+        for d in (None, draft):
+            assert [g.token_ids for g in b.generate(ps, tokens, d)] == want

@@ -559,3 +559,44 @@ def test_tree_cache_past_four_gigabytes():
     t.c = paged.PagedKv(k=kp.data_ptr(), v=vp.data_ptr(), pages=pages, page_size=page, kv_heads=kv_heads, head_dim=hd)
     t.run()
     t.check()
+
+
+# ------------------------------------- pages of more positions than a chunk's
+
+
+def chunk_of(t):
+    """Positions per chunk, as the launch rule has them (no window)."""
+    want = max(1, 1024 // (len(t.lengths) * t.c.kv_heads))
+    return min(1024, max(64, -(-(-(-t.d.max_positions // want)) // 64) * 64))
+
+
+# A chunk that starts inside a page meets one page more than its length fills:
+# (requests, kv_heads, longest, page, chunk).
+CHUNKS_INSIDE_PAGES = [(64, 8, 340, 256, 192), (64, 8, 1400, 1024, 704), (4, 8, 4200, 512, 192), (4, 8, 14000, 256, 448),
+                       (8, 8, 11200, 512, 704), (16, 4, 2200, 256, 192)]
+
+
+@pytest.mark.parametrize("requests, kv_heads, longest, page, chunk", CHUNKS_INSIDE_PAGES)
+@pytest.mark.parametrize("group, nodes, hd", [(1, 1, 64), (3, 9, 20)])
+def test_tree_chunks_that_start_inside_a_page(requests, kv_heads, longest, page, chunk, group, nodes, hd):
+    # One row tile and several; the last shape is the short form's.
+    rng = np.random.default_rng(longest + page)
+    some = requests if nodes == 1 else min(requests, 8)  # the others have no rows
+    lengths = rng.integers(longest // 2, longest - nodes, requests)
+    lengths[0] = longest - nodes
+    t = Tree(rng, lengths.tolist(), [nodes] * some + [0] * (requests - some), group * kv_heads, kv_heads, hd, page=page)
+    assert chunk_of(t) == chunk
+    t.run()
+    t.check()
+
+
+@pytest.mark.parametrize("heads, nodes", [(1, 1), (3, 9)])
+def test_tree_bad_page_behind_a_chunk_that_starts_inside_a_page(heads, nodes):
+    # 512 requests of two chunks of 192: page 1 lies in the second chunk's end.
+    rng = np.random.default_rng(21)
+    t = Tree(rng, [340] + [0] * 511, [nodes] + [0] * 511, heads, 1, 64, page=256)
+    assert chunk_of(t) == 192
+    t.table[0, 1] = t.c.pages
+    t.t["table"].copy_(dev(t.table))
+    t.run()
+    t.check(status=-1)
