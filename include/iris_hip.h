@@ -475,8 +475,8 @@ int iris_paged_store(const IrisPagedKv* cache, const int32_t* k, uint32_t k_stri
  *   scaled      1: scores are the scaled dot product (scale_q32, mistral);
  *               0: the requantized dot product (gemma)
  *   rows        rows of q, k, v and out, rows * heads under 2^26 (and rows *
- *               (heads + 24 kv_heads) under 2^30); rows from
- *               row_start[sequences] on are left as they were
+ *               (heads + 24 kv_heads) under 2^30); rows before row_start[0]
+ *               and from row_start[sequences] on are left as they were
  *   max_length  at least the longest sequence, at most 65535; a row that lies
  *               deeper in its sequence is left as it was
  *   status      (nullable) set to IRIS_E_RANGE where such a row was found;

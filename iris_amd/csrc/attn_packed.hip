@@ -176,7 +176,7 @@ __global__ __launch_bounds__(256) void packed_planes_kernel(const IrisPackedAtte
     const uint32_t t = task * 64 + lane;
     if (t >= a.rows) return;
     int32_t first = -1;
-    if ((int32_t)t < a.row_start[a.sequences]) {
+    if ((int32_t)t >= a.row_start[0] && (int32_t)t < a.row_start[a.sequences]) {
         const int32_t start = min(max(a.row_start[sequence_of(a.row_start, a.sequences, t)], 0), (int32_t)t);
         if (t - (uint32_t)start >= a.max_length) {
             if (a.status) *a.status = IRIS_E_RANGE;

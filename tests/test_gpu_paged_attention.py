@@ -218,6 +218,17 @@ def test_packed_starts_that_cannot_be_stay_in_bounds():
         torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("first, lens", [(1, [30]), (5, [20, 33]), (16, [1, 64]), (70, [3, 100, 20])])
+@pytest.mark.parametrize("window", [0, 9])
+def test_packed_rows_before_the_first_start_are_left(first, lens, window):
+    rng = np.random.default_rng(first)
+    p = Packed(rng, lens, 4, 2, 64, window=window, behind=first + 3)
+    p.starts += first
+    p.row_start.copy_(dev(p.starts))
+    p.run()
+    p.check()
+
+
 def test_packed_result_is_the_same_beside_other_sequences():
     rng = np.random.default_rng(8)
     p = Packed(rng, [70, 200, 33], 4, 2, 128)
