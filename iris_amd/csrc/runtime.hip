@@ -1229,6 +1229,7 @@ int iris_session_make(IrisModel* m, uint32_t max_positions, uint32_t max_rows, I
     if (st == hipSuccess && !batch) st = hipMalloc((void**)&s->sel_partial, (size_t)m->head->tiles * sizeof(uint64_t));
     if (st != hipSuccess) {
         iris_session_free(s);
+        (void)hipGetLastError();  // returned here: not the next launch's to report
         return (int)st;
     }
     *out = s;

@@ -482,6 +482,7 @@ int iris_batch_create(IrisModel* m, uint32_t requests, uint32_t pages, uint32_t 
     if (st == hipSuccess) st = hipDeviceSynchronize();
     if (st != hipSuccess) {
         iris_batch_free(b);
+        (void)hipGetLastError();  // returned here: not the next launch's to report
         return (int)st;
     }
     *out = b;

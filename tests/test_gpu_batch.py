@@ -288,3 +288,17 @@ def test_batch_of_long_requests():
         b = Batch(dm, requests, 8192 // page, page, 2048, 3600)
         for d in (None, draft):
             assert [g.token_ids for g in b.generate(ps, tokens, d)] == want
+
+
+def test_calls_after_a_batch_that_the_device_cannot_hold():
+    # 2^31 - 16 positions of 64 key values in two layers: over two terabytes.
+    name = "mistral"
+    ps = prompts(name, [12, 30], seed=145)
+    want = [alone(name, p, 9).token_ids for p in ps]
+    dm, s, _ = made(name)
+    b = Batch(dm, 2, 8, 16, 64, 64)
+    for _ in range(2):
+        refused(2, lambda: Batch(dm, 2, (1 << 27) - 1, 16, 64, 64))  # hipErrorOutOfMemory
+        assert s.generate(ps[0], 9, use_graph=False).token_ids == want[0]
+        refused(2, lambda: Batch(dm, 2, (1 << 27) - 1, 16, 64, 64))
+        assert [g.token_ids for g in b.generate(ps, 9)] == want
