@@ -541,9 +541,10 @@ int iris_attention_tree(const IrisPagedKv* cache, const IrisTreeAttention* a, vo
  * rows (at most 65535); at most 4096 requests, requests * kv_heads at most
  * 65535. Both families. Every call is synchronous, on a stream of the batch's own; calls
  * of one batch must not overlap. A refused call (IRIS_E_INVALID, _SCALE,
- * _RANGE, _STATE of a request's length) changes nothing; after any other
- * error the batch's state is unknown and every call but iris_batch_free
- * returns IRIS_E_STATE. */
+ * _RANGE, _STATE of a request's length, hipErrorOutOfMemory of a pass whose
+ * work space the device lacks) changes nothing; after any other error the
+ * batch's state is unknown and every call but iris_batch_free returns
+ * IRIS_E_STATE. */
 typedef struct IrisBatch IrisBatch;
 int iris_batch_create(IrisModel* model, uint32_t requests, uint32_t pages, uint32_t page_size, uint32_t max_positions,
                       uint32_t max_rows, IrisBatch** out);

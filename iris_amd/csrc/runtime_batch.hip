@@ -161,8 +161,8 @@ struct IrisBatch {
     int32_t *d_held = nullptr, *table = nullptr, *ring = nullptr, *ring_state = nullptr, *row_start = nullptr;
     int32_t *slots = nullptr, *path = nullptr, *logits = nullptr;
     int64_t* best = nullptr;
-    void* space = nullptr;
-    uint64_t space_bytes = 0;
+    void* space = nullptr;  // of the attention
+    uint64_t space_bytes = 0, space_most = 0;  // now; that a pass can need
     // The pass at hand: its requests' rows and, of prompts, the longest; of
     // newest rows, the most of a request and the last position's end.
     bool prompts = false, trees = false;
@@ -180,13 +180,70 @@ struct IrisBatch {
     size_t out_ints() const { return 1 + (size_t)requests + std::max(s->max_rows, requests); }
 };
 
-static int batch_space(IrisBatch* b, uint64_t bytes) {
-    if (bytes <= b->space_bytes) return 0;
+// The operators' arguments for layer l of the pass at hand.
+static IrisPackedAttention batch_prompts(const IrisBatch* b, uint32_t l, uint32_t rows) {
+    const IrisSession* s = b->s;
+    const IrisModelDesc& d = s->model->d;
+    const LayerWeights& L = s->model->layers[l];
+    const bool gemma = d.family == IRIS_FAMILY_GEMMA_DENSE;
+    const uint32_t qw = L.q_rows, kvw = L.kv_rows, qkvw = qw + 2 * kvw;
+    IrisPackedAttention a{};
+    a.q = gemma ? s->q : s->qkv;
+    a.k = gemma ? b->k_rows[L.kv_source] : s->qkv + qw;
+    a.v = gemma ? b->v_rows[L.kv_source] : s->qkv + qw + kvw;
+    a.out = s->ctx;
+    a.row_start = b->row_start;
+    a.q_stride = gemma ? qw : qkvw, a.k_stride = a.v_stride = gemma ? kvw : qkvw, a.out_stride = qw;
+    a.sequences = b->requests, a.rows = rows, a.max_length = b->longest;
+    a.heads = d.heads, a.kv_heads = d.kv_heads, a.head_dim = L.head_dim, a.window = L.window;
+    a.scaled = !gemma, a.scale_q32 = gemma ? 0 : d.attention_scale_q32;
+    return a;
+}
+
+static IrisTreeAttention batch_newest(const IrisBatch* b, uint32_t l, uint32_t rows) {
+    const IrisSession* s = b->s;
+    const IrisModelDesc& d = s->model->d;
+    const LayerWeights& L = s->model->layers[l];
+    const bool gemma = d.family == IRIS_FAMILY_GEMMA_DENSE;
+    IrisTreeAttention a{};
+    a.q = gemma ? s->q : s->qkv, a.out = s->ctx;
+    a.row_start = b->row_start, a.lengths = b->lengths(), a.parents = b->trees ? b->parents() : nullptr, a.table = b->table;
+    a.q_stride = gemma ? L.q_rows : L.q_rows + 2 * L.kv_rows, a.out_stride = L.q_rows;
+    a.requests = b->requests, a.rows = rows, a.table_stride = b->table_stride;
+    a.max_nodes = b->longest, a.max_positions = b->end;
+    a.heads = d.heads, a.window = L.window;
+    a.scaled = !gemma, a.scale_q32 = gemma ? 0 : d.attention_scale_q32;
+    return a;
+}
+
+// Work space for the pass at hand, before it begins: where the device has
+// none, the pass is refused (hipErrorOutOfMemory) and the requests stay as they
+// were. It grows by halves up to what the largest pass takes, since positions
+// grow from pass to pass and each growth waits for the device.
+static int batch_space(IrisBatch* b, uint32_t rows) {
+    uint64_t need = 0;
+    for (uint32_t l = 0; rows && l < b->s->model->d.layers; l++) {
+        if (b->prompts) {
+            const IrisPackedAttention a = batch_prompts(b, l, rows);
+            need = std::max(need, iris_attention_packed_workspace_bytes(&a));
+        } else {
+            const IrisTreeAttention a = batch_newest(b, l, rows);
+            need = std::max(need, iris_attention_tree_workspace_bytes(&b->caches[b->s->model->layers[l].kv_source], &a));
+        }
+    }
+    if (need <= b->space_bytes) return 0;
+    uint64_t bytes = std::max(need, std::min(b->space_bytes + b->space_bytes / 2, b->space_most));
     RT_CHECK(hipStreamSynchronize(b->s->stream));
     (void)hipFree(b->space);
     b->space = nullptr;
     b->space_bytes = 0;
-    RT_CHECK(hipMalloc(&b->space, bytes));
+    hipError_t st = hipMalloc(&b->space, bytes);
+    if (st != hipSuccess && bytes > need) st = hipMalloc(&b->space, bytes = need);
+    if (st != hipSuccess) {
+        b->space = nullptr;
+        (void)hipGetLastError();  // returned here: not the next launch's to report
+        return (int)st;
+    }
     b->space_bytes = bytes;
     return 0;
 }
@@ -199,9 +256,6 @@ int iris_batch_attention(IrisSession* s, uint32_t l, uint32_t rows) {
     const bool gemma = d.family == IRIS_FAMILY_GEMMA_DENSE, own = L.kv_source == (int32_t)l;
     const uint32_t hd = L.head_dim, qw = L.q_rows, kvw = L.kv_rows, qkvw = qw + 2 * kvw;
     hipStream_t st = s->stream;
-    // The layer's queries, and the keys and values its attention reads.
-    const int32_t *q = s->qkv, *k = s->qkv + qw, *v = s->qkv + qw + kvw;
-    uint32_t q_stride = qkvw, kv_stride = qkvw;
     if (gemma) {
         GemmaQkvArgs qa{};
         qa.qkv = s->qkv;
@@ -217,38 +271,20 @@ int iris_batch_attention(IrisSession* s, uint32_t l, uint32_t rows) {
         qa.positions = s->d_pos;
         qa.q_out = s->q;
         qa.q_stride = qw;
-        k = b->k_rows[L.kv_source], v = b->v_rows[L.kv_source];
         if (own) qa.k_rows = b->k_rows[l], qa.v_rows = b->v_rows[l];
         RT_CHECK(iris_gemma_qkv_finish_launch(qa, rows, st));
-        q = s->q, q_stride = qw, kv_stride = kvw;
     } else {
         hipLaunchKernelGGL(batch_rotate_kernel, dim3(((qw + kvw) / 2 + 255) / 256, rows), dim3(256), 0, st, s->qkv, qkvw, qw + kvw,
                            hd, s->rope_sc, s->d_pos);
         RT_CHECK(hipGetLastError());
     }
+    // The layer's queries, and the keys and values its attention reads.
+    const IrisPackedAttention prompts = batch_prompts(b, l, rows);
     const IrisPagedKv& cache = b->caches[L.kv_source];
-    if (own) RT_CHECK(iris_paged_store(&cache, k, kv_stride, v, kv_stride, b->slots, rows, st));
-    if (b->prompts) {
-        IrisPackedAttention a{};
-        a.q = q, a.k = k, a.v = v, a.out = s->ctx;
-        a.row_start = b->row_start;
-        a.q_stride = q_stride, a.k_stride = a.v_stride = kv_stride, a.out_stride = qw;
-        a.sequences = b->requests, a.rows = rows, a.max_length = b->longest;
-        a.heads = d.heads, a.kv_heads = d.kv_heads, a.head_dim = hd, a.window = L.window;
-        a.scaled = !gemma, a.scale_q32 = gemma ? 0 : d.attention_scale_q32;
-        RT_CHECK(batch_space(b, iris_attention_packed_workspace_bytes(&a)));
-        return iris_attention_packed(&a, b->space, b->space_bytes, st);
-    }
-    IrisTreeAttention a{};
-    a.q = q, a.out = s->ctx;
-    a.row_start = b->row_start, a.lengths = b->lengths(), a.parents = b->trees ? b->parents() : nullptr, a.table = b->table;
-    a.q_stride = q_stride, a.out_stride = qw;
-    a.requests = b->requests, a.rows = rows, a.table_stride = b->table_stride;
-    a.max_nodes = b->longest, a.max_positions = b->end;
-    a.heads = d.heads, a.window = L.window;
-    a.scaled = !gemma, a.scale_q32 = gemma ? 0 : d.attention_scale_q32;
-    RT_CHECK(batch_space(b, iris_attention_tree_workspace_bytes(&cache, &a)));
-    return iris_attention_tree(&cache, &a, b->space, b->space_bytes, st);
+    if (own) RT_CHECK(iris_paged_store(&cache, prompts.k, prompts.k_stride, prompts.v, prompts.v_stride, b->slots, rows, st));
+    if (b->prompts) return iris_attention_packed(&prompts, b->space, b->space_bytes, st);
+    const IrisTreeAttention newest = batch_newest(b, l, rows);
+    return iris_attention_tree(&cache, &newest, b->space, b->space_bytes, st);
 }
 
 // First maxima of the logits of `count` rows of x, as SELECT_PARTS keys each.
@@ -366,6 +402,7 @@ static int batch_run(IrisBatch* b, const int32_t* ids, const int32_t* parents, c
     b->trees = parents != nullptr;
     b->longest = (uint32_t)most;
     b->end = (uint32_t)end;
+    RT_CHECK(batch_space(b, (uint32_t)rows));
     b->broken = true;  // until the pass has ended well
     if (grow > b->pages - held) {
         // The plan takes pages before it gives others back, so those of
@@ -393,6 +430,7 @@ int iris_batch_create(IrisModel* m, uint32_t requests, uint32_t pages, uint32_t 
     // What the paged operators take, layer by layer (the addresses stand for
     // the pass's; nothing is read).
     int32_t* some = (int32_t*)256;
+    uint64_t most = 0;
     IrisPagedKv shape{some, some, pages, page_size, 1, 4};
     RT_CHECK(iris_paged_check(&shape));
     for (const LayerWeights& L : m->layers) {
@@ -410,10 +448,13 @@ int iris_batch_create(IrisModel* m, uint32_t requests, uint32_t pages, uint32_t 
         ta.requests = requests, ta.rows = max_rows, ta.table_stride = (max_positions + page_size - 1) / page_size;
         ta.max_nodes = std::min(max_rows, TREE_MAX_NODES), ta.max_positions = max_positions;
         ta.heads = d.heads, ta.window = L.window;
-        if (!iris_attention_packed_workspace_bytes(&pa) || !iris_attention_tree_workspace_bytes(&shape, &ta)) return IRIS_E_RANGE;
+        const uint64_t of_prompts = iris_attention_packed_workspace_bytes(&pa), of_newest = iris_attention_tree_workspace_bytes(&shape, &ta);
+        if (!of_prompts || !of_newest) return IRIS_E_RANGE;
+        most = std::max(most, std::max(of_prompts, of_newest));
     }
     IrisBatch* b = new (std::nothrow) IrisBatch();
     if (!b) return IRIS_E_NOMEM;
+    b->space_most = most;
     b->requests = requests, b->pages = pages, b->page_size = page_size, b->max_positions = max_positions;
     b->table_stride = (max_positions + page_size - 1) / page_size;
     int rc = 0;

@@ -302,3 +302,18 @@ def test_calls_after_a_batch_that_the_device_cannot_hold():
         assert s.generate(ps[0], 9, use_graph=False).token_ids == want[0]
         refused(2, lambda: Batch(dm, 2, (1 << 27) - 1, 16, 64, 64))
         assert [g.token_ids for g in b.generate(ps, 9)] == want
+
+
+def test_batch_pass_without_work_space_changes_nothing():
+    # Trees of 64 rows for each of 4096 requests over 16000 positions would
+    # take hundreds of gigabytes: refused before the pass, and single rows go on.
+    m = synth.mistral_model(128, 1, 32, 1, 4, 64, 64, seed=26, per_row_scale=False)
+    dm, n = DeviceModel(m), 16000
+    p = synth.token_ids(140, n, 64).astype(np.int32)
+    want = Session(dm, n + 8, n).generate(p, 4).token_ids
+    b = Batch(dm, 4096, 40, 1024, n + 100, n)
+    assert b.prefill({7: p}) == {7: want[0]}
+    for j in range(1, 4):
+        refused(2, lambda: b.step({7: [want[j - 1]] * 64}))  # hipErrorOutOfMemory
+        assert b.length(7) == n + j - 1
+        assert b.step({7: [want[j - 1]]}) == {7: [want[j]]}
