@@ -246,6 +246,7 @@ extern "C" {
     pub fn iris_model_finalize(model: *mut IrisModel) -> c_int;
     pub fn iris_model_free(model: *mut IrisModel);
     pub fn iris_model_device_bytes(model: *const IrisModel) -> u64;
+    pub fn iris_model_ids_refused(model: *const IrisModel, ids: *const i32, count: u32, at: *mut u32) -> c_int;
 
     pub fn iris_session_create(
         model: *mut IrisModel,

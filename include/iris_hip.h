@@ -254,6 +254,12 @@ void iris_model_free(IrisModel* model);
 /* Device bytes held by the model's matrices, the digit planes that the first
  * session of more than one row adds to them included. */
 uint64_t iris_model_device_bytes(const IrisModel* model);
+/* Whether the `count` token ids can be embedded: 0; or IRIS_E_INVALID where
+ * one lies outside the vocabulary, IRIS_E_SCALE where its row of the embedding
+ * (or of the per-layer embedding) has a block scale that is not finite, what a
+ * pass over them is refused with. *at (nullable): the first such id's place,
+ * else count. Host code only. */
+int iris_model_ids_refused(const IrisModel* model, const int32_t* ids, uint32_t count, uint32_t* at);
 
 /* A KV cache for positions 0..max_positions and work space for passes of up
  * to max_rows rows. max_positions is at most 65535 (-5 beyond: the

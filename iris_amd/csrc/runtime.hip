@@ -983,6 +983,19 @@ bool iris_embedding_refused(const IrisModel* m, int32_t id) {
     return (!m->embed_bad.empty() && m->embed_bad[id]) || (!m->ple_bad.empty() && m->ple_bad[id]);
 }
 
+extern "C" int iris_model_ids_refused(const IrisModel* m, const int32_t* ids, uint32_t count, uint32_t* at) {
+    if (!m || (count && !ids)) return IRIS_E_INVALID;
+    int rc = 0;
+    uint32_t i = 0;
+    for (; i < count; i++) {
+        if (ids[i] < 0 || (uint32_t)ids[i] >= m->d.vocab) rc = IRIS_E_INVALID;
+        else if (iris_embedding_refused(m, ids[i])) rc = IRIS_E_SCALE;
+        if (rc) break;
+    }
+    if (at) *at = i;
+    return rc;
+}
+
 // The pass's rows: the embedding of `ids` at positions start.., the step
 // counter reset.
 static int session_reset_and_embed(IrisSession* s, const int32_t* ids, uint32_t count, uint32_t start = 0) {

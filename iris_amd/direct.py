@@ -19,6 +19,7 @@ from . import native
 from .model import PREFIX, Model
 
 FAMILY = {"mistral-dense": 0, "gemma-dense": 1}
+E_SCALE = -2  # a block scale that is not finite
 
 
 class ModelDesc(C.Structure):
@@ -46,6 +47,7 @@ def _declare():
         "iris_model_finalize": (C.c_int, [vp]),
         "iris_model_free": (None, [vp]),
         "iris_model_device_bytes": (u64, [vp]),
+        "iris_model_ids_refused": (C.c_int, [vp, vp, u32, C.POINTER(u32)]),
         "iris_session_create": (C.c_int, [vp, u32, u32, pp]),
         "iris_session_free": (None, [vp]),
         "iris_session_generate": (C.c_int, [vp, vp, u32, u32, vp, u32, vp, C.POINTER(u32), vp, i32]),
@@ -162,6 +164,12 @@ class DeviceModel:
 
     def device_bytes(self) -> int:
         return int(native.lib().iris_model_device_bytes(self._h))
+
+    def ids_refused(self, ids) -> tuple:
+        """What a pass over the ids is refused with (0: nothing; the code of the
+        first that cannot be embedded) and that id's place (else their number)."""
+        ids, at = np.ascontiguousarray(ids, dtype=np.int32), C.c_uint32()
+        return native.lib().iris_model_ids_refused(self._h, ids.ctypes.data, ids.size, C.byref(at)), at.value
 
     def free(self):
         if getattr(self, "_h", None):
@@ -376,7 +384,13 @@ class Batch:
         ``draft(index, ids)`` (optional), called with a prompt's index and the
         ids so far, proposes what may follow: (ids, parents), parents[j] the
         place in ``ids`` of row j's parent, -1 for the last of the ids so far;
-        or (ids, None) for a chain. The tokens do not depend on it."""
+        or (ids, None) for a chain. The tokens do not depend on it: proposals
+        that the model cannot embed are dropped, with what lies below them.
+        (Ids outside the vocabulary are refused, as in a prompt.)
+        Prompts with ids that cannot be embedded are refused before any pass.
+        A prompt whose own selection cannot be embedded ends there, as a
+        session's does; the others go on, and at the end IrisError is raised
+        with ``results``: the list, None for each such prompt."""
         prompts = [np.ascontiguousarray(p, dtype=np.int32) for p in prompts]
         eos = self.dm.model.eos_token_ids
         results = [GenerateResult([], None) for _ in prompts]
@@ -391,7 +405,15 @@ class Batch:
                 raise native.IrisError(-5, "batch generate")
         if any(self.length(i) for i in range(self.requests)):
             raise native.IrisError(-4, "batch generate")
+        for p in prompts:
+            native.check(self.dm.ids_refused(p)[0], "batch generate")
         waiting, running = list(range(len(prompts))), {}  # request -> prompt
+        failed = {}  # prompt -> code
+
+        def ended(request):
+            self.release(request)
+            del running[request]
+            return True
 
         def took(request, new):
             """The request's next tokens; True when it has ended."""
@@ -400,9 +422,11 @@ class Batch:
                 r.token_ids.append(t)
                 if t in eos or len(r.token_ids) == tokens:
                     r.stop_reason = "eos" if t in eos else "max_new_tokens"
-                    self.release(request)
-                    del running[request]
-                    return True
+                    return ended(request)
+            code = self.dm.ids_refused(new[-1:])[0]  # the next pass embeds it
+            if code:
+                failed[running[request]] = code
+                return ended(request)
             return False
 
         try:
@@ -431,9 +455,12 @@ class Batch:
                     more = max(min(more, left), 0)
                     if draft is not None and more:
                         drafted, above = draft(p, prompts[p].tolist() + ids)
-                        last += [int(t) for t in drafted[:more]]
+                        drafted = [int(t) for t in drafted[:more]]
+                        above = above if above is None else [int(a) for a in above[:more]]
+                        drafted, above = self._embedded(drafted, above)
+                        last += drafted
                         if above is not None:
-                            trees[request] = [-1] + [int(a) + 1 for a in above[:more]]
+                            trees[request] = [-1] + [a + 1 for a in above]
                     step[request] = last
                     rows += len(last)
                 if step:
@@ -446,7 +473,32 @@ class Batch:
             for i in running:
                 native.lib().iris_batch_release(self._h, i)  # (refused after a failed pass)
             raise
+        if failed:
+            first = min(failed)
+            e = native.IrisError(failed[first], f"batch generate: embedding a selection of prompt {first}")
+            e.results = [None if p in failed else r for p, r in enumerate(results)]
+            raise e
         return results
+
+    def _embedded(self, drafted, above):
+        """The proposals without those whose embedding is refused for its
+        scales, and without what lies below these."""
+        code, at = self.dm.ids_refused(drafted)
+        if code != E_SCALE:
+            return drafted, above
+        if above is None:
+            return drafted[:at], None
+        if len(above) != len(drafted):
+            raise ValueError("parents must name one row per row")
+        place, ids, parents = {-1: -1}, [], []  # place: of a kept proposal
+        for j, (t, a) in enumerate(zip(drafted, above)):
+            inside = -1 <= a < j  # (any other value: no parent)
+            if (inside and a not in place) or self.dm.ids_refused([t])[0] == E_SCALE:
+                continue
+            place[j] = len(ids)
+            ids.append(t)
+            parents.append(place[a] if inside else -2)
+        return ids, parents
 
     def free(self):
         if getattr(self, "_h", None):

@@ -317,3 +317,84 @@ def test_batch_pass_without_work_space_changes_nothing():
         refused(2, lambda: b.step({7: [want[j - 1]] * 64}))  # hipErrorOutOfMemory
         assert b.length(7) == n + j - 1
         assert b.step({7: [want[j - 1]]}) == {7: [want[j]]}
+
+
+def without_embedding(name, token):
+    """The model with a row of the embedding that has no finite scale, and the
+    tokens of its sessions where none embeds it."""
+    m = MODELS[name]()
+    raw = m.tensors["model.language_model.embed_tokens.weight"].copy()
+    raw[token, 35] = 0x7C  # the second block's scale
+    m.tensors["model.language_model.embed_tokens.weight"] = raw
+    return DeviceModel(m)
+
+
+def test_generate_ends_only_the_prompt_whose_selection_is_refused():
+    name, tokens = "mistral wide heads", 12
+    ps = prompts(name, [5, 37, 20, 12], seed=150)
+    want = [alone(name, p, tokens).token_ids for p in ps]
+    others = {int(t) for p in ps for t in p} | {t for w in (want[0], want[2], want[3]) for t in w}
+    at, token = next((i, t) for i, t in enumerate(want[1][:-1]) if t not in others)
+    dm = without_embedding(name, token)
+    refused(-2, lambda: Session(dm, 256, 160).generate(ps[1], tokens))
+    for draft in (None, drafter(name, ps, tokens, 5, True)):
+        b = Batch(dm, 2, 20, 16, 256, 160)
+        with pytest.raises(native.IrisError) as e:
+            b.generate(ps, tokens, draft)
+        assert e.value.code == -2
+        assert [r and r.token_ids for r in e.value.results] == [want[0], None, want[2], want[3]]
+        assert [b.length(0), b.length(1)] == [0, 0]
+        # Selected last it is not embedded.
+        assert [r.token_ids for r in b.generate(ps, at + 1, draft)] == [w[:at + 1] for w in want]
+
+
+@pytest.mark.parametrize("tree", [False, True])
+def test_generate_does_not_depend_on_drafts_that_cannot_be_embedded(tree):
+    name, tokens = "mistral wide heads", 12
+    ps = prompts(name, [5, 37, 20], seed=160)
+    want = [alone(name, p, tokens).token_ids for p in ps]
+    token = next(t for t in range(512) if t not in {int(t) for p in ps for t in p} | {t for w in want for t in w})
+
+    def draft(p, ids):
+        true = want[p][len(ids) - len(ps[p]):]
+        if not tree:
+            return true[:2] + [token] + true[2:], None
+        # The refused row first, rows under it, and true ones beside them.
+        return [token, 3, true[0], token, 4] + true[1:2], [-1, 0, -1, 2, 3] + [2] * len(true[1:2])
+
+    b = Batch(without_embedding(name, token), 2, 20, 16, 256, 160)
+    assert [r.token_ids for r in b.generate(ps, tokens, draft)] == want
+
+
+def test_generate_refuses_a_prompt_before_any_pass():
+    name = "mistral wide heads"
+    ps = prompts(name, [5, 37, 20], seed=170)
+    dm = without_embedding(name, int(ps[2][7]))
+    b, calls = Batch(dm, 1, 20, 16, 256, 160), []
+    refused(-2, lambda: b.generate(ps, 5, lambda p, ids: calls.append(p)))
+    refused(-1, lambda: b.generate([ps[0], [3, 512]], 5, lambda p, ids: calls.append(p)))
+    assert not calls and b.length(0) == 0
+
+
+def test_ids_refused():
+    dm = without_embedding("mistral", 7)
+    for ids, want in (([], (0, 0)), ([1, 2, 511], (0, 3)), ([1, 7, 512], (-2, 1)), ([0, 512, 7], (-1, 1)), ([-1], (-1, 0))):
+        assert dm.ids_refused(ids) == want
+    m = parity_gemma()
+    raw = m.tensors["model.language_model.embed_tokens_per_layer.weight"].copy()
+    raw[9, 1] = 0x7C  # the first block's scale
+    m.tensors["model.language_model.embed_tokens_per_layer.weight"] = raw
+    assert DeviceModel(m).ids_refused([8, 9]) == (-2, 1)
+
+
+def test_trees_without_the_rows_that_cannot_be_embedded():
+    b = Batch(without_embedding("mistral", 7), 1, 2, 16, 16, 16)
+    for given, want in (
+            (([1, 2], None), ([1, 2], None)), (([1, 7, 2], None), ([1], None)), (([7], None), ([], None)),
+            (([1, 2, 3], [-1, 0, 1]), ([1, 2, 3], [-1, 0, 1])),
+            (([7, 2, 3], [-1, 0, -1]), ([3], [-1])),
+            (([1, 7, 3, 4, 5, 6], [-1, -1, 1, 2, 0, 4]), ([1, 5, 6], [-1, 0, 1])),
+            (([7, 1, 2], [-1, 9, 1]), ([1, 2], [-2, 0])), (([512, 7], [-1, 0]), ([512, 7], [-1, 0]))):
+        assert b._embedded(*given) == want
+    with pytest.raises(ValueError):
+        b._embedded([1, 7], [-1])

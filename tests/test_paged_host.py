@@ -158,3 +158,9 @@ def test_batch_refuses_null_handles():
     assert L.iris_batch_release(None, 0) == -1
     assert L.iris_batch_length(None, 0, C.byref(n)) == -1
     L.iris_batch_free(None)
+
+
+def test_ids_refused_refuses_null_handles():
+    import ctypes as C
+    from iris_amd import direct
+    assert direct._declare().iris_model_ids_refused(None, A, 1, C.byref(C.c_uint32())) == -1
