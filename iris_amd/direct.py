@@ -20,6 +20,7 @@ from .model import PREFIX, Model
 
 FAMILY = {"mistral-dense": 0, "gemma-dense": 1}
 E_SCALE = -2  # a block scale that is not finite
+HIP_OUT_OF_MEMORY = 2  # hipErrorOutOfMemory
 
 
 class ModelDesc(C.Structure):
@@ -386,7 +387,8 @@ class Batch:
         place in ``ids`` of row j's parent, -1 for the last of the ids so far;
         or (ids, None) for a chain. The tokens do not depend on it: proposals
         that the model cannot embed are dropped, with what lies below them.
-        (Ids outside the vocabulary are refused, as in a prompt.)
+        (Ids outside the vocabulary are refused, as in a prompt.) Where the
+        device has no work space for a pass with its drafts, it runs without.
         Prompts with ids that cannot be embedded are refused before any pass.
         A prompt whose own selection cannot be embedded ends there, as a
         session's does; the others go on, and at the end IrisError is raised
@@ -464,7 +466,12 @@ class Batch:
                     step[request] = last
                     rows += len(last)
                 if step:
-                    done = self.step(step, trees)
+                    try:
+                        done = self.step(step, trees)
+                    except native.IrisError as e:
+                        if e.code != HIP_OUT_OF_MEMORY or all(len(r) == 1 for r in step.values()):
+                            raise
+                        done = self.step({request: r[:1] for request, r in step.items()})
                     # A request that has had its turn goes to the back.
                     for request, new in done.items():
                         if not took(request, new):

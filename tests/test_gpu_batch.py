@@ -398,3 +398,18 @@ def test_trees_without_the_rows_that_cannot_be_embedded():
         assert b._embedded(*given) == want
     with pytest.raises(ValueError):
         b._embedded([1, 7], [-1])
+
+
+def test_generate_without_work_space_for_its_drafts():
+    m = synth.mistral_model(128, 1, 32, 1, 4, 64, 64, seed=26, per_row_scale=False)
+    dm, n = DeviceModel(m), 16000
+    p = synth.token_ids(140, n, 64).astype(np.int32)
+    want = Session(dm, n + 100, n).generate(p, 90).token_ids
+    b, asked = Batch(dm, 4096, 40, 1024, n + 100, n), []
+
+    def draft(index, ids):  # 63 rows at the first step, then one
+        asked.append(len(ids))
+        return ([1] * 63 if len(asked) == 1 else [want[len(ids) - n]]), None
+
+    assert b.generate([p], 90, draft)[0].token_ids == want
+    assert asked[:2] == [n + 1, n + 2]  # the first pass kept its last token's row only
