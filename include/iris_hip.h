@@ -468,8 +468,10 @@ int iris_paged_plan(const IrisPagedPlan* plan, void* stream);
 
 /* Writes rows of keys and values (kv_heads * head_dim values each, strides in
  * values, multiples of 4, 16-byte aligned) to their slots; a row whose slot is
- * outside the cache (-1) is skipped. Two rows of one slot: either one. At most
- * 2^24 - 1 rows. */
+ * outside the cache (-1) is skipped. The rows' slots are distinct: what a slot
+ * that two rows name then holds is not specified (values of either row, the
+ * keys of one beside the values of the other); all others are as they should
+ * be. At most 2^24 - 1 rows. */
 int iris_paged_store(const IrisPagedKv* cache, const int32_t* k, uint32_t k_stride, const int32_t* v,
                      uint32_t v_stride, const int32_t* slots, uint32_t rows, void* stream);
 

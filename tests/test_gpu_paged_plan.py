@@ -235,3 +235,27 @@ def test_store_past_four_gigabytes():
     for r, s in enumerate(slots.tolist()):
         assert torch.equal(kp[s // page, :, s % page].reshape(-1), k[r])
     assert int((kp != 0).sum()) == rows * 1024 - 1
+
+
+def test_store_of_two_rows_of_one_slot():
+    # The slot's contents are not specified, every other value is.
+    kv_heads, hd, page, pages, rows = 2, 64, 16, 4, 40
+    rng = np.random.default_rng(30)
+    k, v = (rng.integers(-2 ** 31, 2 ** 31, (rows, kv_heads * hd)).astype(np.int32) for _ in range(2))
+    slots = rng.permutation(pages * page)[:rows].astype(np.int32)
+    slots[[7, 30]] = slots[3]
+    margin, left = 4096, 123456789
+    big = [torch.full((2 * margin + pages * kv_heads * page * hd,), left, dtype=torch.int32, device="cuda") for _ in range(2)]
+    kp, vp = (b[margin:-margin].view(pages, kv_heads, page, hd) for b in big)
+    c = paged.PagedKv(k=kp.data_ptr(), v=vp.data_ptr(), pages=pages, page_size=page, kv_heads=kv_heads, head_dim=hd)
+    tk, tv, ts = dev(k), dev(v), dev(slots)
+    paged.store(c, tk.data_ptr(), kv_heads * hd, tv.data_ptr(), kv_heads * hd, ts.data_ptr(), rows)
+    torch.cuda.synchronize()
+    for b, cache, x in zip(big, (kp, vp), (k, v)):
+        got, want = cache.cpu().numpy(), np.full(cache.shape, left, np.int32)
+        for r, s in enumerate(slots.tolist()):
+            want[s // page, :, s % page] = x[r].reshape(kv_heads, hd)
+        s = int(slots[3])
+        got[s // page, :, s % page] = want[s // page, :, s % page] = 0
+        assert np.array_equal(got, want)
+        assert bool((b[:margin] == left).all()) and bool((b[-margin:] == left).all())
