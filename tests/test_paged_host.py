@@ -119,6 +119,17 @@ def test_tree_workspace():
     paged.attend_tree(cache(), tree(requests=0), None, 0)
 
 
+@pytest.mark.parametrize("kw", [{}, dict(requests=1, rows=1, max_nodes=1, max_positions=1), dict(window=5),
+                                dict(requests=64, max_positions=9000, table_stride=600),
+                                dict(heads=32, q_stride=2048, out_stride=2048, max_nodes=64, rows=128)])
+def test_tree_workspace_of_a_valid_call_is_checked(kw):
+    size = paged.tree_workspace_bytes(cache(), tree(**kw))
+    assert size > 0
+    refused(lambda: paged.attend_tree(cache(), tree(**kw), A, size - 1), -5)
+    refused(lambda: paged.attend_tree(cache(), tree(**kw), None, size), -1)
+    refused(lambda: paged.attend_tree(cache(), tree(**kw), A + 4, size), -1)
+
+
 C_TYPES = {paged._P: "*", paged._U: "uint32_t", paged._I: "int32_t"}
 
 
