@@ -611,3 +611,65 @@ def test_tree_bad_page_behind_a_chunk_that_starts_inside_a_page(heads, nodes):
     t.t["table"].copy_(dev(t.table))
     t.run()
     t.check(status=-1)
+
+
+# ------------------------------------------------- the ends of the ranges
+
+
+@pytest.mark.parametrize("kinds", [("sharp", "normal", "normal"), ("same", "same", "ends"), ("wide", "wide", "wide")])
+@pytest.mark.parametrize("hd", [4, 68])
+def test_packed_longest_sequence(kinds, hd):
+    rng = np.random.default_rng(hd)
+    p = Packed(rng, [65535, 1], 1, 1, hd, kinds=kinds, extra=(4, 0, 0, 0))
+    p.run()
+    torch.cuda.synchronize()
+    got = p.out.cpu().numpy()
+    rows = [0, 1, 32767, 43690, 65518, 65519, 65533, 65534]
+    seen = np.arange(65535)[None, :] <= np.array(rows)[:, None]
+    want = ref.attend(p.q[rows], p.k[:65535], p.v[:65535], seen, p.scale)
+    assert np.array_equal(got[rows, :hd], want)
+    assert np.array_equal(got[65535, :hd], ref.attend(p.q[65535:], p.k[65535:], p.v[65535:], np.ones((1, 1), bool), p.scale)[0])
+    assert p.status.item() == 0
+
+
+@pytest.mark.parametrize("kinds", [("sharp", "normal", "normal"), ("same", "same", "ends"), ("wide", "wide", "wide")])
+@pytest.mark.parametrize("page, nodes", [(1024, 1), (256, 2), (4, 33)])
+def test_tree_most_positions(kinds, page, nodes):
+    rng = np.random.default_rng(page)
+    t = Tree(rng, [(1 << 20) - nodes], [nodes], 1, 1, 4, page=page, kinds=kinds, parents=None)
+    t.run()
+    torch.cuda.synchronize()
+    n, at = nodes - 1, np.arange(1 << 20)
+    ids = t.table[0][at // page]
+    k, v = t.kp[ids, 0, at % page], t.vp[ids, 0, at % page]
+    for i in {0, n // 2, n}:
+        seen = (at <= (1 << 20) - nodes + i)[None, :]
+        assert np.array_equal(t.out[i].cpu().numpy(), ref.attend(t.q[i:i + 1], k, v, seen, t.scale)[0])
+    assert t.t["status"].item() == 0
+
+
+@pytest.mark.parametrize("scale", [1, 1 << 16, (1 << 31) + 12345, (1 << 32) - 1])
+@pytest.mark.parametrize("kind", ["normal", "mixed", "ends"])
+def test_scales(scale, kind):
+    rng = np.random.default_rng(scale % 1000)
+    p = Packed(rng, [40, 3], 4, 2, 64, kinds=(kind,) * 3)
+    t = Tree(rng, [70, 5], [3, 9], 4, 2, 64, kinds=(kind,) * 3)
+    for c in (p, t):
+        c.scale = c.d.scale_q32 = scale
+        c.run()
+        c.check()
+
+
+@pytest.mark.parametrize("window", [2 ** 31, 2 ** 32 - 1])
+def test_windows_past_every_position(window):
+    rng = np.random.default_rng(40)
+    p = Packed(rng, [90, 40], 4, 2, 64)
+    t = Tree(rng, [200, 5], [3, 9], 4, 2, 64, max_positions=2600)
+    want = p.want(), t.want()
+    for c, w in zip((p, t), want):
+        c.d.window = window
+        c.size = paged.packed_workspace_bytes(c.d) if c is p else paged.tree_workspace_bytes(c.c, c.d)
+        c.space = torch.full((c.size,), 0xA5, dtype=torch.uint8, device="cuda")
+        c.run()
+        torch.cuda.synchronize()
+        assert np.array_equal(c.out.cpu().numpy(), w)
