@@ -413,3 +413,17 @@ def test_generate_without_work_space_for_its_drafts():
 
     assert b.generate([p], 90, draft)[0].token_ids == want
     assert asked[:2] == [n + 1, n + 2]  # the first pass kept its last token's row only
+
+
+def test_two_batches_at_once():
+    # Each on a thread of its own, over one model.
+    from concurrent.futures import ThreadPoolExecutor
+    name, tokens = "mistral wide heads", 24
+    sets = [prompts(name, [5, 37, 64], seed=180), prompts(name, [90, 12], seed=190)]
+    want = [[alone(name, p, tokens).token_ids for p in ps] for ps in sets]
+    bs = [Batch(made(name)[0], 2, 30, 16, 256, 160) for _ in sets]
+    drafts = [drafter(name, sets[0], tokens, 3, True), None]
+    with ThreadPoolExecutor(2) as pool:
+        for _ in range(3):
+            runs = [pool.submit(b.generate, ps, tokens, d) for b, ps, d in zip(bs, sets, drafts)]
+            assert [[g.token_ids for g in r.result()] for r in runs] == want
