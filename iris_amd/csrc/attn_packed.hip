@@ -599,8 +599,6 @@ __global__ __launch_bounds__(NW * 64, HD >= 512 ? 2 : 4) void packed_spill_kerne
     }
 }
 
-bool misaligned(const void* p) { return ((uintptr_t)p & 15) != 0; }
-
 int packed_check(const IrisPackedAttention* a) {
     if (!a || !a->q || !a->k || !a->v || !a->out || !a->row_start) return IRIS_E_INVALID;
     if (misaligned(a->q) || misaligned(a->k) || misaligned(a->v) || misaligned(a->out)) return IRIS_E_INVALID;
@@ -619,8 +617,6 @@ int packed_check(const IrisPackedAttention* a) {
     return 0;
 }
 
-uint32_t padded_head(uint32_t hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : 512; }
-
 constexpr uint32_t LDS_BYTES = 160 * 1024;
 constexpr uint32_t CUS = 256;  // an MI355X
 
@@ -635,7 +631,7 @@ struct PackedShape {
 // Tiles of up to a half (a quarter) of LDS: workgroups of eight (four) waves,
 // so that one's waits are another's work. More than that: where the items are
 // many, still two workgroups of eight waves to a CU with the tiles past 76 in
-// the work space, else one of sixteen waves with 157 tiles. us, two of eight /
+// the work space, else one of sixteen waves with 156 tiles. us, two of eight /
 // one of sixteen: 4096 rows x 32 heads of 128 1349 / 1419, 2048 x 32 of 128 357
 // / 371, 1300 x 32 of 128 159 / 172, 2000 x 8 of 512 256 / 307; 2300 x 8 of 256
 // 175 / 161, 2000 x 4 of 64 52 / 44. Few items: sixteen waves for each, eight

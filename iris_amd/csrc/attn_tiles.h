@@ -30,6 +30,9 @@ constexpr int DIGITS = 5;              // of any int32
 constexpr int NARROW = 3;              // of the usual values
 constexpr int32_t BIG_WEIGHT = 32640;  // the first weight that needs a third digit
 
+// The dimensions that a head's operand tiles hold.
+constexpr uint32_t padded_head(uint32_t hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : 512; }
+
 // The wave's index in its workgroup, known to be the same in every lane (what
 // follows from it stays in scalar registers).
 __device__ __forceinline__ uint32_t wave_index() { return (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }

@@ -1100,8 +1100,6 @@ __global__ __launch_bounds__(SHORT_WAVES * 64, 4) void tree_short_kernel(const I
         dn::requantize((int64_t)t);
 }
 
-bool misaligned(const void* p) { return ((uintptr_t)p & 15) != 0; }
-
 int tree_check(const IrisPagedKv* c, const IrisTreeAttention* a) {
     const int rc = iris_paged_check(c);
     if (rc) return rc;
@@ -1118,8 +1116,6 @@ int tree_check(const IrisPagedKv* c, const IrisTreeAttention* a) {
         return IRIS_E_RANGE;
     return 0;
 }
-
-uint32_t padded_head(uint32_t hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : 512; }
 
 // Carves the work space (base may be null) and returns its bytes.
 uint64_t tree_space(const IrisPagedKv& c, const IrisTreeAttention& a, uint8_t* base, TreeSpace* s) {

@@ -14,6 +14,8 @@ constexpr uint32_t TREE_MAX_POSITIONS = 1u << 20;
 // 0, or why the cache cannot be used (host checks).
 int iris_paged_check(const IrisPagedKv* c);
 
+inline bool misaligned(const void* p) { return ((uintptr_t)p & 15) != 0; }
+
 // Raises a kernel's dynamic LDS limit where a launch needs more than 64 KB.
 // (Not a stream operation: it can precede a captured launch.)
 inline hipError_t paged_lds_limit(const void* kernel, size_t bytes) {

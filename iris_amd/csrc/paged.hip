@@ -167,8 +167,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(const IrisPagedPlan 
 // pieces, keys then values. Bound by memory: 6007 rows of 8 heads of 128, 98 MB
 // read and written, 15.9 us (6.2 TB/s, a large copy reaches 4.6); 8 rows 2.6 us.
 __global__ __launch_bounds__(256) void store_kernel(const IrisPagedKv c, const int32_t* k, uint32_t k_stride,
-                                                    const int32_t* v, uint32_t v_stride, const int32_t* slots,
-                                                    uint32_t rows) {
+                                                    const int32_t* v, uint32_t v_stride, const int32_t* slots) {
     const uint32_t hd4 = c.head_dim / 4, w4 = c.kv_heads * hd4, page_log = 31 - __clz((int)c.page_size);
     const uint32_t row = blockIdx.x;
     const int32_t slot = slots[row];
@@ -183,8 +182,6 @@ __global__ __launch_bounds__(256) void store_kernel(const IrisPagedKv c, const i
         ((int4*)c.v)[at] = vs[i];
     }
 }
-
-bool misaligned(const void* p) { return ((uintptr_t)p & 15) != 0; }
 
 }  // namespace
 
@@ -231,8 +228,7 @@ int iris_paged_store(const IrisPagedKv* c, const int32_t* k, uint32_t k_stride, 
         return IRIS_E_INVALID;
     if (rows >= 1u << 24) return IRIS_E_RANGE;  // a launch has under 2^32 threads
     if (!rows) return 0;
-    hipLaunchKernelGGL(store_kernel, dim3(rows), dim3(256), 0, (hipStream_t)stream, *c, k, k_stride, v, v_stride, slots,
-                       rows);
+    hipLaunchKernelGGL(store_kernel, dim3(rows), dim3(256), 0, (hipStream_t)stream, *c, k, k_stride, v, v_stride, slots);
     return (int)hipGetLastError();
 }
 
