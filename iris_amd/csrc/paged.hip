@@ -165,7 +165,9 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(const IrisPagedPlan 
 
 // Four values of one row to their slot per thread and turn: rows of width / 4
 // pieces, keys then values. Bound by memory: 6007 rows of 8 heads of 128, 98 MB
-// read and written, 15.9 us (6.2 TB/s, a large copy reaches 4.6); 8 rows 2.6 us.
+// read and written, 15.2 us where the same buffers come again and the last-level
+// cache holds them (a copy of as many bytes 14.5), 18.9 us over sixteen sets in
+// turn (the copy 20.4); 8 rows 2.1 us.
 __global__ __launch_bounds__(256) void store_kernel(const IrisPagedKv c, const int32_t* k, uint32_t k_stride,
                                                     const int32_t* v, uint32_t v_stride, const int32_t* slots) {
     const uint32_t hd4 = c.head_dim / 4, w4 = c.kv_heads * hd4, page_log = 31 - __clz((int)c.page_size);
