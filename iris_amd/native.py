@@ -18,6 +18,8 @@ _lib = None
 
 
 class IrisError(RuntimeError):
+    results = None  # direct.Batch.generate: what its other prompts came to
+
     def __init__(self, code: int, what: str):
         self.code = code
         super().__init__(f"{what} failed: {error_text(code)} (code {code})")

@@ -320,8 +320,8 @@ def test_batch_pass_without_work_space_changes_nothing():
 
 
 def without_embedding(name, token):
-    """The model with a row of the embedding that has no finite scale, and the
-    tokens of its sessions where none embeds it."""
+    """The model, with no finite scale in the token's row of the embedding (its
+    selections are the other model's while none embeds that row)."""
     m = MODELS[name]()
     raw = m.tensors["model.language_model.embed_tokens.weight"].copy()
     raw[token, 35] = 0x7C  # the second block's scale
