@@ -673,3 +673,95 @@ def test_windows_past_every_position(window):
         c.run()
         torch.cuda.synchronize()
         assert np.array_equal(c.out.cpu().numpy(), w)
+
+
+def test_packed_rows_past_four_giga_values():
+    # 1.1 million rows of 32 heads of 128: queries, outputs and digit planes
+    # with offsets past 2^32 values; the rows that are looked at lie at both ends.
+    rows, heads, kv_heads, hd, n = 1_100_003, 32, 1, 128, 300
+    g = torch.Generator(device="cuda").manual_seed(50)
+    q, k, v = (torch.randint(-200000, 200000, (rows, x * hd), dtype=torch.int32, device="cuda", generator=g)
+               for x in (heads, kv_heads, kv_heads))
+    out = torch.full((rows, heads * hd), LEFT, dtype=torch.int32, device="cuda")
+    starts = torch.tensor(list(range(0, rows - 50, n)) + [rows - 1], dtype=torch.int32, device="cuda")
+    status = dev([0])
+    d = paged.PackedAttention(
+        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), row_start=starts.data_ptr(),
+        status=status.data_ptr(), q_stride=heads * hd, k_stride=hd, v_stride=hd, out_stride=heads * hd,
+        sequences=len(starts) - 1, rows=rows, max_length=n + 50, heads=heads, kv_heads=kv_heads, head_dim=hd, window=0,
+        scaled=1, scale_q32=scale_of(hd, True))
+    size = paged.packed_workspace_bytes(d)
+    assert size > 1 << 34
+    space = torch.empty(size, dtype=torch.uint8, device="cuda")
+    paged.attend_packed(d, space.data_ptr(), size)
+    torch.cuda.synchronize()
+    assert status.item() == 0 and bool((out[-1] == LEFT).all())
+    for i in (0, len(starts) // 2, len(starts) - 2):
+        a, b = int(starts[i]), int(starts[i + 1])
+        qs, ks, vs, got = (x[a:b].cpu().numpy() for x in (q, k, v, out))
+        pick = [0, 1, b - a - 17, b - a - 1]
+        seen = np.arange(b - a)[None, :] <= np.array(pick)[:, None]
+        for h in (0, 17, heads - 1):
+            cols = slice(h * hd, h * hd + hd)
+            assert np.array_equal(got[pick, cols], ref.attend(qs[pick][:, cols], ks, vs, seen, d.scale_q32))
+
+
+def test_tree_work_space_past_four_gigabytes():
+    # 64 trees of 64 rows at up to 12000 positions: 6.4 GB of scores.
+    requests, nodes, heads, kv_heads, hd, page, longest = 64, 64, 32, 8, 64, 128, 12000
+    g = torch.Generator(device="cuda").manual_seed(51)
+    held = -(-(longest + nodes) // page)
+    pages = requests * held
+    kp, vp = (torch.randint(-300000, 300000, (pages, kv_heads, page, hd), dtype=torch.int32, device="cuda", generator=g)
+              for _ in range(2))
+    q = torch.randint(-300000, 300000, (requests * nodes, heads * hd), dtype=torch.int32, device="cuda", generator=g)
+    table = torch.randperm(pages, device="cuda", generator=g).to(torch.int32).reshape(requests, held)
+    r = random.Random(52)
+    lengths = [longest - r.randrange(3000) for _ in range(requests - 1)] + [longest]
+    parents = [r.randrange(-1, i) if i else -1 for _ in range(requests) for i in range(nodes)]
+    out = torch.full_like(q, LEFT)
+    t = dict(row_start=dev(range(0, requests * nodes + 1, nodes)), lengths=dev(lengths), parents=dev(parents), table=table,
+             status=dev([0]))
+    c = paged.PagedKv(k=kp.data_ptr(), v=vp.data_ptr(), pages=pages, page_size=page, kv_heads=kv_heads, head_dim=hd)
+    d = paged.TreeAttention(
+        q=q.data_ptr(), out=out.data_ptr(), **{n: x.data_ptr() for n, x in t.items()}, q_stride=heads * hd,
+        out_stride=heads * hd, requests=requests, rows=requests * nodes, table_stride=held, max_nodes=nodes,
+        max_positions=longest + nodes, heads=heads, window=0, scaled=1, scale_q32=scale_of(hd, True))
+    size = paged.tree_workspace_bytes(c, d)
+    assert size > 6 << 30
+    space = torch.empty(size, dtype=torch.uint8, device="cuda")
+    paged.attend_tree(c, d, space.data_ptr(), size)
+    torch.cuda.synchronize()
+    assert t["status"].item() == 0
+    for b in (0, requests - 1):
+        seen, _ = ref.tree_mask(lengths[b], parents[b * nodes:b * nodes + nodes], 0)
+        at = np.arange(seen.shape[1])
+        ids, rows = table[b].cpu().numpy()[at // page], slice(b * nodes, b * nodes + nodes)
+        qs, got, pick = q[rows].cpu().numpy(), out[rows].cpu().numpy(), [0, 30, 63]
+        own = torch.from_numpy(ids).long().cuda()
+        for h in (0, heads - 1):
+            cols, kv = slice(h * hd, h * hd + hd), h // (heads // kv_heads)
+            ks, vs = (x[own, kv, torch.from_numpy(at % page).cuda()].cpu().numpy() for x in (kp, vp))
+            assert np.array_equal(got[pick, cols], ref.attend(qs[pick][:, cols], ks, vs, seen[pick], d.scale_q32))
+
+
+@pytest.mark.parametrize("heads, kv_heads", [(3000, 3000), (3000, 3), (1200, 600)])
+def test_many_heads(heads, kv_heads):
+    rng = np.random.default_rng(heads + kv_heads)
+    p = Packed(rng, [3, 18], heads, kv_heads, 4)
+    t = Tree(rng, [20, 3], [1, 2], heads, kv_heads, 4)
+    for c in (p, t):
+        c.run()
+        c.check()
+
+
+def test_tree_requests_that_share_pages():
+    # Three requests over the pages of one prompt, their newest rows in pages of their own.
+    rng = np.random.default_rng(53)
+    t = Tree(rng, [64, 64, 64], [3, 1, 5], 4, 2, 64)
+    t.table[1:, :4] = t.table[0, :4]
+    t.t["table"].copy_(dev(t.table))
+    t.d.status = t.d.parents = None
+    t.parents = None
+    t.run()
+    t.check()
