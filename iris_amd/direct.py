@@ -476,7 +476,7 @@ class Batch:
                     for request, new in done.items():
                         if not took(request, new):
                             running[request] = running.pop(request)
-        except Exception:
+        except BaseException:  # an interrupt too: the requests are empty again
             for i in running:
                 native.lib().iris_batch_release(self._h, i)  # (refused after a failed pass)
             raise

@@ -427,3 +427,16 @@ def test_two_batches_at_once():
         for _ in range(3):
             runs = [pool.submit(b.generate, ps, tokens, d) for b, ps, d in zip(bs, sets, drafts)]
             assert [[g.token_ids for g in r.result()] for r in runs] == want
+
+
+def test_generate_after_an_interrupt():
+    ps = prompts("mistral", [12, 30], seed=200)
+    b = Batch(made("mistral")[0], 2, 8, 16, 64, 64)
+
+    def interrupted(p, ids):
+        raise KeyboardInterrupt
+
+    with pytest.raises(KeyboardInterrupt):
+        b.generate(ps, 9, interrupted)
+    assert [b.length(0), b.length(1)] == [0, 0]
+    assert [g.token_ids for g in b.generate(ps, 9)] == [alone("mistral", p, 9).token_ids for p in ps]
