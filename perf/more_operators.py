@@ -11,8 +11,8 @@ Three kinds of call:
 - ``rules``: penalties for repeated tokens, biases and grammar masks on rows of
   logits; drafted rows count the drafted tokens above them too.
 - ``draw``: a token for each row of logits: the first maximum, or drawn with a
-  temperature, top-k, top-p and min-p bounds from a random number that is an
-  input.
+  temperature and bounds on their number (top-k), their share (top-p) and their
+  distance from the first, from a random number that is an input.
 
 All values are Q16.16 integers, and every result is an integer that the
 arithmetic fixes bit for bit: sums are exact, each rounding goes to the nearest
@@ -265,17 +265,18 @@ def _prepare_rules(case, seed):
 
 
 def _drawings(case):
-    """[row]: inverse temperature, k, p, min-p."""
+    """[row]: inverse temperature, k, p, the largest distance from the first (0: any)."""
     r = random.Random(case["mix"])
     out = []
     for _ in range(case["rows"]):
-        kind = case["kind"] if case["kind"] != "mixed" else r.choice(["greedy", "plain", "top_k", "top_p", "both", "min_p"])
+        kind = case["kind"] if case["kind"] != "mixed" else r.choice(["greedy", "plain", "top_k", "top_p", "both", "gap"])
         beta = 0 if kind == "greedy" else int(ONE / r.choice([0.3, 0.7, 0.8, 1.0, 1.5]))
         k = r.choice([1, 5, 40, 50, 1000]) if kind in ("top_k", "both") else 0
         p = int(r.choice([0.1, 0.5, 0.9, 0.95, 0.999]) * 2 ** 32) if kind in ("top_p", "both") else 0
         if case["kind"] == "both":
             k, p = 40, int(0.95 * 2 ** 32)
-        out.append([beta, k, p, int(r.choice([0.01, 0.05, 0.2]) * 2 ** 32) if kind == "min_p" else 0])
+        # A distance of -ln(0.05) keeps tokens of at least a twentieth of the first's weight.
+        out.append([beta, k, p, int(-math.log(r.choice([0.01, 0.05, 0.2])) * ONE) if kind == "gap" else 0])
     return out
 
 
@@ -419,18 +420,19 @@ def _scaled_floor(value, share):
 
 
 def _plain_draw(s):
-    beta, k, p, floor = (s["drawings"][:, i].long() & 0xFFFFFFFF for i in range(4))
+    beta, k, p, most = (s["drawings"][:, i].long() & 0xFFFFFFFF for i in range(4))
     number = s["numbers"].long() & 0xFFFFFFFF
     l, index = torch.sort(s["logits"].long(), dim=1, descending=True, stable=True)
     is_open = l > LOWEST
     gap = l[:, :1] - l
-    e = _exp(_rte(torch.minimum(gap, torch.full_like(gap, (1 << 31) - 1)) * beta[:, None], 16).clamp(max=1 << 20)) * is_open
+    gap = _rte(torch.minimum(gap, torch.full_like(gap, (1 << 31) - 1)) * beta[:, None], 16).clamp(max=1 << 20)
+    e = _exp(gap) * is_open * ((most == 0)[:, None] | (gap <= most[:, None]))
     place = torch.arange(l.shape[1], device="cuda")[None, :]
     e = e * ((k == 0)[:, None] | (place < k[:, None]))
     total = e.cumsum(1)
     whole, cut = _scaled_floor(total[:, -1], p)
     before = total - e
-    e = e * ((p == 0)[:, None] | (before < (whole + cut)[:, None])) * (e >= floor[:, None])
+    e = e * ((p == 0)[:, None] | (before < (whole + cut)[:, None]))
     total = e.cumsum(1)
     target, _ = _scaled_floor(total[:, -1], number)
     at = (total > target[:, None]).to(torch.int8).argmax(1)
@@ -573,7 +575,7 @@ def _exact_draw(s):
     numbers = s["numbers"].cpu().numpy().view(np.uint32)
     tokens, mass = [], []
     for i, l in enumerate(logits):
-        beta, k, p, least = (int(v) for v in drawings[i])
+        beta, k, p, most = (int(v) for v in drawings[i])
         order = np.lexsort((np.arange(l.size), -l))
         order = order[l[order] > LOWEST]
         if not order.size:
@@ -587,12 +589,12 @@ def _exact_draw(s):
         if k:
             order = order[:k]
         gap = _nearest((l[order[0]] - l[order]) * beta, 65536)
-        order, gap = order[gap < 1 << 20], gap[gap < 1 << 20]
+        gap = gap[gap <= (most or HIGHEST)]
+        gap = gap[gap < 1 << 20]
         terms = _exact_term(gap)
         if p:
             need = -(-p * int(terms.sum()) >> 32)
             terms = terms[:np.searchsorted(np.cumsum(terms), need) + 1]
-        terms = terms[terms >= least]
         whole = int(terms.sum())
         at = int(np.searchsorted(np.cumsum(terms), whole * int(numbers[i]) >> 32, side="right"))
         tokens.append(int(order[at]))
