@@ -147,6 +147,110 @@ pub struct IrisTreeAttention {
     pub scale_q32: u32,
 }
 
+/// The header's 16-bit integers, by its own name for them.
+#[allow(non_camel_case_types)]
+pub type int16_t = i16;
+
+/// A product's part for its adapters: output i is column first + i * step
+/// (include/iris_hip.h `IrisAdapterPart`).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct IrisAdapterPart {
+    pub rows: u32,
+    pub first: u32,
+    pub step: u32,
+}
+
+/// The low-rank adapters of one product on the device.
+#[repr(C)]
+pub struct IrisAdapterBank {
+    _private: [u8; 0],
+}
+
+/// Rows with an adapter each (`IrisAdapterRows`).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct IrisAdapterRows {
+    pub x: *const i32,
+    pub y: *const i32,
+    pub out: *mut i32,
+    pub slots: *const i32,
+    pub status: *mut i32,
+    pub x_stride: u32,
+    pub y_stride: u32,
+    pub out_stride: u32,
+    pub rows: u32,
+}
+
+/// One request's penalties and biases (`IrisTokenRule`).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct IrisTokenRule {
+    pub repetition: i32,
+    pub frequency: i32,
+    pub presence: i32,
+    pub window: u32,
+    pub bias_start: u32,
+    pub bias_count: u32,
+}
+
+/// Rules on rows of logits (`IrisLogitsRules`).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct IrisLogitsRules {
+    pub logits: *const i32,
+    pub out: *mut i32,
+    pub request: *const i32,
+    pub rules: *const IrisTokenRule,
+    pub history: *const i32,
+    pub lengths: *const i32,
+    pub row_start: *const i32,
+    pub ids: *const i32,
+    pub parents: *const i32,
+    pub bias_ids: *const i32,
+    pub bias_values: *const i32,
+    pub masks: *const u32,
+    pub mask_of: *const i32,
+    pub status: *mut i32,
+    pub rows: u32,
+    pub first_row: u32,
+    pub vocab: u32,
+    pub logits_stride: u32,
+    pub out_stride: u32,
+    pub requests: u32,
+    pub history_stride: u32,
+    pub biases: u32,
+    pub mask_rows: u32,
+    pub mask_stride: u32,
+}
+
+/// How a request draws its tokens (`IrisDrawing`).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct IrisDrawing {
+    pub inverse_temperature: i32,
+    pub top_k: u32,
+    pub top_p: u32,
+    pub max_gap: u32,
+}
+
+/// A token for each row of logits (`IrisLogitsDraw`).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct IrisLogitsDraw {
+    pub logits: *const i32,
+    pub request: *const i32,
+    pub drawings: *const IrisDrawing,
+    pub numbers: *const u32,
+    pub tokens: *mut i32,
+    pub mass: *mut i64,
+    pub status: *mut i32,
+    pub rows: u32,
+    pub vocab: u32,
+    pub logits_stride: u32,
+    pub requests: u32,
+}
+
 extern "C" {
     pub fn q8gpu_error(code: c_int) -> *const c_char;
     pub fn q8gpu_init() -> c_int;
@@ -371,6 +475,42 @@ extern "C" {
     pub fn iris_attention_tree(
         cache: *const IrisPagedKv,
         a: *const IrisTreeAttention,
+        d_workspace: *mut c_void,
+        workspace_bytes: u64,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn iris_adapters_create(
+        cols: u32,
+        parts: *const IrisAdapterPart,
+        part_count: u32,
+        slots: u32,
+        max_rank: u32,
+        out: *mut *mut IrisAdapterBank,
+    ) -> c_int;
+    pub fn iris_adapters_free(bank: *mut IrisAdapterBank);
+    pub fn iris_adapters_device_bytes(bank: *const IrisAdapterBank) -> u64;
+    pub fn iris_adapters_load(
+        bank: *mut IrisAdapterBank,
+        slot: u32,
+        part: u32,
+        a: *const int16_t,
+        a_bits: u32,
+        b: *const int16_t,
+        b_bits: u32,
+        rank: u32,
+    ) -> c_int;
+    pub fn iris_adapters_workspace_bytes(bank: *const IrisAdapterBank, rows: u32) -> u64;
+    pub fn iris_adapters_apply(
+        bank: *const IrisAdapterBank,
+        a: *const IrisAdapterRows,
+        d_workspace: *mut c_void,
+        workspace_bytes: u64,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn iris_logits_rules(a: *const IrisLogitsRules, stream: *mut c_void) -> c_int;
+    pub fn iris_logits_draw_workspace_bytes(a: *const IrisLogitsDraw) -> u64;
+    pub fn iris_logits_draw(
+        a: *const IrisLogitsDraw,
         d_workspace: *mut c_void,
         workspace_bytes: u64,
         stream: *mut c_void,

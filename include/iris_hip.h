@@ -543,6 +543,174 @@ uint64_t iris_attention_tree_workspace_bytes(const IrisPagedKv* cache, const Iri
 int iris_attention_tree(const IrisPagedKv* cache, const IrisTreeAttention* a, void* d_workspace,
                         uint64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Requests with their own adapters, rules and draws (no counterpart in the
+ * reference, which runs one sequence and takes first maxima,
+ * crates/inference/direct/src/executor.rs:143-185). Results are integers that
+ * the definitions below fix bit for bit, whichever rows share a launch. As
+ * with the paged operators, every pointer inside the structs is device memory
+ * of the current device, calls enqueue on `stream`, allocate nothing, do not
+ * synchronise and can be captured into a graph, and calls that may run at once
+ * need work spaces of their own. What the device finds wrong it reports in
+ * *status (nullable, set and never cleared here); nothing is read or written
+ * out of bounds. "Rounded" is to the nearest integer, ties to even.
+ * ---------------------------------------------------------------------- */
+
+/* A bank of low-rank adapters of one product of `cols` columns. The product
+ * has up to IRIS_ADAPTER_PARTS parts, stacked or interleaved: output i of a
+ * part is column first + i * step of the product's rows. Each of `slots`
+ * adapters has for each part a pair of matrices A [rank][cols] and B
+ * [rows][rank] of 16-bit integers of at most IRIS_ADAPTER_WEIGHT in magnitude,
+ * each matrix with a number of fraction bits, its weights being a / 2^bits.
+ * cols: a multiple of 32, at most 65504; max_rank 1 to IRIS_ADAPTER_RANK; parts
+ * that do not share an output; slots at most 65535. The bank is device memory
+ * of the device that is current when it is made. Slots are empty at first. */
+#define IRIS_ADAPTER_PARTS 3
+#define IRIS_ADAPTER_RANK 256
+#define IRIS_ADAPTER_WEIGHT 32639
+#define IRIS_ADAPTER_BITS 40
+typedef struct IrisAdapterPart {
+    uint32_t rows, first, step;
+} IrisAdapterPart;
+typedef struct IrisAdapterBank IrisAdapterBank;
+
+int iris_adapters_create(uint32_t cols, const IrisAdapterPart* parts, uint32_t part_count, uint32_t slots, uint32_t max_rank,
+                         IrisAdapterBank** out);
+void iris_adapters_free(IrisAdapterBank* bank);
+/* Device bytes that the bank holds: about 2 slots max_rank (cols + rows) a part. */
+uint64_t iris_adapters_device_bytes(const IrisAdapterBank* bank);
+
+/* Copies one part of an adapter from host memory: A and B row by row, their
+ * fraction bits (at most IRIS_ADAPTER_BITS) and the rank; rank 0 empties the
+ * part (a and b are not read then). Waits for the device first, so that no
+ * call still reads the slot. IRIS_E_RANGE for a weight or a rank past the
+ * bounds; the part is then as it was. */
+int iris_adapters_load(IrisAdapterBank* bank, uint32_t slot, uint32_t part, const int16_t* a, uint32_t a_bits,
+                       const int16_t* b, uint32_t b_bits, uint32_t rank);
+
+/* Row r with adapter s = slots[r]: for each part that s holds
+ *   t[j]   = A[j] . x[r] / 2^a_bits, rounded and clamped to 32 bits
+ *   u[i]   = B[i] . t / 2^b_bits, rounded and clamped to 32 bits
+ *   out[r][first + i step] = y[r][first + i step] + u[i], clamped
+ * with exact sums; rows of slot -1 and empty parts have out = y. out may be y
+ * (of the same stride: such rows are then left alone), else overlaps none of
+ * the others; columns that belong to no part are left as they were. x is
+ * 16-byte aligned, its stride a multiple of 4; strides in values, at least
+ * cols, or the parts' last column + 1. At most 65535 rows.
+ *   status  IRIS_E_INVALID where a slot lies outside the bank (as slot -1) */
+typedef struct IrisAdapterRows {
+    const int32_t* x;
+    const int32_t* y;
+    int32_t* out;
+    const int32_t* slots;
+    int32_t* status;
+    uint32_t x_stride, y_stride, out_stride;
+    uint32_t rows;
+} IrisAdapterRows;
+
+/* Bytes of work space for up to `rows` rows (0 for a null bank or no rows). */
+uint64_t iris_adapters_workspace_bytes(const IrisAdapterBank* bank, uint32_t rows);
+int iris_adapters_apply(const IrisAdapterBank* bank, const IrisAdapterRows* a, void* d_workspace, uint64_t workspace_bytes,
+                        void* stream);
+
+/* One request's rule (a record in device memory).
+ *   repetition           Q16.16, above 0; 65536: none
+ *   frequency, presence  Q16.16, taken off per occurrence, and once
+ *   window               the last tokens of its text that count; 0: all
+ *   bias_start, _count   its entries of bias_ids and bias_values */
+typedef struct IrisTokenRule {
+    int32_t repetition, frequency, presence;
+    uint32_t window, bias_start, bias_count;
+} IrisTokenRule;
+
+/* Rules on rows of logits. Row r of the call belongs to request q =
+ * request[r] (-1: to none; only its mask counts). The request's text is
+ * history[q][0 .. lengths[q]) and, with ids, the drafted rows from the root to
+ * row first_row + r of the pass, that row's token the last: ids and parents
+ * (null: chains) are the pass's rows, request q's from row_start[q] to
+ * row_start[q + 1] (at most 64), as IrisTreeAttention's. With c the
+ * occurrences of token v in the window's part of the text:
+ *   l = logits[r][v]; where c is not 0, l / repetition if l > 0, else
+ *       l * repetition (in Q16.16, rounded)
+ *   out[r][v] = l - c frequency - (c > 0) presence + the sum of v's biases,
+ *       summed exactly, then clamped to [INT32_MIN + 1, INT32_MAX];
+ *   INT32_MIN where logits[r][v] is (a place closed before) and where bit v %
+ *       32 of word v / 32 of masks[mask_of[r]] is 0 (mask_of null or -1: no
+ *       mask).
+ * Tokens outside the vocabulary count nowhere. out may be logits (of the same
+ * stride), else overlaps nothing. vocab is at most 2^20, rows at most 65535,
+ * history_stride at most 2^20, biases (entries of the two arrays) at most
+ * 2^20; without `rules` no row has a request (request and what follows to
+ * bias_values are not read).
+ *   status  IRIS_E_INVALID for a request, mask, repetition or bias range that
+ *           cannot be, IRIS_E_RANGE where a request's length or rows pass these
+ *           bounds; such a row has no request (or no mask) */
+typedef struct IrisLogitsRules {
+    const int32_t* logits;
+    int32_t* out;
+    const int32_t* request;
+    const IrisTokenRule* rules;
+    const int32_t* history;
+    const int32_t* lengths;
+    const int32_t* row_start;
+    const int32_t* ids;
+    const int32_t* parents;
+    const int32_t* bias_ids;
+    const int32_t* bias_values;
+    const uint32_t* masks;
+    const int32_t* mask_of;
+    int32_t* status;
+    uint32_t rows, first_row, vocab, logits_stride, out_stride;
+    uint32_t requests, history_stride, biases, mask_rows, mask_stride;
+} IrisLogitsRules;
+
+int iris_logits_rules(const IrisLogitsRules* a, void* stream);
+
+/* How a request draws (a record in device memory).
+ *   inverse_temperature  Q16.16; 0 or below: the first maximum
+ *   top_k                the most tokens kept; 0: all
+ *   top_p                the share of the weights kept, in 32 fraction bits; 0: all
+ *   max_gap              Q16.16: the farthest below the first that a token may
+ *                        lie, in its scaled gap (a share p of the first's
+ *                        weight is -ln p); 0: any */
+typedef struct IrisDrawing {
+    int32_t inverse_temperature;
+    uint32_t top_k, top_p, max_gap;
+} IrisDrawing;
+
+/* A token for each row of logits, INT32_MIN being a place that a mask closed.
+ * With m the row's largest logit, a token's gap is (m - l) inverse_temperature
+ * rounded to Q16.16, and its weight the attention's exp term of the gap
+ * (crates/det-num/src/ops.rs:508-556; 2^32 for the largest, 0 from a gap of 16
+ * on), 0 past max_gap. The tokens in order of falling logits, of equal ones the
+ * smaller index first: top_k keeps the first top_k, top_p of these the shortest
+ * run from the first whose weights add to at least top_p / 2^32 of theirs. With
+ * S the sum of the weights kept and numbers[r] the row's random 32 bits, the
+ * token is the first whose running sum passes floor(numbers[r] S / 2^32).
+ *   request   (nullable) each row's request, -1 as a null `drawings`: the
+ *             first maximum. Null: row r is request r's
+ *   drawings  (nullable) the requests' records
+ *   numbers   (nullable where drawings is)
+ *   tokens    -1 for a row whose every place is closed
+ *   mass      (nullable) [rows][2]: the token's weight and S (2^32 and 2^32 for
+ *             a first maximum, 0 and 0 for token -1)
+ *   status    IRIS_E_INVALID for a request that cannot be (the first maximum)
+ * vocab is at most 2^20, rows at most 65535. */
+typedef struct IrisLogitsDraw {
+    const int32_t* logits;
+    const int32_t* request;
+    const IrisDrawing* drawings;
+    const uint32_t* numbers;
+    int32_t* tokens;
+    int64_t* mass;
+    int32_t* status;
+    uint32_t rows, vocab, logits_stride, requests;
+} IrisLogitsDraw;
+
+/* Bytes of work space a call needs (0 for one that is refused). */
+uint64_t iris_logits_draw_workspace_bytes(const IrisLogitsDraw* a);
+int iris_logits_draw(const IrisLogitsDraw* a, void* d_workspace, uint64_t workspace_bytes, void* stream);
+
 /* Greedy generation of several requests at a time over one paged cache of
  * `pages` pages of page_size positions (of every layer that has keys of its
  * own), each up to max_positions (at most 2^20), in passes of up to max_rows
