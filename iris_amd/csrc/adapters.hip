@@ -2,10 +2,15 @@
 // gets out = y + B_s (A_s x), both products exact over 16-bit weights and
 // rounded once each.
 //
-// Two launches, since every output needs the whole of A x: t = A x for each
-// row into the work space, then B t added to y.
+// Two launches, since every output needs the whole of A x: the sums of A x for
+// each row into the work space, then B t added to y. Few rows take a workgroup
+// per value of A x and a thread per output, on the vector units; more rows tiles
+// of 32 on the int8 matrix cores, a tile's adapters one after the other.
+//
+// A weight is kept as two signed byte digits, w = 256 high + low, in 16 bits;
+// a value of x or t is up to five (three below 2^23 in magnitude, split4 in
+// attn_tiles.h). Digit products of one weight 2^8s share an int32 accumulator.
 #include <algorithm>
-#include <cstring>
 #include <new>
 #include <vector>
 
@@ -28,6 +33,19 @@ struct AdapterShape {
     uint32_t cols, part_count, slots, max_rank;
     IrisAdapterPart parts[IRIS_ADAPTER_PARTS];
 };
+
+// Rows up to which a call takes the kernels of single rows.
+constexpr uint32_t FEW_ROWS = 48;
+constexpr uint32_t TILE_ROWS = 32;
+constexpr uint32_t TILE_RANKS = 64;    // of A x a workgroup forms at a time: four 16-rank tiles
+constexpr uint32_t MAX_SPLITS = 16;    // pieces of the columns, each with sums of its own
+constexpr uint32_t CHUNK_OUTPUTS = 512;  // of a tile of rows that a workgroup forms
+
+// A weight's two digits, and the weight from them.
+inline uint16_t digits_of(int16_t w) { return (uint16_t)(((w + 128) & ~255) | (w & 255)); }
+__device__ __forceinline__ int32_t weight_of(uint32_t digits) {
+    return (int32_t)(int16_t)digits - (int32_t)((digits & 0x80u) << 1);
+}
 
 // A sum of products as the Q16.16 value it stands for.
 __device__ __forceinline__ int32_t rounded(int64_t sum, uint32_t bits) {
@@ -66,8 +84,8 @@ __global__ __launch_bounds__(256) void shrink_row_kernel(const IrisAdapterRows a
         const int32_t q[4] = {p.x, p.y, p.z, p.w}, v[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
 #pragma unroll
         for (int c = 0; c < 4; c++) {
-            sum += (int64_t)(int16_t)q[c] * v[2 * c];
-            sum += (int64_t)(q[c] >> 16) * v[2 * c + 1];
+            sum += (int64_t)weight_of((uint32_t)q[c]) * v[2 * c];
+            sum += (int64_t)weight_of((uint32_t)q[c] >> 16) * v[2 * c + 1];
         }
     }
     sum = wave_sum(sum);
@@ -93,10 +111,353 @@ __global__ __launch_bounds__(256) void expand_row_kernel(const IrisAdapterRows a
         const int32_t* tr = t + ((size_t)row * sh.part_count + part) * sh.max_rank;
         const int16_t* w = e.b + (size_t)i * stride_of(e.rank);
         int64_t sum = 0;
-        for (uint32_t j = 0; j < e.rank; j++) sum += (int64_t)w[j] * tr[j];
+        for (uint32_t j = 0; j < e.rank; j++) sum += (int64_t)weight_of((uint16_t)w[j]) * tr[j];
         v = dn::add_sat(v, rounded(sum, e.b_bits));
     }
     a.out[(size_t)row * a.out_stride + column] = v;
+}
+
+// ------------------------------------------------------------------ tiles of rows
+
+struct Tile {
+    uint32_t lane, wave;
+    int32_t slot;      // of row lane % 32
+    uint32_t pending;  // rows whose adapter is still to come
+};
+
+__device__ __forceinline__ Tile tile_of(const IrisAdapterRows& a, const AdapterShape& sh, uint32_t row0, bool report) {
+    Tile t;
+    t.lane = threadIdx.x & 63, t.wave = wave_index();
+    const uint32_t row = row0 + t.lane % TILE_ROWS;
+    t.slot = row < a.rows ? slot_of(a, sh.slots, row, report && threadIdx.x < TILE_ROWS) : -1;
+    t.pending = (uint32_t)__ballot(t.slot >= 0);
+    return t;
+}
+
+// The next adapter of the tile and its rows.
+__device__ __forceinline__ uint32_t next_slot(Tile& t, int32_t& slot) {
+    slot = __builtin_amdgcn_readlane(t.slot, __builtin_ctz(t.pending));
+    const uint32_t rows = (uint32_t)__ballot(t.slot == slot);
+    t.pending &= ~rows;
+    return rows;
+}
+
+// Sixteen weights' digits as two operands of the matrix cores.
+__device__ __forceinline__ void weight_digits(const int16_t* w, bool valid, v4i& low, v4i& high) {
+    int4 p{}, q{};
+    if (valid) p = load4((const int32_t*)w), q = load4((const int32_t*)w + 4);
+    const uint32_t d[8] = {(uint32_t)p.x, (uint32_t)p.y, (uint32_t)p.z, (uint32_t)p.w,
+                           (uint32_t)q.x, (uint32_t)q.y, (uint32_t)q.z, (uint32_t)q.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        low[i] = (int)__builtin_amdgcn_perm(d[2 * i + 1], d[2 * i], 0x06040200u);
+        high[i] = (int)__builtin_amdgcn_perm(d[2 * i + 1], d[2 * i], 0x07050301u);
+    }
+}
+
+// Three digits of sixteen values: the low three, or with HIGH the two above.
+template <bool HIGH>
+__device__ __forceinline__ void value_digits(const int4 (&v)[4], v4i (&digit)[3], uint32_t& seen) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t plane[4];
+        split4(v[i], plane, seen);
+        digit[0][i] = (int)(HIGH ? plane[3] : plane[0]);
+        digit[1][i] = (int)(HIGH ? fifth4(v[i]) : plane[1]);
+        digit[2][i] = HIGH ? 0 : (int)plane[2];
+    }
+}
+
+// One step's products of two weight digits and DIGITS value digits.
+template <int DIGITS>
+__device__ __forceinline__ void digit_products(v4i low, v4i high, const v4i (&digit)[3], v4i (&acc)[4]) {
+#pragma unroll
+    for (int d = 0; d < DIGITS; d++) {
+        acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(low, digit[d], acc[d], 0, 0, 0);
+        acc[d + 1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(high, digit[d], acc[d + 1], 0, 0, 0);
+    }
+}
+
+// A rank tile's place: sixteen values of A x of one part.
+struct RankTile {
+    const int16_t* a;  // this lane's weights row
+    uint32_t at;       // of the tile's first value among the row's part_count max_rank
+    uint32_t ranks;    // of the sixteen that there are
+};
+
+// The sums of A x over a piece of the columns for a tile of rows: waves take the
+// piece's 64-column steps in turn, each with up to four rank tiles, and add
+// their int64 sums in LDS (exact, so the order does not matter).
+template <bool HIGH>
+__device__ __forceinline__ bool shrink_steps(const IrisAdapterRows& a, uint32_t cols, const RankTile (&tile)[4], uint32_t tiles,
+                                             uint32_t row0, uint32_t step0, uint32_t step1, const Tile& t, int64_t* s_sum) {
+    v4i acc[2][4][4] = {};
+    uint32_t seen = 0;
+    const uint32_t n = t.lane & 15, group = t.lane >> 4;
+    const int32_t* x[2];
+#pragma unroll
+    for (int g = 0; g < 2; g++) x[g] = a.x + (size_t)min(row0 + 16 * g + n, a.rows - 1) * a.x_stride;
+    for (uint32_t step = step0 + t.wave; step < step1; step += 4) {
+        const uint32_t k = step * 64 + 16 * group;
+        const bool valid = k < cols;
+        int4 v[2][4] = {};
+        if (valid) {
+#pragma unroll
+            for (int g = 0; g < 2; g++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[g][i] = load4(x[g] + k + 4 * i);
+        }
+        v4i digit[2][3];
+#pragma unroll
+        for (int g = 0; g < 2; g++) value_digits<HIGH>(v[g], digit[g], seen);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (i >= (int)tiles) break;
+            v4i low, high;
+            weight_digits(tile[i].a + k, valid, low, high);
+#pragma unroll
+            for (int g = 0; g < 2; g++) digit_products<HIGH ? 2 : 3>(low, high, digit[g], acc[g][i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (i >= (int)tiles) break;
+#pragma unroll
+        for (int g = 0; g < 2; g++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                int64_t sum = 0;
+#pragma unroll
+                for (int d = 3; d >= 0; d--) sum = (sum << 8) + acc[g][i][d][c];
+                if (HIGH) sum <<= 24;
+                atomicAdd((unsigned long long*)&s_sum[(16 * g + n) * (TILE_RANKS + 1) + 16 * i + 4 * group + c],
+                          (unsigned long long)sum);
+            }
+    }
+    return is_wide(seen);
+}
+
+// Workgroup: piece blockIdx.x of the columns, row tile blockIdx.y. sums:
+// [piece][row][part_count max_rank].
+__global__ __launch_bounds__(256, 2) void shrink_tile_kernel(const IrisAdapterRows a, const AdapterShape sh,
+                                                             const AdapterEntry* table, int64_t* sums) {
+    __shared__ int64_t s_sum[TILE_ROWS * (TILE_RANKS + 1)];
+    __shared__ uint32_t s_wide;
+    const uint32_t row0 = blockIdx.y * TILE_ROWS, tid = threadIdx.x, steps = (sh.cols + 63) / 64;
+    const uint32_t per = (steps + gridDim.x - 1) / gridDim.x, step0 = min(blockIdx.x * per, steps), step1 = min(step0 + per, steps);
+    const uint32_t width = sh.part_count * sh.max_rank;
+    Tile t = tile_of(a, sh, row0, blockIdx.x == 0);
+    while (t.pending) {
+        int32_t slot;
+        const uint32_t rows = next_slot(t, slot);
+        const AdapterEntry* entry = table + (size_t)slot * sh.part_count;
+        uint32_t part = 0, j = 0;  // the next rank tile
+        while (true) {
+            RankTile tile[4];
+            uint32_t tiles = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                while (part < sh.part_count && j >= entry[part].rank) part++, j = 0;
+                if (part == sh.part_count) break;
+                const AdapterEntry e = entry[part];
+                tile[i].a = e.a + (size_t)min(j + (t.lane & 15), e.rank - 1) * sh.cols;
+                tile[i].at = part * sh.max_rank + j;
+                tile[i].ranks = min(e.rank - j, 16u);
+                j += 16;
+                tiles++;
+            }
+            if (!tiles) break;
+            __syncthreads();  // the sums before are read
+            for (uint32_t i = tid; i < TILE_ROWS * (TILE_RANKS + 1); i += 256) s_sum[i] = 0;
+            if (tid == 0) s_wide = 0;
+            __syncthreads();
+            if (shrink_steps<false>(a, sh.cols, tile, tiles, row0, step0, step1, t, s_sum) && t.lane == 0) s_wide = 1;
+            __syncthreads();
+            if (s_wide) {
+                shrink_steps<true>(a, sh.cols, tile, tiles, row0, step0, step1, t, s_sum);
+                __syncthreads();
+            }
+            // A row of 64 values a wave and turn.
+            for (uint32_t r = t.wave; r < TILE_ROWS; r += 4) {
+                if (!(rows >> r & 1)) continue;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (i < (int)tiles && t.lane / 16 == i && t.lane % 16 < tile[i].ranks)
+                        sums[((size_t)blockIdx.x * a.rows + row0 + r) * width + tile[i].at + t.lane % 16] =
+                            s_sum[r * (TILE_RANKS + 1) + t.lane];
+            }
+        }
+    }
+}
+
+// Four neighbouring outputs' columns of a row.
+template <bool VEC>
+__device__ __forceinline__ int4 load_columns(const int32_t* p, uint32_t step, uint32_t count) {
+    if (VEC && count == 4) return load4(p);
+    int4 v{};
+    if (count > 0) v.x = load1(p);
+    if (count > 1) v.y = load1(p + step);
+    if (count > 2) v.z = load1(p + 2 * step);
+    if (count > 3) v.w = load1(p + 3 * step);
+    return v;
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store_columns(int32_t* p, uint32_t step, uint32_t count, int4 v) {
+    if (VEC && count == 4) {
+        *(int4*)p = v;
+        return;
+    }
+    if (count > 0) p[0] = v.x;
+    if (count > 1) p[step] = v.y;
+    if (count > 2) p[2 * (size_t)step] = v.z;
+    if (count > 3) p[3 * (size_t)step] = v.w;
+}
+
+// y + sum / 2^bits from the sum's exact double, below 2^53.
+__device__ __forceinline__ int32_t added(int32_t y, double sum, double unit) {
+    const double u = fmin(fmax(rint(sum * unit), -2147483648.0), 2147483647.0);
+    return (int32_t)fmin(fmax((double)y + u, -2147483648.0), 2147483647.0);
+}
+
+// Workgroup: outputs from blockIdx.x CHUNK_OUTPUTS of part blockIdx.z, row tile
+// blockIdx.y. LDS: t of the tile's rows, [32][whole 64-rank steps and 4 more].
+template <bool VEC>
+__global__ __launch_bounds__(256) void expand_tile_kernel(const IrisAdapterRows a, const AdapterShape sh, const AdapterEntry* table,
+                                                          const int64_t* sums, uint32_t splits) {
+    extern __shared__ int32_t s_t[];
+    __shared__ uint32_t s_wide;
+    const uint32_t row0 = blockIdx.y * TILE_ROWS, tid = threadIdx.x, part = blockIdx.z;
+    const IrisAdapterPart p = sh.parts[part];
+    const uint32_t i0 = blockIdx.x * CHUNK_OUTPUTS, i1 = min(i0 + CHUNK_OUTPUTS, p.rows);
+    if (i0 >= p.rows) return;
+    const uint32_t padded = (sh.max_rank + 63) & ~63u, stride = padded + 4, width = sh.part_count * sh.max_rank;
+    Tile t = tile_of(a, sh, row0, false);
+    const uint32_t n = t.lane & 15, group = t.lane >> 4;
+    uint32_t copied = ~t.pending;  // rows that no adapter changes
+    while (t.pending) {
+        int32_t slot;
+        const uint32_t rows = next_slot(t, slot);
+        const AdapterEntry e = table[(size_t)slot * sh.part_count + part];
+        if (!e.rank) {
+            copied |= rows;
+            continue;
+        }
+        const uint32_t blocks = (e.rank + 63) / 64, b_stride = stride_of(e.rank);
+        __syncthreads();  // the adapter before is done with s_t
+        if (tid == 0) s_wide = 0;
+        __syncthreads();
+        uint32_t far = 0;
+        for (uint32_t i = tid; i < TILE_ROWS * blocks * 64; i += 256) {
+            const uint32_t r = i / (blocks * 64), j = i % (blocks * 64);
+            int32_t v = 0;
+            if (j < e.rank && (rows >> r & 1)) {
+                const int64_t* from = sums + (size_t)(row0 + r) * width + part * sh.max_rank + j;
+                int64_t sum = 0;
+                for (uint32_t q = 0; q < splits; q++) sum += from[(size_t)q * a.rows * width];
+                v = rounded(sum, e.a_bits);
+            }
+            s_t[r * stride + j] = v;
+            far |= (uint32_t)(v > 8355711 || v < -8421504);
+        }
+        if (far) s_wide = 1;
+        __syncthreads();
+        const bool wide = s_wide != 0;
+        const double unit = ldexp(1.0, -(int)e.b_bits);
+        for (uint32_t i = i0 + 16 * t.wave; i < i1; i += 64) {
+            const int16_t* w = e.b + (size_t)min(i + n, p.rows - 1) * b_stride;
+            const uint32_t first = i + 4 * group, count = first < i1 ? min(i1 - first, 4u) : 0;
+            int4 y[2];
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+                const uint32_t r = 16 * g + n;
+                y[g] = load_columns<VEC>(a.y + (size_t)(row0 + r) * a.y_stride + p.first + (size_t)first * p.step, p.step,
+                                         rows >> r & 1 ? count : 0);
+            }
+            v4i acc[2][4] = {}, top[2][4] = {};
+            for (uint32_t block = 0; block < blocks; block++) {
+                const uint32_t k = 64 * block + 16 * group;
+                // The rank's padding ends at 8 of 16: those behind it are another row's.
+                v4i low, high;
+                {
+                    int4 b0{}, b1{};
+                    if (k < b_stride) b0 = load4((const int32_t*)(w + k));
+                    if (k + 8 < b_stride) b1 = load4((const int32_t*)(w + k) + 4);
+                    const uint32_t d[8] = {(uint32_t)b0.x, (uint32_t)b0.y, (uint32_t)b0.z, (uint32_t)b0.w,
+                                           (uint32_t)b1.x, (uint32_t)b1.y, (uint32_t)b1.z, (uint32_t)b1.w};
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        low[c] = (int)__builtin_amdgcn_perm(d[2 * c + 1], d[2 * c], 0x06040200u);
+                        high[c] = (int)__builtin_amdgcn_perm(d[2 * c + 1], d[2 * c], 0x07050301u);
+                    }
+                }
+#pragma unroll
+                for (int g = 0; g < 2; g++) {
+                    int4 v[4];
+#pragma unroll
+                    for (int c = 0; c < 4; c++) v[c] = *(const int4*)&s_t[(16 * g + n) * stride + k + 4 * c];
+                    v4i digit[3];
+                    uint32_t seen = 0;
+                    value_digits<false>(v, digit, seen);
+                    digit_products<3>(low, high, digit, acc[g]);
+                    if (wide) {
+                        value_digits<true>(v, digit, seen);
+                        digit_products<2>(low, high, digit, top[g]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+                const uint32_t r = 16 * g + n;
+                const int32_t old[4] = {y[g].x, y[g].y, y[g].z, y[g].w};
+                int32_t out[4];
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    if (!wide) {
+                        // Below 2^23 2^15 256 = 2^46: exact.
+                        double sum = (double)acc[g][3][c];
+#pragma unroll
+                        for (int d = 2; d >= 0; d--) sum = fma(sum, 256.0, (double)acc[g][d][c]);
+                        out[c] = added(old[c], sum, unit);
+                    } else {
+                        int64_t sum = 0, high = 0;
+#pragma unroll
+                        for (int d = 3; d >= 0; d--) sum = (sum << 8) + acc[g][d][c], high = (high << 8) + top[g][d][c];
+                        out[c] = dn::add_sat(old[c], rounded(sum + (high << 24), e.b_bits));
+                    }
+                }
+                if (rows >> r & 1)
+                    store_columns<VEC>(a.out + (size_t)(row0 + r) * a.out_stride + p.first + (size_t)first * p.step, p.step, count,
+                                       make_int4(out[0], out[1], out[2], out[3]));
+            }
+        }
+    }
+    if (a.out == a.y) return;
+    for (uint32_t r = t.wave; r < TILE_ROWS && row0 + r < a.rows; r += 4) {
+        if (!(copied >> r & 1)) continue;
+        for (uint32_t i = i0 + 4 * t.lane; i < i1; i += 256) {
+            const size_t column = p.first + (size_t)i * p.step;
+            const uint32_t count = min(i1 - i, 4u);
+            store_columns<VEC>(a.out + (size_t)(row0 + r) * a.out_stride + column, p.step, count,
+                               load_columns<VEC>(a.y + (size_t)(row0 + r) * a.y_stride + column, p.step, count));
+        }
+    }
+}
+
+// Pieces of the columns for a call of tiles: enough workgroups for the card,
+// each with a step for every wave.
+uint32_t splits_of(const AdapterShape& s, uint32_t rows) {
+    const uint32_t tiles = (rows + TILE_ROWS - 1) / TILE_ROWS, steps = (s.cols + 63) / 64;
+    // A piece's accumulators hold 2^14 2 64 a step: 32768 columns at most.
+    const uint32_t least = (s.cols + 32767) / 32768;
+    return std::max(least, std::min(std::min(256 / tiles, (steps + 3) / 4), MAX_SPLITS));
+}
+
+// Bytes of work space of a call: t itself for few rows, its sums by pieces for
+// tiles.
+uint64_t space_of(const AdapterShape& s, uint32_t rows) {
+    const uint64_t values = (uint64_t)rows * s.part_count * s.max_rank;
+    return rows <= FEW_ROWS ? values * 4 : values * splits_of(s, rows) * 8;
 }
 
 }  // namespace
@@ -172,22 +533,28 @@ int iris_adapters_load(IrisAdapterBank* b, uint32_t slot, uint32_t part, const i
     const AdapterShape& s = b->shape;
     if (rank > s.max_rank || (rank && (a_bits > IRIS_ADAPTER_BITS || b_bits > IRIS_ADAPTER_BITS))) return IRIS_E_RANGE;
     const uint32_t rows = s.parts[part].rows, stride = stride_of(rank);
-    auto past = [](const int16_t* v, uint64_t n) {
-        for (uint64_t i = 0; i < n; i++)
-            if (v[i] > IRIS_ADAPTER_WEIGHT || v[i] < -IRIS_ADAPTER_WEIGHT) return true;
-        return false;
-    };
-    if (past(a, (uint64_t)rank * s.cols) || past(w, (uint64_t)rank * rows)) return IRIS_E_RANGE;
-    std::vector<int16_t> padded;
-    if (stride != rank) {
-        try {
-            padded.assign((size_t)rows * stride, 0);
-        } catch (const std::bad_alloc&) {
-            return IRIS_E_NOMEM;
-        }
-        for (uint32_t i = 0; i < rows; i++) std::memcpy(&padded[(size_t)i * stride], w + (size_t)i * rank, rank * 2);
-        w = padded.data();
+    // The two digits of each weight, A and then B with its rows padded by zeros.
+    std::vector<uint16_t> digits;
+    const size_t a_count = (size_t)rank * s.cols, count = a_count + (size_t)rows * stride;
+    try {
+        digits.assign(count, 0);
+    } catch (const std::bad_alloc&) {
+        return IRIS_E_NOMEM;
     }
+    uint32_t past = 0;
+    auto convert = [&past](const int16_t* from, uint16_t* to, size_t n) {
+        uint32_t bad = 0;
+        for (size_t i = 0; i < n; i++) {
+            bad |= (uint32_t)(from[i] > IRIS_ADAPTER_WEIGHT) | (uint32_t)(from[i] < -IRIS_ADAPTER_WEIGHT);
+            to[i] = digits_of(from[i]);
+        }
+        past |= bad;
+    };
+    convert(a, digits.data(), a_count);
+    if (stride == rank) convert(w, digits.data() + a_count, (size_t)rows * rank);
+    else
+        for (uint32_t i = 0; i < rows; i++) convert(w + (size_t)i * rank, digits.data() + a_count + (size_t)i * stride, rank);
+    if (past) return IRIS_E_RANGE;
     int16_t* to = b->weights + slot * b->slot_weights + b->part_at[part];
     AdapterEntry* entry = b->table + (size_t)slot * s.part_count + part;
     AdapterEntry e{};
@@ -196,10 +563,9 @@ int iris_adapters_load(IrisAdapterBank* b, uint32_t slot, uint32_t part, const i
     // (A copy that fails on the way leaves the part empty.)
     st = hipMemcpy(entry, &e, sizeof(e), hipMemcpyHostToDevice);
     if (st == hipSuccess && rank) {
-        e.a = to, e.b = to + (((uint64_t)s.max_rank * s.cols + 7) & ~7ull);
+        e.a = to, e.b = to + a_count;
         e.rank = rank, e.a_bits = a_bits, e.b_bits = b_bits;
-        st = hipMemcpy((void*)e.a, a, (size_t)rank * s.cols * 2, hipMemcpyHostToDevice);
-        if (st == hipSuccess) st = hipMemcpy((void*)e.b, w, (size_t)rows * stride * 2, hipMemcpyHostToDevice);
+        st = hipMemcpy(to, digits.data(), count * 2, hipMemcpyHostToDevice);
         if (st == hipSuccess) st = hipMemcpy(entry, &e, sizeof(e), hipMemcpyHostToDevice);
     }
     return (int)st;
@@ -207,7 +573,10 @@ int iris_adapters_load(IrisAdapterBank* b, uint32_t slot, uint32_t part, const i
 
 uint64_t iris_adapters_workspace_bytes(const IrisAdapterBank* b, uint32_t rows) {
     if (!b || !rows || rows > 65535) return 0;
-    return (uint64_t)rows * b->shape.part_count * b->shape.max_rank * 4;
+    // What any number of rows up to these takes: whole tiles take the most.
+    uint64_t bytes = space_of(b->shape, rows);
+    for (uint32_t n = rows / TILE_ROWS * TILE_ROWS; n; n -= TILE_ROWS) bytes = std::max(bytes, space_of(b->shape, n));
+    return std::max(bytes, space_of(b->shape, std::min(rows, FEW_ROWS)));
 }
 
 int iris_adapters_apply(const IrisAdapterBank* b, const IrisAdapterRows* a, void* space, uint64_t space_bytes, void* stream) {
@@ -219,11 +588,24 @@ int iris_adapters_apply(const IrisAdapterBank* b, const IrisAdapterRows* a, void
     if (a->x_stride < s.cols || a->y_stride < b->width || a->out_stride < b->width) return IRIS_E_INVALID;
     if (a->out == a->y && a->out_stride != a->y_stride) return IRIS_E_INVALID;
     if (a->rows > 65535) return IRIS_E_RANGE;
-    if (space_bytes < iris_adapters_workspace_bytes(b, a->rows)) return IRIS_E_RANGE;
-    hipLaunchKernelGGL(shrink_row_kernel, dim3(s.part_count * s.max_rank, a->rows), dim3(256), 0, (hipStream_t)stream, *a, s,
-                       b->table, (int32_t*)space);
-    hipLaunchKernelGGL(expand_row_kernel, dim3((b->most_rows + 255) / 256, a->rows, s.part_count), dim3(256), 0,
-                       (hipStream_t)stream, *a, s, b->table, (const int32_t*)space);
+    if (space_bytes < space_of(s, a->rows)) return IRIS_E_RANGE;
+    hipStream_t st = (hipStream_t)stream;
+    if (a->rows > FEW_ROWS) {
+        const uint32_t tiles = (a->rows + TILE_ROWS - 1) / TILE_ROWS, splits = splits_of(s, a->rows);
+        const size_t lds = TILE_ROWS * (((s.max_rank + 63) & ~63u) + 4) * 4;
+        // Sixteen bytes of a row at a time where every part allows it.
+        bool vec = !misaligned(a->y) && !misaligned(a->out) && a->y_stride % 4 == 0 && a->out_stride % 4 == 0;
+        for (uint32_t p = 0; p < s.part_count; p++) vec = vec && s.parts[p].step == 1 && s.parts[p].first % 4 == 0;
+        const dim3 grid((b->most_rows + CHUNK_OUTPUTS - 1) / CHUNK_OUTPUTS, tiles, s.part_count);
+        hipLaunchKernelGGL(shrink_tile_kernel, dim3(splits, tiles), dim3(256), 0, st, *a, s, b->table, (int64_t*)space);
+        if (vec) hipLaunchKernelGGL(expand_tile_kernel<true>, grid, dim3(256), lds, st, *a, s, b->table, (const int64_t*)space, splits);
+        else hipLaunchKernelGGL(expand_tile_kernel<false>, grid, dim3(256), lds, st, *a, s, b->table, (const int64_t*)space, splits);
+        return (int)hipGetLastError();
+    }
+    hipLaunchKernelGGL(shrink_row_kernel, dim3(s.part_count * s.max_rank, a->rows), dim3(256), 0, st, *a, s, b->table,
+                       (int32_t*)space);
+    hipLaunchKernelGGL(expand_row_kernel, dim3((b->most_rows + 255) / 256, a->rows, s.part_count), dim3(256), 0, st, *a,
+                       s, b->table, (const int32_t*)space);
     return (int)hipGetLastError();
 }
 

@@ -112,14 +112,14 @@ def test_rows_of_many_adapters(rows, parts):
 
 
 @pytest.mark.parametrize("rank", [1, 2, 7, 8, 9, 15, 16, 17, 31, 32, 33, 63, 64, 65, 100, 128, 129, 255, 256])
-@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("rows", [1, 40, 75])
 def test_ranks(rank, rows):
     rng = np.random.default_rng(rank)
     Call(rng, 96, QKV, [[rank] * 3, [max(1, rank // 2), rank, 0]], rows, rng.integers(0, 2, rows)).check()
 
 
 @pytest.mark.parametrize("cols", [32, 64, 96, 224, 416, 1024, 2080, 14336, 65504])
-@pytest.mark.parametrize("rows", [1, 3, 35])
+@pytest.mark.parametrize("rows", [1, 3, 35, 64])
 def test_columns(cols, rows):
     rng = np.random.default_rng(cols)
     Call(rng, cols, ODD, [[9, 16], [16, 3]], rows, np.arange(rows) % 2).check()
@@ -127,7 +127,7 @@ def test_columns(cols, rows):
 
 @pytest.mark.parametrize("kind", ["normal", "wide", "mixed", "sharp", "ends", "same"])
 @pytest.mark.parametrize("weights", ["normal", "ends", "top", "uniform"])
-@pytest.mark.parametrize("rows", [3, 40])
+@pytest.mark.parametrize("rows", [3, 40, 83])
 def test_values(kind, weights, rows):
     # Every digit of the values and both clamps.
     rng = np.random.default_rng(5)
@@ -140,16 +140,16 @@ def test_the_largest_sums():
     # 65504 products of 2^31 and 32639, without and with shifts, of either sign.
     rng = np.random.default_rng(1)
     for bits in ((0, 0), (40, 40), (38, 20)):
-        for rows in (2, 40):
+        for rows in (2, 40, 66):
             c = Call(rng, 65504, ONE, [[3]], rows, [0] * rows, weights="top", bits=bits)
             c.x[:] = np.where(np.arange(rows) % 2, -2 ** 31, 2 ** 31 - 1)[:, None]
             c.d_x.copy_(Call.strided(c.x, 65504))
             c.check()
 
 
-def test_ties_round_to_even():
+@pytest.mark.parametrize("rows", [41, 95])
+def test_ties_round_to_even(rows):
     # One column of one, weights of halves: sums at every tie of two bits.
-    rows = 41
     c = Call(np.random.default_rng(0), 32, ONE, [[1]], rows, [0] * rows, bits=(2, 1))
     a = np.zeros((1, 32), np.int16)
     a[0, 5] = 1
@@ -157,7 +157,7 @@ def test_ties_round_to_even():
     c.bank.load(0, 0, a, 2, b, 1)
     c.weights = [[(a, 2, b, 1)]]
     c.x[:] = 0
-    c.x[:, 5] = np.arange(rows) - 20
+    c.x[:, 5] = np.arange(rows) - rows // 2
     c.d_x.copy_(Call.strided(c.x, 32))
     c.check()
 
@@ -178,7 +178,7 @@ def test_no_row_has_an_adapter(rows, in_place):
     Call(rng, 64, QKV, [[0, 0, 0], [4, 4, 4]], rows, [0] * rows, in_place=in_place).check()
 
 
-@pytest.mark.parametrize("rows", [3, 40])
+@pytest.mark.parametrize("rows", [3, 40, 90])
 def test_slots_outside_the_bank_are_reported(rows):
     rng = np.random.default_rng(3)
     for bad in (-2, 2, 65535, 2 ** 31 - 1, -2 ** 31):
@@ -187,9 +187,9 @@ def test_slots_outside_the_bank_are_reported(rows):
         Call(rng, 64, QKV, [[4, 4, 4], [9, 2, 0]], rows, slots).check(status=-1)
 
 
-def test_slots_load_again_and_empty():
+@pytest.mark.parametrize("rows", [37, 70])
+def test_slots_load_again_and_empty(rows):
     rng = np.random.default_rng(8)
-    rows = 37
     c = Call(rng, 96, QKV, [[16, 16, 16], [8, 8, 8]], rows, rng.integers(-1, 2, rows))
     c.check()
     a, b = Call.some(rng, (5, 96), "uniform"), Call.some(rng, (32, 5), "uniform")
