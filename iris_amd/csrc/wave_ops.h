@@ -74,3 +74,15 @@ __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
     }
     return t;
 }
+
+// Wrapping running sum over the wave, inclusive: lanes one, two, four and eight
+// before within each row, then the rows before through scalar registers.
+__device__ __forceinline__ uint64_t wave_running_sum_u64(uint64_t v) {
+    v += (uint64_t)dpp64<0x111>((int64_t)v);  // row_shr (0 from outside the row)
+    v += (uint64_t)dpp64<0x112>((int64_t)v);
+    v += (uint64_t)dpp64<0x114>((int64_t)v);
+    v += (uint64_t)dpp64<0x118>((int64_t)v);
+    const uint64_t t0 = readlane64(v, 15), t1 = readlane64(v, 31), t2 = readlane64(v, 47);
+    const uint32_t row = (threadIdx.x & 63) / 16;
+    return v + (row > 0 ? t0 : 0) + (row > 1 ? t1 : 0) + (row > 2 ? t2 : 0);
+}

@@ -175,6 +175,14 @@ def test_rules_of_drafted_rows(nodes, trees, window):
     Rules(rng, 300, [int(rng.integers(0, 30)) for _ in nodes], nodes=nodes, trees=trees, window=window, masks=3, biases=4).check()
 
 
+@pytest.mark.parametrize("vocab, biases", [(600, 3000), (5000, 9000), (9001, 1500)])
+def test_rules_of_many_biases(vocab, biases):
+    # More biased tokens than the sums that a workgroup keeps; each several times.
+    rng = np.random.default_rng(biases)
+    Rules(rng, vocab, [40, 3, 900], biases=biases).check()
+    Rules(rng, vocab, [40, 3], biases=biases, rules=[[ONE, 0, 0, 0, 0, biases], [ONE, 0, 1, 0, biases // 2, biases]], masks=2).check()
+
+
 def test_rules_of_a_part_of_a_pass():
     rng = np.random.default_rng(2)
     for first in (1, 5, 9):
