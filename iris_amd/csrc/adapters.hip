@@ -41,6 +41,10 @@ constexpr uint32_t TILE_RANKS = 64;    // of A x a workgroup forms at a time: fo
 constexpr uint32_t MAX_SPLITS = 16;    // pieces of the columns, each with sums of its own
 constexpr uint32_t CHUNK_OUTPUTS = 512;  // of a tile of rows that a workgroup forms
 
+// Workgroups that share the adapters of a tile of rows: most tiles have one or
+// two, those of short prompts many (2309 rows of 19 prompts: 151 us with one).
+constexpr uint32_t SLOT_GROUPS = 4;
+
 // A weight's two digits, and the weight from them.
 inline uint16_t digits_of(int16_t w) { return (uint16_t)(((w + 128) & ~255) | (w & 255)); }
 __device__ __forceinline__ int32_t weight_of(uint32_t digits) {
@@ -143,9 +147,7 @@ __device__ __forceinline__ uint32_t next_slot(Tile& t, int32_t& slot) {
 }
 
 // Sixteen weights' digits as two operands of the matrix cores.
-__device__ __forceinline__ void weight_digits(const int16_t* w, bool valid, v4i& low, v4i& high) {
-    int4 p{}, q{};
-    if (valid) p = load4((const int32_t*)w), q = load4((const int32_t*)w + 4);
+__device__ __forceinline__ void split_weights(int4 p, int4 q, v4i& low, v4i& high) {
     const uint32_t d[8] = {(uint32_t)p.x, (uint32_t)p.y, (uint32_t)p.z, (uint32_t)p.w,
                            (uint32_t)q.x, (uint32_t)q.y, (uint32_t)q.z, (uint32_t)q.w};
 #pragma unroll
@@ -213,8 +215,10 @@ __device__ __forceinline__ bool shrink_steps(const IrisAdapterRows& a, uint32_t 
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             if (i >= (int)tiles) break;
+            int4 w0{}, w1{};
+            if (valid) w0 = load4((const int32_t*)(tile[i].a + k)), w1 = load4((const int32_t*)(tile[i].a + k) + 4);
             v4i low, high;
-            weight_digits(tile[i].a + k, valid, low, high);
+            split_weights(w0, w1, low, high);
 #pragma unroll
             for (int g = 0; g < 2; g++) digit_products<HIGH ? 2 : 3>(low, high, digit[g], acc[g][i]);
         }
@@ -237,8 +241,9 @@ __device__ __forceinline__ bool shrink_steps(const IrisAdapterRows& a, uint32_t 
     return is_wide(seen);
 }
 
-// Workgroup: piece blockIdx.x of the columns, row tile blockIdx.y. sums:
-// [piece][row][part_count max_rank].
+// Workgroup: piece blockIdx.x of the columns, row tile blockIdx.y, and of
+// blockIdx.z which of the tile's adapters and which four rank tiles of them.
+// sums: [piece][row][part_count max_rank].
 __global__ __launch_bounds__(256, 2) void shrink_tile_kernel(const IrisAdapterRows a, const AdapterShape sh,
                                                              const AdapterEntry* table, int64_t* sums) {
     __shared__ int64_t s_sum[TILE_ROWS * (TILE_RANKS + 1)];
@@ -246,46 +251,53 @@ __global__ __launch_bounds__(256, 2) void shrink_tile_kernel(const IrisAdapterRo
     const uint32_t row0 = blockIdx.y * TILE_ROWS, tid = threadIdx.x, steps = (sh.cols + 63) / 64;
     const uint32_t per = (steps + gridDim.x - 1) / gridDim.x, step0 = min(blockIdx.x * per, steps), step1 = min(step0 + per, steps);
     const uint32_t width = sh.part_count * sh.max_rank;
-    Tile t = tile_of(a, sh, row0, blockIdx.x == 0);
-    while (t.pending) {
+    const uint32_t turn = blockIdx.z % SLOT_GROUPS, rank_group = blockIdx.z / SLOT_GROUPS;
+    Tile t = tile_of(a, sh, row0, blockIdx.x == 0 && blockIdx.z == 0);
+    for (uint32_t at = 0; t.pending; at++) {
         int32_t slot;
         const uint32_t rows = next_slot(t, slot);
+        if (at % SLOT_GROUPS != turn) continue;
         const AdapterEntry* entry = table + (size_t)slot * sh.part_count;
-        uint32_t part = 0, j = 0;  // the next rank tile
-        while (true) {
-            RankTile tile[4];
-            uint32_t tiles = 0;
+        RankTile tile[4];
+        uint32_t tiles = 0, skip = 4 * rank_group;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                while (part < sh.part_count && j >= entry[part].rank) part++, j = 0;
-                if (part == sh.part_count) break;
-                const AdapterEntry e = entry[part];
+        for (uint32_t part = 0; part < IRIS_ADAPTER_PARTS; part++) {
+            if (part >= sh.part_count) break;
+            const AdapterEntry e = entry[part];
+            const uint32_t of_part = (e.rank + 15) / 16;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+                // The part's tile that is this workgroup's i-th, if it is.
+                const uint32_t at = skip + i - tiles;
+                if (i < tiles || at >= of_part) continue;
+                const uint32_t j = 16 * at;
                 tile[i].a = e.a + (size_t)min(j + (t.lane & 15), e.rank - 1) * sh.cols;
                 tile[i].at = part * sh.max_rank + j;
                 tile[i].ranks = min(e.rank - j, 16u);
-                j += 16;
-                tiles++;
             }
-            if (!tiles) break;
-            __syncthreads();  // the sums before are read
-            for (uint32_t i = tid; i < TILE_ROWS * (TILE_RANKS + 1); i += 256) s_sum[i] = 0;
-            if (tid == 0) s_wide = 0;
+            const uint32_t taken = min(of_part - min(skip, of_part), 4 - tiles);
+            skip = skip > of_part ? skip - of_part : 0;
+            tiles += taken;
+        }
+        if (!tiles) continue;
+        __syncthreads();  // the sums before are read
+        for (uint32_t i = tid; i < TILE_ROWS * (TILE_RANKS + 1); i += 256) s_sum[i] = 0;
+        if (tid == 0) s_wide = 0;
+        __syncthreads();
+        if (shrink_steps<false>(a, sh.cols, tile, tiles, row0, step0, step1, t, s_sum) && t.lane == 0) s_wide = 1;
+        __syncthreads();
+        if (s_wide) {
+            shrink_steps<true>(a, sh.cols, tile, tiles, row0, step0, step1, t, s_sum);
             __syncthreads();
-            if (shrink_steps<false>(a, sh.cols, tile, tiles, row0, step0, step1, t, s_sum) && t.lane == 0) s_wide = 1;
-            __syncthreads();
-            if (s_wide) {
-                shrink_steps<true>(a, sh.cols, tile, tiles, row0, step0, step1, t, s_sum);
-                __syncthreads();
-            }
-            // A row of 64 values a wave and turn.
-            for (uint32_t r = t.wave; r < TILE_ROWS; r += 4) {
-                if (!(rows >> r & 1)) continue;
+        }
+        // A row of 64 values a wave and turn.
+        for (uint32_t r = t.wave; r < TILE_ROWS; r += 4) {
+            if (!(rows >> r & 1)) continue;
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (i < (int)tiles && t.lane / 16 == i && t.lane % 16 < tile[i].ranks)
-                        sums[((size_t)blockIdx.x * a.rows + row0 + r) * width + tile[i].at + t.lane % 16] =
-                            s_sum[r * (TILE_RANKS + 1) + t.lane];
-            }
+            for (int i = 0; i < 4; i++)
+                if (i < (int)tiles && t.lane / 16 == i && t.lane % 16 < tile[i].ranks)
+                    sums[((size_t)blockIdx.x * a.rows + row0 + r) * width + tile[i].at + t.lane % 16] =
+                        s_sum[r * (TILE_RANKS + 1) + t.lane];
         }
     }
 }
@@ -293,8 +305,11 @@ __global__ __launch_bounds__(256, 2) void shrink_tile_kernel(const IrisAdapterRo
 // Four neighbouring outputs' columns of a row.
 template <bool VEC>
 __device__ __forceinline__ int4 load_columns(const int32_t* p, uint32_t step, uint32_t count) {
-    if (VEC && count == 4) return load4(p);
     int4 v{};
+    if constexpr (VEC) {  // (fours are whole)
+        if (count) v = load4(p);
+        return v;
+    }
     if (count > 0) v.x = load1(p);
     if (count > 1) v.y = load1(p + step);
     if (count > 2) v.z = load1(p + 2 * step);
@@ -304,8 +319,8 @@ __device__ __forceinline__ int4 load_columns(const int32_t* p, uint32_t step, ui
 
 template <bool VEC>
 __device__ __forceinline__ void store_columns(int32_t* p, uint32_t step, uint32_t count, int4 v) {
-    if (VEC && count == 4) {
-        *(int4*)p = v;
+    if constexpr (VEC) {
+        if (count) *(int4*)p = v;
         return;
     }
     if (count > 0) p[0] = v.x;
@@ -320,119 +335,160 @@ __device__ __forceinline__ int32_t added(int32_t y, double sum, double unit) {
     return (int32_t)fmin(fmax((double)y + u, -2147483648.0), 2147483647.0);
 }
 
-// Workgroup: outputs from blockIdx.x CHUNK_OUTPUTS of part blockIdx.z, row tile
-// blockIdx.y. LDS: t of the tile's rows, [32][whole 64-rank steps and 4 more].
+// The digits of t of a tile's rows as operands of the matrix cores, in LDS:
+// [64-rank step][16 rows][digit][lane].
+struct Operand {
+    v4i lane[64];
+};
+constexpr uint32_t DIGIT_PLANES = 5;
+__device__ __forceinline__ uint32_t operand_at(uint32_t step, uint32_t g, uint32_t digit) { return (step * 2 + g) * DIGIT_PLANES + digit; }
+
+// Sixteen weights of a row of B from k on. The rank's padding may end at 8 of
+// them: those behind it are another row's.
+__device__ __forceinline__ void load_weights(const int16_t* w, uint32_t k, uint32_t stride, int4& b0, int4& b1) {
+    b0 = k < stride ? load4((const int32_t*)(w + k)) : int4{};
+    b1 = k + 8 < stride ? load4((const int32_t*)(w + k) + 4) : int4{};
+}
+
+// Tiles of 16 outputs for the rows of one adapter, into out. WIDE: values past
+// three digits. One step's operands stay in registers where they are all (ONE).
+template <bool VEC, bool WIDE, bool ONE>
+__device__ __forceinline__ void expand_outputs(const IrisAdapterRows& a, const IrisAdapterPart& p, const AdapterEntry& e,
+                                               const Operand* s_digits, const Tile& t, uint32_t row0, uint32_t rows, uint32_t i0,
+                                               uint32_t i1) {
+    constexpr int SUMS = WIDE ? 6 : 4;
+    const uint32_t n = t.lane & 15, group = t.lane >> 4, steps = ONE ? 1 : (e.rank + 63) / 64, b_stride = stride_of(e.rank);
+    const double unit = ldexp(1.0, -(int)e.b_bits);
+    constexpr int DIGITS = WIDE ? 5 : 3;
+    v4i kept[2][DIGITS];
+    if (ONE) {
+#pragma unroll
+        for (int g = 0; g < 2; g++)
+#pragma unroll
+            for (int d = 0; d < DIGITS; d++) kept[g][d] = s_digits[operand_at(0, g, d)].lane[t.lane];
+    }
+    // The next tile's y and first weights are under way while one is computed.
+    int4 y[2], b0{}, b1{};
+    auto load = [&](uint32_t i) {
+        const int16_t* w = e.b + (size_t)min(i + n, p.rows - 1) * b_stride;
+        const uint32_t first = i + 4 * group, count = first < i1 ? min(i1 - first, 4u) : 0;
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+            const uint32_t r = 16 * g + n;
+            y[g] = load_columns<VEC>(a.y + (size_t)(row0 + r) * a.y_stride + p.first + (size_t)first * p.step, p.step,
+                                     rows >> r & 1 ? count : 0);
+        }
+        load_weights(w, 16 * group, b_stride, b0, b1);
+    };
+    if (i0 + 16 * t.wave < i1) load(i0 + 16 * t.wave);
+#pragma unroll 1
+    for (uint32_t i = i0 + 16 * t.wave; i < i1; i += 64) {
+        const uint32_t first = i + 4 * group, count = first < i1 ? min(i1 - first, 4u) : 0;
+        const int4 was[2] = {y[0], y[1]};
+        v4i acc[2][SUMS] = {};
+        v4i low, high;
+        split_weights(b0, b1, low, high);
+        if (i + 64 < i1) load(i + 64);
+#pragma unroll 1
+        for (uint32_t step = 0;;) {
+#pragma unroll
+            for (int g = 0; g < 2; g++)
+#pragma unroll
+                for (int d = 0; d < DIGITS; d++) {
+                    const v4i digit = ONE ? kept[g][d] : s_digits[operand_at(step, g, d)].lane[t.lane];
+                    acc[g][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(low, digit, acc[g][d], 0, 0, 0);
+                    acc[g][d + 1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(high, digit, acc[g][d + 1], 0, 0, 0);
+                }
+            if (ONE || ++step == steps) break;
+            int4 c0{}, c1{};
+            load_weights(e.b + (size_t)min(i + n, p.rows - 1) * b_stride, 64 * step + 16 * group, b_stride, c0, c1);
+            split_weights(c0, c1, low, high);
+        }
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+            const uint32_t r = 16 * g + n;
+            const int32_t old[4] = {was[g].x, was[g].y, was[g].z, was[g].w};
+            int32_t out[4];
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                if constexpr (!WIDE) {
+                    // Below 2^23 2^15 256 = 2^46: exact.
+                    double sum = (double)acc[g][3][c];
+#pragma unroll
+                    for (int d = 2; d >= 0; d--) sum = fma(sum, 256.0, (double)acc[g][d][c]);
+                    out[c] = added(old[c], sum, unit);
+                } else {
+                    int64_t sum = 0;
+#pragma unroll
+                    for (int d = SUMS - 1; d >= 0; d--) sum = (sum << 8) + acc[g][d][c];
+                    out[c] = dn::add_sat(old[c], rounded(sum, e.b_bits));
+                }
+            }
+            if (rows >> r & 1)
+                store_columns<VEC>(a.out + (size_t)(row0 + r) * a.out_stride + p.first + (size_t)first * p.step, p.step, count,
+                                   make_int4(out[0], out[1], out[2], out[3]));
+        }
+    }
+}
+
+// Workgroup: outputs from blockIdx.x CHUNK_OUTPUTS on, row tile blockIdx.y, and of
+// blockIdx.z the part and which of the tile's adapters. LDS: operands of the
+// steps of max_rank.
 template <bool VEC>
 __global__ __launch_bounds__(256) void expand_tile_kernel(const IrisAdapterRows a, const AdapterShape sh, const AdapterEntry* table,
                                                           const int64_t* sums, uint32_t splits) {
-    extern __shared__ int32_t s_t[];
+    extern __shared__ Operand s_digits[];
     __shared__ uint32_t s_wide;
-    const uint32_t row0 = blockIdx.y * TILE_ROWS, tid = threadIdx.x, part = blockIdx.z;
+    const uint32_t row0 = blockIdx.y * TILE_ROWS, tid = threadIdx.x, part = blockIdx.z / SLOT_GROUPS, turn = blockIdx.z % SLOT_GROUPS;
     const IrisAdapterPart p = sh.parts[part];
     const uint32_t i0 = blockIdx.x * CHUNK_OUTPUTS, i1 = min(i0 + CHUNK_OUTPUTS, p.rows);
     if (i0 >= p.rows) return;
-    const uint32_t padded = (sh.max_rank + 63) & ~63u, stride = padded + 4, width = sh.part_count * sh.max_rank;
+    const uint32_t width = sh.part_count * sh.max_rank;
     Tile t = tile_of(a, sh, row0, false);
-    const uint32_t n = t.lane & 15, group = t.lane >> 4;
     uint32_t copied = ~t.pending;  // rows that no adapter changes
-    while (t.pending) {
+    const bool copies = turn == 0 && a.out != a.y;
+    for (uint32_t at = 0; t.pending; at++) {
         int32_t slot;
         const uint32_t rows = next_slot(t, slot);
+        if (at % SLOT_GROUPS != turn && !copies) continue;
         const AdapterEntry e = table[(size_t)slot * sh.part_count + part];
-        if (!e.rank) {
-            copied |= rows;
-            continue;
-        }
-        const uint32_t blocks = (e.rank + 63) / 64, b_stride = stride_of(e.rank);
-        __syncthreads();  // the adapter before is done with s_t
+        if (!e.rank) copied |= rows;
+        if (!e.rank || at % SLOT_GROUPS != turn) continue;
+        const uint32_t steps = (e.rank + 63) / 64;
+        __syncthreads();  // the adapter before is done with the operands
         if (tid == 0) s_wide = 0;
         __syncthreads();
-        uint32_t far = 0;
-        for (uint32_t i = tid; i < TILE_ROWS * blocks * 64; i += 256) {
-            const uint32_t r = i / (blocks * 64), j = i % (blocks * 64);
-            int32_t v = 0;
-            if (j < e.rank && (rows >> r & 1)) {
+        uint32_t seen = 0;
+        // Four values of a row a thread and turn (zeros past the rank and for
+        // others' rows).
+        for (uint32_t i = tid; i < TILE_ROWS * steps * 16; i += 256) {
+            const uint32_t r = i / (steps * 16), j = i % (steps * 16) * 4;
+            int32_t v[4] = {};
+            if (rows >> r & 1) {
                 const int64_t* from = sums + (size_t)(row0 + r) * width + part * sh.max_rank + j;
-                int64_t sum = 0;
-                for (uint32_t q = 0; q < splits; q++) sum += from[(size_t)q * a.rows * width];
-                v = rounded(sum, e.a_bits);
+                int64_t sum[4] = {};
+                for (uint32_t q = 0; q < splits; q++)
+#pragma unroll
+                    for (uint32_t c = 0; c < 4; c++)
+                        if (j + c < e.rank) sum[c] += from[(size_t)q * a.rows * width + c];
+#pragma unroll
+                for (int c = 0; c < 4; c++) v[c] = rounded(sum[c], e.a_bits);
             }
-            s_t[r * stride + j] = v;
-            far |= (uint32_t)(v > 8355711 || v < -8421504);
+            const int4 x = make_int4(v[0], v[1], v[2], v[3]);
+            uint32_t plane[4];
+            split4(x, plane, seen);
+            const uint32_t lane = (j % 64 / 16) * 16 + r % 16, c = j % 16 / 4;
+#pragma unroll
+            for (uint32_t d = 0; d < DIGIT_PLANES; d++)
+                ((uint32_t*)&s_digits[operand_at(j / 64, r / 16, d)].lane[lane])[c] = d < 4 ? plane[d] : fifth4(x);
         }
-        if (far) s_wide = 1;
+        if (seen >> 24) s_wide = 1;
         __syncthreads();
-        const bool wide = s_wide != 0;
-        const double unit = ldexp(1.0, -(int)e.b_bits);
-        for (uint32_t i = i0 + 16 * t.wave; i < i1; i += 64) {
-            const int16_t* w = e.b + (size_t)min(i + n, p.rows - 1) * b_stride;
-            const uint32_t first = i + 4 * group, count = first < i1 ? min(i1 - first, 4u) : 0;
-            int4 y[2];
-#pragma unroll
-            for (int g = 0; g < 2; g++) {
-                const uint32_t r = 16 * g + n;
-                y[g] = load_columns<VEC>(a.y + (size_t)(row0 + r) * a.y_stride + p.first + (size_t)first * p.step, p.step,
-                                         rows >> r & 1 ? count : 0);
-            }
-            v4i acc[2][4] = {}, top[2][4] = {};
-            for (uint32_t block = 0; block < blocks; block++) {
-                const uint32_t k = 64 * block + 16 * group;
-                // The rank's padding ends at 8 of 16: those behind it are another row's.
-                v4i low, high;
-                {
-                    int4 b0{}, b1{};
-                    if (k < b_stride) b0 = load4((const int32_t*)(w + k));
-                    if (k + 8 < b_stride) b1 = load4((const int32_t*)(w + k) + 4);
-                    const uint32_t d[8] = {(uint32_t)b0.x, (uint32_t)b0.y, (uint32_t)b0.z, (uint32_t)b0.w,
-                                           (uint32_t)b1.x, (uint32_t)b1.y, (uint32_t)b1.z, (uint32_t)b1.w};
-#pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        low[c] = (int)__builtin_amdgcn_perm(d[2 * c + 1], d[2 * c], 0x06040200u);
-                        high[c] = (int)__builtin_amdgcn_perm(d[2 * c + 1], d[2 * c], 0x07050301u);
-                    }
-                }
-#pragma unroll
-                for (int g = 0; g < 2; g++) {
-                    int4 v[4];
-#pragma unroll
-                    for (int c = 0; c < 4; c++) v[c] = *(const int4*)&s_t[(16 * g + n) * stride + k + 4 * c];
-                    v4i digit[3];
-                    uint32_t seen = 0;
-                    value_digits<false>(v, digit, seen);
-                    digit_products<3>(low, high, digit, acc[g]);
-                    if (wide) {
-                        value_digits<true>(v, digit, seen);
-                        digit_products<2>(low, high, digit, top[g]);
-                    }
-                }
-            }
-#pragma unroll
-            for (int g = 0; g < 2; g++) {
-                const uint32_t r = 16 * g + n;
-                const int32_t old[4] = {y[g].x, y[g].y, y[g].z, y[g].w};
-                int32_t out[4];
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    if (!wide) {
-                        // Below 2^23 2^15 256 = 2^46: exact.
-                        double sum = (double)acc[g][3][c];
-#pragma unroll
-                        for (int d = 2; d >= 0; d--) sum = fma(sum, 256.0, (double)acc[g][d][c]);
-                        out[c] = added(old[c], sum, unit);
-                    } else {
-                        int64_t sum = 0, high = 0;
-#pragma unroll
-                        for (int d = 3; d >= 0; d--) sum = (sum << 8) + acc[g][d][c], high = (high << 8) + top[g][d][c];
-                        out[c] = dn::add_sat(old[c], rounded(sum + (high << 24), e.b_bits));
-                    }
-                }
-                if (rows >> r & 1)
-                    store_columns<VEC>(a.out + (size_t)(row0 + r) * a.out_stride + p.first + (size_t)first * p.step, p.step, count,
-                                       make_int4(out[0], out[1], out[2], out[3]));
-            }
-        }
+        if (s_wide) expand_outputs<VEC, true, false>(a, p, e, s_digits, t, row0, rows, i0, i1);
+        else if (steps == 1) expand_outputs<VEC, false, true>(a, p, e, s_digits, t, row0, rows, i0, i1);
+        else expand_outputs<VEC, false, false>(a, p, e, s_digits, t, row0, rows, i0, i1);
     }
-    if (a.out == a.y) return;
+    if (!copies) return;
     for (uint32_t r = t.wave; r < TILE_ROWS && row0 + r < a.rows; r += 4) {
         if (!(copied >> r & 1)) continue;
         for (uint32_t i = i0 + 4 * t.lane; i < i1; i += 256) {
@@ -444,13 +500,16 @@ __global__ __launch_bounds__(256) void expand_tile_kernel(const IrisAdapterRows 
     }
 }
 
+// Workgroups that share the rank tiles of an adapter.
+uint32_t rank_groups(const AdapterShape& s) { return (s.part_count * ((s.max_rank + 15) / 16) + 3) / 4; }
+
 // Pieces of the columns for a call of tiles: enough workgroups for the card,
 // each with a step for every wave.
 uint32_t splits_of(const AdapterShape& s, uint32_t rows) {
     const uint32_t tiles = (rows + TILE_ROWS - 1) / TILE_ROWS, steps = (s.cols + 63) / 64;
     // A piece's accumulators hold 2^14 2 64 a step: 32768 columns at most.
     const uint32_t least = (s.cols + 32767) / 32768;
-    return std::max(least, std::min(std::min(256 / tiles, (steps + 3) / 4), MAX_SPLITS));
+    return std::max(least, std::min(std::min(512 / (tiles * rank_groups(s)), (steps + 3) / 4), MAX_SPLITS));
 }
 
 // Bytes of work space of a call: t itself for few rows, its sums by pieces for
@@ -592,12 +651,13 @@ int iris_adapters_apply(const IrisAdapterBank* b, const IrisAdapterRows* a, void
     hipStream_t st = (hipStream_t)stream;
     if (a->rows > FEW_ROWS) {
         const uint32_t tiles = (a->rows + TILE_ROWS - 1) / TILE_ROWS, splits = splits_of(s, a->rows);
-        const size_t lds = TILE_ROWS * (((s.max_rank + 63) & ~63u) + 4) * 4;
+        const size_t lds = (s.max_rank + 63) / 64 * 2 * DIGIT_PLANES * sizeof(Operand);
         // Sixteen bytes of a row at a time where every part allows it.
         bool vec = !misaligned(a->y) && !misaligned(a->out) && a->y_stride % 4 == 0 && a->out_stride % 4 == 0;
-        for (uint32_t p = 0; p < s.part_count; p++) vec = vec && s.parts[p].step == 1 && s.parts[p].first % 4 == 0;
-        const dim3 grid((b->most_rows + CHUNK_OUTPUTS - 1) / CHUNK_OUTPUTS, tiles, s.part_count);
-        hipLaunchKernelGGL(shrink_tile_kernel, dim3(splits, tiles), dim3(256), 0, st, *a, s, b->table, (int64_t*)space);
+        for (uint32_t p = 0; p < s.part_count; p++) vec = vec && s.parts[p].step == 1 && s.parts[p].first % 4 == 0 && s.parts[p].rows % 4 == 0;
+        const dim3 grid((b->most_rows + CHUNK_OUTPUTS - 1) / CHUNK_OUTPUTS, tiles, s.part_count * SLOT_GROUPS);
+        hipLaunchKernelGGL(shrink_tile_kernel, dim3(splits, tiles, rank_groups(s) * SLOT_GROUPS), dim3(256), 0, st, *a, s, b->table,
+                           (int64_t*)space);
         if (vec) hipLaunchKernelGGL(expand_tile_kernel<true>, grid, dim3(256), lds, st, *a, s, b->table, (const int64_t*)space, splits);
         else hipLaunchKernelGGL(expand_tile_kernel<false>, grid, dim3(256), lds, st, *a, s, b->table, (const int64_t*)space, splits);
         return (int)hipGetLastError();

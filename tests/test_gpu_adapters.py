@@ -111,6 +111,15 @@ def test_rows_of_many_adapters(rows, parts):
     Call(rng, 128, parts, ranks, rows, rng.integers(-1, 5, rows)).check()
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+def test_a_tile_of_many_adapters(in_place):
+    # Every row its own adapter, a few without, some parts empty.
+    rng = np.random.default_rng(21)
+    ranks = [[int(rng.integers(0, 20)) for _ in QKV] for _ in range(90)]
+    Call(rng, 160, QKV, ranks, 100, np.arange(100) % 91 - 1, in_place=in_place).check()
+    Call(rng, 160, QKV, ranks, 100, rng.integers(-1, 7, 100), in_place=in_place, kind="mixed").check()
+
+
 @pytest.mark.parametrize("rank", [1, 2, 7, 8, 9, 15, 16, 17, 31, 32, 33, 63, 64, 65, 100, 128, 129, 255, 256])
 @pytest.mark.parametrize("rows", [1, 40, 75])
 def test_ranks(rank, rows):
