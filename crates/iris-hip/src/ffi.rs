@@ -167,6 +167,12 @@ pub struct IrisAdapterBank {
     _private: [u8; 0],
 }
 
+/// The low-rank adapters of a model's layers.
+#[repr(C)]
+pub struct IrisModelAdapters {
+    _private: [u8; 0],
+}
+
 /// Rows with an adapter each (`IrisAdapterRows`).
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
@@ -541,5 +547,48 @@ extern "C" {
     ) -> c_int;
     pub fn iris_batch_release(batch: *mut IrisBatch, request: u32) -> c_int;
     pub fn iris_batch_length(batch: *const IrisBatch, request: u32, out: *mut u32) -> c_int;
+    pub fn iris_model_adapters_create(
+        model: *mut IrisModel,
+        slots: u32,
+        max_rank: u32,
+        out: *mut *mut IrisModelAdapters,
+    ) -> c_int;
+    pub fn iris_model_adapters_free(set: *mut IrisModelAdapters);
+    pub fn iris_model_adapters_device_bytes(set: *const IrisModelAdapters) -> u64;
+    pub fn iris_model_adapters_load(
+        set: *mut IrisModelAdapters,
+        slot: u32,
+        name: *const c_char,
+        a: *const int16_t,
+        a_bits: u32,
+        b: *const int16_t,
+        b_bits: u32,
+        rank: u32,
+    ) -> c_int;
+    pub fn iris_model_adapters_clear(set: *mut IrisModelAdapters, slot: u32) -> c_int;
+    pub fn iris_batch_adapters(batch: *mut IrisBatch, set: *const IrisModelAdapters) -> c_int;
+    pub fn iris_batch_adapter(batch: *mut IrisBatch, request: u32, slot: i32) -> c_int;
+    pub fn iris_batch_rule(
+        batch: *mut IrisBatch,
+        request: u32,
+        rule: *const IrisTokenRule,
+        bias_ids: *const i32,
+        bias_values: *const i32,
+    ) -> c_int;
+    pub fn iris_batch_drawing(
+        batch: *mut IrisBatch,
+        request: u32,
+        drawing: *const IrisDrawing,
+        numbers: *const u32,
+        first: u32,
+        count: u32,
+    ) -> c_int;
+    pub fn iris_batch_masks(
+        batch: *mut IrisBatch,
+        masks: *const u32,
+        mask_rows: u32,
+        mask_of: *const i32,
+        rows: u32,
+    ) -> c_int;
     pub fn iris_sha256_bytes(data: *const u8, len: u64, out: *mut u8) -> c_int;
 }

@@ -748,10 +748,60 @@ int iris_batch_prefill(IrisBatch* batch, const int32_t* ids, const uint32_t* cou
 int iris_batch_step(IrisBatch* batch, const int32_t* ids, const int32_t* parents, const uint32_t* counts,
                     int32_t* out_tokens, uint32_t* out_kept);
 
-/* Empties a request: its length is 0 and its pages are free for the next call. */
+/* Empties a request: its length is 0, its pages are free for the next call, and
+ * it has no adapter, rule or drawing. */
 int iris_batch_release(IrisBatch* batch, uint32_t request);
 /* Positions a request holds. */
 int iris_batch_length(const IrisBatch* batch, uint32_t request, uint32_t* out);
+
+/* The low-rank adapters of a model's layers: up to `slots` of them, each of rank
+ * up to max_rank, with device memory (a bank for all slots) for the products
+ * that any of them touches. Freed before the model, and after the batches that
+ * use it are done with it. */
+typedef struct IrisModelAdapters IrisModelAdapters;
+int iris_model_adapters_create(IrisModel* model, uint32_t slots, uint32_t max_rank, IrisModelAdapters** out);
+void iris_model_adapters_free(IrisModelAdapters* set);
+uint64_t iris_model_adapters_device_bytes(const IrisModelAdapters* set);
+/* One matrix's pair A [rank][cols], B [rows][rank] under the matrix's DETWGT
+ * name (a layer's self_attn.{q,k,v,o}_proj.weight or
+ * mlp.{gate,up,down}_proj.weight), as iris_adapters_load takes it. */
+int iris_model_adapters_load(IrisModelAdapters* set, uint32_t slot, const char* name, const int16_t* a, uint32_t a_bits,
+                             const int16_t* b, uint32_t b_bits, uint32_t rank);
+/* Empties a slot. */
+int iris_model_adapters_clear(IrisModelAdapters* set, uint32_t slot);
+
+/* A batch's requests with adapters, rules and draws of their own. Each setting
+ * holds from the next pass on until it is set again or the request is released;
+ * requests without any run as ever. The calls are synchronous; a refused one
+ * changes nothing.
+ *
+ * iris_batch_adapters: the set that the requests' slots name (null: none, and
+ * no request has an adapter then). iris_batch_adapter: a request's slot, -1 for
+ * none (IRIS_E_STATE without a set). A row's product is the layer's, plus its
+ * residual where the layer adds it in the same step, plus the adapter's
+ * (IrisAdapterRows); gate and up have theirs before the activation. Keys and
+ * values that a request holds stay those of the adapter they were made with. */
+int iris_batch_adapters(IrisBatch* batch, const IrisModelAdapters* set);
+int iris_batch_adapter(IrisBatch* batch, uint32_t request, int32_t slot);
+
+/* A request's rule on its logits (IrisLogitsRules), its text being all the
+ * positions it holds: bias_count entries of bias_ids and bias_values (host
+ * memory; bias_start is not read). Null: none. IRIS_E_RANGE past 2^20 entries
+ * of all requests. */
+int iris_batch_rule(IrisBatch* batch, uint32_t request, const IrisTokenRule* rule, const int32_t* bias_ids,
+                    const int32_t* bias_values);
+/* How a request draws (IrisLogitsDraw), and the numbers of the rows at positions
+ * first .. first + count (host memory): a row's selection takes the number of
+ * its position, so drafts change nothing. A pass with a row past them is refused
+ * (IRIS_E_RANGE). Null: the first maximum. */
+int iris_batch_drawing(IrisBatch* batch, uint32_t request, const IrisDrawing* drawing, const uint32_t* numbers, uint32_t first,
+                       uint32_t count);
+/* Masks (host memory, [mask_rows][(vocab + 31) / 32]) for the next pass that
+ * succeeds: mask_of has an entry (-1: none) for each of its `rows` ids, of
+ * which a prompt's last counts. A pass of another number of rows is refused
+ * (IRIS_E_INVALID). Null or no rows: none. A selection of which nothing is open
+ * is -1, and a path ends there. */
+int iris_batch_masks(IrisBatch* batch, const uint32_t* masks, uint32_t mask_rows, const int32_t* mask_of, uint32_t rows);
 
 /* SHA-256 (FIPS 180-4) of `len` bytes into out[32]; the hash
  * iris_session_layer_pass uses. Host code only. */

@@ -15,7 +15,7 @@
 #include <vector>
 
 #include "attn_tiles.h"
-#include "q8_internal.h"
+#include "runtime_internal.h"
 
 namespace {
 
@@ -530,6 +530,16 @@ struct IrisAdapterBank {
     uint32_t most_rows = 0, width = 0;
 };
 
+uint64_t iris_adapters_space(uint32_t cols, uint32_t part_count, uint32_t max_rank, uint32_t rows) {
+    if (!rows || rows > 65535) return 0;
+    AdapterShape s{};
+    s.cols = cols, s.part_count = part_count, s.max_rank = max_rank;
+    // What any number of rows up to these takes: whole tiles take the most.
+    uint64_t bytes = space_of(s, rows);
+    for (uint32_t n = rows / TILE_ROWS * TILE_ROWS; n; n -= TILE_ROWS) bytes = std::max(bytes, space_of(s, n));
+    return std::max(bytes, space_of(s, std::min(rows, FEW_ROWS)));
+}
+
 extern "C" {
 
 int iris_adapters_create(uint32_t cols, const IrisAdapterPart* parts, uint32_t part_count, uint32_t slots, uint32_t max_rank,
@@ -631,11 +641,7 @@ int iris_adapters_load(IrisAdapterBank* b, uint32_t slot, uint32_t part, const i
 }
 
 uint64_t iris_adapters_workspace_bytes(const IrisAdapterBank* b, uint32_t rows) {
-    if (!b || !rows || rows > 65535) return 0;
-    // What any number of rows up to these takes: whole tiles take the most.
-    uint64_t bytes = space_of(b->shape, rows);
-    for (uint32_t n = rows / TILE_ROWS * TILE_ROWS; n; n -= TILE_ROWS) bytes = std::max(bytes, space_of(b->shape, n));
-    return std::max(bytes, space_of(b->shape, std::min(rows, FEW_ROWS)));
+    return b ? iris_adapters_space(b->shape.cols, b->shape.part_count, b->shape.max_rank, rows) : 0;
 }
 
 int iris_adapters_apply(const IrisAdapterBank* b, const IrisAdapterRows* a, void* space, uint64_t space_bytes, void* stream) {

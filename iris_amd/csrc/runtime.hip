@@ -36,16 +36,6 @@ constexpr const char* PREFIX = "model.language_model.";
 
 bool starts_with(const std::string& s, const std::string& p) { return s.compare(0, p.size(), p) == 0; }
 
-int layer_of(const std::string& name, std::string* suffix) {
-    const std::string lp = std::string(PREFIX) + "layers.";
-    if (!starts_with(name, lp)) return -1;
-    size_t dot = name.find('.', lp.size());
-    if (dot == std::string::npos) return -1;
-    int layer = std::atoi(name.substr(lp.size(), dot - lp.size()).c_str());
-    *suffix = name.substr(dot + 1);
-    return layer;
-}
-
 #define RT_CHECK(expr)                  \
     do {                                \
         int rc_ = (int)(expr);          \
@@ -84,6 +74,16 @@ static inline void with_gemm_space(GemvArgs& g, const IrisSession* s, uint32_t r
         g.planes = s->planes;
         g.token_limbs = s->token_limbs;
     }
+}
+
+int iris_layer_of(const std::string& name, std::string* suffix) {
+    const std::string lp = std::string(PREFIX) + "layers.";
+    if (!starts_with(name, lp)) return -1;
+    size_t dot = name.find('.', lp.size());
+    if (dot == std::string::npos) return -1;
+    int layer = std::atoi(name.substr(lp.size(), dot - lp.size()).c_str());
+    *suffix = name.substr(dot + 1);
+    return layer;
 }
 
 // ---------------------------------------------------------------- model
@@ -194,7 +194,7 @@ int iris_model_set_tensor(IrisModel* m, const char* cname, int32_t width, const 
         return IRIS_E_INVALID;
     }
     std::string suffix;
-    const int layer = layer_of(name, &suffix);
+    const int layer = iris_layer_of(name, &suffix);
     const IrisModelDesc& d = m->d;
     if (layer >= 0) {
         if ((uint32_t)layer >= d.layers) return IRIS_E_INVALID;
@@ -494,6 +494,10 @@ static int mistral_layer(IrisSession* s, uint32_t l, uint32_t rows, bool slots, 
         }
         with_gemm_space(g, s, rows);
         RT_CHECK(iris_gemv_launch(g, st));
+        if (iris_batch_adapts(s, l, ADAPT_QKV)) {
+            RT_CHECK(iris_batch_norm(s, s->x, L.norm_attn, rows));
+            RT_CHECK(iris_batch_adapt(s, l, ADAPT_QKV, iris_batch_normed(s), H, s->qkv, qw + 2 * kvw, rows));
+        }
         // 2. attention.
         bool ctx_planes = false;
         if (s->batch) {
@@ -541,6 +545,7 @@ static int mistral_layer(IrisSession* s, uint32_t l, uint32_t rows, bool slots, 
         if (ctx_planes) bcast_input(g, s, s->ctx_planes, s->ctx_counts);
         with_gemm_space(g, s, rows);
         RT_CHECK(iris_gemv_launch(g, st));
+        if (iris_batch_adapts(s, l, ADAPT_O)) RT_CHECK(iris_batch_adapt(s, l, ADAPT_O, s->ctx, qw, s->attended, H, rows));
         // 4. gated = mul(silu(W_gate m), W_up m), m = rms_norm(attended).
         g = GemvArgs{};
         g.w = q8_view(L.wgu);
@@ -558,8 +563,15 @@ static int mistral_layer(IrisSession* s, uint32_t l, uint32_t rows, bool slots, 
             g.ssq_in = s->ssq_att;
             g.ssq_n = h_tiles;
         }
+        // Adapters of gate and up come before the gate's activation.
+        const bool adapted = iris_batch_adapts(s, l, ADAPT_GATE_UP);
+        if (adapted) {
+            g.epilogue = EPI_STORE;
+            g.out = iris_batch_gate_up(s);
+            g.out_stride = 2 * d.ffn;
+        }
         // One row: the gated row's digit planes too, for the down product.
-        const bool gated_planes = rows == 1;
+        const bool gated_planes = rows == 1 && !adapted;
         if (gated_planes) {
             g.out_planes = s->gated_planes;
             g.out_counts = s->gated_counts;
@@ -581,8 +593,9 @@ static int mistral_layer(IrisSession* s, uint32_t l, uint32_t rows, bool slots, 
         with_gemm_space(dn, s, rows);
         // Several rows, both products on the matrix cores: the gate/up
         // product writes the gated rows' digit planes for the down product.
-        if (rows > 1 && s->gated_gemm_planes && iris_gemm_applies(g) && iris_gemm_applies(dn)) {
-            g.out = nullptr;  // nothing reads the gated rows themselves
+        const bool down_adapted = iris_batch_adapts(s, l, ADAPT_DOWN);
+        if (rows > 1 && !adapted && s->gated_gemm_planes && iris_gemm_applies(g) && iris_gemm_applies(dn)) {
+            if (!down_adapted) g.out = nullptr;  // nothing reads the gated rows themselves
             g.out_gemm_planes = s->gated_gemm_planes;
             g.out_gemm_limbs = s->gated_gemm_limbs;
             dn.planes = s->gated_gemm_planes;
@@ -590,7 +603,13 @@ static int mistral_layer(IrisSession* s, uint32_t l, uint32_t rows, bool slots, 
             dn.planes_ready = 1;
         }
         RT_CHECK(iris_gemv_launch(g, st));
+        if (adapted) {
+            RT_CHECK(iris_batch_norm(s, s->attended, L.norm_ff, rows));
+            RT_CHECK(iris_batch_adapt(s, l, ADAPT_GATE_UP, iris_batch_normed(s), H, iris_batch_gate_up(s), 2 * d.ffn, rows));
+            RT_CHECK(iris_batch_gate(s, d.ffn, false, rows));
+        }
         RT_CHECK(iris_gemv_launch(dn, st));
+        if (down_adapted) RT_CHECK(iris_batch_adapt(s, l, ADAPT_DOWN, s->gated, d.ffn, s->x, H, rows));
     }
     return 0;
 }
@@ -607,7 +626,8 @@ static int mistral_pass(IrisSession* s, uint32_t rows, const CkptSink* sink) {
     // One row: sums of squares pass from each residual product to the norm
     // after it (hidden rows in 16-row tiles, within the slot count).
     const uint32_t h_tiles = (d.hidden + Q8_TILE_ROWS - 1) / Q8_TILE_ROWS;
-    const bool slots = rows == 1 && h_tiles <= GEMV_SSQ_SLOTS;
+    // (Adapters change those products' rows afterwards.)
+    const bool slots = rows == 1 && h_tiles <= GEMV_SSQ_SLOTS && !iris_batch_adapted(s);
     s->ssq_x_valid = false;
     for (uint32_t l = 0; l < d.layers; l++) {
         RT_CHECK(mistral_layer(s, l, rows, slots, l > 0));
@@ -724,6 +744,10 @@ static int gemma_layer(IrisSession* s, uint32_t l, uint32_t rows, bool carry) {
         g.out_stride = qkvw;
         with_gemm_space(g, s, rows);
         RT_CHECK(iris_gemv_launch(g, st));
+        if (iris_batch_adapts(s, l, ADAPT_QKV)) {
+            RT_CHECK(iris_batch_norm(s, s->x, L.norm_attn, rows));
+            RT_CHECK(iris_batch_adapt(s, l, ADAPT_QKV, iris_batch_normed(s), H, s->qkv, qkvw, rows));
+        }
         bool ctx_planes = false;
         if (s->batch) {
             RT_CHECK(iris_batch_attention(s, l, rows));
@@ -786,6 +810,7 @@ static int gemma_layer(IrisSession* s, uint32_t l, uint32_t rows, bool carry) {
         if (ctx_planes) bcast_input(g, s, s->ctx_planes, s->ctx_counts);
         with_gemm_space(g, s, rows);
         RT_CHECK(iris_gemv_launch(g, st));
+        if (iris_batch_adapts(s, l, ADAPT_O)) RT_CHECK(iris_batch_adapt(s, l, ADAPT_O, s->ctx, qw, s->tmp, H, rows));
         if (!carry)
             RT_CHECK(iris_norm_residual_launch(s->tmp, H, L.norm_post_attn, d.norm_eps, s->x, H, 0, s->attended, H, H,
                                                rows, st));
@@ -810,8 +835,15 @@ static int gemma_layer(IrisSession* s, uint32_t l, uint32_t rows, bool carry) {
         g.epilogue = EPI_GEGLU;
         g.out = s->gated;
         g.out_stride = L.ffn;
+        // Adapters of gate and up come before the gate's activation.
+        const bool adapted = iris_batch_adapts(s, l, ADAPT_GATE_UP);
+        if (adapted) {
+            g.epilogue = EPI_STORE;
+            g.out = iris_batch_gate_up(s);
+            g.out_stride = 2 * L.ffn;
+        }
         // One row: the gated row's digit planes too, for the down product.
-        const bool gated_planes = rows == 1;
+        const bool gated_planes = rows == 1 && !adapted;
         if (gated_planes) {
             g.out_planes = s->gated_planes;
             g.out_counts = s->gated_counts;
@@ -831,8 +863,9 @@ static int gemma_layer(IrisSession* s, uint32_t l, uint32_t rows, bool carry) {
         with_gemm_space(dn, s, rows);
         // Several rows, both products on the matrix cores: the gate/up
         // product writes the gated rows' digit planes for the down product.
-        if (rows > 1 && s->gated_gemm_planes && iris_gemm_applies(g) && iris_gemm_applies(dn)) {
-            g.out = nullptr;  // nothing reads the gated rows themselves
+        const bool down_adapted = iris_batch_adapts(s, l, ADAPT_DOWN);
+        if (rows > 1 && !adapted && s->gated_gemm_planes && iris_gemm_applies(g) && iris_gemm_applies(dn)) {
+            if (!down_adapted) g.out = nullptr;  // nothing reads the gated rows themselves
             g.out_gemm_planes = s->gated_gemm_planes;
             g.out_gemm_limbs = s->gated_gemm_limbs;
             dn.planes = s->gated_gemm_planes;
@@ -840,7 +873,13 @@ static int gemma_layer(IrisSession* s, uint32_t l, uint32_t rows, bool carry) {
             dn.planes_ready = 1;
         }
         RT_CHECK(iris_gemv_launch(g, st));
+        if (adapted) {
+            RT_CHECK(iris_batch_norm(s, s->attended, L.norm_ff, rows));
+            RT_CHECK(iris_batch_adapt(s, l, ADAPT_GATE_UP, iris_batch_normed(s), H, iris_batch_gate_up(s), 2 * L.ffn, rows));
+            RT_CHECK(iris_batch_gate(s, L.ffn, true, rows));
+        }
         RT_CHECK(iris_gemv_launch(dn, st));
+        if (down_adapted) RT_CHECK(iris_batch_adapt(s, l, ADAPT_DOWN, s->gated, L.ffn, s->tmp, H, rows));
         if (!carry)
             RT_CHECK(iris_norm_residual_launch(s->tmp, H, L.norm_post_ffw, d.norm_eps, s->attended, H, 0, s->attended,
                                                H, H, rows, st));

@@ -89,11 +89,28 @@ __global__ __launch_bounds__(64) void batch_token_kernel(const int64_t* best, in
     if (threadIdx.x == 0) tokens[blockIdx.x] = (int32_t)~(uint32_t)k;
 }
 
-// One request's tree, a lane per row: each row's selection, and from the root
-// (row 0) the path of rows whose token is their parent's selection (of equal
-// children the first). tokens: the selections along the path, path: its rows;
-// kept: their number.
-__global__ __launch_bounds__(64) void batch_accept_kernel(const int64_t* best, const int32_t* row_start, const int32_t* ids,
+// Each request's tokens of the pass behind the text it had: a prompt's, or the kept
+// rows' (path).
+__global__ __launch_bounds__(256) void batch_text_kernel(const int32_t* ids, const int32_t* row_start, const int32_t* lengths,
+                                                         const int32_t* path, const int32_t* kept, int32_t* text, uint32_t stride) {
+    const uint32_t b = blockIdx.x, at = row_start[b], n = path ? kept[b] : row_start[b + 1] - at;
+    int32_t* to = text + (size_t)b * stride + lengths[b];
+    for (uint32_t i = threadIdx.x; i < n; i += 256) to[i] = ids[at + (path ? path[at + i] : (int32_t)i)];
+}
+
+// gated = mul(act(gate), up) of rows that interleave the two.
+__global__ __launch_bounds__(256) void batch_gate_kernel(const int32_t* gate_up, uint32_t ffn, int use_gelu, int32_t* gated) {
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= ffn) return;
+    const int2 x = ((const int2*)(gate_up + (size_t)blockIdx.y * 2 * ffn))[i];
+    gated[(size_t)blockIdx.y * ffn + i] = dn::mul_sat(use_gelu ? dn::gelu(x.x) : dn::silu(x.x), x.y);
+}
+
+// One request's tree, a lane per row: each row's selection (from its pieces'
+// first maxima, or as drawn), and from the root (row 0) the path of rows whose
+// token is their parent's selection (of equal children the first). tokens: the
+// selections along the path, path: its rows; kept: their number.
+__global__ __launch_bounds__(64) void batch_accept_kernel(const int64_t* best, const int32_t* drawn, const int32_t* row_start, const int32_t* ids,
                                                           const int32_t* parents, int32_t* tokens, int32_t* path,
                                                           int32_t* kept) {
     const uint32_t b = blockIdx.x, lane = threadIdx.x, at = row_start[b], n = row_start[b + 1] - at;
@@ -101,7 +118,9 @@ __global__ __launch_bounds__(64) void batch_accept_kernel(const int64_t* best, c
     int32_t id = -1, parent = -1;
     if (lane < n) {
         const int64_t* row = best + (size_t)(at + lane) * SELECT_PARTS;
-        for (uint32_t i = 0; i < SELECT_PARTS; i++) k = max(k, row[i]);
+        if (drawn) k = (int64_t)(uint32_t)~drawn[at + lane];
+        else
+            for (uint32_t i = 0; i < SELECT_PARTS; i++) k = max(k, row[i]);
         id = ids[at + lane];
         parent = parents ? parents[at + lane] : (int32_t)lane - 1;
     }
@@ -163,6 +182,38 @@ struct IrisBatch {
     int64_t* best = nullptr;
     void* space = nullptr;  // of the attention
     uint64_t space_bytes = 0, space_most = 0;  // now; that a pass can need
+    // What requests have of their own (host), and the tables of it on the device.
+    std::vector<int32_t> slot;      // per request, its adapter
+    std::vector<uint8_t> ruled, draws;
+    std::vector<IrisTokenRule> rule;
+    std::vector<std::vector<int32_t>> bias_ids, bias_values;
+    std::vector<std::vector<uint32_t>> numbers;
+    std::vector<uint32_t> first_number;
+    std::vector<std::vector<int32_t>> text;  // the ids of the positions held
+    const IrisModelAdapters* adapters = nullptr;
+    IrisTokenRule* d_rules = nullptr;  // [requests]
+    IrisDrawing* d_drawings = nullptr;
+    int32_t *d_bias_ids = nullptr, *d_bias_values = nullptr, *d_text = nullptr;  // d_text: [requests][max_positions]
+    uint32_t biases = 0;
+    // The next pass's masks.
+    uint32_t* d_masks = nullptr;
+    uint64_t mask_space = 0;  // words
+    uint32_t mask_rows = 0;
+    std::vector<int32_t> mask_of;
+    // What the pass at hand brings of it, by row: slots; and by selection:
+    // requests with rules, requests that draw, numbers, masks. Its selections.
+    int32_t *host_own = nullptr, *own = nullptr, *drawn = nullptr;
+    void* draw_space = nullptr;
+    uint64_t draw_bytes = 0;
+    bool adapted = false, rules_now = false, draws_now = false;
+    int32_t *normed = nullptr, *gate_up = nullptr;
+    void* adapter_space = nullptr;
+    uint64_t adapter_bytes = 0;
+    int32_t* own_slots() const { return own; }
+    int32_t* own_ruled() const { return own + s->max_rows; }
+    int32_t* own_draws() const { return own + 2 * (size_t)s->max_rows; }
+    uint32_t* own_numbers() const { return (uint32_t*)own + 3 * (size_t)s->max_rows; }
+    int32_t* own_masks() const { return own + 4 * (size_t)s->max_rows; }
     // The pass at hand: its requests' rows and, of prompts, the longest; of
     // newest rows, the most of a request and the last position's end.
     bool prompts = false, trees = false;
@@ -287,11 +338,13 @@ int iris_batch_attention(IrisSession* s, uint32_t l, uint32_t rows) {
     return iris_attention_tree(&cache, &newest, b->space, b->space_bytes, st);
 }
 
-// First maxima of the logits of `count` rows of x, as SELECT_PARTS keys each.
+// The selections of `count` rows of x: first maxima as SELECT_PARTS keys each, or
+// where the pass has rules, masks or draws the tokens in b->drawn.
 static int batch_select(IrisBatch* b, const int32_t* x, uint32_t count) {
     IrisSession* s = b->s;
     const IrisModel* m = s->model;
     const uint32_t H = m->d.hidden, V = m->d.vocab;
+    const bool own = b->rules_now || b->draws_now;
     for (uint32_t r = 0; r < count; r += LOGITS_ROWS) {
         const uint32_t n = std::min(LOGITS_ROWS, count - r);
         GemvArgs g{};
@@ -311,9 +364,36 @@ static int batch_select(IrisBatch* b, const int32_t* x, uint32_t count) {
             g.token_limbs = s->token_limbs;
         }
         RT_CHECK(iris_gemv_launch(g, s->stream));
-        hipLaunchKernelGGL(batch_select_kernel, dim3(SELECT_PARTS, n), dim3(256), 0, s->stream, b->logits, V,
-                           b->best + (size_t)r * SELECT_PARTS);
-        RT_CHECK(hipGetLastError());
+        if (!own) {
+            hipLaunchKernelGGL(batch_select_kernel, dim3(SELECT_PARTS, n), dim3(256), 0, s->stream, b->logits, V,
+                               b->best + (size_t)r * SELECT_PARTS);
+            RT_CHECK(hipGetLastError());
+            continue;
+        }
+        if (b->rules_now) {
+            IrisLogitsRules a{};
+            a.logits = a.out = b->logits;
+            a.rows = n, a.vocab = a.logits_stride = a.out_stride = V;
+            if (b->d_rules && b->d_text) {
+                a.request = b->own_ruled() + r;
+                a.rules = b->d_rules, a.requests = b->requests;
+                a.history = b->d_text, a.history_stride = b->max_positions;
+                a.bias_ids = b->d_bias_ids, a.bias_values = b->d_bias_values, a.biases = b->biases;
+                if (b->prompts) {  // the texts have the prompts already
+                    a.lengths = b->added();
+                } else {
+                    a.lengths = b->lengths(), a.ids = s->ids, a.parents = b->trees ? b->parents() : nullptr;
+                    a.row_start = b->row_start, a.first_row = r;
+                }
+            }
+            if (!b->mask_of.empty()) a.masks = b->d_masks, a.mask_of = b->own_masks() + r, a.mask_rows = b->mask_rows, a.mask_stride = (V + 31) / 32;
+            RT_CHECK(iris_logits_rules(&a, s->stream));
+        }
+        IrisLogitsDraw d{};
+        d.logits = b->logits, d.tokens = b->drawn + r;
+        d.rows = n, d.vocab = d.logits_stride = V;
+        if (b->draws_now) d.request = b->own_draws() + r, d.drawings = b->d_drawings, d.numbers = b->own_numbers() + r, d.requests = b->requests;
+        RT_CHECK(iris_logits_draw(&d, b->draw_space, b->draw_bytes, s->stream));
     }
     return 0;
 }
@@ -324,6 +404,8 @@ static int batch_pass(IrisBatch* b, uint32_t rows, uint32_t picks) {
     const IrisModel* m = s->model;
     hipStream_t st = s->stream;
     RT_CHECK(hipMemcpyAsync(b->in, b->host_in, b->in_ints() * 4, hipMemcpyHostToDevice, st));
+    if (rows && (b->adapted || b->rules_now || b->draws_now))
+        RT_CHECK(hipMemcpyAsync(b->own, b->host_own, 5 * (size_t)s->max_rows * 4, hipMemcpyHostToDevice, st));
     IrisPagedPlan p{};
     p.lengths = b->lengths(), p.added = b->added(), p.parents = b->trees ? b->parents() : nullptr;
     p.held = p.held_out = b->d_held;
@@ -337,16 +419,24 @@ static int batch_pass(IrisBatch* b, uint32_t rows, uint32_t picks) {
         RT_CHECK(iris_embed_rows_launch(s->ids, rows, m->embed_raw, m->embed_row_bytes, m->d.hidden, m->embed_scale, s->x, st));
         s->rope_ready = false;
         RT_CHECK(iris_session_pass(s, rows, nullptr));
+        const bool own = b->rules_now || b->draws_now;
         if (b->prompts) {
+            if (b->d_text)
+                hipLaunchKernelGGL(batch_text_kernel, dim3(b->requests), dim3(256), 0, st, s->ids, b->row_start, b->lengths(), nullptr,
+                                   nullptr, b->d_text, b->max_positions);
             hipLaunchKernelGGL(batch_gather_kernel, dim3(picks), dim3(256), 0, st, s->x, b->picks(), m->d.hidden, s->attended);
             RT_CHECK(hipGetLastError());
             RT_CHECK(batch_select(b, s->attended, picks));
-            hipLaunchKernelGGL(batch_token_kernel, dim3(picks), dim3(64), 0, st, b->best, b->tokens());
+            if (own) RT_CHECK(hipMemcpyAsync(b->tokens(), b->drawn, picks * 4, hipMemcpyDeviceToDevice, st));
+            else hipLaunchKernelGGL(batch_token_kernel, dim3(picks), dim3(64), 0, st, b->best, b->tokens());
         } else {
             RT_CHECK(batch_select(b, s->x, rows));
-            hipLaunchKernelGGL(batch_accept_kernel, dim3(b->requests), dim3(64), 0, st, b->best, b->row_start, s->ids,
-                               p.parents, b->tokens(), b->path, b->kept());
+            hipLaunchKernelGGL(batch_accept_kernel, dim3(b->requests), dim3(64), 0, st, b->best, own ? b->drawn : nullptr,
+                               b->row_start, s->ids, p.parents, b->tokens(), b->path, b->kept());
             RT_CHECK(hipGetLastError());
+            if (b->d_text)
+                hipLaunchKernelGGL(batch_text_kernel, dim3(b->requests), dim3(256), 0, st, s->ids, b->row_start, b->lengths(), b->path,
+                                   b->kept(), b->d_text, b->max_positions);
             if (b->longest > 2 && b->trees && m->d.layers)
                 hipLaunchKernelGGL(batch_keep_kernel, dim3(b->requests, m->d.layers), dim3(256), 0, st, b->d_caches, b->row_start,
                                    b->path, b->kept(), b->slots);
@@ -360,6 +450,81 @@ static int batch_pass(IrisBatch* b, uint32_t rows, uint32_t picks) {
 
 static uint32_t pages_of(const IrisBatch* b, uint64_t positions) {
     return (uint32_t)((positions + b->page_size - 1) / b->page_size);
+}
+
+template <class T>
+static int batch_alloc(T** p, uint64_t count) {
+    const hipError_t st = hipMalloc((void**)p, std::max<uint64_t>(count * sizeof(T), 16));
+    if (st != hipSuccess) {
+        *p = nullptr;
+        (void)hipGetLastError();  // returned here: not the next launch's to report
+    }
+    return (int)st;
+}
+
+// The buffers of passes whose requests have something of their own, made for the
+// first that does.
+static int batch_own_buffers(IrisBatch* b) {
+    const uint64_t rows = b->s->max_rows;
+    if (!b->own) RT_CHECK(batch_alloc(&b->own, 5 * rows));
+    if (!b->drawn) RT_CHECK(batch_alloc(&b->drawn, rows));
+    if (!b->host_own) {
+        const hipError_t st = hipHostMalloc((void**)&b->host_own, 5 * rows * 4);
+        if (st != hipSuccess) {
+            b->host_own = nullptr;
+            (void)hipGetLastError();
+            return (int)st;
+        }
+        std::memset(b->host_own, 0, 5 * rows * 4);
+    }
+    if (!b->draw_space) {
+        IrisLogitsDraw d{};
+        d.logits = (const int32_t*)256, d.tokens = b->drawn;
+        d.rows = LOGITS_ROWS, d.vocab = d.logits_stride = b->s->model->d.vocab;
+        // (What any number of rows up to these takes.)
+        uint64_t bytes = 0;
+        for (d.rows = 1; d.rows <= LOGITS_ROWS; d.rows++) bytes = std::max(bytes, iris_logits_draw_workspace_bytes(&d));
+        uint8_t* space = nullptr;
+        RT_CHECK(batch_alloc(&space, bytes));
+        b->draw_space = space, b->draw_bytes = bytes;
+    }
+    return 0;
+}
+
+// What the pass's requests have of their own, by row and by selection, into
+// host_own. IRIS_E_RANGE where a drawing's numbers do not reach.
+static int batch_own(IrisBatch* b, const int32_t* parents, const uint32_t* counts, uint32_t rows, bool prompts) {
+    b->adapted = b->rules_now = b->draws_now = false;
+    const bool masked = !b->mask_of.empty();
+    if (masked && b->mask_of.size() != rows) return IRIS_E_INVALID;
+    bool any = masked;
+    for (uint32_t i = 0; i < b->requests; i++) any = any || (counts[i] && (b->slot[i] >= 0 || b->ruled[i] || b->draws[i]));
+    if (!any) return 0;
+    const uint32_t most = b->s->max_rows;
+    int32_t *slots = b->host_own, *ruled = slots + most, *draws = ruled + most, *numbers = draws + most, *masks = numbers + most;
+    bool adapted = false, rules_now = masked, draws_now = false;
+    for (uint32_t i = 0, at = 0, pick = 0; i < b->requests; at += counts[i++]) {
+        if (!counts[i]) continue;
+        adapted = adapted || b->slot[i] >= 0, rules_now = rules_now || b->ruled[i], draws_now = draws_now || b->draws[i];
+        uint32_t depth[TREE_MAX_NODES] = {};
+        for (uint32_t j = 0; j < counts[i]; j++) {
+            slots[at + j] = b->slot[i];
+            if (prompts && j + 1 < counts[i]) continue;
+            if (!prompts) {
+                const int64_t up = parents ? parents[at + j] : (int64_t)j - 1;
+                depth[j] = up >= 0 && up < (int64_t)j ? depth[up] + 1 : 0;
+            }
+            const uint32_t to = prompts ? pick++ : at + j;
+            ruled[to] = b->ruled[i] ? (int32_t)i : -1, draws[to] = b->draws[i] ? (int32_t)i : -1, numbers[to] = 0;
+            masks[to] = masked ? b->mask_of[at + j] : -1;
+            if (!b->draws[i]) continue;
+            const uint64_t position = prompts ? j : b->length[i] + depth[j];
+            if (position < b->first_number[i] || position - b->first_number[i] >= b->numbers[i].size()) return IRIS_E_RANGE;
+            numbers[to] = (int32_t)b->numbers[i][position - b->first_number[i]];
+        }
+    }
+    b->adapted = adapted, b->rules_now = rules_now, b->draws_now = draws_now;
+    return 0;
 }
 
 // The checks of a pass, its inputs into host_in and the pass itself.
@@ -402,7 +567,15 @@ static int batch_run(IrisBatch* b, const int32_t* ids, const int32_t* parents, c
     b->trees = parents != nullptr;
     b->longest = (uint32_t)most;
     b->end = (uint32_t)end;
+    RT_CHECK(batch_own(b, parents, counts, (uint32_t)rows, prompts));
     RT_CHECK(batch_space(b, (uint32_t)rows));
+    try {  // room for the texts to come
+        for (uint32_t i = 0; i < n; i++)
+            if (b->text[i].capacity() < b->text[i].size() + counts[i])
+                b->text[i].reserve(std::max(b->text[i].size() + counts[i], 2 * b->text[i].capacity()));
+    } catch (const std::bad_alloc&) {
+        return IRIS_E_NOMEM;
+    }
     b->broken = true;  // until the pass has ended well
     if (grow > b->pages - held) {
         // The plan takes pages before it gives others back, so those of
@@ -414,7 +587,39 @@ static int batch_run(IrisBatch* b, const int32_t* ids, const int32_t* parents, c
     RT_CHECK(batch_pass(b, (uint32_t)rows, picks));
     for (uint32_t i = 0; i < n; i++) b->held[i] = pages_of(b, b->length[i] + counts[i]);
     b->broken = false;
+    if (rows) b->mask_of.clear();
     return 0;
+}
+
+bool iris_batch_adapted(const IrisSession* s) { return s->batch && s->batch->adapted; }
+
+bool iris_batch_adapts(const IrisSession* s, uint32_t layer, uint32_t product) {
+    return iris_batch_adapted(s) && iris_model_adapters_bank(s->batch->adapters, layer, product);
+}
+
+int32_t* iris_batch_normed(const IrisSession* s) { return s->batch->normed; }
+int32_t* iris_batch_gate_up(const IrisSession* s) { return s->batch->gate_up; }
+
+int iris_batch_norm(IrisSession* s, const int32_t* x, const int32_t* norm_w, uint32_t rows) {
+    const uint32_t H = s->model->d.hidden;
+    // (The residual is one row of zeros, behind the rows.)
+    return iris_norm_residual_launch(x, H, norm_w, s->model->d.norm_eps, s->batch->normed + (size_t)s->max_rows * H, 0, 0,
+                                     s->batch->normed, H, H, rows, s->stream);
+}
+
+int iris_batch_adapt(IrisSession* s, uint32_t layer, uint32_t product, const int32_t* x, uint32_t x_stride, int32_t* y,
+                     uint32_t y_stride, uint32_t rows) {
+    const IrisBatch* b = s->batch;
+    IrisAdapterRows a{};
+    a.x = x, a.y = a.out = y, a.slots = b->own_slots();
+    a.x_stride = x_stride, a.y_stride = a.out_stride = y_stride, a.rows = rows;
+    return iris_adapters_apply(iris_model_adapters_bank(b->adapters, layer, product), &a, b->adapter_space, b->adapter_bytes, s->stream);
+}
+
+int iris_batch_gate(IrisSession* s, uint32_t ffn, bool use_gelu, uint32_t rows) {
+    hipLaunchKernelGGL(batch_gate_kernel, dim3((ffn + 255) / 256, rows), dim3(256), 0, s->stream, s->batch->gate_up, ffn, use_gelu,
+                       s->gated);
+    return (int)hipGetLastError();
 }
 
 extern "C" {
@@ -461,6 +666,15 @@ int iris_batch_create(IrisModel* m, uint32_t requests, uint32_t pages, uint32_t 
     try {
         b->length.assign(requests, 0);
         b->held.assign(requests, 0);
+        b->slot.assign(requests, -1);
+        b->ruled.assign(requests, 0);
+        b->draws.assign(requests, 0);
+        b->rule.assign(requests, IrisTokenRule{});
+        b->bias_ids.resize(requests);
+        b->bias_values.resize(requests);
+        b->numbers.resize(requests);
+        b->first_number.assign(requests, 0);
+        b->text.resize(requests);
         b->caches.assign(d.layers, IrisPagedKv{});
         b->k_rows.assign(d.layers, nullptr);
         b->v_rows.assign(d.layers, nullptr);
@@ -539,6 +753,9 @@ void iris_batch_free(IrisBatch* b) {
     (void)hipFree(b->d_caches);
     for (int32_t* p : {b->in, b->out, b->d_held, b->table, b->ring, b->ring_state, b->row_start, b->slots, b->path, b->logits})
         (void)hipFree(p);
+    for (int32_t* p : {b->d_bias_ids, b->d_bias_values, b->d_text, b->own, b->drawn, b->normed, b->gate_up}) (void)hipFree(p);
+    for (void* p : {(void*)b->d_rules, (void*)b->d_drawings, (void*)b->d_masks, b->draw_space, b->adapter_space}) (void)hipFree(p);
+    if (b->host_own) (void)hipHostFree(b->host_own);
     (void)hipFree(b->best);
     (void)hipFree(b->space);
     if (b->host_in) (void)hipHostFree(b->host_in);
@@ -554,6 +771,8 @@ int iris_batch_prefill(IrisBatch* b, const int32_t* ids, const uint32_t* counts,
     for (uint32_t i = 0, at = 0; i < b->requests; i++) {
         out_tokens[i] = counts[i] ? tokens[at++] : -1;
         b->length[i] += counts[i];
+        b->text[i].insert(b->text[i].end(), ids, ids + counts[i]);  // (room was made)
+        ids += counts[i];
     }
     return 0;
 }
@@ -567,6 +786,8 @@ int iris_batch_step(IrisBatch* b, const int32_t* ids, const int32_t* parents, co
         out_kept[i] = counts[i] ? (uint32_t)kept[i] : 0;
         for (uint32_t j = 0; j < counts[i]; j++) out_tokens[at + j] = j < out_kept[i] ? tokens[at + j] : -1;
         b->length[i] += out_kept[i];
+        // A kept row behind the first has its forerunner's selection as its token.
+        for (uint32_t j = 0; j < out_kept[i]; j++) b->text[i].push_back(j ? tokens[at + j - 1] : ids[at]);
     }
     return 0;
 }
@@ -575,6 +796,188 @@ int iris_batch_release(IrisBatch* b, uint32_t request) {
     if (!b || request >= b->requests) return IRIS_E_INVALID;
     if (b->broken) return IRIS_E_STATE;
     b->length[request] = 0;  // its pages go back to the ring with the next pass's plan
+    b->text[request].clear();
+    b->slot[request] = -1, b->ruled[request] = b->draws[request] = 0;
+    return 0;
+}
+
+int iris_batch_adapters(IrisBatch* b, const IrisModelAdapters* set) {
+    if (!b) return IRIS_E_INVALID;
+    if (b->broken) return IRIS_E_STATE;
+    const IrisModelDesc& d = b->s->model->d;
+    if (set) {
+        uint32_t slots, max_rank;
+        if (iris_model_adapters_model(set, &slots, &max_rank) != b->s->model) return IRIS_E_INVALID;
+        uint64_t bytes = 16;
+        for (uint32_t l = 0; l < d.layers; l++)
+            for (uint32_t product = 0; product < ADAPT_PRODUCTS; product++) {
+                const AdapterProductShape p = iris_adapter_product(b->s->model, l, product);
+                bytes = std::max(bytes, iris_adapters_space(p.cols, p.part_count, max_rank, b->s->max_rows));
+            }
+        RT_CHECK(batch_own_buffers(b));
+        const uint64_t H = d.hidden, rows = b->s->max_rows;
+        if (!b->normed) {  // and a row of zeros
+            int32_t *normed = nullptr, *gate_up = nullptr;
+            RT_CHECK(batch_alloc(&normed, (rows + 1) * H));
+            int rc = batch_alloc(&gate_up, 2 * rows * std::max(b->s->model->max_ffn, 1u));
+            if (!rc) rc = (int)hipMemset(normed + rows * H, 0, H * 4);
+            if (rc) {
+                (void)hipFree(normed);
+                (void)hipFree(gate_up);
+                return rc;
+            }
+            b->normed = normed, b->gate_up = gate_up;
+        }
+        if (bytes > b->adapter_bytes) {
+            uint8_t* space = nullptr;
+            RT_CHECK(batch_alloc(&space, bytes));
+            (void)hipFree(b->adapter_space);
+            b->adapter_space = space, b->adapter_bytes = bytes;
+        }
+    }
+    b->adapters = set;
+    std::fill(b->slot.begin(), b->slot.end(), -1);
+    return 0;
+}
+
+int iris_batch_adapter(IrisBatch* b, uint32_t request, int32_t slot) {
+    if (!b || request >= b->requests || slot < -1) return IRIS_E_INVALID;
+    if (b->broken || (slot >= 0 && !b->adapters)) return IRIS_E_STATE;
+    uint32_t slots = 0, max_rank;
+    if (slot >= 0) (void)iris_model_adapters_model(b->adapters, &slots, &max_rank);
+    if (slot >= 0 && (uint32_t)slot >= slots) return IRIS_E_INVALID;
+    b->slot[request] = slot;
+    return 0;
+}
+
+int iris_batch_rule(IrisBatch* b, uint32_t request, const IrisTokenRule* rule, const int32_t* bias_ids, const int32_t* bias_values) {
+    if (!b || request >= b->requests) return IRIS_E_INVALID;
+    if (b->broken) return IRIS_E_STATE;
+    if (!rule) {
+        b->ruled[request] = 0;
+        return 0;
+    }
+    if (rule->repetition <= 0 || (rule->bias_count && (!bias_ids || !bias_values))) return IRIS_E_INVALID;
+    RT_CHECK(batch_own_buffers(b));
+    try {
+        // All requests' biases, one after the other, with this one's new ones.
+        std::vector<int32_t> ids, values, own_ids, own_values;
+        if (rule->bias_count) {
+            own_ids.assign(bias_ids, bias_ids + rule->bias_count);
+            own_values.assign(bias_values, bias_values + rule->bias_count);
+        }
+        std::vector<IrisTokenRule> rules = b->rule;
+        rules[request] = *rule;
+        uint64_t total = 0;
+        for (uint32_t i = 0; i < b->requests; i++) total += i == request ? own_ids.size() : b->ruled[i] ? b->bias_ids[i].size() : 0;
+        if (total > 1u << 20) return IRIS_E_RANGE;
+        for (uint32_t i = 0; i < b->requests; i++) {
+            rules[i].bias_start = (uint32_t)ids.size(), rules[i].bias_count = 0;
+            if (i != request && !b->ruled[i]) continue;
+            const auto& from = i == request ? own_ids : b->bias_ids[i];
+            const auto& of = i == request ? own_values : b->bias_values[i];
+            ids.insert(ids.end(), from.begin(), from.end());
+            values.insert(values.end(), of.begin(), of.end());
+            rules[i].bias_count = (uint32_t)from.size();
+        }
+        IrisTokenRule* d_rules = b->d_rules;
+        int32_t *d_ids = nullptr, *d_values = nullptr, *d_text = b->d_text;
+        int rc = b->d_rules ? 0 : batch_alloc(&d_rules, b->requests);
+        if (!rc) rc = batch_alloc(&d_ids, std::max<size_t>(ids.size(), 1));
+        if (!rc) rc = batch_alloc(&d_values, std::max<size_t>(ids.size(), 1));
+        if (!rc && !ids.empty()) rc = (int)hipMemcpy(d_ids, ids.data(), ids.size() * 4, hipMemcpyHostToDevice);
+        if (!rc && !ids.empty()) rc = (int)hipMemcpy(d_values, values.data(), ids.size() * 4, hipMemcpyHostToDevice);
+        if (!rc && !b->d_text) {
+            rc = batch_alloc(&d_text, (uint64_t)b->requests * b->max_positions);
+            for (uint32_t i = 0; !rc && i < b->requests; i++)
+                if (!b->text[i].empty())
+                    rc = (int)hipMemcpy(d_text + (size_t)i * b->max_positions, b->text[i].data(), b->text[i].size() * 4, hipMemcpyHostToDevice);
+        }
+        if (!rc) rc = (int)hipMemcpy(d_rules, rules.data(), b->requests * sizeof(IrisTokenRule), hipMemcpyHostToDevice);
+        if (rc) {
+            (void)hipFree(d_ids);
+            (void)hipFree(d_values);
+            if (d_rules != b->d_rules) (void)hipFree(d_rules);
+            if (d_text != b->d_text) (void)hipFree(d_text);
+            return rc;
+        }
+        (void)hipFree(b->d_bias_ids);
+        (void)hipFree(b->d_bias_values);
+        b->d_rules = d_rules, b->d_bias_ids = d_ids, b->d_bias_values = d_values, b->d_text = d_text;
+        b->biases = (uint32_t)ids.size();
+        b->rule.swap(rules);
+        b->bias_ids[request].swap(own_ids);
+        b->bias_values[request].swap(own_values);
+    } catch (const std::bad_alloc&) {
+        return IRIS_E_NOMEM;
+    }
+    b->ruled[request] = 1;
+    return 0;
+}
+
+int iris_batch_drawing(IrisBatch* b, uint32_t request, const IrisDrawing* drawing, const uint32_t* numbers, uint32_t first,
+                       uint32_t count) {
+    if (!b || request >= b->requests) return IRIS_E_INVALID;
+    if (b->broken) return IRIS_E_STATE;
+    if (!drawing) {
+        b->draws[request] = 0;
+        return 0;
+    }
+    if (count && !numbers) return IRIS_E_INVALID;
+    if (count > b->max_positions) return IRIS_E_RANGE;
+    RT_CHECK(batch_own_buffers(b));
+    try {
+        std::vector<uint32_t> own;
+        if (count) own.assign(numbers, numbers + count);
+        IrisDrawing* d = b->d_drawings;
+        if (!d) RT_CHECK(batch_alloc(&d, b->requests));
+        const int rc = (int)hipMemcpy(d + request, drawing, sizeof(*drawing), hipMemcpyHostToDevice);
+        if (rc) {
+            if (d != b->d_drawings) (void)hipFree(d);
+            return rc;
+        }
+        b->d_drawings = d;
+        b->numbers[request].swap(own);
+    } catch (const std::bad_alloc&) {
+        return IRIS_E_NOMEM;
+    }
+    b->first_number[request] = first;
+    b->draws[request] = 1;
+    return 0;
+}
+
+int iris_batch_masks(IrisBatch* b, const uint32_t* masks, uint32_t mask_rows, const int32_t* mask_of, uint32_t rows) {
+    if (!b) return IRIS_E_INVALID;
+    if (b->broken) return IRIS_E_STATE;
+    if (!masks || !rows) {
+        b->mask_of.clear();
+        return 0;
+    }
+    if (!mask_of || !mask_rows) return IRIS_E_INVALID;
+    if (rows > b->s->max_rows || mask_rows > rows) return IRIS_E_RANGE;
+    for (uint32_t r = 0; r < rows; r++)
+        if (mask_of[r] < -1 || mask_of[r] >= (int64_t)mask_rows) return IRIS_E_INVALID;
+    RT_CHECK(batch_own_buffers(b));
+    const uint64_t words = (uint64_t)mask_rows * ((b->s->model->d.vocab + 31) / 32);
+    try {
+        std::vector<int32_t> of(mask_of, mask_of + rows);
+        if (words > b->mask_space) {
+            uint32_t* space = nullptr;
+            RT_CHECK(batch_alloc(&space, words));
+            (void)hipFree(b->d_masks);
+            b->d_masks = space, b->mask_space = words;
+            b->mask_of.clear();  // (of the masks before)
+        }
+        const int rc = (int)hipMemcpy(b->d_masks, masks, words * 4, hipMemcpyHostToDevice);
+        if (rc) {
+            b->mask_of.clear();
+            return rc;
+        }
+        b->mask_of.swap(of);
+    } catch (const std::bad_alloc&) {
+        return IRIS_E_NOMEM;
+    }
+    b->mask_rows = mask_rows;
     return 0;
 }
 

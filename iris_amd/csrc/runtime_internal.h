@@ -170,6 +170,31 @@ int iris_session_pass(IrisSession* s, uint32_t rows, const CkptSink* sink);
 // A batch's step between a layer's q|k|v product (s->qkv) and its O product:
 // rotation, cache store and attention, into s->ctx.
 int iris_batch_attention(IrisSession* s, uint32_t layer, uint32_t rows);
+// Adapters beside a layer's products, in a batch whose rows have some.
+enum AdapterProduct : uint32_t { ADAPT_QKV = 0, ADAPT_O = 1, ADAPT_GATE_UP = 2, ADAPT_DOWN = 3, ADAPT_PRODUCTS = 4 };
+struct AdapterProductShape {
+    uint32_t cols, part_count;
+    IrisAdapterPart parts[IRIS_ADAPTER_PARTS];
+};
+AdapterProductShape iris_adapter_product(const IrisModel* m, uint32_t layer, uint32_t product);
+const IrisAdapterBank* iris_model_adapters_bank(const IrisModelAdapters* set, uint32_t layer, uint32_t product);
+const IrisModel* iris_model_adapters_model(const IrisModelAdapters* set, uint32_t* slots, uint32_t* max_rank);
+// Work space of a call of up to `rows` rows of a bank of that shape.
+uint64_t iris_adapters_space(uint32_t cols, uint32_t part_count, uint32_t max_rank, uint32_t rows);
+// Whether the pass at hand has rows with an adapter (of that product of a layer).
+bool iris_batch_adapted(const IrisSession* s);
+bool iris_batch_adapts(const IrisSession* s, uint32_t layer, uint32_t product);
+// y += the rows' adapters of x.
+int iris_batch_adapt(IrisSession* s, uint32_t layer, uint32_t product, const int32_t* x, uint32_t x_stride, int32_t* y,
+                     uint32_t y_stride, uint32_t rows);
+// The rows rms_norm(x, norm_w) of the hidden size, and the gate and up rows in turn.
+int iris_batch_norm(IrisSession* s, const int32_t* x, const int32_t* norm_w, uint32_t rows);
+int32_t* iris_batch_normed(const IrisSession* s);
+int32_t* iris_batch_gate_up(const IrisSession* s);
+// s->gated = mul(act(gate), up) of them: silu, or gelu.
+int iris_batch_gate(IrisSession* s, uint32_t ffn, bool use_gelu, uint32_t rows);
+// The layer of a tensor's name and what follows; -1 for none.
+int iris_layer_of(const std::string& name, std::string* suffix);
 // True when embedding token `id` is refused.
 bool iris_embedding_refused(const IrisModel* m, int32_t id);
 

@@ -16,6 +16,8 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import native
+from .adapters import to_fixed
+from .logits import Drawing, TokenRule
 from .model import PREFIX, Model
 
 FAMILY = {"mistral-dense": 0, "gemma-dense": 1}
@@ -67,6 +69,16 @@ def _declare():
         "iris_batch_step": (C.c_int, [vp, vp, vp, vp, vp, vp]),
         "iris_batch_release": (C.c_int, [vp, u32]),
         "iris_batch_length": (C.c_int, [vp, u32, C.POINTER(u32)]),
+        "iris_model_adapters_create": (C.c_int, [vp, u32, u32, pp]),
+        "iris_model_adapters_free": (None, [vp]),
+        "iris_model_adapters_device_bytes": (u64, [vp]),
+        "iris_model_adapters_load": (C.c_int, [vp, u32, C.c_char_p, vp, u32, vp, u32, u32]),
+        "iris_model_adapters_clear": (C.c_int, [vp, u32]),
+        "iris_batch_adapters": (C.c_int, [vp, vp]),
+        "iris_batch_adapter": (C.c_int, [vp, u32, i32]),
+        "iris_batch_rule": (C.c_int, [vp, u32, C.POINTER(TokenRule), vp, vp]),
+        "iris_batch_drawing": (C.c_int, [vp, u32, C.POINTER(Drawing), vp, u32, u32]),
+        "iris_batch_masks": (C.c_int, [vp, vp, u32, vp, u32]),
         "iris_sha256_bytes": (C.c_int, [vp, u64, vp]),
     }
     for name, (res, args) in sig.items():
@@ -189,7 +201,8 @@ class GenerateResult:
     token_ids: list
     logits: np.ndarray | None  # [selections, vocab]
     # "eos" when the last selection is an EOS id, else "max_new_tokens"
-    # (the reference's report field, crates/inference/direct/src/executor.rs:157-171)
+    # (the reference's report field, crates/inference/direct/src/executor.rs:157-171);
+    # "closed" where a mask left no token to select (Batch.generate)
     stop_reason: str = "max_new_tokens"
 
     @property
@@ -316,6 +329,79 @@ class Session:
             pass
 
 
+class ModelAdapters:
+    """Up to ``slots`` low-rank adapters of a model's layers, of rank up to
+    ``max_rank`` (iris_model_adapters_*). A batch that uses them must not outlive
+    them."""
+
+    PRODUCTS = ("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj", "self_attn.o_proj", "mlp.gate_proj",
+                "mlp.up_proj", "mlp.down_proj")
+
+    def __init__(self, dm: DeviceModel, slots: int, max_rank: int):
+        h = C.c_void_p()
+        native.check(_declare().iris_model_adapters_create(dm.handle, slots, max_rank, C.byref(h)), "adapters create")
+        self.dm, self.slots, self.max_rank, self._h = dm, slots, max_rank, h
+
+    @property
+    def handle(self):
+        return self._h
+
+    def _cols_rows(self, name: str) -> tuple:
+        m = self.dm.model
+        if not name.startswith(PREFIX + "layers.") or not name.endswith(tuple(p + ".weight" for p in self.PRODUCTS)):
+            raise native.IrisError(-1, "adapters load")
+        w = m.q8(name)
+        return w.shape[1] // 34 * 32, w.shape[0]
+
+    def load(self, slot: int, name: str, a, a_bits: int, b, b_bits: int):
+        """The pair of one matrix (its tensor's name): a [rank][columns], b
+        [rows][rank] (int16), weights a / 2^a_bits and b / 2^b_bits. Waits for
+        the device."""
+        cols, rows = self._cols_rows(name)
+        a, b = np.asarray(a), np.asarray(b)
+        if a.dtype != np.int16 or b.dtype != np.int16 or a.ndim != 2 or a.shape[1] != cols or b.shape != (rows, a.shape[0]):
+            raise ValueError(f"{name} takes int16 [rank][{cols}] and [{rows}][rank]")
+        a, b = np.ascontiguousarray(a), np.ascontiguousarray(b)
+        native.check(native.lib().iris_model_adapters_load(self._h, slot, name.encode(), a.ctypes.data, a_bits, b.ctypes.data,
+                                                           b_bits, a.shape[0]), "adapters load")
+
+    def load_real(self, slot: int, name: str, a, b, scale: float = 1.0):
+        """The pair as real weights, B times ``scale`` (an import-time conversion)."""
+        (qa, a_bits), (qb, b_bits) = to_fixed(a), to_fixed(np.asarray(b, dtype=np.float64) * scale)
+        self.load(slot, name, qa, a_bits, qb, b_bits)
+
+    def clear(self, slot: int):
+        """Empties a slot."""
+        native.check(native.lib().iris_model_adapters_clear(self._h, slot), "adapters clear")
+
+    def device_bytes(self) -> int:
+        return native.lib().iris_model_adapters_device_bytes(self._h)
+
+    def free(self):
+        if getattr(self, "_h", None):
+            native.lib().iris_model_adapters_free(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+@dataclass
+class RequestOptions:
+    """What one prompt of ``Batch.generate`` has of its own."""
+    adapter: int = -1                    # slot of the batch's adapters
+    rule: TokenRule | None = None        # its penalties (bias_start and _count are not read)
+    biases: object = None                # {token: Q16.16 value} or (token, value) pairs
+    drawing: Drawing | None = None       # logits.drawing(...)
+    # The random 32-bit numbers of the tokens to come, in order.
+    numbers: object = None
+    # mask(ids): the tokens open behind the ids so far (bool [vocab]), or None for all.
+    mask: object = None
+
+
 class Batch:
     """Up to ``requests`` requests at a time over one paged K/V cache of
     ``pages`` pages of ``page_size`` positions, each request up to
@@ -332,7 +418,7 @@ class Batch:
         h = C.c_void_p()
         native.check(L.iris_batch_create(dm.handle, requests, pages, page_size, max_positions, max_rows, C.byref(h)),
                      "batch create")
-        self._h = h
+        self._h, self._adapters = h, None
 
     def _gather(self, rows: dict):
         """The requests' rows one after the other: (ids, counts)."""
@@ -369,19 +455,70 @@ class Batch:
         return {i: tokens[at[i]:at[i] + kept[i]].tolist() for i in range(self.requests) if counts[i]}
 
     def release(self, request: int):
-        """Empties a request; its pages are free for the next call."""
+        """Empties a request; its pages are free for the next call, and it has
+        no adapter, rule or drawing."""
         native.check(native.lib().iris_batch_release(self._h, request), "batch release")
+
+    def adapters(self, adapters: ModelAdapters | None):
+        """The adapters that requests' slots name (None: none)."""
+        native.check(native.lib().iris_batch_adapters(self._h, adapters.handle if adapters else None), "batch adapters")
+        self._adapters = adapters  # (kept as long as the batch uses them)
+
+    def adapter(self, request: int, slot: int):
+        """A request's adapter from the next pass on (-1: none)."""
+        native.check(native.lib().iris_batch_adapter(self._h, request, slot), "batch adapter")
+
+    def rule(self, request: int, rule: TokenRule | None, biases=None):
+        """A request's penalties and biases, {token: Q16.16 value} or pairs
+        (None: neither)."""
+        if rule is None and not biases:
+            native.check(native.lib().iris_batch_rule(self._h, request, None, None, None), "batch rule")
+            return
+        pairs = list(biases.items()) if isinstance(biases, dict) else list(biases or ())
+        ids = np.array([t for t, _ in pairs], dtype=np.int32)
+        values = np.array([v for _, v in pairs], dtype=np.int32)
+        r = TokenRule.from_buffer_copy(rule) if rule is not None else TokenRule(repetition=1 << 16)
+        r.bias_start, r.bias_count = 0, len(pairs)
+        native.check(native.lib().iris_batch_rule(self._h, request, C.byref(r), ids.ctypes.data, values.ctypes.data),
+                     "batch rule")
+
+    def drawing(self, request: int, drawing: Drawing | None, numbers=(), first: int = 0):
+        """How a request draws, and the numbers of the rows at positions
+        ``first`` on (None: the first maximum)."""
+        numbers = np.ascontiguousarray(numbers, dtype=np.uint32)
+        native.check(native.lib().iris_batch_drawing(self._h, request, C.byref(drawing) if drawing is not None else None,
+                                                     numbers.ctypes.data, first, numbers.size), "batch drawing")
+
+    def masks(self, masks, mask_of=()):
+        """The open tokens of the next pass's rows: masks [count][vocab] of
+        truth values, mask_of the mask of each of its ids in order (-1: none).
+        None: no masks."""
+        if masks is None:
+            native.check(native.lib().iris_batch_masks(self._h, None, 0, None, 0), "batch masks")
+            return
+        masks = np.asarray(masks, dtype=bool)
+        vocab = self.dm.model.vocab
+        if masks.ndim != 2 or masks.shape[1] != vocab:
+            raise ValueError(f"masks take [count][{vocab}] truth values")
+        words = np.zeros((masks.shape[0], -(-vocab // 32) * 4), dtype=np.uint8)
+        words[:, :-(-vocab // 8)] = np.packbits(masks, axis=1, bitorder="little")
+        mask_of = np.ascontiguousarray(mask_of, dtype=np.int32)
+        native.check(native.lib().iris_batch_masks(self._h, words.ctypes.data, masks.shape[0], mask_of.ctypes.data,
+                                                   mask_of.size), "batch masks")
 
     def length(self, request: int) -> int:
         n = C.c_uint32()
         native.check(native.lib().iris_batch_length(self._h, request, C.byref(n)), "batch length")
         return n.value
 
-    def generate(self, prompts, tokens: int, draft=None) -> list:
+    def generate(self, prompts, tokens: int, draft=None, options=None) -> list:
         """Greedy generation for each prompt: a list of GenerateResult, as
         ``Session.generate`` gives them (without logits), over requests that
         are all empty. Prompts wait until a request and enough pages for all
         their positions are free.
+        ``options`` (optional) has RequestOptions or None for each prompt: its
+        adapter, rules, mask and drawing. Its tokens then depend on these and
+        on nothing else.
         ``draft(index, ids)`` (optional), called with a prompt's index and the
         ids so far, proposes what may follow: (ids, parents), parents[j] the
         place in ``ids`` of row j's parent, -1 for the last of the ids so far;
@@ -407,6 +544,12 @@ class Batch:
                 raise native.IrisError(-5, "batch generate")
         if any(self.length(i) for i in range(self.requests)):
             raise native.IrisError(-4, "batch generate")
+        own = list(options) if options is not None else [None] * len(prompts)
+        if len(own) != len(prompts):
+            raise ValueError("options must have an entry for each prompt")
+        for o in own:
+            if o is not None and o.drawing is not None and len(o.numbers if o.numbers is not None else ()) < tokens:
+                raise ValueError(f"a drawing takes a number for each of the {tokens} tokens")
         for p in prompts:
             native.check(self.dm.ids_refused(p)[0], "batch generate")
         waiting, running = list(range(len(prompts))), {}  # request -> prompt
@@ -421,6 +564,9 @@ class Batch:
             """The request's next tokens; True when it has ended."""
             r = results[running[request]]
             for t in new:
+                if t < 0:
+                    r.stop_reason = "closed"
+                    return ended(request)
                 r.token_ids.append(t)
                 if t in eos or len(r.token_ids) == tokens:
                     r.stop_reason = "eos" if t in eos else "max_new_tokens"
@@ -430,6 +576,45 @@ class Batch:
                 failed[running[request]] = code
                 return ended(request)
             return False
+
+        def begin(request, p):
+            """The request is prompt p's: what p has of its own."""
+            o = own[p]
+            if o is None:
+                return
+            if o.adapter >= 0:
+                self.adapter(request, o.adapter)
+            if o.rule is not None or o.biases:
+                self.rule(request, o.rule, o.biases)
+            if o.drawing is not None:
+                self.drawing(request, o.drawing, o.numbers, prompts[p].size - 1)
+
+        def mask_rows(rows, parents):
+            """The masks of the pass over {request: ids to come}."""
+            if not any(own[running[r]] is not None and own[running[r]].mask is not None for r in rows):
+                return
+            masks, mask_of = [], []
+            for request in sorted(rows):
+                p, ids = running[request], rows[request]
+                mask = own[p].mask if own[p] is not None else None
+                if mask is None:
+                    mask_of += [-1] * len(ids)
+                    continue
+                prompt = len(results[p].token_ids) == 0
+                so_far = [] if prompt else prompts[p].tolist() + results[p].token_ids[:-1]
+                paths = []  # each row's ids from the first on
+                for j, t in enumerate(ids):
+                    up = parents[request][j] if request in parents else j - 1
+                    if prompt:
+                        is_open = mask(list(ids)) if j + 1 == len(ids) else None
+                    else:
+                        paths.append((paths[up] if 0 <= up < j else so_far) + [int(t)])
+                        is_open = mask(paths[-1])
+                    mask_of.append(-1 if is_open is None else len(masks))
+                    if is_open is not None:
+                        masks.append(np.asarray(is_open, dtype=bool))
+            if masks:
+                self.masks(np.stack(masks), mask_of)
 
         try:
             while waiting or running:
@@ -445,6 +630,9 @@ class Batch:
                     free -= pages[p]
                     rows += prompts[p].size
                 if start:
+                    for request, p in start.items():
+                        begin(request, p)
+                    mask_rows({r: prompts[p].tolist() for r, p in start.items()}, {})
                     for request, token in self.prefill({r: prompts[p] for r, p in start.items()}).items():
                         took(request, [token])
                 step, trees, rows = {}, {}, 0
@@ -467,11 +655,15 @@ class Batch:
                     rows += len(last)
                 if step:
                     try:
+                        mask_rows(step, trees)
                         done = self.step(step, trees)
                     except native.IrisError as e:
                         if e.code != HIP_OUT_OF_MEMORY or all(len(r) == 1 for r in step.values()):
                             raise
-                        done = self.step({request: r[:1] for request, r in step.items()})
+                        step = {request: r[:1] for request, r in step.items()}
+                        self.masks(None)
+                        mask_rows(step, {})
+                        done = self.step(step)
                     # A request that has had its turn goes to the back.
                     for request, new in done.items():
                         if not took(request, new):
@@ -479,6 +671,7 @@ class Batch:
         except BaseException:  # an interrupt too: the requests are empty again
             for i in running:
                 native.lib().iris_batch_release(self._h, i)  # (refused after a failed pass)
+            native.lib().iris_batch_masks(self._h, None, 0, None, 0)
             raise
         if failed:
             first = min(failed)
