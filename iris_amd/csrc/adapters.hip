@@ -12,6 +12,7 @@
 // attn_tiles.h). Digit products of one weight 2^8s share an int32 accumulator.
 #include <algorithm>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 #include "attn_tiles.h"
@@ -34,16 +35,15 @@ struct AdapterShape {
     IrisAdapterPart parts[IRIS_ADAPTER_PARTS];
 };
 
-// Rows up to which a call takes the kernels of single rows.
-constexpr uint32_t FEW_ROWS = 48;
+// A call of up to so many rows, and rows times ranks, takes the kernels of single
+// rows: they read an adapter again for each row, but a row's work does not wait
+// for others'.
+constexpr uint32_t FEW_ROWS = 256, FEW_RANKS = 4096;
+__host__ __device__ __forceinline__ bool few(uint32_t rows, uint32_t max_rank) { return rows <= FEW_ROWS && rows * max_rank <= FEW_RANKS; }
 constexpr uint32_t TILE_ROWS = 32;
 constexpr uint32_t TILE_RANKS = 64;    // of A x a workgroup forms at a time: four 16-rank tiles
 constexpr uint32_t MAX_SPLITS = 16;    // pieces of the columns, each with sums of its own
 constexpr uint32_t CHUNK_OUTPUTS = 512;  // of a tile of rows that a workgroup forms
-
-// Workgroups that share the adapters of a tile of rows: most tiles have one or
-// two, those of short prompts many (2309 rows of 19 prompts: 151 us with one).
-constexpr uint32_t SLOT_GROUPS = 4;
 
 // A weight's two digits, and the weight from them.
 inline uint16_t digits_of(int16_t w) { return (uint16_t)(((w + 128) & ~255) | (w & 255)); }
@@ -113,9 +113,18 @@ __global__ __launch_bounds__(256) void expand_row_kernel(const IrisAdapterRows a
     int32_t v = a.y[(size_t)row * a.y_stride + column];
     if (e.rank) {
         const int32_t* tr = t + ((size_t)row * sh.part_count + part) * sh.max_rank;
-        const int16_t* w = e.b + (size_t)i * stride_of(e.rank);
+        const int32_t* w = (const int32_t*)(e.b + (size_t)i * stride_of(e.rank));
         int64_t sum = 0;
-        for (uint32_t j = 0; j < e.rank; j++) sum += (int64_t)weight_of((uint16_t)w[j]) * tr[j];
+#pragma unroll 2
+        for (uint32_t j = 0; j < e.rank; j += 8) {  // (the work space ends behind whole eights; weights there are zero)
+            const int4 d = load4(w + j / 2);
+            const uint32_t q[4] = {(uint32_t)d.x, (uint32_t)d.y, (uint32_t)d.z, (uint32_t)d.w};
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                sum += (int64_t)weight_of(q[c]) * tr[j + 2 * c];
+                sum += (int64_t)weight_of(q[c] >> 16) * tr[j + 2 * c + 1];
+            }
+        }
         v = dn::add_sat(v, rounded(sum, e.b_bits));
     }
     a.out[(size_t)row * a.out_stride + column] = v;
@@ -245,18 +254,18 @@ __device__ __forceinline__ bool shrink_steps(const IrisAdapterRows& a, uint32_t 
 // blockIdx.z which of the tile's adapters and which four rank tiles of them.
 // sums: [piece][row][part_count max_rank].
 __global__ __launch_bounds__(256, 2) void shrink_tile_kernel(const IrisAdapterRows a, const AdapterShape sh,
-                                                             const AdapterEntry* table, int64_t* sums) {
+                                                             const AdapterEntry* table, int64_t* sums, uint32_t slot_groups) {
     __shared__ int64_t s_sum[TILE_ROWS * (TILE_RANKS + 1)];
     __shared__ uint32_t s_wide;
     const uint32_t row0 = blockIdx.y * TILE_ROWS, tid = threadIdx.x, steps = (sh.cols + 63) / 64;
     const uint32_t per = (steps + gridDim.x - 1) / gridDim.x, step0 = min(blockIdx.x * per, steps), step1 = min(step0 + per, steps);
     const uint32_t width = sh.part_count * sh.max_rank;
-    const uint32_t turn = blockIdx.z % SLOT_GROUPS, rank_group = blockIdx.z / SLOT_GROUPS;
+    const uint32_t turn = blockIdx.z % slot_groups, rank_group = blockIdx.z / slot_groups;
     Tile t = tile_of(a, sh, row0, blockIdx.x == 0 && blockIdx.z == 0);
     for (uint32_t at = 0; t.pending; at++) {
         int32_t slot;
         const uint32_t rows = next_slot(t, slot);
-        if (at % SLOT_GROUPS != turn) continue;
+        if (at % slot_groups != turn) continue;
         const AdapterEntry* entry = table + (size_t)slot * sh.part_count;
         RankTile tile[4];
         uint32_t tiles = 0, skip = 4 * rank_group;
@@ -329,10 +338,37 @@ __device__ __forceinline__ void store_columns(int32_t* p, uint32_t step, uint32_
     if (count > 3) p[3 * (size_t)step] = v.w;
 }
 
-// y + sum / 2^bits from the sum's exact double, below 2^53.
-__device__ __forceinline__ int32_t added(int32_t y, double sum, double unit) {
-    const double u = fmin(fmax(rint(sum * unit), -2147483648.0), 2147483647.0);
-    return (int32_t)fmin(fmax((double)y + u, -2147483648.0), 2147483647.0);
+// u of output c of a lane's four from its accumulators; unit = 2^-bits. The
+// vector units' part of a tile, so few operations: neighbouring accumulators
+// share an int32 where they fit (NARROW: up to three steps, 2^29 a step), powers
+// of two scale exactly, and an addend of 1.5 2^52 rounds to even.
+enum class Sums { NARROW, LONG, WIDE };
+template <Sums KIND, int SUMS>
+__device__ __forceinline__ int32_t output_sum(const v4i (&acc)[SUMS], int c, uint32_t bits, double unit) {
+    if constexpr (KIND != Sums::WIDE) {
+        // Below 2^23 2^15 256 = 2^46: exact in double.
+        double sum;
+        if constexpr (KIND == Sums::NARROW) {
+            const int32_t low = acc[0][c] + (acc[1][c] << 8), high = acc[2][c] + (acc[3][c] << 8);
+            sum = fma((double)high, 65536.0 * unit, (double)low * unit);
+        } else {
+            sum = (double)acc[3][c];
+#pragma unroll
+            for (int d = 2; d >= 0; d--) sum = fma(sum, 256.0, (double)acc[d][c]);
+            sum *= unit;
+        }
+        return (int32_t)(uint32_t)softmax_bits(fmin(fmax(sum, -2147483648.0), 2147483647.0) + SOFTMAX_ROUND);
+    } else {
+        int64_t sum = 0;
+#pragma unroll
+        for (int d = SUMS - 1; d >= 0; d--) sum = (sum << 8) + acc[d][c];
+        return rounded(sum, bits);
+    }
+}
+
+// The kind of an adapter's sums, its rank and whether its t is wide known.
+__device__ __forceinline__ Sums kind_of(uint32_t rank, bool wide) {
+    return wide ? Sums::WIDE : rank <= 192 ? Sums::NARROW : Sums::LONG;
 }
 
 // The digits of t of a tile's rows as operands of the matrix cores, in LDS:
@@ -343,6 +379,52 @@ struct Operand {
 constexpr uint32_t DIGIT_PLANES = 5;
 __device__ __forceinline__ uint32_t operand_at(uint32_t step, uint32_t g, uint32_t digit) { return (step * 2 + g) * DIGIT_PLANES + digit; }
 
+// t of the rows of one adapter's part, from its sums by pieces, as operands in
+// s_digits; by a workgroup of 256. What it returns tells whether a fourth digit
+// was needed (above bit 23).
+__device__ __forceinline__ uint32_t stage_digits(const IrisAdapterRows& a, const AdapterEntry& e, const int64_t* sums, uint32_t width,
+                                                 uint32_t splits, uint32_t row0, uint32_t rows, Operand* s_digits) {
+    const uint32_t steps = (e.rank + 63) / 64;
+    uint32_t seen = 0;
+    // Four values of a row a thread and turn (zeros past the rank and for
+    // others' rows).
+    for (uint32_t i = threadIdx.x; i < TILE_ROWS * steps * 16; i += 256) {
+        const uint32_t r = i / (steps * 16), j = i % (steps * 16) * 4;
+        int32_t v[4] = {};
+        if (rows >> r & 1) {
+            const int64_t* from = sums + (size_t)(row0 + r) * width + min(j, e.rank - 1);
+            int64_t sum[4] = {};
+            // Several pieces' loads at once; a value past the rank is the last again.
+            const uint32_t last = e.rank - 1 - min(j, e.rank - 1);
+            const size_t piece = (size_t)a.rows * width;
+            auto add = [&](auto count, uint32_t q) {
+                int64_t x[count][4];
+#pragma unroll
+                for (uint32_t k = 0; k < count; k++)
+#pragma unroll
+                    for (uint32_t c = 0; c < 4; c++) x[k][c] = from[min(q + k, splits - 1) * piece + min(c, last)];
+#pragma unroll
+                for (uint32_t k = 0; k < count; k++)
+#pragma unroll
+                    for (uint32_t c = 0; c < 4; c++) sum[c] += q + k < splits ? x[k][c] : 0;
+            };
+            if (splits <= 2) add(std::integral_constant<uint32_t, 2>{}, 0);
+            else
+                for (uint32_t q = 0; q < splits; q += 4) add(std::integral_constant<uint32_t, 4>{}, q);
+#pragma unroll
+            for (uint32_t c = 0; c < 4; c++) v[c] = j + c < e.rank ? rounded(sum[c], e.a_bits) : 0;
+        }
+        const int4 x = make_int4(v[0], v[1], v[2], v[3]);
+        uint32_t plane[4];
+        split4(x, plane, seen);
+        const uint32_t lane = (j % 64 / 16) * 16 + r % 16, c = j % 16 / 4;
+#pragma unroll
+        for (uint32_t d = 0; d < DIGIT_PLANES; d++)
+            ((uint32_t*)&s_digits[operand_at(j / 64, r / 16, d)].lane[lane])[c] = d < 4 ? plane[d] : fifth4(x);
+    }
+    return seen;
+}
+
 // Sixteen weights of a row of B from k on. The rank's padding may end at 8 of
 // them: those behind it are another row's.
 __device__ __forceinline__ void load_weights(const int16_t* w, uint32_t k, uint32_t stride, int4& b0, int4& b1) {
@@ -352,14 +434,13 @@ __device__ __forceinline__ void load_weights(const int16_t* w, uint32_t k, uint3
 
 // Tiles of 16 outputs for the rows of one adapter, into out. WIDE: values past
 // three digits. One step's operands stay in registers where they are all (ONE).
-template <bool VEC, bool WIDE, bool ONE>
+template <bool VEC, Sums KIND, bool ONE>
 __device__ __forceinline__ void expand_outputs(const IrisAdapterRows& a, const IrisAdapterPart& p, const AdapterEntry& e,
                                                const Operand* s_digits, const Tile& t, uint32_t row0, uint32_t rows, uint32_t i0,
                                                uint32_t i1) {
-    constexpr int SUMS = WIDE ? 6 : 4;
+    constexpr int SUMS = KIND == Sums::WIDE ? 6 : 4, DIGITS = KIND == Sums::WIDE ? 5 : 3;
     const uint32_t n = t.lane & 15, group = t.lane >> 4, steps = ONE ? 1 : (e.rank + 63) / 64, b_stride = stride_of(e.rank);
     const double unit = ldexp(1.0, -(int)e.b_bits);
-    constexpr int DIGITS = WIDE ? 5 : 3;
     v4i kept[2][DIGITS];
     if (ONE) {
 #pragma unroll
@@ -410,20 +491,7 @@ __device__ __forceinline__ void expand_outputs(const IrisAdapterRows& a, const I
             const int32_t old[4] = {was[g].x, was[g].y, was[g].z, was[g].w};
             int32_t out[4];
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                if constexpr (!WIDE) {
-                    // Below 2^23 2^15 256 = 2^46: exact.
-                    double sum = (double)acc[g][3][c];
-#pragma unroll
-                    for (int d = 2; d >= 0; d--) sum = fma(sum, 256.0, (double)acc[g][d][c]);
-                    out[c] = added(old[c], sum, unit);
-                } else {
-                    int64_t sum = 0;
-#pragma unroll
-                    for (int d = SUMS - 1; d >= 0; d--) sum = (sum << 8) + acc[g][d][c];
-                    out[c] = dn::add_sat(old[c], rounded(sum, e.b_bits));
-                }
-            }
+            for (int c = 0; c < 4; c++) out[c] = __builtin_elementwise_add_sat(old[c], output_sum<KIND>(acc[g], c, e.b_bits, unit));
             if (rows >> r & 1)
                 store_columns<VEC>(a.out + (size_t)(row0 + r) * a.out_stride + p.first + (size_t)first * p.step, p.step, count,
                                    make_int4(out[0], out[1], out[2], out[3]));
@@ -436,10 +504,10 @@ __device__ __forceinline__ void expand_outputs(const IrisAdapterRows& a, const I
 // steps of max_rank.
 template <bool VEC>
 __global__ __launch_bounds__(256) void expand_tile_kernel(const IrisAdapterRows a, const AdapterShape sh, const AdapterEntry* table,
-                                                          const int64_t* sums, uint32_t splits) {
+                                                          const int64_t* sums, uint32_t splits, uint32_t slot_groups) {
     extern __shared__ Operand s_digits[];
     __shared__ uint32_t s_wide;
-    const uint32_t row0 = blockIdx.y * TILE_ROWS, tid = threadIdx.x, part = blockIdx.z / SLOT_GROUPS, turn = blockIdx.z % SLOT_GROUPS;
+    const uint32_t row0 = blockIdx.y * TILE_ROWS, tid = threadIdx.x, part = blockIdx.z / slot_groups, turn = blockIdx.z % slot_groups;
     const IrisAdapterPart p = sh.parts[part];
     const uint32_t i0 = blockIdx.x * CHUNK_OUTPUTS, i1 = min(i0 + CHUNK_OUTPUTS, p.rows);
     if (i0 >= p.rows) return;
@@ -450,43 +518,22 @@ __global__ __launch_bounds__(256) void expand_tile_kernel(const IrisAdapterRows 
     for (uint32_t at = 0; t.pending; at++) {
         int32_t slot;
         const uint32_t rows = next_slot(t, slot);
-        if (at % SLOT_GROUPS != turn && !copies) continue;
+        if (at % slot_groups != turn && !copies) continue;
         const AdapterEntry e = table[(size_t)slot * sh.part_count + part];
         if (!e.rank) copied |= rows;
-        if (!e.rank || at % SLOT_GROUPS != turn) continue;
+        if (!e.rank || at % slot_groups != turn) continue;
         const uint32_t steps = (e.rank + 63) / 64;
         __syncthreads();  // the adapter before is done with the operands
         if (tid == 0) s_wide = 0;
         __syncthreads();
-        uint32_t seen = 0;
-        // Four values of a row a thread and turn (zeros past the rank and for
-        // others' rows).
-        for (uint32_t i = tid; i < TILE_ROWS * steps * 16; i += 256) {
-            const uint32_t r = i / (steps * 16), j = i % (steps * 16) * 4;
-            int32_t v[4] = {};
-            if (rows >> r & 1) {
-                const int64_t* from = sums + (size_t)(row0 + r) * width + part * sh.max_rank + j;
-                int64_t sum[4] = {};
-                for (uint32_t q = 0; q < splits; q++)
-#pragma unroll
-                    for (uint32_t c = 0; c < 4; c++)
-                        if (j + c < e.rank) sum[c] += from[(size_t)q * a.rows * width + c];
-#pragma unroll
-                for (int c = 0; c < 4; c++) v[c] = rounded(sum[c], e.a_bits);
-            }
-            const int4 x = make_int4(v[0], v[1], v[2], v[3]);
-            uint32_t plane[4];
-            split4(x, plane, seen);
-            const uint32_t lane = (j % 64 / 16) * 16 + r % 16, c = j % 16 / 4;
-#pragma unroll
-            for (uint32_t d = 0; d < DIGIT_PLANES; d++)
-                ((uint32_t*)&s_digits[operand_at(j / 64, r / 16, d)].lane[lane])[c] = d < 4 ? plane[d] : fifth4(x);
-        }
+        const uint32_t seen = stage_digits(a, e, sums + part * sh.max_rank, width, splits, row0, rows, s_digits);
         if (seen >> 24) s_wide = 1;
         __syncthreads();
-        if (s_wide) expand_outputs<VEC, true, false>(a, p, e, s_digits, t, row0, rows, i0, i1);
-        else if (steps == 1) expand_outputs<VEC, false, true>(a, p, e, s_digits, t, row0, rows, i0, i1);
-        else expand_outputs<VEC, false, false>(a, p, e, s_digits, t, row0, rows, i0, i1);
+        const Sums kind = kind_of(e.rank, s_wide != 0);
+        if (kind == Sums::WIDE) expand_outputs<VEC, Sums::WIDE, false>(a, p, e, s_digits, t, row0, rows, i0, i1);
+        else if (kind == Sums::LONG) expand_outputs<VEC, Sums::LONG, false>(a, p, e, s_digits, t, row0, rows, i0, i1);
+        else if (steps == 1) expand_outputs<VEC, Sums::NARROW, true>(a, p, e, s_digits, t, row0, rows, i0, i1);
+        else expand_outputs<VEC, Sums::NARROW, false>(a, p, e, s_digits, t, row0, rows, i0, i1);
     }
     if (!copies) return;
     for (uint32_t r = t.wave; r < TILE_ROWS && row0 + r < a.rows; r += 4) {
@@ -500,8 +547,114 @@ __global__ __launch_bounds__(256) void expand_tile_kernel(const IrisAdapterRows 
     }
 }
 
+// u of four outputs of both row groups, 16 outputs a wave from output i on.
+template <Sums KIND>
+__device__ __forceinline__ void tile_sums(const AdapterEntry& e, const IrisAdapterPart& p, const Operand* s_digits, const Tile& t,
+                                          uint32_t i, int32_t (&u)[2][4]) {
+    constexpr int SUMS = KIND == Sums::WIDE ? 6 : 4, DIGITS = KIND == Sums::WIDE ? 5 : 3;
+    const uint32_t n = t.lane & 15, group = t.lane >> 4, steps = (e.rank + 63) / 64, b_stride = stride_of(e.rank);
+    const int16_t* w = e.b + (size_t)min(i + n, p.rows - 1) * b_stride;
+    const double unit = ldexp(1.0, -(int)e.b_bits);
+    v4i acc[2][SUMS] = {};
+#pragma unroll 1
+    for (uint32_t step = 0; step < steps; step++) {
+        int4 b0, b1;
+        load_weights(w, 64 * step + 16 * group, b_stride, b0, b1);
+        v4i low, high;
+        split_weights(b0, b1, low, high);
+#pragma unroll
+        for (int g = 0; g < 2; g++)
+#pragma unroll
+            for (int d = 0; d < DIGITS; d++) {
+                const v4i digit = s_digits[operand_at(step, g, d)].lane[t.lane];
+                acc[g][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(low, digit, acc[g][d], 0, 0, 0);
+                acc[g][d + 1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(high, digit, acc[g][d + 1], 0, 0, 0);
+            }
+    }
+#pragma unroll
+    for (int g = 0; g < 2; g++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) u[g][c] = output_sum<KIND>(acc[g], c, e.b_bits, unit);
+}
+
+// Two parts whose outputs take turns (gate and up): workgroup as
+// expand_tile_kernel's, of both parts, so that a lane's four outputs of each are
+// eight neighbours of a row. (Part by part every fourth byte of a line would be
+// written at a time: 600 rows of 2 x 14336 at rank 16, 129 us.) LDS: operands of
+// both.
+__global__ __launch_bounds__(256) void expand_pair_kernel(const IrisAdapterRows a, const AdapterShape sh, const AdapterEntry* table,
+                                                          const int64_t* sums, uint32_t splits, uint32_t slot_groups, uint32_t low) {
+    extern __shared__ Operand s_digits[];
+    __shared__ uint32_t s_wide;
+    const uint32_t row0 = blockIdx.y * TILE_ROWS, tid = threadIdx.x, turn = blockIdx.z;
+    const IrisAdapterPart p = sh.parts[low];  // the part of the even columns
+    const uint32_t i0 = blockIdx.x * CHUNK_OUTPUTS, i1 = min(i0 + CHUNK_OUTPUTS, p.rows), width = sh.part_count * sh.max_rank;
+    Operand* s_odd = s_digits + operand_at((sh.max_rank + 63) / 64, 0, 0);
+    Tile t = tile_of(a, sh, row0, false);
+    const uint32_t n = t.lane & 15, group = t.lane >> 4;
+    uint32_t copied = ~t.pending;  // rows that no adapter changes
+    const bool copies = turn == 0 && a.out != a.y;
+    for (uint32_t at = 0; t.pending; at++) {
+        int32_t slot;
+        const uint32_t rows = next_slot(t, slot);
+        if (at % slot_groups != turn && !copies) continue;
+        const AdapterEntry even = table[(size_t)slot * 2 + low], odd = table[(size_t)slot * 2 + 1 - low];
+        const bool none = !even.rank && !odd.rank;
+        if (none) copied |= rows;
+        if (none || at % slot_groups != turn) continue;
+        __syncthreads();  // the adapter before is done with the operands
+        if (tid == 0) s_wide = 0;
+        __syncthreads();
+        const uint32_t seen = stage_digits(a, even, sums + low * sh.max_rank, width, splits, row0, rows, s_digits) |
+                              stage_digits(a, odd, sums + (1 - low) * sh.max_rank, width, splits, row0, rows, s_odd);
+        if (seen >> 24) s_wide = 1;
+        __syncthreads();
+        const Sums kind = kind_of(max(even.rank, odd.rank), s_wide != 0);
+#pragma unroll 1
+        for (uint32_t i = i0 + 16 * t.wave; i < i1; i += 64) {
+            const uint32_t first = i + 4 * group;  // (fours are whole)
+            int4 y[2][2];
+#pragma unroll
+            for (int g = 0; g < 2; g++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    if (first < i1 && (rows >> (16 * g + n) & 1))
+                        y[g][h] = load4(a.y + (size_t)(row0 + 16 * g + n) * a.y_stride + p.first + 2 * first + 4 * h);
+            int32_t u[2][4], v[2][4];
+            if (kind == Sums::NARROW) {
+                tile_sums<Sums::NARROW>(even, p, s_digits, t, i, u), tile_sums<Sums::NARROW>(odd, p, s_odd, t, i, v);
+            } else if (kind == Sums::LONG) {
+                tile_sums<Sums::LONG>(even, p, s_digits, t, i, u), tile_sums<Sums::LONG>(odd, p, s_odd, t, i, v);
+            } else {
+                tile_sums<Sums::WIDE>(even, p, s_digits, t, i, u), tile_sums<Sums::WIDE>(odd, p, s_odd, t, i, v);
+            }
+#pragma unroll
+            for (int g = 0; g < 2; g++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    if (first < i1 && (rows >> (16 * g + n) & 1))
+                        *(int4*)(a.out + (size_t)(row0 + 16 * g + n) * a.out_stride + p.first + 2 * first + 4 * h) =
+                            make_int4(__builtin_elementwise_add_sat(y[g][h].x, u[g][2 * h]), __builtin_elementwise_add_sat(y[g][h].y, v[g][2 * h]),
+                                      __builtin_elementwise_add_sat(y[g][h].z, u[g][2 * h + 1]),
+                                      __builtin_elementwise_add_sat(y[g][h].w, v[g][2 * h + 1]));
+        }
+    }
+    if (!copies) return;
+    for (uint32_t r = t.wave; r < TILE_ROWS && row0 + r < a.rows; r += 4) {
+        if (!(copied >> r & 1)) continue;
+        for (uint32_t i = 2 * i0 + 4 * t.lane; i < 2 * i1; i += 256)
+            *(int4*)(a.out + (size_t)(row0 + r) * a.out_stride + p.first + i) = load4(a.y + (size_t)(row0 + r) * a.y_stride + p.first + i);
+    }
+}
+
 // Workgroups that share the rank tiles of an adapter.
 uint32_t rank_groups(const AdapterShape& s) { return (s.part_count * ((s.max_rank + 15) / 16) + 3) / 4; }
+
+// Workgroups that share the adapters of a tile of rows: most tiles of prompts have
+// one or two, those of short prompts or single tokens up to 32, and where tiles
+// are few there is room for a workgroup each. (2309 rows of 19 prompts, sums of
+// A x: 63 us with one, 42 with four.)
+uint32_t slot_groups_of(uint32_t tiles) { return tiles <= 8 ? 32 : tiles <= 32 ? 16 : tiles <= 64 ? 8 : 4; }
 
 // Pieces of the columns for a call of tiles: enough workgroups for the card,
 // each with a step for every wave.
@@ -516,7 +669,7 @@ uint32_t splits_of(const AdapterShape& s, uint32_t rows) {
 // tiles.
 uint64_t space_of(const AdapterShape& s, uint32_t rows) {
     const uint64_t values = (uint64_t)rows * s.part_count * s.max_rank;
-    return rows <= FEW_ROWS ? values * 4 : values * splits_of(s, rows) * 8;
+    return few(rows, s.max_rank) ? values * 4 + 32 : values * splits_of(s, rows) * 8;
 }
 
 }  // namespace
@@ -537,7 +690,7 @@ uint64_t iris_adapters_space(uint32_t cols, uint32_t part_count, uint32_t max_ra
     // What any number of rows up to these takes: whole tiles take the most.
     uint64_t bytes = space_of(s, rows);
     for (uint32_t n = rows / TILE_ROWS * TILE_ROWS; n; n -= TILE_ROWS) bytes = std::max(bytes, space_of(s, n));
-    return std::max(bytes, space_of(s, std::min(rows, FEW_ROWS)));
+    return std::max(bytes, space_of(s, std::min(std::min(rows, FEW_ROWS), std::max(FEW_RANKS / max_rank, 1u))));
 }
 
 extern "C" {
@@ -655,17 +808,32 @@ int iris_adapters_apply(const IrisAdapterBank* b, const IrisAdapterRows* a, void
     if (a->rows > 65535) return IRIS_E_RANGE;
     if (space_bytes < space_of(s, a->rows)) return IRIS_E_RANGE;
     hipStream_t st = (hipStream_t)stream;
-    if (a->rows > FEW_ROWS) {
+    if (!few(a->rows, s.max_rank)) {
         const uint32_t tiles = (a->rows + TILE_ROWS - 1) / TILE_ROWS, splits = splits_of(s, a->rows);
         const size_t lds = (s.max_rank + 63) / 64 * 2 * DIGIT_PLANES * sizeof(Operand);
         // Sixteen bytes of a row at a time where every part allows it.
-        bool vec = !misaligned(a->y) && !misaligned(a->out) && a->y_stride % 4 == 0 && a->out_stride % 4 == 0;
+        const bool aligned = !misaligned(a->y) && !misaligned(a->out) && a->y_stride % 4 == 0 && a->out_stride % 4 == 0;
+        bool vec = aligned;
         for (uint32_t p = 0; p < s.part_count; p++) vec = vec && s.parts[p].step == 1 && s.parts[p].first % 4 == 0 && s.parts[p].rows % 4 == 0;
-        const dim3 grid((b->most_rows + CHUNK_OUTPUTS - 1) / CHUNK_OUTPUTS, tiles, s.part_count * SLOT_GROUPS);
-        hipLaunchKernelGGL(shrink_tile_kernel, dim3(splits, tiles, rank_groups(s) * SLOT_GROUPS), dim3(256), 0, st, *a, s, b->table,
-                           (int64_t*)space);
-        if (vec) hipLaunchKernelGGL(expand_tile_kernel<true>, grid, dim3(256), lds, st, *a, s, b->table, (const int64_t*)space, splits);
-        else hipLaunchKernelGGL(expand_tile_kernel<false>, grid, dim3(256), lds, st, *a, s, b->table, (const int64_t*)space, splits);
+        // Two parts in turn whose fours of both are eight aligned neighbours.
+        const uint32_t low = s.part_count == 2 && s.parts[1].first < s.parts[0].first;
+        const bool pair = s.part_count == 2 && s.parts[0].step == 2 && s.parts[1].step == 2 && s.parts[0].rows == s.parts[1].rows &&
+                          s.parts[1 - low].first == s.parts[low].first + 1 && s.parts[low].first % 4 == 0 && s.parts[0].rows % 4 == 0 &&
+                          aligned;
+        const uint32_t groups = slot_groups_of(tiles);
+        const dim3 grid((b->most_rows + CHUNK_OUTPUTS - 1) / CHUNK_OUTPUTS, tiles, (pair ? 1 : s.part_count) * groups);
+        hipLaunchKernelGGL(shrink_tile_kernel, dim3(splits, tiles, rank_groups(s) * groups), dim3(256), 0, st, *a, s, b->table,
+                           (int64_t*)space, groups);
+        const int64_t* sums = (const int64_t*)space;
+        if (pair) {
+            const hipError_t limit = paged_lds_limit((const void*)expand_pair_kernel, 2 * lds);
+            if (limit != hipSuccess) return (int)limit;
+            hipLaunchKernelGGL(expand_pair_kernel, grid, dim3(256), 2 * lds, st, *a, s, b->table, sums, splits, groups, low);
+        } else if (vec) {
+            hipLaunchKernelGGL(expand_tile_kernel<true>, grid, dim3(256), lds, st, *a, s, b->table, sums, splits, groups);
+        } else {
+            hipLaunchKernelGGL(expand_tile_kernel<false>, grid, dim3(256), lds, st, *a, s, b->table, sums, splits, groups);
+        }
         return (int)hipGetLastError();
     }
     hipLaunchKernelGGL(shrink_row_kernel, dim3(s.part_count * s.max_rank, a->rows), dim3(256), 0, st, *a, s, b->table,

@@ -587,7 +587,7 @@ class Batch:
             if o.rule is not None or o.biases:
                 self.rule(request, o.rule, o.biases)
             if o.drawing is not None:
-                self.drawing(request, o.drawing, o.numbers, prompts[p].size - 1)
+                self.drawing(request, o.drawing, np.asarray(o.numbers)[:tokens], prompts[p].size - 1)
 
         def mask_rows(rows, parents):
             """The masks of the pass over {request: ids to come}."""

@@ -15,6 +15,8 @@ MARGIN = 1 << 14
 
 QKV = [(64, 0, 1), (32, 64, 1), (32, 96, 1)]
 GATED = [(150, 0, 2), (150, 1, 2)]
+PAIRS = [(152, 0, 2), (152, 1, 2)]
+TURNED = [(60, 5, 2), (60, 4, 2)]
 ODD = [(77, 0, 1), (131, 80, 1)]
 ONE = [(40, 3, 1)]
 
@@ -102,13 +104,15 @@ class Call:
             assert bool((t[:MARGIN] == v).all()) and bool((t[-MARGIN:] == v).all())
 
 
-@pytest.mark.parametrize("rows", [1, 2, 5, 15, 16, 17, 33, 70, 129, 300])
-@pytest.mark.parametrize("parts", [QKV, GATED, ODD, ONE], ids=["qkv", "gated", "odd", "one"])
+@pytest.mark.parametrize("rows", [1, 2, 5, 15, 16, 17, 33, 70, 129, 256, 257, 300, 417])
+@pytest.mark.parametrize("parts", [QKV, GATED, PAIRS, TURNED, ODD, ONE], ids=["qkv", "gated", "pairs", "turned", "odd", "one"])
 def test_rows_of_many_adapters(rows, parts):
     rng = np.random.default_rng(rows)
     n = len(parts)
     ranks = [[16] * n, [5] * n, [1] * n, [33] + [8] * (n - 1), [40] + [0] * (n - 1)]
     Call(rng, 128, parts, ranks, rows, rng.integers(-1, 5, rows)).check()
+    Call(rng, 128, parts, [[0] * (n - 1) + [7], [70] * n], rows, rng.integers(-1, 2, rows), in_place=rows % 2 == 0,
+         extra=(4, 4, 8)).check()
 
 
 @pytest.mark.parametrize("in_place", [False, True])
@@ -116,8 +120,10 @@ def test_a_tile_of_many_adapters(in_place):
     # Every row its own adapter, a few without, some parts empty.
     rng = np.random.default_rng(21)
     ranks = [[int(rng.integers(0, 20)) for _ in QKV] for _ in range(90)]
-    Call(rng, 160, QKV, ranks, 100, np.arange(100) % 91 - 1, in_place=in_place).check()
-    Call(rng, 160, QKV, ranks, 100, rng.integers(-1, 7, 100), in_place=in_place, kind="mixed").check()
+    for rows in (100, 300):
+        Call(rng, 160, QKV, ranks, rows, np.arange(rows) % 91 - 1, in_place=in_place).check()
+        Call(rng, 160, QKV, ranks, rows, rng.integers(-1, 7, rows), in_place=in_place, kind="mixed").check()
+        Call(rng, 160, PAIRS, [r[:2] for r in ranks], rows, np.arange(rows) % 91 - 1, in_place=in_place).check()
 
 
 @pytest.mark.parametrize("rank", [1, 2, 7, 8, 9, 15, 16, 17, 31, 32, 33, 63, 64, 65, 100, 128, 129, 255, 256])
@@ -128,7 +134,7 @@ def test_ranks(rank, rows):
 
 
 @pytest.mark.parametrize("cols", [32, 64, 96, 224, 416, 1024, 2080, 14336, 65504])
-@pytest.mark.parametrize("rows", [1, 3, 35, 64])
+@pytest.mark.parametrize("rows", [1, 3, 35, 260])
 def test_columns(cols, rows):
     rng = np.random.default_rng(cols)
     Call(rng, cols, ODD, [[9, 16], [16, 3]], rows, np.arange(rows) % 2).check()
@@ -137,26 +143,28 @@ def test_columns(cols, rows):
 @pytest.mark.parametrize("kind", ["normal", "wide", "mixed", "sharp", "ends", "same"])
 @pytest.mark.parametrize("weights", ["normal", "ends", "top", "uniform"])
 @pytest.mark.parametrize("rows", [3, 40, 83])
-def test_values(kind, weights, rows):
+@pytest.mark.parametrize("parts", [QKV, PAIRS], ids=["qkv", "pairs"])
+def test_values(kind, weights, rows, parts):
     # Every digit of the values and both clamps.
     rng = np.random.default_rng(5)
     for bits in ((18, 16), (0, 0), (40, 40), (1, 33)):
-        Call(rng, 160, QKV, [[20, 3, 16], [16, 16, 70]], rows, rng.integers(-1, 2, rows), kind=kind, weights=weights,
-             bits=bits, y_kind=kind).check()
+        for ranks in ([[20, 3, 16], [16, 16, 70]], [[8, 200, 1], [130, 256, 9]]):
+            Call(rng, 160, parts, [r[:len(parts)] for r in ranks], rows, rng.integers(-1, 2, rows), kind=kind, weights=weights,
+                 bits=bits, y_kind=kind).check()
 
 
 def test_the_largest_sums():
     # 65504 products of 2^31 and 32639, without and with shifts, of either sign.
     rng = np.random.default_rng(1)
     for bits in ((0, 0), (40, 40), (38, 20)):
-        for rows in (2, 40, 66):
+        for rows in (2, 40, 261):
             c = Call(rng, 65504, ONE, [[3]], rows, [0] * rows, weights="top", bits=bits)
             c.x[:] = np.where(np.arange(rows) % 2, -2 ** 31, 2 ** 31 - 1)[:, None]
             c.d_x.copy_(Call.strided(c.x, 65504))
             c.check()
 
 
-@pytest.mark.parametrize("rows", [41, 95])
+@pytest.mark.parametrize("rows", [41, 95, 301])
 def test_ties_round_to_even(rows):
     # One column of one, weights of halves: sums at every tie of two bits.
     c = Call(np.random.default_rng(0), 32, ONE, [[1]], rows, [0] * rows, bits=(2, 1))
@@ -179,7 +187,7 @@ def test_strides_and_places(rows, in_place):
         Call(rng, 128, ODD, [[16, 7], [0, 40]], rows, rng.integers(-1, 2, rows), extra=extra, in_place=in_place).check()
 
 
-@pytest.mark.parametrize("rows", [1, 20, 100])
+@pytest.mark.parametrize("rows", [1, 20, 300])
 @pytest.mark.parametrize("in_place", [False, True])
 def test_no_row_has_an_adapter(rows, in_place):
     rng = np.random.default_rng(2)
@@ -187,7 +195,7 @@ def test_no_row_has_an_adapter(rows, in_place):
     Call(rng, 64, QKV, [[0, 0, 0], [4, 4, 4]], rows, [0] * rows, in_place=in_place).check()
 
 
-@pytest.mark.parametrize("rows", [3, 40, 90])
+@pytest.mark.parametrize("rows", [3, 40, 290])
 def test_slots_outside_the_bank_are_reported(rows):
     rng = np.random.default_rng(3)
     for bad in (-2, 2, 65535, 2 ** 31 - 1, -2 ** 31):
@@ -196,7 +204,7 @@ def test_slots_outside_the_bank_are_reported(rows):
         Call(rng, 64, QKV, [[4, 4, 4], [9, 2, 0]], rows, slots).check(status=-1)
 
 
-@pytest.mark.parametrize("rows", [37, 70])
+@pytest.mark.parametrize("rows", [37, 270])
 def test_slots_load_again_and_empty(rows):
     rng = np.random.default_rng(8)
     c = Call(rng, 96, QKV, [[16, 16, 16], [8, 8, 8]], rows, rng.integers(-1, 2, rows))
@@ -246,11 +254,11 @@ def test_refused_calls_run_nothing():
 def test_rows_do_not_depend_on_the_rows_beside_them():
     rng = np.random.default_rng(6)
     ranks = [[16, 8, 8], [3, 40, 0]]
-    c = Call(rng, 256, QKV, ranks, 90, rng.integers(-1, 2, 90))
+    c = Call(rng, 256, QKV, ranks, 290, rng.integers(-1, 2, 290))
     c.fill()
     c.run()
     whole = c.out.cpu().numpy()
-    for r in (0, 17, 89):
+    for r in (0, 17, 289):
         d = adapters.AdapterRows.from_buffer_copy(c.d)
         d.x, d.y, d.out = (v + 4 * r * s for v, s in ((d.x, d.x_stride), (d.y, d.y_stride), (d.out, d.out_stride)))
         d.slots, d.rows = d.slots + 4 * r, 1
@@ -259,7 +267,7 @@ def test_rows_do_not_depend_on_the_rows_beside_them():
         assert np.array_equal(c.out.cpu().numpy()[r], whole[r])
 
 
-@pytest.mark.parametrize("rows", [2, 60])
+@pytest.mark.parametrize("rows", [2, 60, 270])
 def test_captured_calls_and_other_streams(rows):
     rng = np.random.default_rng(7)
     c = Call(rng, 224, GATED, [[16, 8], [5, 33]], rows, rng.integers(-1, 2, rows))

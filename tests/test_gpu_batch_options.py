@@ -134,12 +134,12 @@ def test_adapters_of_several_requests(name, names):
 
 
 def test_adapters_of_many_rows():
-    # Past the rows of the single-row kernels, and one row alone.
+    # Past the rows and ranks of the single-row kernels, and one row alone.
     name = "mistral rows"
     rng = np.random.default_rng(8)
-    adapters = [some_adapter(rng, made(name).model, ALL, r) for r in (20, 3)]
-    run_and_check(name, [60, 30], 2, [RequestOptions(adapter=1), RequestOptions(adapter=0)], adapters, max_rank=20, drafts=False)
-    run_and_check(name, [1], 3, [RequestOptions(adapter=1)], adapters, max_rank=20)
+    adapters = [some_adapter(rng, made(name).model, ALL, r) for r in (40, 3)]
+    run_and_check(name, [60, 30], 2, [RequestOptions(adapter=1), RequestOptions(adapter=0)], adapters, max_rank=64, drafts=False)
+    run_and_check(name, [1], 3, [RequestOptions(adapter=1)], adapters, max_rank=64)
 
 
 RULE = logits.TokenRule(repetition=int(1.4 * ONE), frequency=ONE // 3, presence=ONE // 4, window=0)
