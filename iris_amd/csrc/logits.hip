@@ -227,7 +227,7 @@ __global__ __launch_bounds__(256) void rules_kernel(const IrisLogitsRules a, con
 // they can lie. Of long rows a launch in between gathers those, by pieces: one
 // workgroup has too little in flight (256000 tokens: 30 us).
 
-constexpr uint32_t BUCKETS = 1024;
+constexpr uint32_t BUCKETS = 2048;
 constexpr uint32_t PICK_THREADS = 512;
 constexpr uint32_t LIST = 512;        // tokens put in order at a time
 constexpr uint32_t GATHER = 4096;     // tokens held in LDS
@@ -312,8 +312,8 @@ __device__ __forceinline__ RowDraw row_draw(const IrisLogitsDraw& a, uint32_t ro
     d.end = min((bound + twice - 1) / twice, 1ull << 32);
     // The least shift with (end - 1) >> shift below BUCKETS.
     const uint32_t bits = 64 - __builtin_clzll(d.end - 1 | 1);
-    d.shift = bits > 10 ? bits - 10 : 0;
-    static_assert(BUCKETS == 1u << 10, "bits of a bucket");
+    d.shift = bits > 11 ? bits - 11 : 0;
+    static_assert(BUCKETS == 1u << 11, "bits of a bucket");
     return d;
 }
 
@@ -408,7 +408,7 @@ struct PickSpace : BucketSpace {
             uint64_t token[GATHER];  // as found, then in order
             uint64_t key[GATHER], upto[GATHER];
             uint32_t part[GATHER];   // parts of the buckets: counts, then first places
-            uint32_t behind[GATHER];  // of a token as found: those before it in its part
+            uint16_t behind[GATHER];  // of a token as found: those before it in its part
         };
         // or those of one bucket at a time: its parts, and the tokens of the last.
         struct {
@@ -745,7 +745,7 @@ __global__ __launch_bounds__(PICK_THREADS) void draw_pick_kernel(const IrisLogit
     uint32_t held, buckets;
     runs.find(p.d, number, s, held, buckets);
     auto before = [&](uint32_t bucket) { return bucket ? s.sum[bucket - 1] : 0; };
-    static_assert(Runs<PICK_THREADS>::OWN == 2, "two buckets a thread");
+    constexpr uint32_t MINE = Runs<PICK_THREADS>::OWN;
     const uint32_t n = runs.wanted_tokens;
     const bool gathered = n <= GATHER;
     uint32_t have = 0;  // the gathered (all n)
@@ -753,11 +753,15 @@ __global__ __launch_bounds__(PICK_THREADS) void draw_pick_kernel(const IrisLogit
     // The gathered tokens in order: s.token, and the running sums of their weights,
     // s.upto.
     if (gathered) {
-        // first0, first1: each of the thread's two buckets' first place.
-        const bool has0 = runs.wanted(2 * tid), has1 = runs.wanted(2 * tid + 1);
-        const uint32_t first1 = held - (has1 ? runs.tokens[1] : 0), first0 = first1 - (has0 ? runs.tokens[0] : 0);
-        s.place_of[2 * tid] = (buckets - has1 - has0) << 16 | first0;
-        s.place_of[2 * tid + 1] = (buckets - has1) << 16 | first1;
+        // Each of the thread's buckets' first place, and the place behind them.
+        uint32_t first_of[MINE + 1], ordinal = buckets;
+        first_of[MINE] = held;
+#pragma unroll
+        for (uint32_t i = MINE; i-- > 0;) {
+            const bool has = runs.wanted(MINE * tid + i);
+            first_of[i] = first_of[i + 1] - (has ? runs.tokens[i] : 0), ordinal -= has;
+            s.place_of[MINE * tid + i] = ordinal << 16 | first_of[i];
+        }
         constexpr uint32_t OWN = GATHER / PICK_THREADS;
 #pragma unroll
         for (uint32_t i = 0; i < OWN; i++) s.part[tid + i * PICK_THREADS] = 0;
@@ -785,7 +789,7 @@ __global__ __launch_bounds__(PICK_THREADS) void draw_pick_kernel(const IrisLogit
             return min((s.place_of[bucket_at(key)] >> 16 << fine) + inside, GATHER - 1);
         };
 #pragma unroll 1
-        for (uint32_t i = tid; i < have; i += PICK_THREADS) s.behind[i] = atomicAdd(&s.part[part_at(s.token[i])], 1u);
+        for (uint32_t i = tid; i < have; i += PICK_THREADS) s.behind[i] = (uint16_t)atomicAdd(&s.part[part_at(s.token[i])], 1u);
         __syncthreads();
         static_assert(OWN == 8, "a thread's parts are two times four");
         uint4* parts = (uint4*)s.part + 2 * tid;
@@ -822,20 +826,24 @@ __global__ __launch_bounds__(PICK_THREADS) void draw_pick_kernel(const IrisLogit
         for (uint32_t i = t0; i < t1; i++) s.upto[i] = sum += s.upto[i];
         __syncthreads();
         if (counts_only) {
-            const uint64_t at1 = sum_before(first1);
-            const uint64_t of[2] = {has0 ? at1 - sum_before(first0) : 0, has1 ? sum_before(held) - at1 : 0};
+            uint64_t of[MINE];
+#pragma unroll
+            for (uint32_t i = 0; i < MINE; i++) of[i] = sum_before(first_of[i + 1]) - sum_before(first_of[i]);
             runs.add_up(of, s);
         }
     } else if (counts_only) {
         // The weights of the buckets up to the k-th token's, from the row.
-        s.sum[2 * tid] = s.sum[2 * tid + 1] = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < MINE; i++) s.sum[MINE * tid + i] = 0;
         __syncthreads();
         p.each(0, 63, [&](uint64_t, uint32_t gap) {
             if (gap >> p.d.shift <= runs.k_bucket)
                 atomicAdd((unsigned long long*)&s.sum[gap >> p.d.shift], (unsigned long long)weight_of(p.d, gap));
         });
         __syncthreads();
-        const uint64_t w[2] = {s.sum[2 * tid], s.sum[2 * tid + 1]};
+        uint64_t w[MINE];
+#pragma unroll
+        for (uint32_t i = 0; i < MINE; i++) w[i] = s.sum[MINE * tid + i];
         __syncthreads();
         runs.add_up(w, s);
     }
