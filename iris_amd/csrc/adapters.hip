@@ -45,6 +45,20 @@ constexpr uint32_t TILE_RANKS = 64;    // of A x a workgroup forms at a time: fo
 constexpr uint32_t MAX_SPLITS = 16;    // pieces of the columns, each with sums of its own
 constexpr uint32_t CHUNK_OUTPUTS = 512;  // of a tile of rows that a workgroup forms
 
+// Chunks of so many outputs that the parts have, and the part of one of them
+// (chunk: its number among that part's). Parts differ in size: a grid of as many
+// chunks for each would leave k's and v's to two of eight chiplets.
+inline uint32_t chunks_of(const AdapterShape& s, uint32_t outputs) {
+    uint32_t n = 0;
+    for (uint32_t p = 0; p < s.part_count; p++) n += (s.parts[p].rows + outputs - 1) / outputs;
+    return n;
+}
+__device__ __forceinline__ uint32_t part_of(const AdapterShape& sh, uint32_t outputs, uint32_t& chunk) {
+    uint32_t part = 0;
+    for (uint32_t n; chunk >= (n = (sh.parts[part].rows + outputs - 1) / outputs); part++) chunk -= n;
+    return part;
+}
+
 // A weight's two digits, and the weight from them.
 inline uint16_t digits_of(int16_t w) { return (uint16_t)(((w + 128) & ~255) | (w & 255)); }
 __device__ __forceinline__ int32_t weight_of(uint32_t digits) {
@@ -99,10 +113,11 @@ __global__ __launch_bounds__(256) void shrink_row_kernel(const IrisAdapterRows a
         t[((size_t)row * sh.part_count + part) * sh.max_rank + j] = rounded(s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3], e.a_bits);
 }
 
-// One output a thread: row blockIdx.y, part blockIdx.z.
+// One output a thread: chunk blockIdx.x of the parts' outputs, row blockIdx.y.
 __global__ __launch_bounds__(256) void expand_row_kernel(const IrisAdapterRows a, const AdapterShape sh,
                                                          const AdapterEntry* table, const int32_t* t) {
-    const uint32_t row = blockIdx.y, part = blockIdx.z, i = blockIdx.x * 256 + threadIdx.x;
+    uint32_t chunk = blockIdx.x;
+    const uint32_t row = blockIdx.y, part = part_of(sh, 256, chunk), i = chunk * 256 + threadIdx.x;
     const IrisAdapterPart p = sh.parts[part];
     if (i >= p.rows) return;
     const size_t column = p.first + (size_t)i * p.step;
@@ -499,18 +514,18 @@ __device__ __forceinline__ void expand_outputs(const IrisAdapterRows& a, const I
     }
 }
 
-// Workgroup: outputs from blockIdx.x CHUNK_OUTPUTS on, row tile blockIdx.y, and of
-// blockIdx.z the part and which of the tile's adapters. LDS: operands of the
-// steps of max_rank.
+// Workgroup: chunk blockIdx.x of the parts' outputs, row tile blockIdx.y, and
+// blockIdx.z which of the tile's adapters. LDS: operands of the steps of max_rank.
 template <bool VEC>
 __global__ __launch_bounds__(256) void expand_tile_kernel(const IrisAdapterRows a, const AdapterShape sh, const AdapterEntry* table,
                                                           const int64_t* sums, uint32_t splits, uint32_t slot_groups) {
     extern __shared__ Operand s_digits[];
     __shared__ uint32_t s_wide;
-    const uint32_t row0 = blockIdx.y * TILE_ROWS, tid = threadIdx.x, part = blockIdx.z / slot_groups, turn = blockIdx.z % slot_groups;
+    const uint32_t row0 = blockIdx.y * TILE_ROWS, tid = threadIdx.x, turn = blockIdx.z;
+    uint32_t chunk = blockIdx.x;
+    const uint32_t part = part_of(sh, CHUNK_OUTPUTS, chunk);
     const IrisAdapterPart p = sh.parts[part];
-    const uint32_t i0 = blockIdx.x * CHUNK_OUTPUTS, i1 = min(i0 + CHUNK_OUTPUTS, p.rows);
-    if (i0 >= p.rows) return;
+    const uint32_t i0 = chunk * CHUNK_OUTPUTS, i1 = min(i0 + CHUNK_OUTPUTS, p.rows);
     const uint32_t width = sh.part_count * sh.max_rank;
     Tile t = tile_of(a, sh, row0, false);
     uint32_t copied = ~t.pending;  // rows that no adapter changes
@@ -821,7 +836,7 @@ int iris_adapters_apply(const IrisAdapterBank* b, const IrisAdapterRows* a, void
                           s.parts[1 - low].first == s.parts[low].first + 1 && s.parts[low].first % 4 == 0 && s.parts[0].rows % 4 == 0 &&
                           aligned;
         const uint32_t groups = slot_groups_of(tiles);
-        const dim3 grid((b->most_rows + CHUNK_OUTPUTS - 1) / CHUNK_OUTPUTS, tiles, (pair ? 1 : s.part_count) * groups);
+        const dim3 grid(pair ? (b->most_rows + CHUNK_OUTPUTS - 1) / CHUNK_OUTPUTS : chunks_of(s, CHUNK_OUTPUTS), tiles, groups);
         hipLaunchKernelGGL(shrink_tile_kernel, dim3(splits, tiles, rank_groups(s) * groups), dim3(256), 0, st, *a, s, b->table,
                            (int64_t*)space, groups);
         const int64_t* sums = (const int64_t*)space;
@@ -838,7 +853,7 @@ int iris_adapters_apply(const IrisAdapterBank* b, const IrisAdapterRows* a, void
     }
     hipLaunchKernelGGL(shrink_row_kernel, dim3(s.part_count * s.max_rank, a->rows), dim3(256), 0, st, *a, s, b->table,
                        (int32_t*)space);
-    hipLaunchKernelGGL(expand_row_kernel, dim3((b->most_rows + 255) / 256, a->rows, s.part_count), dim3(256), 0, st, *a,
+    hipLaunchKernelGGL(expand_row_kernel, dim3(chunks_of(s, 256), a->rows), dim3(256), 0, st, *a,
                        s, b->table, (const int32_t*)space);
     return (int)hipGetLastError();
 }
