@@ -37,7 +37,9 @@ struct AdapterShape {
 
 // A call of up to so many rows, and rows times ranks, takes the kernels of single
 // rows: they read an adapter again for each row, but a row's work does not wait
-// for others'.
+// for others'. Both kernels, q|k|v of 4096 columns: rank 16, 256 rows 26 us of 3
+// or of 40 adapters, tiles 26 us for 300 rows of 3 adapters and 93 for 257 of 40;
+// rank 64, 64 rows 27 us, tiles 31 for 65 rows of one adapter.
 constexpr uint32_t FEW_ROWS = 256, FEW_RANKS = 4096;
 __host__ __device__ __forceinline__ bool few(uint32_t rows, uint32_t max_rank) { return rows <= FEW_ROWS && rows * max_rank <= FEW_RANKS; }
 constexpr uint32_t TILE_ROWS = 32;
@@ -85,7 +87,9 @@ __device__ __forceinline__ int64_t wave_sum(int64_t v) {
 }
 
 // One value of t a workgroup: row blockIdx.y, value blockIdx.x of the parts'
-// max_rank each.
+// max_rank each. 64-bit sums of products on the vector units, exact in any order.
+// Bound by its chain of loads (slot, entry, weights): 3.2 us for one row of 4096
+// columns with ranks of 16 and as much for 32 rows; 18 us for 256 rows, its products.
 __global__ __launch_bounds__(256) void shrink_row_kernel(const IrisAdapterRows a, const AdapterShape sh,
                                                          const AdapterEntry* table, int32_t* t) {
     __shared__ int64_t s_sum[4];
@@ -113,7 +117,10 @@ __global__ __launch_bounds__(256) void shrink_row_kernel(const IrisAdapterRows a
         t[((size_t)row * sh.part_count + part) * sh.max_rank + j] = rounded(s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3], e.a_bits);
 }
 
-// One output a thread: chunk blockIdx.x of the parts' outputs, row blockIdx.y.
+// One output a thread: chunk blockIdx.x of the parts' outputs, row blockIdx.y. A
+// thread's weights are one row of B, 32 bytes at rank 16, and t is the same for the
+// whole workgroup. Bound by the chain of loads before it: 2.9 us for one row of
+// q|k|v, 5.8 us (2.9 TB/s of y, out and weights) for 32 rows of gate|up of 16384.
 __global__ __launch_bounds__(256) void expand_row_kernel(const IrisAdapterRows a, const AdapterShape sh,
                                                          const AdapterEntry* table, const int32_t* t) {
     uint32_t chunk = blockIdx.x;
@@ -268,6 +275,14 @@ __device__ __forceinline__ bool shrink_steps(const IrisAdapterRows& a, uint32_t 
 // Workgroup: piece blockIdx.x of the columns, row tile blockIdx.y, and of
 // blockIdx.z which of the tile's adapters and which four rank tiles of them.
 // sums: [piece][row][part_count max_rank].
+//
+// A value's digits are split by the vector units, the larger part of a step; so a
+// wave forms them once for up to four rank tiles, whose sums fill its registers.
+// Neither is the bound (4096 rows of 14336 columns, rank 32: vector units issue in
+// 21% of the cycles, matrix cores 4%) but the loads of x, 235 MB at 4.2 TB/s
+// (56 us), with two workgroups a CU; 2309 rows of q|k|v at rank 64 take 41 us, where
+// each of a tile's adapters reads x again. Two rank tiles a wave and the next step's
+// loads ahead took 74 us there against 63 then, and 57 against 55 here.
 __global__ __launch_bounds__(256, 2) void shrink_tile_kernel(const IrisAdapterRows a, const AdapterShape sh,
                                                              const AdapterEntry* table, int64_t* sums, uint32_t slot_groups) {
     __shared__ int64_t s_sum[TILE_ROWS * (TILE_RANKS + 1)];
@@ -516,6 +531,13 @@ __device__ __forceinline__ void expand_outputs(const IrisAdapterRows& a, const I
 
 // Workgroup: chunk blockIdx.x of the parts' outputs, row tile blockIdx.y, and
 // blockIdx.z which of the tile's adapters. LDS: operands of the steps of max_rank.
+//
+// t is rounded and split once for a chunk, whose outputs then take a few steps of
+// matrix products each and y's read and out's write in 16 bytes a lane: 4096 rows
+// of 4096 outputs, rank 32, 43 us (134 MB at 3.1 TB/s; vector units issue in 40% of
+// the cycles), 2309 rows of q|k|v at rank 64 39 us (113 MB, 2.9 TB/s). Chunks of 256
+// outputs form t twice as often, of 1024 leave few workgroups: where 512 took 52 and
+// 88 us, 256 took 68 and 96, 1024 51 and 93.
 template <bool VEC>
 __global__ __launch_bounds__(256) void expand_tile_kernel(const IrisAdapterRows a, const AdapterShape sh, const AdapterEntry* table,
                                                           const int64_t* sums, uint32_t splits, uint32_t slot_groups) {
@@ -595,8 +617,8 @@ __device__ __forceinline__ void tile_sums(const AdapterEntry& e, const IrisAdapt
 // Two parts whose outputs take turns (gate and up): workgroup as
 // expand_tile_kernel's, of both parts, so that a lane's four outputs of each are
 // eight neighbours of a row. (Part by part every fourth byte of a line would be
-// written at a time: 600 rows of 2 x 14336 at rank 16, 129 us.) LDS: operands of
-// both.
+// written at a time: 600 rows of 2 x 14336 at rank 16, 129 us against 71, which
+// is 138 MB at 1.9 TB/s.) LDS: operands of both.
 __global__ __launch_bounds__(256) void expand_pair_kernel(const IrisAdapterRows a, const AdapterShape sh, const AdapterEntry* table,
                                                           const int64_t* sums, uint32_t splits, uint32_t slot_groups, uint32_t low) {
     extern __shared__ Operand s_digits[];
@@ -671,8 +693,9 @@ uint32_t rank_groups(const AdapterShape& s) { return (s.part_count * ((s.max_ran
 // A x: 63 us with one, 42 with four.)
 uint32_t slot_groups_of(uint32_t tiles) { return tiles <= 8 ? 32 : tiles <= 32 ? 16 : tiles <= 64 ? 8 : 4; }
 
-// Pieces of the columns for a call of tiles: enough workgroups for the card,
-// each with a step for every wave.
+// Pieces of the columns for a call of tiles: enough workgroups for the card (two
+// a CU, which its registers hold), each with a step for every wave. More would only
+// be more sums to write and add.
 uint32_t splits_of(const AdapterShape& s, uint32_t rows) {
     const uint32_t tiles = (rows + TILE_ROWS - 1) / TILE_ROWS, steps = (s.cols + 63) / 64;
     // A piece's accumulators hold 2^14 2 64 a step: 32768 columns at most.

@@ -16,7 +16,9 @@ constexpr uint32_t MAX_VOCAB = 1u << 20, MAX_ROWS = 65535, MAX_HISTORY = 1u << 2
 
 // Tokens a workgroup takes: their counts and biases in LDS.
 constexpr uint32_t MIN_RULE_PIECE = 1024, MAX_RULE_PIECE = 4096, RULE_GROUPS = 2048;
-constexpr uint32_t LONG_TEXT = 4096;   // from here on fewer pieces, since each reads the text
+// Texts from here on: larger pieces, since each reads the text (64 rows of 32000
+// behind texts of up to 32700: 21.6 us with pieces of 4096, 29 with 1024).
+constexpr uint32_t LONG_TEXT = 4096;
 constexpr uint32_t BIAS_PLACES = 512;  // biased tokens of a piece that have their sums there
 constexpr uint32_t COUNT_BITS = 21;    // of a text's 2^20 tokens and a path's 64
 static_assert((BIAS_PLACES + 1) << COUNT_BITS >> COUNT_BITS == BIAS_PLACES + 1 && (1u << COUNT_BITS) > MAX_HISTORY + TREE_MAX_NODES,
@@ -44,8 +46,12 @@ __device__ __forceinline__ void report(const IrisLogitsRules& a, int32_t code) {
 // biases summed in LDS, then the piece's logits pass once, four to a thread and
 // turn where the rows allow it. (Biased tokens are few, so their sums have places
 // of their own: a sum for every token would leave three workgroups a CU, 50 us
-// against 24 for 63 rows of 256000.) The rule's loads are a chain of four (request,
-// rule, parents, ids), which a workgroup of several pieces pays once.
+// against 40 for 63 rows of 256000.) The rule's loads are a chain of four (request,
+// rule, parents, ids), which a workgroup of several pieces pays once. It is what
+// one row of 32000 costs (6.5 us with the launch); 63 rows of 256000 of drafted trees
+// take 38.5 us, 131 MB read and written at 3.4 TB/s, the counts and the barriers
+// around them between the loads and the stores (vector units issue in 45% of the
+// cycles, and waves wait 65% of their time).
 template <bool VEC>
 __global__ __launch_bounds__(256) void rules_kernel(const IrisLogitsRules a, const uint32_t piece) {
     // A token's occurrences, and above COUNT_BITS the place of its biases' sum.
@@ -225,8 +231,17 @@ __global__ __launch_bounds__(256) void rules_kernel(const IrisLogitsRules a, con
 // Three launches: the row's maximum by pieces; the histogram; the places, by one
 // workgroup, which reads the row once more for the tokens of the buckets where
 // they can lie. Of long rows a launch in between gathers those, by pieces: one
-// workgroup has too little in flight (256000 tokens: 30 us).
+// workgroup has too little in flight (256000 tokens: 30 us). Sums of weights are
+// whole numbers, so their order does not matter.
+//
+// All is short work between barriers: one row of 32000 takes 3.4 + 4.3 + 16.7 us,
+// the last one workgroup's chain, nine rows of 256000 3.9 + 15.9 + 12.2 + 9.4. 108
+// rows of 256000 read 110 MB three times, from the last-level cache after the
+// first: 18 us (6.1 TB/s), 39.6 (the terms' arithmetic and atomics, vector units
+// issue in 70% of the cycles), 29.6 (3.7 TB/s) and 14.1.
 
+// Enough that few tokens share a bucket of a dense row: with 1024 the gathered
+// tokens of some rows passed GATHER, 97 to 196 us for 108 rows by their numbers.
 constexpr uint32_t BUCKETS = 2048;
 constexpr uint32_t PICK_THREADS = 512;
 constexpr uint32_t LIST = 512;        // tokens put in order at a time
@@ -234,7 +249,10 @@ constexpr uint32_t GATHER = 4096;     // tokens held in LDS
 constexpr uint32_t SUB_BITS = 9;      // a crowded bucket's parts
 constexpr uint32_t INDEX_BITS = 20;   // of a token's index
 constexpr uint32_t SUM_BITS = 47;     // of a piece's sum of weights, its count above them
-constexpr uint32_t LONG_ROW = 65536;      // rows past this are gathered by pieces
+// Rows past this are gathered by pieces, a launch more. Gathered and not, for 1 and
+// 108 rows: 32000 tokens 27 and 42 us against 21 and 34, 65536 the same within 1 us,
+// 128000 29 and 73 against 36 and 82, 256000 31 and 110 against 58 and 135.
+constexpr uint32_t LONG_ROW = 65536;
 constexpr uint32_t GATHER_PIECE = 16384, PIECE_LIST = 512;  // tokens of a piece, of them held in LDS
 constexpr uint32_t MAX_PIECE = 16384;  // tokens of a piece: their weights of 2^32 add to at most 2^46
 
