@@ -304,3 +304,33 @@ def test_two_calls_at_once():
     torch.cuda.synchronize()
     for c in calls:
         assert np.array_equal(c.out.cpu().numpy(), c.want())
+
+
+@pytest.mark.parametrize("rows", [3, 40, 257, 300])
+@pytest.mark.parametrize("parts", [[(1300, 0, 1), (513, 1300, 1), (40, 1813, 1)], [(40, 0, 1), (1024, 40, 1), (511, 1064, 1)],
+                                   [(1028, 0, 2), (1028, 1, 2)], [(1028, 1, 2), (1028, 0, 2)], [(700, 3, 2), (1200, 2, 2)]],
+                         ids=["falling", "rising", "pairs", "turned", "uneven"])
+def test_parts_of_several_chunks(rows, parts):
+    rng = np.random.default_rng(rows)
+    n = len(parts)
+    ranks = [[20] * n, [16] * (n - 1) + [0], [0] * (n - 1) + [3]]
+    for in_place in (False, True):
+        Call(rng, 64, parts, ranks, rows, rng.integers(-1, 3, rows), in_place=in_place).check()
+
+
+@pytest.mark.parametrize("parts", [QKV, PAIRS, TURNED], ids=["qkv", "pairs", "turned"])
+def test_captured_calls_beside_eager_ones(parts):
+    rng = np.random.default_rng(23)
+    rows = 290
+    c = Call(rng, 192, parts, [[16] * len(parts), [65, 7, 30][:len(parts)]], rows, rng.integers(-1, 2, rows), in_place=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.run(torch.cuda.current_stream().cuda_stream)
+    for _ in range(4):
+        c.slots[:] = rng.integers(-1, 2, rows)
+        c.d_slots.copy_(dev(c.slots))
+        c.fill()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(c.out.cpu().numpy(), c.want())
+        c.check()

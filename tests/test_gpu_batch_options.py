@@ -330,3 +330,27 @@ def test_real_weights_and_cleared_slots():
     assert b.generate([p], 4, options=[RequestOptions(adapter=1)])[0].token_ids == Forward(dm.model).generate(p, 4)[0]
     b.adapters(None)
     assert b.generate([p], 4)[0].token_ids == Forward(dm.model).generate(p, 4)[0]
+
+
+def test_two_batches_of_one_set_in_turn():
+    name, tokens = list(MODELS)[0], 5
+    dm, rng = made(name), np.random.default_rng(31)
+    adapters = [some_adapter(rng, dm.model, ALL, r) for r in (8, 16)]
+    shared = loaded(dm, adapters, 16)
+    ps = prompts(dm, [7, 11])
+    options = [RequestOptions(adapter=i, rule=logits.TokenRule(repetition=80000, frequency=3000),
+                              drawing=logits.drawing(30.0, top_k=200), numbers=rng.integers(0, 2 ** 32, tokens)) for i in (1, 0)]
+    want = [wanted(dm.model, p, tokens, o, adapters)[0] for p, o in zip(ps, options)]
+    batches, got = [], []
+    for p, o in zip(ps, options):
+        b = Batch(dm, 2, 20, 4, 64, 32)
+        b.adapters(shared)
+        b.adapter(1, o.adapter)
+        b.rule(1, o.rule)
+        b.drawing(1, o.drawing, o.numbers, p.size - 1)
+        batches.append(b)
+        got.append([b.prefill({1: p})[1]])
+    for _ in range(tokens - 1):
+        for b, out in zip(batches, got):
+            out += b.step({1: [out[-1]]})[1]
+    assert [g[:len(w)] for g, w in zip(got, want)] == want  # (an end token stops `want`)

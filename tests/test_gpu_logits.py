@@ -448,3 +448,33 @@ def test_rules_then_draw():
     torch.cuda.synchronize()
     d.x = r.want()[:, :4500]
     assert d.got() == d.want()
+
+
+@pytest.mark.parametrize("kind", ["normal", "same", "two"])
+def test_captured_draws_of_long_rows(kind):
+    # Rows whose tokens are gathered by pieces, and crowded ones.
+    rng = np.random.default_rng(24)
+    draws = [[ONE, 0, 0, 0], [ONE, 50, 0, 0], [1 << 18, 0, 4080218931, 0], [30000, 6000, 1 << 31, 0]]
+    c = Draw(some_logits(rng, (4, 70001), kind), draws, some_numbers(rng, 4), extra=3)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.run(torch.cuda.current_stream().cuda_stream)
+    for _ in range(3):
+        c.x[:] = some_logits(rng, c.x.shape, kind)
+        c.x[rng.random(c.x.shape) < 0.2] = ref.LOWEST
+        c.t["logits"][:, :70001].copy_(dev(c.x))
+        c.numbers[:] = rng.integers(0, 2 ** 32, 4)
+        c.t["numbers"].copy_(words(c.numbers))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = c.want()
+        assert c.got() == want
+        c.run()
+        torch.cuda.synchronize()
+        assert c.got() == want
+
+
+@pytest.mark.parametrize("vocab", [65535, 65536, 65537, 66000])
+def test_draw_about_the_longest_row_of_one_workgroup(vocab):
+    rng = np.random.default_rng(vocab)
+    Draw(some_logits(rng, (6, vocab), "normal"), some_drawings(rng, 6), some_numbers(rng, 6)).check()
