@@ -38,7 +38,7 @@ struct AdapterShape {
 // A call of up to so many rows, and rows times ranks, takes the kernels of single
 // rows: they read an adapter again for each row, but a row's work does not wait
 // for others'. Both kernels, q|k|v of 4096 columns: rank 16, 256 rows 26 us of 3
-// or of 40 adapters, tiles 26 us for 300 rows of 3 adapters and 93 for 257 of 40;
+// or of 40 adapters, tiles 26 us for 300 rows of 3 prompts and 93 for 257 of 40;
 // rank 64, 64 rows 27 us, tiles 31 for 65 rows of one adapter.
 constexpr uint32_t FEW_ROWS = 256, FEW_RANKS = 4096;
 __host__ __device__ __forceinline__ bool few(uint32_t rows, uint32_t max_rank) { return rows <= FEW_ROWS && rows * max_rank <= FEW_RANKS; }

@@ -406,8 +406,8 @@ class Batch:
     """Up to ``requests`` requests at a time over one paged K/V cache of
     ``pages`` pages of ``page_size`` positions, each request up to
     ``max_positions``, in passes of up to ``max_rows`` rows (iris_batch_*). A
-    request's tokens are those ``Session.generate`` selects for its prompt,
-    whatever runs beside it."""
+    request's tokens are those ``Session.generate`` selects for its prompt, or
+    those of its own adapter, rule, masks and drawing, whatever runs beside it."""
 
     MAX_STEP_ROWS = 64  # rows of one request in one step
 
@@ -512,9 +512,9 @@ class Batch:
         return n.value
 
     def generate(self, prompts, tokens: int, draft=None, options=None) -> list:
-        """Greedy generation for each prompt: a list of GenerateResult, as
-        ``Session.generate`` gives them (without logits), over requests that
-        are all empty. Prompts wait until a request and enough pages for all
+        """Generation for each prompt, greedy where ``options`` say nothing
+        else: a list of GenerateResult, as ``Session.generate`` gives them
+        (without logits), over requests that are all empty. Prompts wait until a request and enough pages for all
         their positions are free.
         ``options`` (optional) has RequestOptions or None for each prompt: its
         adapter, rules, mask and drawing. Its tokens then depend on these and
