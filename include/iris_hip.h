@@ -798,9 +798,9 @@ int iris_batch_drawing(IrisBatch* batch, uint32_t request, const IrisDrawing* dr
                        uint32_t count);
 /* Masks (host memory, [mask_rows][(vocab + 31) / 32]) for the next pass that
  * succeeds: mask_of has an entry (-1: none) for each of its `rows` ids, of
- * which a prompt's last counts. A pass of another number of rows is refused
- * (IRIS_E_INVALID). Null or no rows: none. A selection of which nothing is open
- * is -1, and a path ends there. */
+ * which a prompt's last counts; mask_rows is at most rows. A pass of another
+ * number of rows is refused (IRIS_E_INVALID). Null or no rows: none. A selection
+ * of which nothing is open is -1, and a path ends there. */
 int iris_batch_masks(IrisBatch* batch, const uint32_t* masks, uint32_t mask_rows, const int32_t* mask_of, uint32_t rows);
 
 /* SHA-256 (FIPS 180-4) of `len` bytes into out[32]; the hash

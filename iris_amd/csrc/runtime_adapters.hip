@@ -102,12 +102,15 @@ int iris_model_adapters_load(IrisModelAdapters* set, uint32_t slot, const char* 
     uint32_t product, part;
     int layer = -1;
     std::string suffix;
+    bool whole = false;  // the name is a layer's number as it is written, and the suffix
     try {
         layer = iris_layer_of(name, &suffix);
+        const std::string full = name, end = "layers." + std::to_string(layer) + "." + suffix;
+        whole = layer >= 0 && full.size() >= end.size() && full.compare(full.size() - end.size(), end.size(), end) == 0;
     } catch (const std::bad_alloc&) {
         return IRIS_E_NOMEM;
     }
-    if (layer < 0 || (uint32_t)layer >= set->model->d.layers || !product_of(suffix.c_str(), &product, &part)) return IRIS_E_INVALID;
+    if (!whole || (uint32_t)layer >= set->model->d.layers || !product_of(suffix.c_str(), &product, &part)) return IRIS_E_INVALID;
     IrisAdapterBank*& bank = set->banks[layer][product];
     if (!bank) {
         if (!rank) return 0;

@@ -858,6 +858,7 @@ int iris_batch_rule(IrisBatch* b, uint32_t request, const IrisTokenRule* rule, c
         return 0;
     }
     if (rule->repetition <= 0 || (rule->bias_count && (!bias_ids || !bias_values))) return IRIS_E_INVALID;
+    if (rule->bias_count > 1u << 20) return IRIS_E_RANGE;
     RT_CHECK(batch_own_buffers(b));
     try {
         // All requests' biases, one after the other, with this one's new ones.

@@ -514,8 +514,9 @@ class Batch:
     def generate(self, prompts, tokens: int, draft=None, options=None) -> list:
         """Generation for each prompt, greedy where ``options`` say nothing
         else: a list of GenerateResult, as ``Session.generate`` gives them
-        (without logits), over requests that are all empty. Prompts wait until a request and enough pages for all
-        their positions are free.
+        (without logits), over requests that are all empty; settings made on
+        them before, and masks, end. Prompts wait until a request and enough
+        pages for all their positions are free.
         ``options`` (optional) has RequestOptions or None for each prompt: its
         adapter, rules, mask and drawing. Its tokens then depend on these and
         on nothing else.
@@ -552,6 +553,7 @@ class Batch:
                 raise ValueError(f"a drawing takes a number for each of the {tokens} tokens")
         for p in prompts:
             native.check(self.dm.ids_refused(p)[0], "batch generate")
+        self.masks(None)
         waiting, running = list(range(len(prompts))), {}  # request -> prompt
         failed = {}  # prompt -> code
 
@@ -579,6 +581,7 @@ class Batch:
 
         def begin(request, p):
             """The request is prompt p's: what p has of its own."""
+            self.release(request)  # (nothing that was set before)
             o = own[p]
             if o is None:
                 return

@@ -354,3 +354,33 @@ def test_two_batches_of_one_set_in_turn():
         for b, out in zip(batches, got):
             out += b.step({1: [out[-1]]})[1]
     assert [g[:len(w)] for g, w in zip(got, want)] == want  # (an end token stops `want`)
+
+
+def test_generation_begins_without_earlier_settings():
+    dm, rng = made("mistral"), np.random.default_rng(41)
+    ps = prompts(dm, [6, 9])
+    want = Batch(dm, 2, 40, 4, 64, 64).generate(ps, 4)
+    b = Batch(dm, 2, 40, 4, 64, 64)
+    s = loaded(dm, [some_adapter(rng, dm.model, ALL, 8)], 8)
+    b.adapters(s)
+    for request in (0, 1):
+        b.adapter(request, 0)
+        b.rule(request, logits.TokenRule(repetition=1 << 20), {int(t): 1 << 28 for t in range(9)})
+        b.drawing(request, logits.drawing(50.0), rng.integers(0, 2 ** 32, 64))
+    b.masks(np.zeros((1, dm.model.vocab), bool), [0])
+    got = b.generate(ps, 4, options=[None, RequestOptions()])
+    assert [r.token_ids for r in got] == [r.token_ids for r in want]
+
+
+def test_names_that_are_no_layers_are_refused():
+    dm = made("mistral")
+    s = ModelAdapters(dm, 1, 4)
+    a = np.zeros((1, 256), np.int16)
+    load = native.lib().iris_model_adapters_load
+    at = b"model.language_model.layers.%s.self_attn.o_proj.weight"
+    assert load(s.handle, 0, at % b"1", a.ctypes.data, 0, a.ctypes.data, 0, 1) == 0
+    held = s.device_bytes()
+    for layer in (b"x", b"", b"00", b" 1", b"+1", b"1x", b"-0", b"4294967296", b"2"):
+        assert load(s.handle, 0, at % layer, a.ctypes.data, 0, a.ctypes.data, 0, 1) == -1
+    assert load(s.handle, 0, at % b"1" + b".x", a.ctypes.data, 0, a.ctypes.data, 0, 1) == -1
+    assert s.device_bytes() == held
