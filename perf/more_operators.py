@@ -188,8 +188,7 @@ def _prepare_adapters(case, seed):
     s = dict(case=case, x=_rows(seed, 1, (rows, cols), 1.0), y=_rows(seed, 2, (rows, width), 2.0), slots=_ints(per_row),
              weights=weights, a_bits=a_bits, b_bits=b_bits,
              by_slot=[(t, [i for i, u in enumerate(per_row) if u == t]) for t in sorted(set(per_row)) if t >= 0])
-    # (A call leaves the columns of no part as they are: those of y.)
-    s["out"] = s["y"].clone()
+    s["out"] = torch.zeros_like(s["y"])
     if own:
         from iris_amd import adapters
         bank = adapters.AdapterBank(cols, parts, slots=case["slots"], max_rank=case["rank"])
