@@ -191,6 +191,8 @@ def _prepare_adapters(case, seed):
     s["out"] = torch.zeros_like(s["y"])
     if own:
         from iris_amd import adapters
+        # (A call leaves the columns of no part as they are.)
+        s["between"] = width > sum(n for n, _, _ in parts)
         bank = adapters.AdapterBank(cols, parts, slots=case["slots"], max_rank=case["rank"])
         for t, ws in enumerate(weights):
             for p, (a, b) in enumerate(ws):
@@ -452,6 +454,8 @@ def _own(s):
     op = s["case"]["op"]
     if op == "adapters":
         bank, call, space, size = s["call"]
+        if s["between"]:
+            s["out"].copy_(s["y"])
         bank.apply(call, space.data_ptr(), size, stream)
         return s["out"]
     if op == "rules":
