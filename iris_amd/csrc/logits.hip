@@ -19,7 +19,7 @@ constexpr uint32_t MIN_RULE_PIECE = 1024, MAX_RULE_PIECE = 4096, RULE_GROUPS = 2
 // Texts from here on: larger pieces, since each reads the text (64 rows of 32000
 // behind texts of up to 32700: 21.6 us with pieces of 4096, 29 with 1024).
 constexpr uint32_t LONG_TEXT = 4096;
-constexpr uint32_t BIAS_PLACES = 512;  // biased tokens of a piece that have their sums there
+constexpr uint32_t BIAS_PLACES = 512;  // sums of biases at a time; a crowded piece has more biased tokens
 constexpr uint32_t COUNT_BITS = 21;    // of a text's 2^20 tokens and a path's 64
 static_assert((BIAS_PLACES + 1) << COUNT_BITS >> COUNT_BITS == BIAS_PLACES + 1 && (1u << COUNT_BITS) > MAX_HISTORY + TREE_MAX_NODES,
               "a count and a place in a word");
@@ -46,7 +46,11 @@ __device__ __forceinline__ void report(const IrisLogitsRules& a, int32_t code) {
 // biases summed in LDS, then the piece's logits pass once, four to a thread and
 // turn where the rows allow it. (Biased tokens are few, so their sums have places
 // of their own: a sum for every token would leave three workgroups a CU, 50 us
-// against 40 for 63 rows of 256000.) The rule's loads are a chain of four (request,
+// against 40 for 63 rows of 256000. A piece with more biased tokens than places, or
+// nearly as many where threads that meet a token at once each take one, is done by
+// parts that have a sum for every token, with a pass over the list each: a bias on
+// each token of one row of 32000 takes 85 us, of 2^20 2.1 ms, of 16 rows of 256000
+// 1.1 ms.) The rule's loads are a chain of four (request,
 // rule, parents, ids), which a workgroup of several pieces pays once. It is what
 // one row of 32000 costs (6.5 us with the launch); 63 rows of 256000 of drafted trees
 // take 38.5 us, 131 MB read and written at 3.4 TB/s, the counts and the barriers
@@ -118,14 +122,9 @@ __global__ __launch_bounds__(256) void rules_kernel(const IrisLogitsRules a, con
     for (uint32_t j = 0; j < HELD; j++) held[j] = tid + 256 * j < words ? text[tid + 256 * j] : -1;
     const uint32_t* bits = a.masks + (size_t)max(mask, 0) * a.mask_stride;
     const double inverse = 1.0 / rule.repetition;
-    // A token that the text or a bias names.
-    auto ruled = [&](int32_t logit, uint32_t v, uint32_t word) {
-        const uint32_t count = word & ((1u << COUNT_BITS) - 1), place = word >> COUNT_BITS;
-        int64_t l = logit, bias = 0;
-        if (place && place <= BIAS_PLACES) bias = (int64_t)s_bias[place - 1];
-        if (place > BIAS_PLACES)  // (more biased tokens than places: the list again)
-            for (uint32_t i = 0; i < rule.bias_count; i++)
-                bias += (uint32_t)a.bias_ids[rule.bias_start + i] == v ? a.bias_values[rule.bias_start + i] : 0;
+    // A token with its occurrences and its biases' sum.
+    auto with_bias = [&](int32_t logit, uint32_t count, int64_t bias) {
+        int64_t l = logit;
         if (count) {
             l = l > 0 ? divided((int32_t)l, rule.repetition, inverse) : dn::rshift_rte(l * rule.repetition, 16);
             l -= (int64_t)count * rule.frequency + rule.presence;
@@ -133,6 +132,12 @@ __global__ __launch_bounds__(256) void rules_kernel(const IrisLogitsRules a, con
         l += bias;
         return logit == INT32_MIN ? INT32_MIN : l < INT32_MIN + 1 ? INT32_MIN + 1 : l > INT32_MAX ? INT32_MAX : (int32_t)l;
     };
+    // A token that the text or a bias names.
+    auto ruled = [&](int32_t logit, uint32_t word) {
+        const uint32_t place = word >> COUNT_BITS;
+        return with_bias(logit, word & ((1u << COUNT_BITS) - 1), place ? (int64_t)s_bias[place - 1] : 0);
+    };
+    auto open = [&](uint32_t v) { return mask < 0 || (bits[v / 32] >> (v % 32) & 1); };
 
 #pragma unroll 1
     for (uint32_t v0 = blockIdx.x * piece; v0 < a.vocab; v0 += gridDim.x * piece) {
@@ -186,11 +191,40 @@ __global__ __launch_bounds__(256) void rules_kernel(const IrisLogitsRules a, con
                     word = old == word ? taken : old;
                 }
                 const uint32_t place = word >> COUNT_BITS;
-                if (place <= BIAS_PLACES)
-                    atomicAdd((unsigned long long*)&s_bias[place - 1], (unsigned long long)(int64_t)a.bias_values[rule.bias_start + i]);
+                if (place > BIAS_PLACES) break;  // (the piece is crowded)
+                atomicAdd((unsigned long long*)&s_bias[place - 1], (unsigned long long)(int64_t)a.bias_values[rule.bias_start + i]);
             }
         }
         if (named) __syncthreads();
+        const bool crowded = biased && s_places > BIAS_PLACES;
+        if (crowded) {
+            // A sum for every token, BIAS_PLACES of them at a time, each time by a
+            // pass over the list, eight loads ahead.
+#pragma unroll 1
+            for (uint32_t u0 = v0; u0 < v1; u0 += BIAS_PLACES) {
+                const uint32_t n = min(BIAS_PLACES, v1 - u0);
+                for (uint32_t i = tid; i < BIAS_PLACES; i += 256) s_bias[i] = 0;
+                __syncthreads();
+#pragma unroll 1
+                for (uint32_t i = tid; i < rule.bias_count; i += 8 * 256) {
+                    int32_t id[8];
+#pragma unroll
+                    for (uint32_t j = 0; j < 8; j++) id[j] = i + 256 * j < rule.bias_count ? a.bias_ids[rule.bias_start + i + 256 * j] : -1;
+#pragma unroll
+                    for (uint32_t j = 0; j < 8; j++) {
+                        const uint32_t k = (uint32_t)id[j] - u0;
+                        if (k < n)
+                            atomicAdd((unsigned long long*)&s_bias[k],
+                                      (unsigned long long)(int64_t)a.bias_values[rule.bias_start + i + 256 * j]);
+                    }
+                }
+                __syncthreads();
+                for (uint32_t v = u0 + tid; v < u0 + n; v += 256)
+                    out[v] = open(v) ? with_bias(in[v], s_count[v - v0] & ((1u << COUNT_BITS) - 1), (int64_t)s_bias[v - u0]) : INT32_MIN;
+                __syncthreads();  // before the next tokens' sums
+            }
+            continue;
+        }
         if constexpr (VEC) {
 #pragma unroll
             for (uint32_t i = 0; i < TURNS; i++) {
@@ -202,7 +236,7 @@ __global__ __launch_bounds__(256) void rules_kernel(const IrisLogitsRules a, con
                 if (c.x | c.y | c.z | c.w) {
 #pragma unroll 1
                     for (uint32_t j = 0; j < 4; j++) {
-                        const int32_t y = ruled(j == 0 ? l.x : j == 1 ? l.y : j == 2 ? l.z : l.w, v + j,
+                        const int32_t y = ruled(j == 0 ? l.x : j == 1 ? l.y : j == 2 ? l.z : l.w,
                                                 j == 0 ? c.x : j == 1 ? c.y : j == 2 ? c.z : c.w);
                         l.x = j == 0 ? y : l.x, l.y = j == 1 ? y : l.y, l.z = j == 2 ? y : l.z, l.w = j == 3 ? y : l.w;
                     }
@@ -212,9 +246,7 @@ __global__ __launch_bounds__(256) void rules_kernel(const IrisLogitsRules a, con
             }
         }
         for (uint32_t v = fours + tid; v < v1; v += 256)
-            out[v] = mask >= 0 && !(bits[v / 32] >> (v % 32) & 1)
-                         ? INT32_MIN
-                         : ruled(in[v], v, named ? s_count[v - v0] : 0);
+            out[v] = open(v) ? ruled(in[v], named ? s_count[v - v0] : 0) : INT32_MIN;
         if (named) __syncthreads();  // before the next piece's counts
     }
 }

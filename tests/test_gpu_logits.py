@@ -478,3 +478,53 @@ def test_captured_draws_of_long_rows(kind):
 def test_draw_about_the_longest_row_of_one_workgroup(vocab):
     rng = np.random.default_rng(vocab)
     Draw(some_logits(rng, (6, vocab), "normal"), some_drawings(rng, 6), some_numbers(rng, 6)).check()
+
+
+@pytest.mark.parametrize("vocab", [513, 1025, 5000, 40001])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_rules_of_a_bias_on_every_token(vocab, in_place):
+    # Lists that no piece has room for, beside short and empty ones.
+    rng = np.random.default_rng(vocab)
+    ids = np.concatenate([rng.permutation(vocab + 4) - 2, rng.integers(0, vocab, vocab)]).astype(np.int32)
+    rules = [[int(1.3 * ONE), ONE, 0, 0, 0, len(ids)], [ONE, 0, 0, 0, 0, vocab], [int(1.3 * ONE), 5, 9, 0, 7, 3], [ONE, 0, 0, 0, 0, 0]]
+    for extra in ((0, 0), (3, 5)):
+        c = Rules(rng, vocab, [60, 5, 9, 0], rules=rules, masks=2, extra=extra, in_place=in_place, biases=len(ids) // 4)
+        values = rng.integers(-2 ** 31, 2 ** 31, len(ids), dtype=np.int64).astype(np.int32)
+        c.bias_ids, c.bias_values = ids, values
+        c.t["bias_ids"], c.t["bias_values"] = dev(ids), dev(values)
+        c.d.bias_ids, c.d.bias_values, c.d.biases = c.t["bias_ids"].data_ptr(), c.t["bias_values"].data_ptr(), len(ids)
+        c.check()
+
+
+def test_rules_of_a_token_with_thousands_of_biases():
+    # Beside as many others as there is room for, one fewer and one more.
+    rng = np.random.default_rng(25)
+    for others in (1, 255, 510, 511, 512, 900):
+        ids = np.concatenate([np.full(7000, 77), 100 + np.arange(others)]).astype(np.int32)
+        ids = ids[rng.permutation(len(ids))]
+        c = Rules(rng, 1024, [30, 4], rules=[[ONE, 9, 0, 0, 0, len(ids)], [2 * ONE, 0, 0, 0, 5000, 2000]], biases=len(ids) // 2)
+        c.bias_ids, c.bias_values = ids, rng.integers(-2 ** 31, 2 ** 31, len(ids), dtype=np.int64).astype(np.int32)
+        c.t["bias_ids"], c.t["bias_values"] = dev(c.bias_ids), dev(c.bias_values)
+        c.d.bias_ids, c.d.bias_values, c.d.biases = c.t["bias_ids"].data_ptr(), c.t["bias_values"].data_ptr(), len(ids)
+        c.check()
+
+
+def test_the_time_of_a_bias_on_every_token():
+    # A pass over the list for each part of a piece, not for each of its tokens:
+    # that took 101 ms here.
+    rng = np.random.default_rng(26)
+    n = 1 << 18
+    t = dict(logits=dev(rng.integers(-9 * ONE, 9 * ONE, (1, n)).astype(np.int32)), out=torch.zeros(n, dtype=torch.int32, device="cuda"),
+             request=dev([0]), rules=words([[ONE, 0, 0, 0, 0, n]]), bias_ids=dev(rng.permutation(n).astype(np.int32)),
+             bias_values=dev(np.full(n, 5, np.int32)))
+    d = logits.LogitsRules(rows=1, vocab=n, logits_stride=n, out_stride=n, requests=1, biases=n, **{k: v.data_ptr() for k, v in t.items()})
+    stream, times = torch.cuda.current_stream().cuda_stream, []
+    for _ in range(4):
+        begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        begin.record()
+        logits.apply_rules(d, stream)
+        end.record()
+        end.synchronize()
+        times.append(begin.elapsed_time(end))
+    assert torch.equal(t["out"], t["logits"][0] + 5)
+    assert min(times) < 10, times
