@@ -39,9 +39,12 @@ struct AdapterShape {
 // rows: they read an adapter again for each row, but a row's work does not wait
 // for others'. Both kernels, q|k|v of 4096 columns: rank 16, 256 rows 26 us of 3
 // or of 40 adapters, tiles 26 us for 300 rows of 3 prompts and 93 for 257 of 40;
-// rank 64, 64 rows 27 us, tiles 31 for 65 rows of one adapter.
+// rank 64, 64 rows 27 us, tiles 31 for 65 rows of one adapter. The rank is the
+// largest that the bank holds, not the largest that it may (of which the work
+// space is): in a bank for ranks up to 256, of 40 adapters of rank 16, 256 rows take
+// 30 us a call so and 193 by what it may hold.
 constexpr uint32_t FEW_ROWS = 256, FEW_RANKS = 4096;
-__host__ __device__ __forceinline__ bool few(uint32_t rows, uint32_t max_rank) { return rows <= FEW_ROWS && rows * max_rank <= FEW_RANKS; }
+inline bool few(uint32_t rows, uint32_t rank) { return rows <= FEW_ROWS && rows * rank <= FEW_RANKS; }
 constexpr uint32_t TILE_ROWS = 32;
 constexpr uint32_t TILE_RANKS = 64;    // of A x a workgroup forms at a time: four 16-rank tiles
 constexpr uint32_t MAX_SPLITS = 16;    // pieces of the columns, each with sums of its own
@@ -87,34 +90,37 @@ __device__ __forceinline__ int64_t wave_sum(int64_t v) {
 }
 
 // One value of t a workgroup: row blockIdx.y, value blockIdx.x of the parts'
-// max_rank each. 64-bit sums of products on the vector units, exact in any order.
+// `ranks` each, the largest rank when the call was made (a captured call's bank may
+// hold larger ones since: then every ranks-th value). 64-bit sums of products on the vector units, exact in any order.
 // Bound by its chain of loads (slot, entry, weights): 3.2 us for one row of 4096
 // columns with ranks of 16 and as much for 32 rows; 18 us for 256 rows, its products.
 __global__ __launch_bounds__(256) void shrink_row_kernel(const IrisAdapterRows a, const AdapterShape sh,
-                                                         const AdapterEntry* table, int32_t* t) {
+                                                         const AdapterEntry* table, int32_t* t, uint32_t ranks) {
     __shared__ int64_t s_sum[4];
-    const uint32_t row = blockIdx.y, part = blockIdx.x / sh.max_rank, j = blockIdx.x % sh.max_rank;
+    const uint32_t row = blockIdx.y, part = blockIdx.x / ranks;
     const int32_t slot = slot_of(a, sh.slots, row, blockIdx.x == 0 && threadIdx.x == 0);
     if (slot < 0) return;
     const AdapterEntry e = table[slot * sh.part_count + part];
-    if (j >= e.rank) return;
     const int4* x = (const int4*)(a.x + (size_t)row * a.x_stride);
-    const int4* w = (const int4*)(e.a + (size_t)j * sh.cols);
-    int64_t sum = 0;
-    for (uint32_t i = threadIdx.x; i < sh.cols / 8; i += 256) {
-        const int4 p = w[i], x0 = x[2 * i], x1 = x[2 * i + 1];
-        const int32_t q[4] = {p.x, p.y, p.z, p.w}, v[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+    for (uint32_t j = blockIdx.x % ranks; j < e.rank; j += ranks) {
+        const int4* w = (const int4*)(e.a + (size_t)j * sh.cols);
+        int64_t sum = 0;
+        for (uint32_t i = threadIdx.x; i < sh.cols / 8; i += 256) {
+            const int4 p = w[i], x0 = x[2 * i], x1 = x[2 * i + 1];
+            const int32_t q[4] = {p.x, p.y, p.z, p.w}, v[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-            sum += (int64_t)weight_of((uint32_t)q[c]) * v[2 * c];
-            sum += (int64_t)weight_of((uint32_t)q[c] >> 16) * v[2 * c + 1];
+            for (int c = 0; c < 4; c++) {
+                sum += (int64_t)weight_of((uint32_t)q[c]) * v[2 * c];
+                sum += (int64_t)weight_of((uint32_t)q[c] >> 16) * v[2 * c + 1];
+            }
         }
+        sum = wave_sum(sum);
+        if (threadIdx.x % 64 == 0) s_sum[threadIdx.x / 64] = sum;
+        __syncthreads();
+        if (threadIdx.x == 0)
+            t[((size_t)row * sh.part_count + part) * sh.max_rank + j] = rounded(s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3], e.a_bits);
+        if (j + ranks < e.rank) __syncthreads();  // before the next value's sums
     }
-    sum = wave_sum(sum);
-    if (threadIdx.x % 64 == 0) s_sum[threadIdx.x / 64] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0)
-        t[((size_t)row * sh.part_count + part) * sh.max_rank + j] = rounded(s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3], e.a_bits);
 }
 
 // One output a thread: chunk blockIdx.x of the parts' outputs, row blockIdx.y. A
@@ -704,7 +710,8 @@ uint32_t splits_of(const AdapterShape& s, uint32_t rows) {
 }
 
 // Bytes of work space of a call: t itself for few rows, its sums by pieces for
-// tiles.
+// tiles. Where it goes by the ranks that the bank holds which of the two a call
+// takes, this is the tiles', the larger.
 uint64_t space_of(const AdapterShape& s, uint32_t rows) {
     const uint64_t values = (uint64_t)rows * s.part_count * s.max_rank;
     return few(rows, s.max_rank) ? values * 4 + 32 : values * splits_of(s, rows) * 8;
@@ -719,6 +726,8 @@ struct IrisAdapterBank {
     uint64_t slot_weights = 0;      // weights of a slot
     uint64_t part_at[IRIS_ADAPTER_PARTS] = {};
     uint32_t most_rows = 0, width = 0;
+    std::vector<uint16_t> ranks;  // [slots][parts], as the table's
+    uint32_t rank = 0;            // the largest of them
 };
 
 uint64_t iris_adapters_space(uint32_t cols, uint32_t part_count, uint32_t max_rank, uint32_t rows) {
@@ -761,6 +770,12 @@ int iris_adapters_create(uint32_t cols, const IrisAdapterPart* parts, uint32_t p
         b->slot_weights = (b->slot_weights + 127) & ~127ull;
         b->most_rows = std::max(b->most_rows, parts[p].rows);
         b->width = std::max(b->width, parts[p].first + (parts[p].rows - 1) * parts[p].step + 1);
+    }
+    try {
+        b->ranks.assign((size_t)slots * part_count, 0);
+    } catch (const std::bad_alloc&) {
+        delete b;
+        return IRIS_E_NOMEM;
     }
     const size_t entries = (size_t)slots * part_count * sizeof(AdapterEntry);
     hipError_t st = hipMalloc((void**)&b->weights, b->slot_weights * slots * 2);
@@ -821,13 +836,17 @@ int iris_adapters_load(IrisAdapterBank* b, uint32_t slot, uint32_t part, const i
     hipError_t st = hipDeviceSynchronize();
     if (st != hipSuccess) return (int)st;
     // (A copy that fails on the way leaves the part empty.)
+    uint16_t& held = b->ranks[(size_t)slot * s.part_count + part];
     st = hipMemcpy(entry, &e, sizeof(e), hipMemcpyHostToDevice);
+    if (st == hipSuccess) held = 0;
     if (st == hipSuccess && rank) {
         e.a = to, e.b = to + a_count;
         e.rank = rank, e.a_bits = a_bits, e.b_bits = b_bits;
         st = hipMemcpy(to, digits.data(), count * 2, hipMemcpyHostToDevice);
         if (st == hipSuccess) st = hipMemcpy(entry, &e, sizeof(e), hipMemcpyHostToDevice);
+        if (st == hipSuccess) held = (uint16_t)rank;
     }
+    b->rank = *std::max_element(b->ranks.begin(), b->ranks.end());
     return (int)st;
 }
 
@@ -846,7 +865,7 @@ int iris_adapters_apply(const IrisAdapterBank* b, const IrisAdapterRows* a, void
     if (a->rows > 65535) return IRIS_E_RANGE;
     if (space_bytes < space_of(s, a->rows)) return IRIS_E_RANGE;
     hipStream_t st = (hipStream_t)stream;
-    if (!few(a->rows, s.max_rank)) {
+    if (!few(a->rows, b->rank)) {
         const uint32_t tiles = (a->rows + TILE_ROWS - 1) / TILE_ROWS, splits = splits_of(s, a->rows);
         const size_t lds = (s.max_rank + 63) / 64 * 2 * DIGIT_PLANES * sizeof(Operand);
         // Sixteen bytes of a row at a time where every part allows it.
@@ -874,8 +893,9 @@ int iris_adapters_apply(const IrisAdapterBank* b, const IrisAdapterRows* a, void
         }
         return (int)hipGetLastError();
     }
-    hipLaunchKernelGGL(shrink_row_kernel, dim3(s.part_count * s.max_rank, a->rows), dim3(256), 0, st, *a, s, b->table,
-                       (int32_t*)space);
+    const uint32_t ranks = std::max(b->rank, 1u);
+    hipLaunchKernelGGL(shrink_row_kernel, dim3(s.part_count * ranks, a->rows), dim3(256), 0, st, *a, s, b->table, (int32_t*)space,
+                       ranks);
     hipLaunchKernelGGL(expand_row_kernel, dim3(chunks_of(s, 256), a->rows), dim3(256), 0, st, *a,
                        s, b->table, (const int32_t*)space);
     return (int)hipGetLastError();

@@ -334,3 +334,77 @@ def test_captured_calls_beside_eager_ones(parts):
         torch.cuda.synchronize()
         assert np.array_equal(c.out.cpu().numpy(), c.want())
         c.check()
+
+
+def in_larger_bank(c, max_rank):
+    """The call's adapters in a bank that may hold larger ones."""
+    c.bank = adapters.AdapterBank(c.cols, c.parts, len(c.weights), max_rank)
+    for s, slot in enumerate(c.weights):
+        for p, pair in enumerate(slot):
+            if pair is not None:
+                c.bank.load(s, p, *pair)
+    c.size = c.bank.workspace_bytes(c.rows)
+    c.space = torch.full((2 * MARGIN + c.size,), 0xA5, dtype=torch.uint8, device="cuda")
+    return c
+
+
+@pytest.mark.parametrize("rows", [1, 17, 70, 256, 257])
+@pytest.mark.parametrize("parts", [QKV, PAIRS, ODD], ids=["qkv", "pairs", "odd"])
+def test_a_bank_that_may_hold_larger_ranks(rows, parts):
+    rng = np.random.default_rng(31)
+    n = len(parts)
+    ranks = [[16] * n, [5] * n, [1] * (n - 1) + [0], [8] * n]
+    for max_rank in (17, 64, 256):
+        c = Call(rng, 160, parts, ranks, rows, rng.integers(-1, 4, rows), in_place=max_rank == 64)
+        in_larger_bank(c, max_rank).check()
+    # None loaded, and the largest one emptied.
+    c = in_larger_bank(Call(rng, 160, parts, [[0] * n, [0] * n], rows, rng.integers(-1, 2, rows)), 256)
+    c.check()
+    a, b = Call.some(rng, (200, 160), "normal"), Call.some(rng, (parts[0][0], 200), "normal")
+    c.bank.load(1, 0, a, 18, b, 16)
+    c.weights[1][0] = (a, 18, b, 16)
+    c.check()
+    c.bank.load(1, 0, None)
+    c.weights[1][0] = None
+    c.check()
+
+
+@pytest.mark.parametrize("rows", [1, 20, 300])
+def test_a_captured_call_takes_larger_ranks_loaded_since(rows):
+    rng = np.random.default_rng(32)
+    c = in_larger_bank(Call(rng, 224, QKV, [[0, 0, 0], [3, 9, 0]], rows, rng.integers(-1, 2, rows), in_place=True), 130)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.run(torch.cuda.current_stream().cuda_stream)
+    for rank in (2, 9, 10, 19, 64, 130, 1):
+        for slot, part in ((0, 0), (1, 2)):
+            a, b = Call.some(rng, (rank, 224), "uniform"), Call.some(rng, (QKV[part][0], rank), "uniform")
+            c.bank.load(slot, part, a, 20, b, 14)
+            c.weights[slot][part] = (a, 20, b, 14)
+        c.fill()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(c.out.cpu().numpy(), c.want())
+        c.check()
+
+
+def test_the_time_goes_by_the_ranks_that_are_loaded():
+    # 256 rows of 40 adapters of rank 16 took 30 us where the bank could hold
+    # such ranks, and 193 where it could hold ranks of 256.
+    rng = np.random.default_rng(33)
+    parts, rows, best = [(4096, 0, 1), (1024, 4096, 1), (1024, 5120, 1)], 256, []
+    c = Call(rng, 4096, parts, [[16] * 3] * 40, rows, np.arange(rows) % 40)
+    for max_rank in (16, 256):
+        in_larger_bank(c, max_rank)
+        times = []
+        for _ in range(5):
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            stream = torch.cuda.current_stream().cuda_stream
+            begin.record()
+            for _ in range(20):
+                c.run(stream)
+            end.record()
+            end.synchronize()
+            times.append(begin.elapsed_time(end))
+        best.append(min(times))
+    assert best[1] < 3 * best[0], best
