@@ -775,7 +775,8 @@ int iris_model_adapters_clear(IrisModelAdapters* set, uint32_t slot);
 /* A batch's requests with adapters, rules and draws of their own. Each setting
  * holds from the next pass on until it is set again or the request is released;
  * requests without any run as ever. The calls are synchronous; a refused one
- * changes nothing.
+ * changes nothing. Rules, draws and masks are refused (IRIS_E_RANGE) for a model
+ * of more than 2^20 tokens.
  *
  * iris_batch_adapters: the set that the requests' slots name (null: none, and
  * no request has an adapter then). iris_batch_adapter: a request's slot, -1 for

@@ -463,9 +463,17 @@ static int batch_alloc(T** p, uint64_t count) {
 }
 
 // The buffers of passes whose requests have something of their own, made for the
-// first that does.
-static int batch_own_buffers(IrisBatch* b) {
+// first that does; IRIS_E_RANGE where they `select` by it and the vocabulary is
+// larger than the operators on logits take.
+static int batch_own_buffers(IrisBatch* b, bool select) {
     const uint64_t rows = b->s->max_rows;
+    uint64_t bytes = 0;  // what any number of rows of a draw takes
+    IrisLogitsDraw d{};
+    d.logits = (const int32_t*)256, d.tokens = (int32_t*)256;
+    d.vocab = d.logits_stride = b->s->model->d.vocab;
+    for (d.rows = 1; select && !b->draw_space && d.rows <= LOGITS_ROWS; d.rows++)
+        bytes = std::max(bytes, iris_logits_draw_workspace_bytes(&d));
+    if (select && !b->draw_space && !bytes) return IRIS_E_RANGE;
     if (!b->own) RT_CHECK(batch_alloc(&b->own, 5 * rows));
     if (!b->drawn) RT_CHECK(batch_alloc(&b->drawn, rows));
     if (!b->host_own) {
@@ -477,13 +485,7 @@ static int batch_own_buffers(IrisBatch* b) {
         }
         std::memset(b->host_own, 0, 5 * rows * 4);
     }
-    if (!b->draw_space) {
-        IrisLogitsDraw d{};
-        d.logits = (const int32_t*)256, d.tokens = b->drawn;
-        d.rows = LOGITS_ROWS, d.vocab = d.logits_stride = b->s->model->d.vocab;
-        // (What any number of rows up to these takes.)
-        uint64_t bytes = 0;
-        for (d.rows = 1; d.rows <= LOGITS_ROWS; d.rows++) bytes = std::max(bytes, iris_logits_draw_workspace_bytes(&d));
+    if (bytes) {
         uint8_t* space = nullptr;
         RT_CHECK(batch_alloc(&space, bytes));
         b->draw_space = space, b->draw_bytes = bytes;
@@ -814,7 +816,7 @@ int iris_batch_adapters(IrisBatch* b, const IrisModelAdapters* set) {
                 const AdapterProductShape p = iris_adapter_product(b->s->model, l, product);
                 bytes = std::max(bytes, iris_adapters_space(p.cols, p.part_count, max_rank, b->s->max_rows));
             }
-        RT_CHECK(batch_own_buffers(b));
+        RT_CHECK(batch_own_buffers(b, false));
         const uint64_t H = d.hidden, rows = b->s->max_rows;
         if (!b->normed) {  // and a row of zeros
             int32_t *normed = nullptr, *gate_up = nullptr;
@@ -859,7 +861,7 @@ int iris_batch_rule(IrisBatch* b, uint32_t request, const IrisTokenRule* rule, c
     }
     if (rule->repetition <= 0 || (rule->bias_count && (!bias_ids || !bias_values))) return IRIS_E_INVALID;
     if (rule->bias_count > 1u << 20) return IRIS_E_RANGE;
-    RT_CHECK(batch_own_buffers(b));
+    RT_CHECK(batch_own_buffers(b, true));
     try {
         // All requests' biases, one after the other, with this one's new ones.
         std::vector<int32_t> ids, values, own_ids, own_values;
@@ -926,7 +928,7 @@ int iris_batch_drawing(IrisBatch* b, uint32_t request, const IrisDrawing* drawin
     }
     if (count && !numbers) return IRIS_E_INVALID;
     if (count > b->max_positions) return IRIS_E_RANGE;
-    RT_CHECK(batch_own_buffers(b));
+    RT_CHECK(batch_own_buffers(b, true));
     try {
         std::vector<uint32_t> own;
         if (count) own.assign(numbers, numbers + count);
@@ -958,7 +960,7 @@ int iris_batch_masks(IrisBatch* b, const uint32_t* masks, uint32_t mask_rows, co
     if (rows > b->s->max_rows || mask_rows > rows) return IRIS_E_RANGE;
     for (uint32_t r = 0; r < rows; r++)
         if (mask_of[r] < -1 || mask_of[r] >= (int64_t)mask_rows) return IRIS_E_INVALID;
-    RT_CHECK(batch_own_buffers(b));
+    RT_CHECK(batch_own_buffers(b, true));
     const uint64_t words = (uint64_t)mask_rows * ((b->s->model->d.vocab + 31) / 32);
     try {
         std::vector<int32_t> of(mask_of, mask_of + rows);

@@ -384,3 +384,26 @@ def test_names_that_are_no_layers_are_refused():
         assert load(s.handle, 0, at % layer, a.ctypes.data, 0, a.ctypes.data, 0, 1) == -1
     assert load(s.handle, 0, at % b"1" + b".x", a.ctypes.data, 0, a.ctypes.data, 0, 1) == -1
     assert s.device_bytes() == held
+
+
+def test_rules_and_draws_of_a_larger_vocabulary_are_refused():
+    # The operators on logits take 2^20 tokens; such a model generates greedily
+    # as ever, with adapters too.
+    model = synth.mistral_model(32, 1, 1, 1, 32, 64, (1 << 20) + 32, seed=27)
+    dm, rng = DeviceModel(model), np.random.default_rng(42)
+    p, = prompts(dm, [5])
+    want = Session(dm, 16, 8).generate(p, 3).token_ids
+    b = Batch(dm, 1, 8, 4, 32, 16)
+    for call in (lambda: b.rule(0, RULE), lambda: b.drawing(0, logits.drawing(), [0] * 9),
+                 lambda: b.masks(np.ones((1, model.vocab), bool), [0] * 5)):
+        with pytest.raises(native.IrisError) as e:
+            call()
+        assert e.value.code == -5
+    b.rule(0, None)
+    b.drawing(0, None)
+    b.masks(None)
+    assert b.generate([p], 3)[0].token_ids == want
+    pairs = some_adapter(rng, model, ALL, 8)
+    b.adapters(loaded(dm, [pairs], 8))
+    assert b.generate([p], 3, options=[RequestOptions(adapter=0)])[0].token_ids == \
+        Forward(model, pairs).generate(p, 3)[0]
