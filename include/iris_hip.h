@@ -779,7 +779,8 @@ int iris_model_adapters_clear(IrisModelAdapters* set, uint32_t slot);
  * of more than 2^20 tokens.
  *
  * iris_batch_adapters: the set that the requests' slots name (null: none, and
- * no request has an adapter then). iris_batch_adapter: a request's slot, -1 for
+ * no request has an adapter then). Requests keep their slots; a set that lacks one
+ * of them is refused (IRIS_E_INVALID). iris_batch_adapter: a request's slot, -1 for
  * none (IRIS_E_STATE without a set). A row's product is the layer's, plus its
  * residual where the layer adds it in the same step, plus the adapter's
  * (IrisAdapterRows); gate and up have theirs before the activation. Keys and

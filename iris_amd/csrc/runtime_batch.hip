@@ -810,6 +810,8 @@ int iris_batch_adapters(IrisBatch* b, const IrisModelAdapters* set) {
     if (set) {
         uint32_t slots, max_rank;
         if (iris_model_adapters_model(set, &slots, &max_rank) != b->s->model) return IRIS_E_INVALID;
+        for (const int32_t slot : b->slot)
+            if (slot >= 0 && (uint32_t)slot >= slots) return IRIS_E_INVALID;
         uint64_t bytes = 16;
         for (uint32_t l = 0; l < d.layers; l++)
             for (uint32_t product = 0; product < ADAPT_PRODUCTS; product++) {
@@ -838,7 +840,7 @@ int iris_batch_adapters(IrisBatch* b, const IrisModelAdapters* set) {
         }
     }
     b->adapters = set;
-    std::fill(b->slot.begin(), b->slot.end(), -1);
+    if (!set) std::fill(b->slot.begin(), b->slot.end(), -1);
     return 0;
 }
 

@@ -460,7 +460,8 @@ class Batch:
         native.check(native.lib().iris_batch_release(self._h, request), "batch release")
 
     def adapters(self, adapters: ModelAdapters | None):
-        """The adapters that requests' slots name (None: none)."""
+        """The adapters that requests' slots name (None: none, and no request has
+        an adapter then). Requests keep their slots, which the set must have."""
         native.check(native.lib().iris_batch_adapters(self._h, adapters.handle if adapters else None), "batch adapters")
         self._adapters = adapters  # (kept as long as the batch uses them)
 

@@ -407,3 +407,45 @@ def test_rules_and_draws_of_a_larger_vocabulary_are_refused():
     b.adapters(loaded(dm, [pairs], 8))
     assert b.generate([p], 3, options=[RequestOptions(adapter=0)])[0].token_ids == \
         Forward(model, pairs).generate(p, 3)[0]
+
+
+def test_requests_keep_their_slots_when_the_set_is_given_again():
+    name = "mistral"
+    dm, rng = made(name), np.random.default_rng(43)
+    adapters = [some_adapter(rng, dm.model, ALL, 8) for _ in range(4)]
+    first, second = loaded(dm, adapters[:2], 8), loaded(dm, adapters[2:], 8)
+    p, = prompts(dm, [6])
+    numbers = rng.integers(0, 2 ** 32, 64)
+
+    def tokens(pairs):
+        return Forward(dm.model, pairs).generate(p, 1, drawing=(logits.drawing(40.0).inverse_temperature, 0, 0, 0),
+                                                 numbers=numbers[p.size - 1:])[0]
+    want = [tokens(a) for a in adapters] + [tokens(None)]
+    assert len({t[0] for t in want}) > 3
+    b = Batch(dm, 2, 20, 4, 64, 32)
+
+    def got(slot):
+        b.drawing(0, logits.drawing(40.0), numbers)
+        out = [b.prefill({0: p})[0]]
+        b.release(0)
+        b.adapter(0, slot)  # (a released request has none)
+        return out
+
+    b.adapters(first)
+    b.adapter(0, 1)
+    b.adapters(first)
+    assert got(1) == want[1]
+    b.adapters(second)  # the slot of the other set
+    assert got(1) == want[3]
+    # A set without a request's slot is refused and changes nothing.
+    small = loaded(dm, adapters[:1], 8)
+    with pytest.raises(native.IrisError) as e:
+        b.adapters(small)
+    assert e.value.code == -1
+    assert got(0) == want[3]
+    b.adapters(small)
+    assert got(0) == want[0]
+    b.adapters(None)
+    assert got(-1) == want[4]
+    b.adapters(first)
+    assert got(-1) == want[4]
