@@ -389,12 +389,26 @@ class ModelAdapters:
             pass
 
 
+def _biases(biases) -> np.ndarray:
+    """{token: value} or (token, value) pairs as int32 [count][2]."""
+    if isinstance(biases, np.ndarray):
+        pairs = biases
+        if pairs.ndim != 2 or pairs.shape[1] != 2 or pairs.dtype.kind not in "iu":
+            raise ValueError("an array of biases takes integers [count][2]")
+        if pairs.size and (pairs.min() < -(1 << 31) or pairs.max() >= 1 << 31):
+            raise OverflowError("biased tokens and biases are 32-bit integers")
+    else:
+        pairs = list(biases.items()) if isinstance(biases, dict) else list(biases) if biases is not None else []
+        pairs = [(int(t), int(v)) for t, v in pairs]
+    return np.array(pairs, dtype=np.int32).reshape(-1, 2)
+
+
 @dataclass
 class RequestOptions:
     """What one prompt of ``Batch.generate`` has of its own."""
     adapter: int = -1                    # slot of the batch's adapters
     rule: TokenRule | None = None        # its penalties (bias_start and _count are not read)
-    biases: object = None                # {token: Q16.16 value} or (token, value) pairs
+    biases: object = None                # {token: Q16.16 value} or (token, value) pairs, an array of them too
     drawing: Drawing | None = None       # logits.drawing(...)
     # The random 32-bit numbers of the tokens to come, in order.
     numbers: object = None
@@ -472,14 +486,12 @@ class Batch:
     def rule(self, request: int, rule: TokenRule | None, biases=None):
         """A request's penalties and biases, {token: Q16.16 value} or pairs
         (None: neither)."""
-        if rule is None and not biases:
+        ids, values = np.ascontiguousarray(_biases(biases).T)
+        if rule is None and not ids.size:
             native.check(native.lib().iris_batch_rule(self._h, request, None, None, None), "batch rule")
             return
-        pairs = list(biases.items()) if isinstance(biases, dict) else list(biases or ())
-        ids = np.array([t for t, _ in pairs], dtype=np.int32)
-        values = np.array([v for _, v in pairs], dtype=np.int32)
         r = TokenRule.from_buffer_copy(rule) if rule is not None else TokenRule(repetition=1 << 16)
-        r.bias_start, r.bias_count = 0, len(pairs)
+        r.bias_start, r.bias_count = 0, ids.size
         native.check(native.lib().iris_batch_rule(self._h, request, C.byref(r), ids.ctypes.data, values.ctypes.data),
                      "batch rule")
 
@@ -588,8 +600,9 @@ class Batch:
                 return
             if o.adapter >= 0:
                 self.adapter(request, o.adapter)
-            if o.rule is not None or o.biases:
-                self.rule(request, o.rule, o.biases)
+            biases = _biases(o.biases)
+            if o.rule is not None or len(biases):
+                self.rule(request, o.rule, biases)
             if o.drawing is not None:
                 self.drawing(request, o.drawing, np.asarray(o.numbers)[:tokens], prompts[p].size - 1)
 

@@ -449,3 +449,20 @@ def test_requests_keep_their_slots_when_the_set_is_given_again():
     assert got(-1) == want[4]
     b.adapters(first)
     assert got(-1) == want[4]
+
+
+def test_biases_as_an_array():
+    dm = made("mistral")
+    p, = prompts(dm, [6])
+    b = Batch(dm, 1, 20, 4, 64, 32)
+    plain = b.generate([p], 3)[0].token_ids
+    pairs = [(int(plain[0]), -100 * ONE), (5, ONE), (5, ONE)]
+    want = wanted(dm.model, p, 3, RequestOptions(biases=pairs), ())[0]
+    assert want != plain
+    for biases in (pairs, np.array(pairs), np.array(pairs, np.int32)):
+        assert b.generate([p], 3, options=[RequestOptions(biases=biases)])[0].token_ids == want
+        b.rule(0, None, biases)
+        assert b.prefill({0: p})[0] == want[0]
+        b.release(0)
+    for none in (None, {}, [], np.zeros((0, 2), np.int32)):
+        assert b.generate([p], 3, options=[RequestOptions(biases=none)])[0].token_ids == plain
