@@ -540,7 +540,9 @@ class Batch:
         that the model cannot embed are dropped, with what lies below them.
         (Ids outside the vocabulary are refused, as in a prompt.) Where the
         device has no work space for a pass with its drafts, it runs without.
-        Prompts with ids that cannot be embedded are refused before any pass.
+        Prompts with ids that cannot be embedded are refused before any pass,
+        and so are options that cannot be: an adapter that the batch's set
+        lacks, a rule, biases or numbers out of range.
         A prompt whose own selection cannot be embedded ends there, as a
         session's does; the others go on, and at the end IrisError is raised
         with ``results``: the list, None for each such prompt."""
@@ -561,9 +563,7 @@ class Batch:
         own = list(options) if options is not None else [None] * len(prompts)
         if len(own) != len(prompts):
             raise ValueError("options must have an entry for each prompt")
-        for o in own:
-            if o is not None and o.drawing is not None and len(o.numbers if o.numbers is not None else ()) < tokens:
-                raise ValueError(f"a drawing takes a number for each of the {tokens} tokens")
+        settings = [self._settings(o, tokens) for o in own]
         for p in prompts:
             native.check(self.dm.ids_refused(p)[0], "batch generate")
         self.masks(None)
@@ -595,16 +595,15 @@ class Batch:
         def begin(request, p):
             """The request is prompt p's: what p has of its own."""
             self.release(request)  # (nothing that was set before)
-            o = own[p]
-            if o is None:
+            if own[p] is None:
                 return
-            if o.adapter >= 0:
-                self.adapter(request, o.adapter)
-            biases = _biases(o.biases)
-            if o.rule is not None or len(biases):
-                self.rule(request, o.rule, biases)
-            if o.drawing is not None:
-                self.drawing(request, o.drawing, np.asarray(o.numbers)[:tokens], prompts[p].size - 1)
+            biases, numbers = settings[p]
+            if own[p].adapter >= 0:
+                self.adapter(request, own[p].adapter)
+            if own[p].rule is not None or len(biases):
+                self.rule(request, own[p].rule, biases)
+            if own[p].drawing is not None:
+                self.drawing(request, own[p].drawing, numbers, prompts[p].size - 1)
 
         def mask_rows(rows, parents):
             """The masks of the pass over {request: ids to come}."""
@@ -696,6 +695,25 @@ class Batch:
             e.results = [None if p in failed else r for p, r in enumerate(results)]
             raise e
         return results
+
+    def _settings(self, o, tokens: int) -> tuple:
+        """What the options bring as arrays: (biases [count][2], the numbers of
+        the tokens). Raises for what the batch would refuse whenever it came."""
+        if o is None:
+            return (), ()
+        if o.adapter >= 0 and self._adapters is None:
+            raise native.IrisError(-4, "batch generate")
+        if o.adapter < -1 or (o.adapter >= 0 and o.adapter >= self._adapters.slots) or \
+                (o.rule is not None and o.rule.repetition <= 0):
+            raise native.IrisError(-1, "batch generate")
+        biases = _biases(o.biases)
+        selects = o.rule is not None or len(biases) or o.drawing is not None or o.mask is not None
+        if len(biases) > 1 << 20 or (selects and self.dm.model.vocab > 1 << 20):
+            raise native.IrisError(-5, "batch generate")
+        numbers = np.ascontiguousarray(o.numbers if o.drawing is not None and o.numbers is not None else (), dtype=np.uint32)
+        if o.drawing is not None and numbers.size < tokens:
+            raise ValueError(f"a drawing takes a number for each of the {tokens} tokens")
+        return biases, numbers[:tokens]
 
     def _embedded(self, drafted, above):
         """The proposals without those whose embedding is refused for its

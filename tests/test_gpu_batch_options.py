@@ -466,3 +466,32 @@ def test_biases_as_an_array():
         b.release(0)
     for none in (None, {}, [], np.zeros((0, 2), np.int32)):
         assert b.generate([p], 3, options=[RequestOptions(biases=none)])[0].token_ids == plain
+
+
+def test_options_that_cannot_be_are_refused_before_any_pass():
+    dm, rng = made("mistral"), np.random.default_rng(44)
+    ps = prompts(dm, [5, 7, 4])
+    want = [r.token_ids for r in Batch(dm, 1, 20, 4, 64, 32).generate(ps, 3)]
+    b, passes = Batch(dm, 1, 20, 4, 64, 32), []  # one request: the last prompt's turn comes late
+    prefill = b.prefill
+    b.prefill = lambda rows: passes.append(rows) or prefill(rows)
+
+    def refused(error, code=None, **kw):
+        with pytest.raises(error) as e:
+            b.generate(ps, 3, options=[None, None, RequestOptions(**kw)])
+        assert code is None or e.value.code == code
+        assert not passes and b.length(0) == 0
+
+    refused(native.IrisError, -4, adapter=0)
+    b.adapters(loaded(dm, [some_adapter(rng, dm.model, ALL, 4)] * 2, 4))
+    for slot in (2, -2, 1 << 20):
+        refused(native.IrisError, -1, adapter=slot)
+    for repetition in (0, -5):
+        refused(native.IrisError, -1, rule=logits.TokenRule(repetition=repetition))
+    refused(native.IrisError, -5, biases=np.zeros(((1 << 20) + 1, 2), np.int32))
+    refused(OverflowError, biases={1: 1 << 31})
+    refused(OverflowError, biases=np.array([[1 << 31, 0]]))
+    refused(ValueError, biases=np.zeros((4, 3), np.int32))
+    refused(OverflowError, drawing=logits.drawing(), numbers=[1, 1 << 32, 2])
+    refused(ValueError, drawing=logits.drawing(), numbers=[1, 2])
+    assert [r.token_ids for r in b.generate(ps, 3, options=[None, RequestOptions(), None])] == want
