@@ -544,8 +544,10 @@ class Batch:
         and so are options that cannot be: an adapter that the batch's set
         lacks, a rule, biases or numbers out of range.
         A prompt whose own selection cannot be embedded ends there, as a
-        session's does; the others go on, and at the end IrisError is raised
-        with ``results``: the list, None for each such prompt."""
+        session's does, and one whose options find no room when its turn comes
+        (all requests' biases, memory) does not begin; the others go on, and at
+        the end IrisError is raised with ``results``: the list, None for each
+        such prompt."""
         prompts = [np.ascontiguousarray(p, dtype=np.int32) for p in prompts]
         eos = self.dm.model.eos_token_ids
         results = [GenerateResult([], None) for _ in prompts]
@@ -568,7 +570,7 @@ class Batch:
             native.check(self.dm.ids_refused(p)[0], "batch generate")
         self.masks(None)
         waiting, running = list(range(len(prompts))), {}  # request -> prompt
-        failed = {}  # prompt -> code
+        failed = {}  # prompt -> (code, at what)
 
         def ended(request):
             self.release(request)
@@ -588,22 +590,29 @@ class Batch:
                     return ended(request)
             code = self.dm.ids_refused(new[-1:])[0]  # the next pass embeds it
             if code:
-                failed[running[request]] = code
+                failed[running[request]] = code, "embedding a selection of"
                 return ended(request)
             return False
 
         def begin(request, p):
-            """The request is prompt p's: what p has of its own."""
+            """The request is prompt p's: what p has of its own. False where
+            there is no room for it."""
             self.release(request)  # (nothing that was set before)
             if own[p] is None:
-                return
+                return True
             biases, numbers = settings[p]
-            if own[p].adapter >= 0:
-                self.adapter(request, own[p].adapter)
-            if own[p].rule is not None or len(biases):
-                self.rule(request, own[p].rule, biases)
-            if own[p].drawing is not None:
-                self.drawing(request, own[p].drawing, numbers, prompts[p].size - 1)
+            try:
+                if own[p].adapter >= 0:
+                    self.adapter(request, own[p].adapter)
+                if own[p].rule is not None or len(biases):
+                    self.rule(request, own[p].rule, biases)
+                if own[p].drawing is not None:
+                    self.drawing(request, own[p].drawing, numbers, prompts[p].size - 1)
+            except native.IrisError as e:
+                failed[p] = e.code, "the options of"
+                ended(request)
+                return False
+            return True
 
         def mask_rows(rows, parents):
             """The masks of the pass over {request: ids to come}."""
@@ -646,8 +655,8 @@ class Batch:
                     free -= pages[p]
                     rows += prompts[p].size
                 if start:
-                    for request, p in start.items():
-                        begin(request, p)
+                    start = {request: p for request, p in start.items() if begin(request, p)}
+                if start:
                     mask_rows({r: prompts[p].tolist() for r, p in start.items()}, {})
                     for request, token in self.prefill({r: prompts[p] for r, p in start.items()}).items():
                         took(request, [token])
@@ -691,7 +700,8 @@ class Batch:
             raise
         if failed:
             first = min(failed)
-            e = native.IrisError(failed[first], f"batch generate: embedding a selection of prompt {first}")
+            code, what = failed[first]
+            e = native.IrisError(code, f"batch generate: {what} prompt {first}")
             e.results = [None if p in failed else r for p, r in enumerate(results)]
             raise e
         return results

@@ -451,23 +451,6 @@ def test_requests_keep_their_slots_when_the_set_is_given_again():
     assert got(-1) == want[4]
 
 
-def test_biases_as_an_array():
-    dm = made("mistral")
-    p, = prompts(dm, [6])
-    b = Batch(dm, 1, 20, 4, 64, 32)
-    plain = b.generate([p], 3)[0].token_ids
-    pairs = [(int(plain[0]), -100 * ONE), (5, ONE), (5, ONE)]
-    want = wanted(dm.model, p, 3, RequestOptions(biases=pairs), ())[0]
-    assert want != plain
-    for biases in (pairs, np.array(pairs), np.array(pairs, np.int32)):
-        assert b.generate([p], 3, options=[RequestOptions(biases=biases)])[0].token_ids == want
-        b.rule(0, None, biases)
-        assert b.prefill({0: p})[0] == want[0]
-        b.release(0)
-    for none in (None, {}, [], np.zeros((0, 2), np.int32)):
-        assert b.generate([p], 3, options=[RequestOptions(biases=none)])[0].token_ids == plain
-
-
 def test_options_that_cannot_be_are_refused_before_any_pass():
     dm, rng = made("mistral"), np.random.default_rng(44)
     ps = prompts(dm, [5, 7, 4])
@@ -495,3 +478,39 @@ def test_options_that_cannot_be_are_refused_before_any_pass():
     refused(OverflowError, drawing=logits.drawing(), numbers=[1, 1 << 32, 2])
     refused(ValueError, drawing=logits.drawing(), numbers=[1, 2])
     assert [r.token_ids for r in b.generate(ps, 3, options=[None, RequestOptions(), None])] == want
+
+
+def test_biases_as_an_array():
+    dm = made("mistral")
+    p, = prompts(dm, [6])
+    b = Batch(dm, 1, 20, 4, 64, 32)
+    plain = b.generate([p], 3)[0].token_ids
+    pairs = [(int(plain[0]), -100 * ONE), (5, ONE), (5, ONE)]
+    want = wanted(dm.model, p, 3, RequestOptions(biases=pairs), ())[0]
+    assert want != plain
+    for biases in (pairs, np.array(pairs), np.array(pairs, np.int32)):
+        assert b.generate([p], 3, options=[RequestOptions(biases=biases)])[0].token_ids == want
+        b.rule(0, None, biases)
+        assert b.prefill({0: p})[0] == want[0]
+        b.release(0)
+    for none in (None, {}, [], np.zeros((0, 2), np.int32)):
+        assert b.generate([p], 3, options=[RequestOptions(biases=none)])[0].token_ids == plain
+
+
+def test_prompts_whose_options_find_no_room_leave_the_others_results():
+    dm = made("mistral")
+    ps = prompts(dm, [5, 7, 4])
+    plain = Batch(dm, 3, 40, 4, 64, 64).generate(ps, 4)
+    # Two requests' biases together pass the most that all may have.
+    many = np.zeros((700000, 2), np.int32)
+    many[:, 0] = dm.model.vocab  # (outside the vocabulary: no token changes)
+    options = [None, RequestOptions(biases=many), RequestOptions(biases=many)]
+    b = Batch(dm, 3, 40, 4, 64, 64)
+    with pytest.raises(native.IrisError) as e:
+        b.generate(ps, 4, options=options)
+    assert e.value.code == -5 and "prompt 2" in str(e.value)
+    assert [r and r.token_ids for r in e.value.results] == [plain[0].token_ids, plain[1].token_ids, None]
+    assert [b.length(i) for i in range(3)] == [0, 0, 0]
+    # One after the other they fit.
+    got = Batch(dm, 1, 40, 4, 64, 64).generate(ps, 4, options=options)
+    assert [r.token_ids for r in got] == [r.token_ids for r in plain]
