@@ -62,7 +62,8 @@ def to_fixed(weights: np.ndarray) -> tuple:
     most = float(np.abs(w).max()) if w.size else 0.0
     if not math.isfinite(most) or most > MAX_WEIGHT:
         raise ValueError("an adapter's weights must be finite and at most 32639")
-    bits = MAX_BITS if most == 0.0 else min(MAX_BITS, int(math.floor(math.log2(MAX_WEIGHT / most))))
+    # (Below 2^-MAX_BITS all have the most bits; the quotient of the smallest would be infinite.)
+    bits = MAX_BITS if most < 2.0 ** -MAX_BITS else min(MAX_BITS, int(math.floor(math.log2(MAX_WEIGHT / most))))
     while np.rint(most * 2.0 ** bits) > MAX_WEIGHT:
         bits -= 1
     return np.rint(w * 2.0 ** bits).astype(np.int16), bits

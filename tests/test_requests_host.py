@@ -169,3 +169,12 @@ def test_reference_draw():
     assert ref.draw(l, far, 0) == (1, one, 2 * one) and ref.draw(l, far, (1 << 31) - 1) == (1, one, 2 * one)
     assert ref.draw(l, far, 1 << 31)[0] == 2 and ref.draw(l, None, 7) == (1, one, one)
     assert ref.draw(np.full(3, ref.LOWEST, np.int32), far, 5) == (-1, 0, 0)
+
+
+@pytest.mark.parametrize("scale", [5e-324, 1e-310, 1e-300, 1e-20, 2.0 ** -41, 2.0 ** -40, 2.0 ** -26, 2.0 ** -25])
+def test_tiny_weights_to_fixed(scale):
+    # The smallest overflowed in the number of bits.
+    w = np.array([[scale, -scale, 0.0]])
+    q, bits = adapters.to_fixed(w)
+    assert bits == (adapters.MAX_BITS if scale < 2.0 ** -25 else 39)
+    assert np.array_equal(q, np.rint(w * 2.0 ** bits))
