@@ -514,3 +514,44 @@ def test_prompts_whose_options_find_no_room_leave_the_others_results():
     # One after the other they fit.
     got = Batch(dm, 1, 40, 4, 64, 64).generate(ps, 4, options=options)
     assert [r.token_ids for r in got] == [r.token_ids for r in plain]
+
+
+def own_of(rng, i, vocab, tokens):
+    """Options that differ from request to request in all that is kept by row."""
+    return RequestOptions(rule=logits.TokenRule(repetition=ONE + 3000 * i, frequency=200 * i, presence=0, window=i % 5) if i % 3 else None,
+                          biases={int(t): 3 * ONE for t in rng.integers(0, vocab, i % 4)},
+                          mask=mask_of(i, vocab) if i % 4 != 1 else None,
+                          drawing=logits.drawing(20.0 + i, top_k=(0, 9, 100)[i % 3]) if i % 5 else None,
+                          numbers=rng.integers(0, 2 ** 32, tokens))
+
+
+@pytest.mark.parametrize("name", ["mistral", "gemma"])
+def test_drafts_of_more_rows_than_logits_are_held_for(name):
+    # Up to 120 rows a pass, a request's on both sides of the 64th.
+    dm, rng = made(name), np.random.default_rng(51)
+    n, tokens, vocab = 20, 6, dm.model.vocab
+    options = [own_of(rng, i, vocab, tokens) for i in range(n)]
+    ps = prompts(dm, [3 + i % 5 for i in range(n)])
+    want = [wanted(dm.model, p, tokens, o, ()) for p, o in zip(ps, options)]
+    known = [p.tolist() + w[0] for p, w in zip(ps, want)]
+    b, most = Batch(dm, n, 100, 4, 64, 120), []
+    step = b.step
+    b.step = lambda rows, parents=None: most.append(sum(len(r) for r in rows.values())) or step(rows, parents)
+    for seed in range(3):
+        got = b.generate(ps, tokens, draft=drafter(known, vocab, seed), options=options)
+        assert [(r.token_ids, r.stop_reason) for r in got] == want
+    assert max(most) > 64
+
+
+def test_more_prompts_than_logits_are_held_for():
+    dm, rng = made("mistral odd"), np.random.default_rng(52)
+    n, tokens, vocab = 70, 2, dm.model.vocab
+    options = [own_of(rng, i, vocab, tokens) for i in range(n)]
+    ps = prompts(dm, [1 + i % 3 for i in range(n)])
+    want = [wanted(dm.model, p, tokens, o, ()) for p, o in zip(ps, options)]
+    b, most = Batch(dm, n, 2 * n, 4, 64, 150), []
+    prefill = b.prefill
+    b.prefill = lambda rows: most.append(len(rows)) or prefill(rows)
+    got = b.generate(ps, tokens, options=options)
+    assert [(r.token_ids, r.stop_reason) for r in got] == want
+    assert max(most) == n
