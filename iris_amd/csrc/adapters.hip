@@ -701,12 +701,11 @@ uint32_t slot_groups_of(uint32_t tiles) { return tiles <= 8 ? 32 : tiles <= 32 ?
 
 // Pieces of the columns for a call of tiles: enough workgroups for the card (two
 // a CU, which its registers hold), each with a step for every wave. More would only
-// be more sums to write and add.
+// be more sums to write and add. (One piece holds any columns: a step adds at most
+// 2 64 2^14 to an accumulator, and a wave has a quarter of at most 1024 steps.)
 uint32_t splits_of(const AdapterShape& s, uint32_t rows) {
     const uint32_t tiles = (rows + TILE_ROWS - 1) / TILE_ROWS, steps = (s.cols + 63) / 64;
-    // A piece's accumulators hold 2^14 2 64 a step: 32768 columns at most.
-    const uint32_t least = (s.cols + 32767) / 32768;
-    return std::max(least, std::min(std::min(512 / (tiles * rank_groups(s)), (steps + 3) / 4), MAX_SPLITS));
+    return std::max(1u, std::min(std::min(512 / (tiles * rank_groups(s)), (steps + 3) / 4), MAX_SPLITS));
 }
 
 // Bytes of work space of a call: t itself for few rows, its sums by pieces for

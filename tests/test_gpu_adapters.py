@@ -408,3 +408,19 @@ def test_the_time_goes_by_the_ranks_that_are_loaded():
             times.append(begin.elapsed_time(end))
         best.append(min(times))
     assert best[1] < 3 * best[0], best
+
+
+def test_the_largest_sums_in_one_piece():
+    # So many tiles and ranks that the columns are not divided: every digit at
+    # its end in each of 65504 products, with a sum of either sign.
+    rng, rows = np.random.default_rng(34), 700
+    parts = [(2, 0, 1), (2, 2, 1), (2, 4, 1)]
+    for x in (-2 ** 31, 2 ** 31 - 1, -(128 << 16 | 128 << 8 | 128), 127 << 16 | 127 << 8 | 127):
+        c = Call(rng, 65504, parts, [[2, 1, 1]], rows, [0] * rows, weights="top", bits=(33, 15))
+        for p, pair in enumerate(c.weights[0]):
+            c.weights[0][p] = (np.full_like(pair[0], (127 * 257, -32639, -126 * 256 - 128)[p]), *pair[1:])
+        in_larger_bank(c, 256)
+        c.x[:] = x
+        c.x[::3] = -1 - x
+        c.d_x.copy_(Call.strided(c.x, 65504))
+        c.check()
