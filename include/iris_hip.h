@@ -582,8 +582,8 @@ uint64_t iris_adapters_device_bytes(const IrisAdapterBank* bank);
 
 /* Copies one part of an adapter from host memory: A and B row by row, their
  * fraction bits (at most IRIS_ADAPTER_BITS) and the rank; rank 0 empties the
- * part (a and b are not read then). Waits for the device first, so that no
- * call still reads the slot. IRIS_E_RANGE for a weight or a rank past the
+ * part (a and b are not read then). Waits for the current device, which is to be
+ * the bank's, first, so that no call still reads the slot. IRIS_E_RANGE for a weight or a rank past the
  * bounds; the part is then as it was. */
 int iris_adapters_load(IrisAdapterBank* bank, uint32_t slot, uint32_t part, const int16_t* a, uint32_t a_bits,
                        const int16_t* b, uint32_t b_bits, uint32_t rank);

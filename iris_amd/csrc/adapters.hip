@@ -287,7 +287,8 @@ __device__ __forceinline__ bool shrink_steps(const IrisAdapterRows& a, uint32_t 
 // Neither is the bound (4096 rows of 14336 columns, rank 32: vector units issue in
 // 21% of the cycles, matrix cores 4%) but the loads of x, 235 MB at 4.2 TB/s
 // (56 us), with two workgroups a CU; 2309 rows of q|k|v at rank 64 take 41 us, where
-// each of a tile's adapters reads x again. Two rank tiles a wave and the next step's
+// each of a tile's adapters reads x again, by three workgroups of four of its twelve
+// rank tiles each. Two rank tiles a wave and the next step's
 // loads ahead took 74 us there against 63 then, and 57 against 55 here.
 __global__ __launch_bounds__(256, 2) void shrink_tile_kernel(const IrisAdapterRows a, const AdapterShape sh,
                                                              const AdapterEntry* table, int64_t* sums, uint32_t slot_groups) {
@@ -623,8 +624,9 @@ __device__ __forceinline__ void tile_sums(const AdapterEntry& e, const IrisAdapt
 // Two parts whose outputs take turns (gate and up): workgroup as
 // expand_tile_kernel's, of both parts, so that a lane's four outputs of each are
 // eight neighbours of a row. (Part by part every fourth byte of a line would be
-// written at a time: 600 rows of 2 x 14336 at rank 16, 129 us against 71, which
-// is 138 MB at 1.9 TB/s.) LDS: operands of both.
+// written at a time: 600 rows of 2 x 14336 at rank 16, 129 us against 75, which
+// is 138 MB at 1.8 TB/s: y's loads wait for the sums before them.) LDS: operands of
+// both.
 __global__ __launch_bounds__(256) void expand_pair_kernel(const IrisAdapterRows a, const AdapterShape sh, const AdapterEntry* table,
                                                           const int64_t* sums, uint32_t splits, uint32_t slot_groups, uint32_t low) {
     extern __shared__ Operand s_digits[];
